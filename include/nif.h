@@ -34,9 +34,11 @@ extern "C" {
 #define NIF_ERR_LAUNCH (-4)        /* hipGetLastError() != hipSuccess after a launch */
 #define NIF_ERR_NO_DEVICE (-5)
 
-/* element types of nif_xty inputs */
+/* element types: nif_xty takes the first two, the head losses F32, BF16 and F16 */
 #define NIF_F32 0
 #define NIF_F64 1
+#define NIF_BF16 2
+#define NIF_F16 3
 
 /* nif_xty flags */
 #define NIF_RELU_A 1      /* clamp A's elements at 0 while loading (git_rebasin.py:97) */
@@ -485,6 +487,62 @@ int nif_lsq_refit_f32(const float* X, int64_t ldx, int64_t m, int d, const float
 size_t nif_lsq_solve_workspace_bytes(int d, int N);
 int nif_lsq_solve_f64(const double* G, int64_t ldg, const double* R, int64_t ldr, int d, int N, double cutoff_rel,
                       double* W, int64_t ldw, int32_t* rank_host, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- losses of a linear head over many classes, the logits not kept ---------------------------------------------
+ * z = hidden weight^T + bias, u = z / tau, lse = logsumexp(u) along the classes, and per row a target distribution p:
+ *   loss[n] = tau^2 ( sum_k p[n][k] (log p[n][k] - u[n][at(n,k)]) + P[n] lse[n] ),  P[n] = sum_k p[n][k].
+ * labels: one class with p = 1 and tau = 1 (softmax cross entropy); a row whose label is ignore_index is left out.
+ * top_indices / top_values (rows x top, contiguous): a teacher's top logits t, p = exp(t / tau - L) with L = top_lse[n]
+ * (the teacher's log-sum-exp of t / tau over all classes) or, when NULL, over the row's entries.  Entries of a negative
+ * index or of value -inf carry nothing; a row of none is left out.  Equal indices in a row add up.  A label or index
+ * that is not a class makes its row NaN.  Rows that are left out have loss 0 and gradient 0, whatever they hold.
+ * Reductions: NONE: loss[rows]; SUM; MEAN over the rows that count (0 when there are none).
+ * hidden rows x features (ldh), weight classes x features (ldw), bias classes or NULL, all of `dtype`; any alignment.
+ * Products accumulate in 32 bits; f32 operands are split into three bf16 parts (f32-level accuracy).
+ * `state` carries the forward pass's results to the backward pass, which needs the same inputs; the workspaces are
+ * scratch of each call.  dhidden, dweight, dbias: of `dtype`, written in full; NULL where not wanted. */
+#define NIF_REDUCE_NONE 0
+#define NIF_REDUCE_MEAN 1
+#define NIF_REDUCE_SUM 2
+#define NIF_TOP_MAX_K 1024
+typedef struct nif_head_desc {
+  const void* hidden;
+  int64_t ldh;
+  const void* weight;
+  int64_t ldw;
+  const void* bias;
+  int64_t rows;
+  int32_t features, classes, dtype, reduction;
+  const int64_t* labels;
+  int64_t ignore_index;
+  const int32_t* top_indices;
+  const float* top_values;
+  const float* top_lse;
+  int32_t top; /* entries a row; 0 with labels */
+  float temperature;
+} nif_head_desc;
+size_t nif_head_state_bytes(const nif_head_desc* h);
+size_t nif_head_forward_workspace_bytes(const nif_head_desc* h);
+size_t nif_head_backward_workspace_bytes(const nif_head_desc* h);
+int nif_head_forward(const nif_head_desc* h, float* loss, void* state, size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
+/* grad_loss: one f32 (MEAN, SUM) or rows of them (NONE), on the device */
+int nif_head_backward(const nif_head_desc* h, const float* grad_loss, const void* state, size_t state_bytes, void* dhidden,
+                      int64_t lddh, void* dweight, int64_t lddw, void* dbias, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- the same distillation loss of given logits (rows x classes, ld; F32, BF16 or F16) --------------------------- */
+size_t nif_distill_state_bytes(int64_t rows, int top);
+size_t nif_distill_workspace_bytes(int64_t rows);
+int nif_distill_forward(const void* logits, int64_t ld, int64_t rows, int classes, int dtype, const int32_t* top_indices,
+                        const float* top_values, const float* top_lse, int top, float temperature, int reduction, float* loss,
+                        void* state, size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
+int nif_distill_backward(const void* logits, int64_t ld, int64_t rows, int classes, int dtype, int top, float temperature,
+                         int reduction, const float* grad_loss, const void* state, size_t state_bytes, void* dlogits, int64_t ldd,
+                         void* stream);
+
+/* ---- a teacher's top logits: the `top` largest of each row, larger first and equal ones by the lower class (NaN before
+ * everything), their classes, and logsumexp(row / temperature).  values: rows x top of `dtype`; contiguous outputs. */
+int nif_top_logits(const void* logits, int64_t ld, int64_t rows, int classes, int dtype, int top, float temperature, void* values,
+                   int32_t* indices, float* lse, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,9 @@ import torch  # noqa: F401
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libnif.so')
 
-NIF_F32, NIF_F64 = 0, 1
+NIF_F32, NIF_F64, NIF_BF16, NIF_F16 = 0, 1, 2, 3
+NIF_REDUCE_NONE, NIF_REDUCE_MEAN, NIF_REDUCE_SUM = 0, 1, 2
+NIF_TOP_MAX_K = 1024
 NIF_RELU_A, NIF_RELU_B, NIF_SYMMETRIC, NIF_TRANS_A, NIF_TRANS_B, NIF_XTY_SPLIT_BF16 = 1, 2, 4, 8, 16, 32
 NIF_LAP_MAX_N = 8192
 NIF_LAP_STATIC_MAX_N = 2048
@@ -35,6 +37,17 @@ NIF_ERR_UNSUPPORTED = -3
 
 _c = ctypes
 _vp, _i32, _i64, _sz = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_size_t
+
+
+class HeadDesc(_c.Structure):
+    """nif_head_desc"""
+    _fields_ = [('hidden', _vp), ('ldh', _i64), ('weight', _vp), ('ldw', _i64), ('bias', _vp), ('rows', _i64),
+                ('features', _c.c_int32), ('classes', _c.c_int32), ('dtype', _c.c_int32), ('reduction', _c.c_int32),
+                ('labels', _vp), ('ignore_index', _i64), ('top_indices', _vp), ('top_values', _vp), ('top_lse', _vp),
+                ('top', _c.c_int32), ('temperature', _c.c_float)]
+
+
+_desc = _c.POINTER(HeadDesc)
 
 # name -> (restype, argtypes); mirrors include/nif.h one to one
 SIGNATURES = {
@@ -105,6 +118,16 @@ SIGNATURES = {
     'nif_lsq_solve_workspace_bytes': (_sz, [_i32, _i32]),
     'nif_lsq_solve_f64': (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _c.c_double, _vp, _i64, _c.POINTER(_c.c_int32), _vp, _sz,
                                  _vp]),
+    'nif_head_state_bytes': (_sz, [_desc]),
+    'nif_head_forward_workspace_bytes': (_sz, [_desc]),
+    'nif_head_backward_workspace_bytes': (_sz, [_desc]),
+    'nif_head_forward': (_i32, [_desc, _vp, _vp, _sz, _vp, _sz, _vp]),
+    'nif_head_backward': (_i32, [_desc, _vp, _vp, _sz, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
+    'nif_distill_state_bytes': (_sz, [_i64, _i32]),
+    'nif_distill_workspace_bytes': (_sz, [_i64]),
+    'nif_distill_forward': (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _c.c_float, _i32, _vp, _vp, _sz, _vp, _sz, _vp]),
+    'nif_distill_backward': (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _c.c_float, _i32, _vp, _vp, _sz, _vp, _i64, _vp]),
+    'nif_top_logits': (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _c.c_float, _vp, _vp, _vp, _vp]),
     'nif_kmeans_farthest_init_redo_count': (_i32, [_c.POINTER(_c.c_uint32), _vp]),
     'nif_eigh_trd_launch_counts': (_i32, [_c.POINTER(_c.c_uint64)]),
     'nif_eigh_kept_workspace_bytes': (_sz, [_i32]),

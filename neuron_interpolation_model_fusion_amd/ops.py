@@ -985,6 +985,236 @@ def weighted_mse(pred, truth, w=None):
     return _WeightedMSE.apply(pred, truth, w)
 
 
+# ---- losses of a head over many classes ----------------------------------------------------------------
+
+_HEAD_DT = {torch.float32: _lib.NIF_F32, torch.bfloat16: _lib.NIF_BF16, torch.float16: _lib.NIF_F16}
+_REDUCTIONS = {'none': _lib.NIF_REDUCE_NONE, 'mean': _lib.NIF_REDUCE_MEAN, 'sum': _lib.NIF_REDUCE_SUM}
+
+
+def _bytes(n, device):
+    return torch.empty(max(int(n), 1), dtype=torch.uint8, device=device)
+
+
+def _same_device(what, *ts):
+    _need_gpu(*ts)
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f'{what}: tensors are on different devices: {sorted(map(str, devices))}')
+
+
+def _reduction(what, reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{what}: reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    return _REDUCTIONS[reduction]
+
+
+def _head_type(what, *ts):
+    types = {t.dtype for t in ts if t is not None}
+    if len(types) != 1 or next(iter(types)) not in _HEAD_DT:
+        raise TypeError(f'{what} needs matching float32, bfloat16 or float16 inputs, got {sorted(map(str, types))}')
+
+
+def _temperature(what, temperature):
+    temperature = float(temperature)
+    if not 0.0 < temperature < float('inf') or not 1e-30 < temperature < 1e30:
+        raise ValueError(f'{what}: temperature must be positive and finite, got {temperature}')
+    return temperature
+
+
+def _check_top(what, lead, values, indices, lse):
+    if values.shape != indices.shape or values.dim() < 1 or tuple(values.shape[:-1]) != tuple(lead):
+        raise ValueError(f'{what}: top_values / top_indices must be {tuple(lead)} + (k,), got {tuple(values.shape)} / '
+                         f'{tuple(indices.shape)}')
+    k = values.shape[-1]
+    if not 1 <= k <= _lib.NIF_TOP_MAX_K:
+        raise ValueError(f'{what}: 1 to {_lib.NIF_TOP_MAX_K} top logits a row, got {k}')
+    if not values.is_floating_point() or indices.is_floating_point() or indices.dtype == torch.bool:
+        raise TypeError(f'{what}: top_values must be floating and top_indices integers, got {values.dtype} / {indices.dtype}')
+    if lse is not None and (tuple(lse.shape) != tuple(lead) or not lse.is_floating_point()):
+        raise ValueError(f'{what}: top_lse must be floating of shape {tuple(lead)}, got {lse.dtype} {tuple(lse.shape)}')
+
+
+def _top_targets(values, indices, lse):
+    """Contiguous (indices int32, values f32, lse f32 or None) of a teacher's top logits, a row each."""
+    k = values.shape[-1]
+    if indices.dtype == torch.int64:
+        indices = indices.clamp(-1, 2 ** 31 - 1)
+    indices = indices.detach().to(torch.int32).reshape(-1, k).contiguous()
+    values = values.detach().float().reshape(-1, k).contiguous()
+    return indices, values, None if lse is None else lse.detach().float().reshape(-1).contiguous()
+
+
+def _head_desc(hidden, weight, bias, labels, indices, values, lse, settings):
+    temperature, ignore_index, reduction = settings
+    d = _lib.HeadDesc()
+    d.hidden, d.ldh, d.weight, d.ldw, d.bias = _ptr(hidden), _ld(hidden), _ptr(weight), _ld(weight), _ptr(bias)
+    d.rows, d.features, d.classes = hidden.shape[0], hidden.shape[1], weight.shape[0]
+    d.dtype, d.reduction = _HEAD_DT[hidden.dtype], reduction
+    d.labels, d.ignore_index = _ptr(labels), ignore_index
+    d.top_indices, d.top_values, d.top_lse = _ptr(indices), _ptr(values), _ptr(lse)
+    d.top, d.temperature = 0 if indices is None else indices.shape[1], temperature
+    return ctypes.byref(d)
+
+
+class _LinearHead(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, labels, indices, values, lse, settings):
+        dev = hidden.device
+        d = _head_desc(hidden, weight, bias, labels, indices, values, lse, settings)
+        with torch.cuda.device(dev):
+            per_row = settings[2] == _lib.NIF_REDUCE_NONE
+            loss = torch.empty((hidden.shape[0],) if per_row else (), dtype=torch.float32, device=dev)
+            state = _bytes(lib.nif_head_state_bytes(d), dev)
+            ws = _bytes(lib.nif_head_forward_workspace_bytes(d), dev)
+            check(lib.nif_head_forward(d, _ptr(loss), _ptr(state), state.numel(), _ptr(ws), ws.numel(), _stream()),
+                  'nif_head_forward')
+        ctx.save_for_backward(hidden, weight, bias, labels, indices, values, lse, state)
+        ctx.settings = settings
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        hidden, weight, bias, labels, indices, values, lse, state = ctx.saved_tensors
+        dev = hidden.device
+        d = _head_desc(hidden, weight, bias, labels, indices, values, lse, ctx.settings)
+        grad_out = grad_out.to(torch.float32).contiguous()
+        with torch.cuda.device(dev):
+            dh, dw, db = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+                          for t, need in zip((hidden, weight, bias), ctx.needs_input_grad))
+            ws = _bytes(lib.nif_head_backward_workspace_bytes(d), dev)
+            check(lib.nif_head_backward(d, _ptr(grad_out), _ptr(state), state.numel(), _ptr(dh), hidden.shape[1], _ptr(dw),
+                                        weight.shape[1], _ptr(db), _ptr(ws), ws.numel(), _stream()), 'nif_head_backward')
+        return dh, dw, db, None, None, None, None, None
+
+
+def _check_head(what, hidden, weight, bias):
+    _head_type(what, hidden, weight, bias)
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f'{what}: hidden must be [..., features] and weight [classes, features], got '
+                         f'{tuple(hidden.shape)} and {tuple(weight.shape)}')
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f'{what}: bias has shape {tuple(bias.shape)} for {weight.shape[0]} classes')
+
+
+def _linear_head(hidden, weight, bias, labels, targets, settings):
+    lead = hidden.shape[:-1]
+    hidden = _mat(hidden.reshape(-1, hidden.shape[-1]), 'hidden')
+    loss = _LinearHead.apply(hidden, _mat(weight, 'weight'), None if bias is None else bias.contiguous(), labels, *targets,
+                             settings)
+    return loss.reshape(lead) if settings[2] == _lib.NIF_REDUCE_NONE else loss
+
+
+def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100, reduction='mean'):
+    """Softmax cross entropy of the logits ``hidden @ weight.T + bias`` against ``target``, the logits not kept.
+
+    hidden: [..., features], weight: [classes, features], bias: [classes] or None -- float32, bfloat16 or float16, all
+    alike; target: integers of hidden's leading shape.  Rows with ``ignore_index`` are left out: they cost nothing, get
+    zero gradients whatever they hold, and 'mean' runs over the others (0 when there are none).  A target that is no class
+    makes its row NaN.  Differentiable once w.r.t. hidden, weight and bias; the loss is f32, f32 inputs compute at f32
+    accuracy and 16-bit ones accumulate in 32 bits.  Memory beyond the gradients: the packed hidden rows and pieces of
+    the classes of about 256 MiB."""
+    what = 'linear_cross_entropy'
+    reduction = _reduction(what, reduction)
+    if target.is_floating_point() or target.dtype == torch.bool or tuple(target.shape) != tuple(hidden.shape[:-1]):
+        raise ValueError(f'{what}: target must be integers of shape {tuple(hidden.shape[:-1])}, got {target.dtype} '
+                         f'{tuple(target.shape)}')
+    _check_head(what, hidden, weight, bias)
+    _same_device(what, hidden, weight, target, bias)
+    labels = target.detach().to(torch.int64).reshape(-1).contiguous()
+    return _linear_head(hidden, weight, bias, labels, (None, None, None), (1.0, int(ignore_index), reduction))
+
+
+def linear_topk_distillation(hidden, weight, top_values, top_indices, bias=None, *, temperature=1.0, top_lse=None,
+                             reduction='mean'):
+    """``topk_distillation`` of the logits ``hidden @ weight.T + bias``, the logits not kept; types, reductions and memory
+    as in ``linear_cross_entropy``, targets as in ``topk_distillation``."""
+    what = 'linear_topk_distillation'
+    reduction, temperature = _reduction(what, reduction), _temperature(what, temperature)
+    _check_head(what, hidden, weight, bias)
+    _check_top(what, hidden.shape[:-1], top_values, top_indices, top_lse)
+    _same_device(what, hidden, weight, top_values, top_indices, bias, top_lse)
+    return _linear_head(hidden, weight, bias, None, _top_targets(top_values, top_indices, top_lse), (temperature, 0, reduction))
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, indices, values, lse, settings):
+        temperature, reduction = settings
+        n, classes = logits.shape
+        k, dev = indices.shape[1], logits.device
+        with torch.cuda.device(dev):
+            per_row = reduction == _lib.NIF_REDUCE_NONE
+            loss = torch.empty((n,) if per_row else (), dtype=torch.float32, device=dev)
+            state = _bytes(lib.nif_distill_state_bytes(n, k), dev)
+            ws = _bytes(lib.nif_distill_workspace_bytes(n), dev)
+            check(lib.nif_distill_forward(_ptr(logits), _ld(logits), n, classes, _HEAD_DT[logits.dtype], _ptr(indices),
+                                          _ptr(values), _ptr(lse), k, temperature, reduction, _ptr(loss), _ptr(state),
+                                          state.numel(), _ptr(ws), ws.numel(), _stream()), 'nif_distill_forward')
+        ctx.save_for_backward(logits, state)
+        ctx.settings = settings + (k,)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        logits, state = ctx.saved_tensors
+        temperature, reduction, k = ctx.settings
+        n, classes = logits.shape
+        grad_out = grad_out.to(torch.float32).contiguous()
+        with torch.cuda.device(logits.device):
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            check(lib.nif_distill_backward(_ptr(logits), _ld(logits), n, classes, _HEAD_DT[logits.dtype], k, temperature,
+                                           reduction, _ptr(grad_out), _ptr(state), state.numel(), _ptr(grad), classes,
+                                           _stream()), 'nif_distill_backward')
+        return grad, None, None, None, None
+
+
+def topk_distillation(logits, top_values, top_indices, *, temperature=1.0, top_lse=None, reduction='mean'):
+    """temperature^2 * KL(teacher || softmax(logits / temperature)), the teacher given by its top logits.
+
+    logits: [..., classes] float32, bfloat16 or float16; top_values / top_indices: [..., k], a teacher's top logits and
+    their classes (``top_logits``).  The teacher's distribution is softmax(top_values / temperature) over the row's
+    entries, or exp(top_values / temperature - top_lse) with ``top_lse`` its log-sum-exp at that temperature over all
+    classes (the divergence is then cut off behind the entries).  Entries of a negative index or of value -inf carry
+    nothing; rows of none are left out (loss and gradient 0 whatever they hold; 'mean' runs over the others, 0 when there
+    are none); equal indices add up; an index that is no class makes its row NaN.  f32 loss; differentiable once w.r.t.
+    logits."""
+    what = 'topk_distillation'
+    _head_type(what, logits)
+    reduction, temperature = _reduction(what, reduction), _temperature(what, temperature)
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f'{what}: logits must be [..., classes], got {tuple(logits.shape)}')
+    lead = logits.shape[:-1]
+    _check_top(what, lead, top_values, top_indices, top_lse)
+    _same_device(what, logits, top_values, top_indices, top_lse)
+    loss = _Distill.apply(_mat(logits.reshape(-1, logits.shape[-1]), 'logits'), *_top_targets(top_values, top_indices, top_lse),
+                          (temperature, reduction))
+    return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE else loss
+
+
+def top_logits(logits, k, *, temperature=1.0):
+    """The k largest logits of each row, what ``topk_distillation`` takes of a teacher: (values [..., k] of logits' type,
+    indices [..., k] int32, lse [...] f32 = logsumexp(logits / temperature) over all classes).  Larger ones first, equal
+    ones by the lower class, NaN before everything.  No gradient."""
+    what = 'top_logits'
+    _head_type(what, logits)
+    temperature, k = _temperature(what, temperature), int(k)
+    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], _lib.NIF_TOP_MAX_K):
+        raise ValueError(f'{what}: 1 to min(classes, {_lib.NIF_TOP_MAX_K}) top logits, got {k} of {tuple(logits.shape)}')
+    _same_device(what, logits)
+    lead = logits.shape[:-1]
+    z = _mat(logits.detach().reshape(-1, logits.shape[-1]), 'logits')
+    n, dev = z.shape[0], z.device
+    with torch.cuda.device(dev):
+        values = torch.empty((n, k), dtype=z.dtype, device=dev)
+        indices = torch.empty((n, k), dtype=torch.int32, device=dev)
+        lse = torch.empty((n,), dtype=torch.float32, device=dev)
+        check(lib.nif_top_logits(_ptr(z), _ld(z), n, z.shape[1], _HEAD_DT[z.dtype], k, temperature, _ptr(values), _ptr(indices),
+                                 _ptr(lse), _stream()), 'nif_top_logits')
+    return values.reshape(*lead, k), indices.reshape(*lead, k), lse.reshape(lead)
+
+
 # ---- exact transport with general marginals and the sparse refit --------------------------------------
 
 class SparsePlan:
