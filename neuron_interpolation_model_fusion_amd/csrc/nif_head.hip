@@ -1,0 +1,1059 @@
+// nif_head.hip -- losses of a linear head over many classes, computed without keeping its logits: softmax cross
+// entropy against labels, and distillation from a teacher's top logits, each with its gradients.
+//
+//   z[n][v] = hidden[n] . weight[v] + bias[v],   u = z / tau,   s[n][v] = exp(u[n][v] - lse[n]),
+//   loss[n] = tau^2 ( sum_k p[n][k] (log p[n][k] - u[n][at(n,k)]) + P[n] lse[n] ),   P[n] = sum_k p[n][k],
+//   dloss[n] / dz[n][v] = tau ( P[n] s[n][v] - sum_{k : at(n,k) = v} p[n][k] ).
+//
+// Cross entropy is the case of one target k with p = 1 and tau = 1, so both share every kernel.  A row without a
+// target (ignored label, padding) is left out: the rows that count are packed to the front (`rows`, `count` on the
+// device), and tiles behind them end at once -- such rows cost nothing and nothing in them reaches a result.
+//
+// Forward: one matrix product whose epilogue reduces each tile of u to (maximum, sum of exponentials) per row; the
+// logits never leave registers.  Backward, in pieces of the classes: the product again, its epilogue writing
+// dz = coef * (P s) in 16 bits; the targets' entries are then rewritten with their -p; dW of the piece = dz^T hidden,
+// and dhidden += dz W.  Recomputing costs 8 n d v operations in place of 6 and saves n * v logits.
+//
+// 16-bit inputs run on v_mfma_f32_16x16x32 with 32-bit accumulation.  f32 inputs are split exactly into three bf16
+// planes (x = h + m + l, 24 bits) and a product runs as the six plane pairs above 2^-24: f32-level accuracy.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/nif.h"
+#include "nif_common.h"
+#include "nif_target.h"
+
+namespace nif {
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+struct Bf16 {
+  typedef __bf16 t;
+  static constexpr int PLANES = 1;
+  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+struct F32 : Bf16 {  // as three bf16 planes
+  static constexpr int PLANES = 3;
+};
+struct F16 {
+  typedef _Float16 t;
+  static constexpr int PLANES = 1;
+  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+
+template <class T>
+__device__ __forceinline__ short to16(float x) {
+  return __builtin_bit_cast(short, (typename T::t)x);  // round to nearest even
+}
+
+// 16-bit outputs: the hardware's exponential (about 2^-21 relative); f32: the library's
+template <class T>
+__device__ __forceinline__ float head_exp(float x) {
+  return T::PLANES == 3 ? expf(x) : __expf(x);
+}
+
+constexpr int HEAD_PAD = 256;  // packed rows are padded to a multiple of the largest tile
+
+// One side of a product.  Plain side: element (r, k) at base[r * ld + k]; transposed side: base[k * ld + r].
+struct Side {
+  const short* base;
+  int64_t plane;  // elements between the planes of a split f32 operand
+  int64_t ld;
+  int rlim;       // rows that exist (plain) / row extent rounded up to 8 (transposed); reads behind are clamped
+  int64_t klim;   // k that exist: plain: multiple of 8, zeros are read behind it; transposed: clamped
+};
+
+enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
+enum { OUT_F32 = 0, OUT_ADD = 1, OUT_FINAL = 2 };
+
+struct GemmArgs {
+  Side A, B;
+  const short* zero;    // 16 bytes of zeros
+  int M, N;             // extents that are computed (N: at most *n_dev when given)
+  const int* n_dev;
+  int64_t K;            // contraction length (at most *k_dev when given)
+  const int* k_dev;
+  int mt, nt, splits;
+  // EPI_STATS / EPI_DZ: the logit's last steps
+  const void* bias;     // of the first class of the piece; f32 or the 16-bit type
+  float inv_tau;
+  float2* stats;        // [m tile * waves in m][stat_ld]
+  int64_t stat_ld;
+  const float* lse;
+  const float* cp;      // coef * P of each packed row
+  short* dz;            // [planes][rows][ldz]
+  int64_t dz_plane, ldz;
+  // EPI_OUT
+  int out_kind;
+  float* acc;           // OUT_F32 / OUT_ADD target, [split][n][acc_ld]; OUT_FINAL: added when not null
+  int64_t acc_ld, acc_split;
+  void* out;
+  int64_t out_ld;
+  const int* rowmap;    // packed row -> row of out
+  const float* inv_scale;
+};
+
+// blockIdx -> tile: blocks b and b + 8 share an XCD (and its L2), so each XCD takes a contiguous range of ids; inside,
+// tiles go in groups of 8 along n for each step along m, so that the blocks in flight on an XCD share their panels.
+__device__ __forceinline__ void tile_of(int id, int total, int mt, int nt, int& tm, int& tn) {
+  const int q = total >> 3, rr = total & 7, xcd = id & 7;
+  const int wg = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + (id >> 3);
+  const int G = 8;
+  const int group = wg / (G * mt), first = group * G;
+  const int width = min(G, nt - first);
+  const int in = wg - group * G * mt;
+  tm = in / width;
+  tn = first + in % width;
+}
+
+// Copies a 64-deep tile of one side into LDS with direct 16-byte loads.  Plain: [BT rows][8 units of 16 bytes], unit
+// u of row r at u ^ (r & 7).  Transposed: [64 k][BT / 8 units], pairs of units xor-ed with (k & 3) | (k >> 3 & 1) << 2:
+// both keep the fragment reads free of bank conflicts.
+template <int BT, int NW, bool TR>
+struct Stager {
+  static constexpr int CW = BT / 8 / NW;  // 1 KiB pieces per wave
+  static constexpr int U = BT / 8;
+  const char* p[CW];
+  int64_t step;
+  int k_of[CW];
+  __device__ __forceinline__ void init(const Side& s, int r0, int wave, int lane) {
+#pragma unroll
+    for (int q = 0; q < CW; ++q) {
+      const int c = wave * CW + q;
+      if (!TR) {
+        const int row = 8 * c + (lane >> 3);
+        const int64_t r = min(r0 + row, s.rlim - 1);
+        k_of[q] = ((lane & 7) ^ (row & 7)) * 8;
+        p[q] = (const char*)(s.base + r * s.ld + k_of[q]);
+      } else {
+        const int k = c * (64 / U) + lane / U, d = lane % U;
+        const int f = ((k & 3) | ((k >> 3 & 1) << 2)) & (U / 2 - 1);
+        const int unit = min(r0 / 8 + (d ^ (f << 1)), s.rlim / 8 - 1);
+        k_of[q] = k;
+        p[q] = (const char*)(s.base + (int64_t)unit * 8);
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(const Side& s, const char* zero, int plane, int64_t k0, char* lds, int wave) const {
+    const int64_t po = (int64_t)plane * s.plane * 2;
+#pragma unroll
+    for (int q = 0; q < CW; ++q) {
+      const char* a;
+      if (!TR) {
+        a = k0 + k_of[q] < s.klim ? p[q] + po + k0 * 2 : zero;
+      } else {
+        const int64_t k = min(k0 + k_of[q], s.klim - 1);
+        a = p[q] + po + k * s.ld * 2;
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)a,
+                                       (__attribute__((address_space(3))) void*)(lds + (wave * CW + q) * 1024), 16, 0, 0);
+    }
+  }
+};
+
+template <int BT, bool TR>
+struct Reader {
+  int base, lane_f;
+  __device__ __forceinline__ void init(int w0, int lane) {
+    if (!TR) {
+      base = (w0 + (lane & 15)) * 128;
+      lane_f = (lane >> 4) ^ (lane & 7);
+    } else {
+      const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
+      lane_f = (q | ((g & 1) << 2)) & (BT / 16 - 1);
+      base = (8 * g + q) * (BT * 2) + pp * 8;
+    }
+  }
+  // fragment i (16 rows from w0 + 16 i) of k step ks (32 deep)
+  __device__ __forceinline__ s16x8 get(const char* lds, int w0, int i, int ks) const {
+    if (!TR) {
+      return *(const s16x8*)(lds + base + i * 2048 + ((lane_f ^ (ks * 4)) << 4));
+    } else {
+      const char* a = lds + base + ks * 32 * BT * 2 + (((w0 / 16 + i) ^ lane_f) << 5);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * BT * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+template <class T, int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
+__global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
+  constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
+  __shared__ __attribute__((aligned(1024))) char lds_a[2][BM * 128];
+  __shared__ __attribute__((aligned(1024))) char lds_b[2][BN * 128];
+  const int split = blockIdx.x / (g.mt * g.nt);
+  int tm, tn;
+  tile_of(blockIdx.x % (g.mt * g.nt), g.mt * g.nt, g.mt, g.nt, tm, tn);
+  const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
+  const int m0 = tm * BM, n0 = tn * BN;
+  // dz is the next products' operand in steps of 64 rows: rows up to there are written as zeros
+  if (n0 >= (EPI == EPI_DZ ? (N + 63) / 64 * 64 : N)) return;
+  const int64_t K = g.k_dev ? min(g.K, (int64_t)*g.k_dev) : g.K;
+  const int ktiles = (int)((K + 63) / 64);
+  const int total = ktiles * (T::PLANES == 3 ? 6 : 1);
+  const int per = (total + g.splits - 1) / g.splits;
+  const int t0 = min(split * per, total), t1 = min(t0 + per, total);
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const char* zero = (const char*)g.zero;
+  Stager<BM, NW, TRA> sa;
+  Stager<BN, NW, TRB> sb;
+  sa.init(g.A, m0, wave, lane);
+  sb.init(g.B, n0, wave, lane);
+  Reader<BM, TRA> ra;
+  Reader<BN, TRB> rb;
+  ra.init(wm * WTM, lane);
+  rb.init(wn * WTN, lane);
+
+  f32x4 acc[FI][FJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // plane pairs, smallest products first: (l, h) (h, l) (m, m) (m, h) (h, m) (h, h)
+  auto issue = [&](int t, int buf) {
+    const int pair = t / ktiles;
+    const int64_t k0 = (int64_t)(t - pair * ktiles) * 64;
+    const int pa = T::PLANES == 3 ? (0x001102 >> (4 * pair)) & 3 : 0;
+    const int pb = T::PLANES == 3 ? (0x010120 >> (4 * pair)) & 3 : 0;
+    sa.issue(g.A, zero, pa, k0, lds_a[buf], wave);
+    sb.issue(g.B, zero, pb, k0, lds_b[buf], wave);
+  };
+  if (t0 < t1) issue(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    __syncthreads();  // the tile has landed for every wave, and every wave is done with the other buffer
+    if (t + 1 < t1) issue(t + 1, buf ^ 1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      s16x8 a[FI], b[FJ];
+#pragma unroll
+      for (int i = 0; i < FI; ++i) a[i] = ra.get(lds_a[buf], wm * WTM, i, ks);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) b[j] = rb.get(lds_b[buf], wn * WTN, j, ks);
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) acc[i][j] = T::mfma(a[i], b[j], acc[i][j]);
+    }
+  }
+
+  // acc[i][j][r]: m = .. + 16 i + 4 (lane / 16) + r, n = .. + 16 j + lane % 16 -- a lane holds four neighbours along m
+  const int mw = m0 + wm * WTM + 4 * (lane >> 4), nw = n0 + wn * WTN + (lane & 15);
+  if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
+    float bias[FI][4];
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = min(mw + 16 * i + r, g.M - 1);
+        bias[i][r] = !g.bias ? 0.f : T::PLANES == 3 ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m];
+      }
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int n = nw + 16 * j;
+      if constexpr (EPI == EPI_STATS) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float u = (acc[i][j][r] + bias[i][r]) * g.inv_tau;
+            u = mw + 16 * i + r < g.M ? u : -INFINITY;
+            acc[i][j][r] = u;
+            top = fmaxf(top, u);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        float sum = 0.f;
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum += head_exp<T>(acc[i][j][r] - ref);  // a NaN stays in the sum
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lane < 16 && n < N) g.stats[(int64_t)(tm * WM + wm) * g.stat_ld + n] = make_float2(top, sum);
+      } else {
+        const bool live = n < N;
+        const float lse = live ? g.lse[n] : 0.f, cp = live ? g.cp[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+          const int m = mw + 16 * i;
+          s16x4 w[T::PLANES];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float u = (acc[i][j][r] + bias[i][r]) * g.inv_tau;
+            // Rounded to the 16-bit type (half a step, 2^-8 bf16 / 2^-11 f16, of each element; f16 after scaling by a
+            // power of two): the size of the rounding that the gradients themselves get.  f32: three exact planes.
+            float x = live && m + r < g.M ? cp * head_exp<T>(u - lse) : 0.f;
+#pragma unroll
+            for (int pl = 0; pl < T::PLANES; ++pl) {
+              const short h = to16<T>(x);
+              w[pl][r] = h;
+              x -= (float)__builtin_bit_cast(typename T::t, h);
+            }
+          }
+          if (m < g.ldz)
+#pragma unroll
+            for (int pl = 0; pl < T::PLANES; ++pl) *(s16x4*)(g.dz + pl * g.dz_plane + (int64_t)n * g.ldz + m) = w[pl];
+        }
+      }
+    }
+  } else {
+    const float inv = g.inv_scale ? *g.inv_scale : 1.f;
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int n = nw + 16 * j;
+      if (n >= N) continue;
+      float* arow = g.acc ? g.acc + split * g.acc_split + (int64_t)n * g.acc_ld : nullptr;
+      const int64_t orow = (int64_t)(g.rowmap ? g.rowmap[n] : n) * g.out_ld;
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+        const int m = mw + 16 * i;
+        f32x4 x = acc[i][j];
+        if (m >= g.M) continue;
+        if (g.out_kind != OUT_FINAL) {  // acc rows are padded to a multiple of 4
+          f32x4* dst = (f32x4*)(arow + m);
+          *dst = g.out_kind == OUT_ADD ? *dst + x : x;
+          continue;
+        }
+        if (arow) x += *(const f32x4*)(arow + m);
+        x *= inv;
+        if constexpr (T::PLANES == 3) {
+          float* o = (float*)g.out + orow + m;
+          if (m + 4 <= g.M && !(((uintptr_t)o) & 15)) {
+            *(f32x4*)o = x;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (m + r < g.M) o[r] = x[r];
+          }
+        } else {
+          s16x4 w;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[r] = to16<T>(x[r]);
+          short* o = (short*)g.out + orow + m;
+          if (m + 4 <= g.M && !(((uintptr_t)o) & 7)) {
+            *(s16x4*)o = w;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (m + r < g.M) o[r] = w[r];
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---- the rows that count ------------------------------------------------------------------------------
+// One workgroup: rows[i] = i-th row with a target, inv[r] = its place or -1, count; also 16 zero bytes.
+__global__ __launch_bounds__(1024) void head_rows_kernel(const float* __restrict__ P, int64_t n, int* __restrict__ rows,
+                                                         int* __restrict__ inv, int* __restrict__ count, int* __restrict__ zero) {
+  __shared__ int sh[17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x < 4) zero[threadIdx.x] = 0;
+  int base = 0;
+  for (int64_t r0 = 0; r0 < n; r0 += 1024) {
+    const int64_t r = r0 + threadIdx.x;
+    const bool live = r < n && P[r] != NO_TARGET;
+    const unsigned long long m = __ballot(live);
+    if (lane == 0) sh[wave] = __popcll(m);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int s = 0;
+      for (int w = 0; w < 16; ++w) {
+        const int c = sh[w];
+        sh[w] = s;
+        s += c;
+      }
+      sh[16] = s;
+    }
+    __syncthreads();
+    const int at = base + sh[wave] + __popcll(m & ((1ull << lane) - 1));
+    if (live) rows[at] = (int)r;
+    if (r < n) inv[r] = live ? at : -1;
+    base += sh[16];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+// x = h + m + l: three bf16 values, exact for 24 bits; infinities and NaN stay in the first one
+__device__ __forceinline__ void split3(float x, short (&w)[3]) {
+#pragma unroll
+  for (int pl = 0; pl < 3; ++pl) {
+    const __bf16 h = (__bf16)x;
+    w[pl] = __builtin_bit_cast(short, h);
+    x -= (float)h;
+  }
+}
+
+// dst[plane][i][0 .. ldd) = src[rows ? rows[i] : i][0 .. d), zeros behind d and in rows behind the last one.
+// One block per row, or per rows of a piece of the weight.
+template <bool F32>
+__global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__ src, int64_t lds, int d, const int* __restrict__ rows,
+                                                        const int* __restrict__ count, int64_t nrows, short* __restrict__ dst,
+                                                        int64_t plane, int ldd) {
+  const int64_t i = blockIdx.x;
+  const bool have = i < (count ? (int64_t)*count : nrows);
+  const int64_t r = have ? (rows ? rows[i] : i) : 0;
+  for (int c = threadIdx.x * 8; c < ldd; c += 256 * 8) {
+    s16x8 w[3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[0][e] = w[1][e] = w[2][e] = 0;
+    if (have && c < d) {
+      if (F32) {
+        const float* p = (const float*)src + r * lds + c;
+        float x[8];
+        if (c + 8 <= d && !((uintptr_t)p & 15)) {
+          *(f32x4*)x = ((const f32x4*)p)[0];
+          *(f32x4*)(x + 4) = ((const f32x4*)p)[1];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = c + e < d ? p[e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          short t[3];
+          split3(x[e], t);
+          w[0][e] = t[0], w[1][e] = t[1], w[2][e] = t[2];
+        }
+      } else {
+        const short* p = (const short*)src + r * lds + c;
+        if (c + 8 <= d && !((uintptr_t)p & 15)) {
+          w[0] = *(const s16x8*)p;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[0][e] = c + e < d ? p[e] : (short)0;
+        }
+      }
+    }
+#pragma unroll
+    for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) *(s16x8*)(dst + pl * plane + i * ldd + c) = w[pl];
+  }
+}
+
+// ---- the loss of each row -------------------------------------------------------------------------------
+// One block per 16 packed rows: joins the tiles' (maximum, sum) pairs into lse, takes the targets' logits as dot
+// products of the inputs (32-bit accumulation), and writes the row's loss to its own place.
+template <int DT>
+__global__ __launch_bounds__(256) void head_finish_kernel(const void* __restrict__ hidden, int64_t ldh, const void* __restrict__ weight,
+                                                          int64_t ldw, const void* __restrict__ bias, int d,
+                                                          const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
+                                                          const int* __restrict__ rows, const int* __restrict__ count,
+                                                          float* __restrict__ lse, float* __restrict__ uk, float* __restrict__ loss) {
+  __shared__ float sh_top[16][17], sh_sum[16][17], sh_lse[16];
+  const int i0 = blockIdx.x * 16, n = *count;
+  if (i0 >= n) return;
+  const int r = threadIdx.x & 15, part = threadIdx.x >> 4;
+  float top = -INFINITY, sum = 0.f;
+  if (i0 + r < n)
+    for (int t = part; t < tiles; t += 16) {
+      const float2 x = stats[(int64_t)t * stat_ld + i0 + r];
+      join(top, sum, x.x, x.y);
+    }
+  sh_top[r][part] = top;
+  sh_sum[r][part] = sum;
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    top = sh_top[threadIdx.x][0], sum = sh_sum[threadIdx.x][0];
+    for (int p = 1; p < 16; ++p) join(top, sum, sh_top[threadIdx.x][p], sh_sum[threadIdx.x][p]);
+    const float l = top + logf(sum);
+    sh_lse[threadIdx.x] = l;
+    if (i0 + (int)threadIdx.x < n) lse[i0 + threadIdx.x] = l;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rn = min(16, n - i0);
+  for (int q = wave; q < rn * tg.k; q += 4) {
+    const int i = i0 + q / tg.k, k = q % tg.k;
+    const int64_t src = rows[i];
+    const int at = tg.at[src * tg.k + k];
+    float u = 0.f;
+    if (at >= 0) {
+      u = wave_dot<DT>(hidden, src * ldh, weight, (int64_t)at * ldw, d, lane);
+      if (bias) u += Elem<DT>::load(bias, at);
+      u *= tg.inv_tau;
+    }
+    if (lane == 0) uk[(int64_t)i * tg.k + k] = u;
+  }
+  __syncthreads();
+  for (int q = wave; q < rn; q += 4) {
+    const int i = i0 + q;
+    const int64_t src = rows[i];
+    double s = 0.0;
+    for (int k = lane; k < tg.k; k += 64) s += target_term(tg, src, k, uk[(int64_t)i * tg.k + k], sh_lse[q]);
+    s = wave_sum_f64(s);
+    if (lane == 0) loss[src] = (float)(s * tg.tau2);
+  }
+}
+
+// sum or mean over the rows that count, in a fixed order and 64 bits; rows without a target hold 0
+__global__ __launch_bounds__(1024) void head_reduce_kernel(const float* __restrict__ row_loss, int64_t n, const int* __restrict__ count,
+                                                           int mean, float* __restrict__ loss) {
+  __shared__ double sh[16];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)row_loss[i];
+  s = wave_sum_f64(s);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < 16; ++w) s += sh[w];
+    loss[0] = (float)(mean ? s / max(1, *count) : s);
+  }
+}
+
+// rows without a target: loss 0 (before the finish kernel), gradient 0
+__global__ __launch_bounds__(256) void head_clear_loss_kernel(const int* __restrict__ inv, int64_t n, float* __restrict__ loss) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n && inv[i] < 0) loss[i] = 0.f;
+}
+
+template <typename W>
+__global__ __launch_bounds__(256) void head_clear_rows_kernel(const int* __restrict__ inv, W* __restrict__ out, int64_t ld, int d) {
+  const int64_t r = blockIdx.x;
+  if (inv[r] >= 0) return;
+  for (int c = threadIdx.x; c < d; c += 256) out[r * ld + c] = 0;
+}
+
+// coef[i] = (gradient that arrives at row i) * tau * scale and cp[i] = coef[i] * P[i].  scale: f16 holds nothing below
+// 2^-24, so dz is scaled by the power of two that takes the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger);
+// the gradients' epilogues divide by it again.  bf16 and f32 need none.
+__global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict__ grad, int per_row, int mean, Targets tg,
+                                                         const int* __restrict__ rows, const int* __restrict__ count, int f16,
+                                                         float* __restrict__ coef, float* __restrict__ cp, float* __restrict__ inv_scale) {
+  __shared__ float sh[16];
+  const int n = *count;
+  const float w = tg.tau * (mean ? 1.f / max(1, n) : 1.f);
+  float scale = 1.f;
+  if (f16) {
+    float top = 0.f;
+    for (int i = threadIdx.x; i < n; i += 1024) {
+      const float c = fabsf(grad[per_row ? rows[i] : 0] * w) * fmaxf(1.f, tg.P[rows[i]]);
+      top = c < INFINITY ? fmaxf(top, c) : top;
+    }
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (int v = 0; v < 16; ++v) top = fmaxf(top, sh[v]);
+    if (top > 0.f && top < INFINITY) {
+      int e;
+      frexpf(top, &e);  // top in [2^(e-1), 2^e)
+      scale = ldexpf(1.f, max(-100, min(100, 14 - e)));
+    }
+  }
+  if (threadIdx.x == 0) *inv_scale = 1.f / scale;
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float c = (per_row ? grad[rows[i]] : grad[0]) * w * scale;
+    coef[i] = c;
+    cp[i] = c * tg.P[rows[i]];
+  }
+}
+
+// The targets' entries of a piece of dz: coef (P s - sum of the row's p with that class).  The first of equal classes
+// writes, with the sum over all of them in order.  One wave per packed row.
+template <class T>
+__global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
+                                                           const float* __restrict__ uk, const float* __restrict__ lse,
+                                                           const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
+                                                           short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int planes) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= *count) return;
+  const int64_t src = rows[i];
+  const int* at = tg.at + src * tg.k;
+  const float* p = tg.p + src * tg.k;
+  for (int k = lane; k < tg.k; k += 64) {
+    const int v = at[k];
+    if (v < v0 || v >= v1) continue;
+    float sum = 0.f;
+    bool first = true;
+    if (tg.k > 1)
+      for (int q = 0; q < tg.k; ++q)
+        if (at[q] == v) {
+          if (q < k) first = false;
+          sum += p[q];
+        }
+    if (tg.k == 1) sum = p[0];
+    if (!first) continue;
+    float x = cp[i] * expf(uk[(int64_t)i * tg.k + k] - lse[i]) - coef[i] * sum;
+    for (int pl = 0; pl < planes; ++pl) {
+      const short w = to16<T>(x);
+      dz[pl * dz_plane + (int64_t)i * ldz + (v - v0)] = w;
+      x -= (float)__builtin_bit_cast(typename T::t, w);
+    }
+  }
+}
+
+// dbias of a piece: column sums of dz over the packed rows; 64 columns a block, 4 waves over the rows
+template <class T>
+__global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int planes,
+                                                        const int* __restrict__ count, int cols, const float* __restrict__ inv_scale,
+                                                        void* __restrict__ out, int out_f32) {
+  __shared__ float sh[4][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+  const int n = *count;
+  float s = 0.f;
+  if (c < cols)
+    for (int i = part; i < n; i += 4)
+      for (int pl = 0; pl < planes; ++pl)
+        s += (float)__builtin_bit_cast(typename T::t, dz[pl * dz_plane + (int64_t)i * ldz + c]);
+  sh[part][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (part == 0 && c < cols) {
+    s = ((sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x])) * *inv_scale;
+    if (out_f32)
+      ((float*)out)[c] = s;
+    else
+      ((short*)out)[c] = to16<T>(s);
+  }
+}
+
+// out = (sum of the splits' partial sums, in order, + acc) * inv_scale, or acc = that sum
+template <class T>
+__global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict__ part, int splits, int64_t part_split, int64_t part_ld,
+                                                        int n, const int* __restrict__ n_dev, int m, float* __restrict__ acc, int first,
+                                                        int last, void* __restrict__ out, int64_t out_ld, int out_f32,
+                                                        const int* __restrict__ rowmap, const float* __restrict__ inv_scale) {
+  const int64_t i = blockIdx.x;
+  if (i >= (n_dev ? min(n, *n_dev) : n)) return;
+  const float inv = *inv_scale;
+  const int64_t o = (int64_t)(rowmap ? rowmap[i] : i) * out_ld;
+  for (int c = threadIdx.x; c < m; c += 256) {
+    float s = first ? 0.f : acc[i * part_ld + c];
+    for (int q = 0; q < splits; ++q) s += part[q * part_split + i * part_ld + c];
+    if (!last)
+      acc[i * part_ld + c] = s;
+    else if (out_f32)
+      ((float*)out)[o + c] = s * inv;
+    else
+      ((short*)out)[o + c] = to16<T>(s * inv);
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------
+
+static inline int64_t round_up(int64_t x, int64_t q) { return (x + q - 1) / q * q; }
+
+struct Plan {
+  int64_t n, cap;
+  int d, ldd, v, planes, k;
+  bool pack_w;       // the weight is copied by pieces: f32, or rows that 16-byte loads cannot take
+  int piece;         // classes per piece (multiple of 256, or all)
+  // state: what the backward pass reads
+  size_t s_p, s_at, s_P, s_rows, s_inv, s_count, s_zero, s_lse, s_uk, s_h, state;
+};
+
+static constexpr size_t PIECE_BYTES = (size_t)256 << 20;
+
+static size_t take(size_t& at, size_t bytes) {
+  const size_t r = at;
+  at += (bytes + 255) / 256 * 256;
+  return r;
+}
+
+static bool make_plan(const nif_head_desc* h, Plan& p) {
+  if (!h || h->rows < 0 || h->features <= 0 || h->classes <= 0 || h->top < 0) return false;
+  if (h->dtype != NIF_F32 && h->dtype != NIF_BF16 && h->dtype != NIF_F16) return false;
+  if (h->rows > (1 << 30) || h->features > (1 << 20) || h->classes > (1 << 28) || h->top > NIF_TOP_MAX_K) return false;
+  p.n = h->rows;
+  p.cap = round_up(p.n > 0 ? p.n : 1, HEAD_PAD);
+  p.d = h->features;
+  p.ldd = (int)round_up(p.d, 64);
+  p.v = h->classes;
+  p.k = h->top > 0 ? h->top : 1;
+  p.planes = h->dtype == NIF_F32 ? 3 : 1;
+  p.pack_w = h->dtype == NIF_F32 || p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0;
+  const int64_t per = (p.pack_w && p.ldd > p.cap ? (int64_t)p.ldd : p.cap) * 2 * p.planes;  // bytes of one class of a piece
+  int64_t c = (int64_t)(PIECE_BYTES / per) / 256 * 256;
+  if (c < 1024) c = 1024;
+  if (c > p.v) c = p.v;
+  p.piece = (int)c;
+  size_t at = 0;
+  p.s_p = take(at, (size_t)p.n * p.k * 4);
+  p.s_at = take(at, (size_t)p.n * p.k * 4);
+  p.s_P = take(at, (size_t)p.n * 4);
+  p.s_rows = take(at, (size_t)p.cap * 4);
+  p.s_inv = take(at, (size_t)p.cap * 4);
+  p.s_count = take(at, 4);
+  p.s_zero = take(at, 16);
+  p.s_lse = take(at, (size_t)p.cap * 4);
+  p.s_uk = take(at, (size_t)p.cap * p.k * 4);
+  p.s_h = take(at, (size_t)p.cap * p.ldd * 2 * p.planes);
+  p.state = at;
+  return true;
+}
+
+static Targets targets_of(const nif_head_desc* h, const Plan& p, char* state) {
+  Targets t;
+  t.p = (float*)(state + p.s_p);
+  t.at = (int*)(state + p.s_at);
+  t.P = (float*)(state + p.s_P);
+  t.k = p.k;
+  t.tau = h->labels ? 1.f : h->temperature;
+  t.inv_tau = 1.f / t.tau;
+  t.tau2 = (double)t.tau * t.tau;
+  return t;
+}
+
+struct Shape {
+  int bm, bn, wm;
+};
+// tile of a product with extents m x n
+static Shape shape_of(int64_t m, int64_t n) {
+  (void)m;
+  if (n <= 32) return {128, 32, 4};
+  return {128, 128, 2};
+}
+
+template <class T, bool TRA, bool TRB, int EPI>
+static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
+  g.mt = (g.M + s.bm - 1) / s.bm;
+  g.nt = (g.N + s.bn - 1) / s.bn;
+  const dim3 grid((unsigned)((int64_t)g.mt * g.nt * g.splits));
+  if (grid.x == 0) return;
+  if (s.bn == 32)
+    hipLaunchKernelGGL((head_gemm_kernel<T, 128, 32, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+  else
+    hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+}
+
+static int splits_for(const Shape& s, int64_t m, int64_t n, int64_t ktiles) {
+  const int64_t tiles = ((m + s.bm - 1) / s.bm) * ((n + s.bn - 1) / s.bn);
+  int64_t q = 512 / (tiles > 0 ? tiles : 1);  // no rows: no tiles
+  if (q > ktiles / 4) q = ktiles / 4;
+  if (q > 32) q = 32;
+  return (int)(q < 1 ? 1 : q);
+}
+
+struct FwdSpace {
+  size_t stats, w, bytes;
+};
+static FwdSpace forward_space(const Plan& p) {
+  FwdSpace f;
+  size_t at = 0;
+  const Shape s = shape_of(p.v, p.n);
+  const int64_t tiles = (p.v / s.bm + p.v / p.piece + 2) * s.wm;
+  f.stats = take(at, (size_t)tiles * p.cap * 8);
+  f.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * 2 * p.planes : 0);
+  f.bytes = at;
+  return f;
+}
+
+// the weight rows of a piece as a side with classes along its rows
+static Side weight_side(const nif_head_desc* h, const Plan& p, int v0, int vc, short* packed, hipStream_t st) {
+  Side s;
+  if (p.pack_w) {
+    const size_t e = h->dtype == NIF_F32 ? 4 : 2;
+    const char* src = (const char*)h->weight + (size_t)v0 * h->ldw * e;
+    const int64_t plane = (int64_t)vc * p.ldd;
+    if (h->dtype == NIF_F32)
+      hipLaunchKernelGGL(head_pack_kernel<true>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, nullptr, nullptr, (int64_t)vc, packed,
+                         plane, p.ldd);
+    else
+      hipLaunchKernelGGL(head_pack_kernel<false>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, nullptr, nullptr, (int64_t)vc, packed,
+                         plane, p.ldd);
+    s = Side{packed, plane, p.ldd, vc, p.ldd};
+  } else {
+    s = Side{(const short*)h->weight + (int64_t)v0 * h->ldw, 0, h->ldw, vc, p.d};
+  }
+  return s;
+}
+
+static const void* bias_at(const nif_head_desc* h, int v0) {
+  return h->bias ? (const char*)h->bias + (size_t)v0 * (h->dtype == NIF_F32 ? 4 : 2) : nullptr;
+}
+
+template <class T>
+static void forward_products(const nif_head_desc* h, const Plan& p, char* state, char* ws, const FwdSpace& f, int& tiles, hipStream_t st) {
+  const Shape s = shape_of(p.v, p.n);
+  tiles = 0;
+  for (int v0 = 0; v0 < p.v; v0 += p.pack_w ? p.piece : p.v) {
+    const int vc = p.pack_w ? (p.v - v0 < p.piece ? p.v - v0 : p.piece) : p.v;
+    GemmArgs g = {};
+    g.A = weight_side(h, p, v0, vc, (short*)(ws + f.w), st);
+    g.B = Side{(const short*)(state + p.s_h), p.cap * p.ldd, p.ldd, (int)p.cap, p.ldd};
+    g.zero = (const short*)(state + p.s_zero);
+    g.M = vc;
+    g.N = (int)p.n;
+    g.n_dev = (const int*)(state + p.s_count);
+    g.K = p.ldd;
+    g.splits = 1;
+    g.bias = bias_at(h, v0);
+    g.inv_tau = h->labels ? 1.f : 1.f / h->temperature;
+    g.stats = (float2*)(ws + f.stats) + (int64_t)tiles * p.cap;
+    g.stat_ld = p.cap;
+    run_gemm<T, false, false, EPI_STATS>(s, g, st);
+    tiles += g.mt * s.wm;
+  }
+}
+
+template <int DT>
+static void finish(const nif_head_desc* h, const Plan& p, char* state, const float2* stats, int tiles, float* row_loss, hipStream_t st) {
+  hipLaunchKernelGGL(head_finish_kernel<DT>, dim3((unsigned)((p.n + 15) / 16)), dim3(256), 0, st, h->hidden, h->ldh, h->weight, h->ldw,
+                     h->bias, p.d, stats, p.cap, tiles, targets_of(h, p, state), (const int*)(state + p.s_rows),
+                     (const int*)(state + p.s_count), (float*)(state + p.s_lse), (float*)(state + p.s_uk), row_loss);
+}
+
+struct BwdSpace {
+  size_t coef, cp, scale, dz, w, acc, part, bytes;
+  int64_t ldz, dh_ld;
+  int dh_splits, dw_splits;
+  Shape dh, dw;
+};
+static BwdSpace backward_space(const Plan& p) {
+  BwdSpace b;
+  b.ldz = round_up(p.piece, 64);
+  b.dh_ld = round_up(p.d, 4);
+  b.dh = shape_of(p.d, p.n);
+  b.dw = shape_of(p.d, p.piece);
+  const int pairs = p.planes == 3 ? 6 : 1;
+  b.dh_splits = splits_for(b.dh, p.d, p.n, b.ldz / 64 * pairs);
+  b.dw_splits = splits_for(b.dw, p.d, p.piece, (p.cap / 64) * pairs);
+  size_t at = 0;
+  b.coef = take(at, (size_t)p.cap * 4);
+  b.cp = take(at, (size_t)p.cap * 4);
+  b.scale = take(at, 4);
+  b.dz = take(at, (size_t)p.cap * b.ldz * 2 * p.planes);
+  b.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * 2 * p.planes : 0);
+  b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
+  const size_t part_h = b.dh_splits > 1 ? (size_t)b.dh_splits * p.cap * b.dh_ld * 4 : 0;
+  const size_t part_w = b.dw_splits > 1 ? (size_t)b.dw_splits * p.piece * b.dh_ld * 4 : 0;
+  b.part = take(at, part_h > part_w ? part_h : part_w);
+  b.bytes = at;
+  return b;
+}
+
+template <class T>
+static void backward_products(const nif_head_desc* h, const Plan& p, const char* state, char* ws, const BwdSpace& b, void* dhidden,
+                              int64_t lddh, void* dweight, int64_t lddw, void* dbias, hipStream_t st) {
+  const int* count = (const int*)(state + p.s_count);
+  const int* rows = (const int*)(state + p.s_rows);
+  const short* hp = (const short*)(state + p.s_h);
+  const Targets tg = targets_of(h, p, (char*)state);
+  const float* lse = (const float*)(state + p.s_lse);
+  const float* uk = (const float*)(state + p.s_uk);
+  const float* coef = (const float*)(ws + b.coef);
+  const float* cp = (const float*)(ws + b.cp);
+  const float* inv_scale = (const float*)(ws + b.scale);
+  short* dz = (short*)(ws + b.dz);
+  float* acc = (float*)(ws + b.acc);
+  float* part = (float*)(ws + b.part);
+  const int f32 = h->dtype == NIF_F32;
+  const int64_t dz_plane = p.cap * b.ldz;
+  for (int v0 = 0; v0 < p.v; v0 += p.piece) {
+    const int vc = p.v - v0 < p.piece ? p.v - v0 : p.piece;
+    const bool first = v0 == 0, last = v0 + vc == p.v;
+    const Side w = weight_side(h, p, v0, vc, (short*)(ws + b.w), st);
+    const int64_t kz = round_up(vc, 64);  // columns of dz that are written
+    {
+      GemmArgs g = {};
+      g.A = w;
+      g.B = Side{hp, p.cap * p.ldd, p.ldd, (int)p.cap, p.ldd};
+      g.zero = (const short*)(state + p.s_zero);
+      g.M = vc;
+      g.N = (int)round_up(p.n, 64);
+      g.n_dev = count;
+      g.K = p.ldd;
+      g.splits = 1;
+      g.bias = bias_at(h, v0);
+      g.inv_tau = tg.inv_tau;
+      g.lse = lse;
+      g.cp = cp;
+      g.dz = dz;
+      g.dz_plane = dz_plane;
+      g.ldz = b.ldz;
+      run_gemm<T, false, false, EPI_DZ>(shape_of(vc, p.n), g, st);
+    }
+    if (p.n > 0)
+      hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
+                       v0 + vc, dz, dz_plane, b.ldz, p.planes);
+    if (dbias)
+      hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 63) / 64), dim3(256), 0, st, dz, dz_plane, b.ldz, p.planes, count, vc, inv_scale,
+                         (char*)dbias + (size_t)v0 * (f32 ? 4 : 2), f32);
+    if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
+      GemmArgs g = {};
+      g.A = Side{hp, p.cap * p.ldd, p.ldd, p.ldd, p.cap};
+      g.B = Side{dz, dz_plane, b.ldz, (int)kz, p.cap};
+      g.zero = (const short*)(state + p.s_zero);
+      g.M = p.d;
+      g.N = vc;
+      g.K = p.cap;
+      g.k_dev = count;
+      g.splits = b.dw_splits;
+      g.out = (char*)dweight + (size_t)v0 * lddw * (f32 ? 4 : 2);
+      g.out_ld = lddw;
+      g.inv_scale = inv_scale;
+      g.out_kind = OUT_FINAL;
+      if (g.splits > 1) {
+        g.out_kind = OUT_F32;
+        g.acc = part;
+        g.acc_ld = b.dh_ld;
+        g.acc_split = (int64_t)p.piece * b.dh_ld;
+      }
+      run_gemm<T, true, true, EPI_OUT>(b.dw, g, st);
+      if (g.splits > 1)
+        hipLaunchKernelGGL(head_join_kernel<T>, dim3(vc), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, vc, nullptr, p.d,
+                           nullptr, 1, 1, g.out, lddw, f32, nullptr, inv_scale);
+    }
+    if (dhidden) {  // [packed rows][features] += dz W, contraction over the classes of the piece
+      GemmArgs g = {};
+      g.A = w;
+      g.A.klim = w.rlim;
+      g.A.rlim = p.pack_w ? p.ldd : p.d;
+      g.B = Side{dz, dz_plane, b.ldz, (int)p.cap, kz};
+      g.zero = (const short*)(state + p.s_zero);
+      g.M = p.d;
+      g.N = (int)p.n;
+      g.n_dev = count;
+      g.K = kz;
+      g.splits = b.dh_splits;
+      g.out = dhidden;
+      g.out_ld = lddh;
+      g.rowmap = rows;
+      g.inv_scale = inv_scale;
+      if (g.splits > 1) {
+        g.out_kind = OUT_F32;
+        g.acc = part;
+        g.acc_split = p.cap * b.dh_ld;
+      } else {
+        g.out_kind = last ? OUT_FINAL : first ? OUT_F32 : OUT_ADD;
+        g.acc = first && last ? nullptr : acc;
+      }
+      g.acc_ld = b.dh_ld;
+      run_gemm<T, true, false, EPI_OUT>(b.dh, g, st);
+      if (g.splits > 1 && p.n > 0)
+        hipLaunchKernelGGL(head_join_kernel<T>, dim3((unsigned)p.n), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, (int)p.n, count,
+                           p.d, acc, first, last, dhidden, lddh, f32, rows, inv_scale);
+    }
+  }
+}
+
+static int check_desc(const nif_head_desc* h, Plan& p) {
+  if (!make_plan(h, p)) return NIF_ERR_INVALID_ARG;
+  if (!h->weight || (h->rows > 0 && !h->hidden) || h->ldh < h->features || h->ldw < h->features) return NIF_ERR_INVALID_ARG;
+  if (h->reduction < NIF_REDUCE_NONE || h->reduction > NIF_REDUCE_SUM) return NIF_ERR_INVALID_ARG;
+  if (h->rows > 0) {
+    if (!h->labels == !h->top_indices) return NIF_ERR_INVALID_ARG;  // one of the two
+    if (h->labels && h->top != 0) return NIF_ERR_INVALID_ARG;
+    if (!h->labels && (h->top < 1 || !h->top_values || !(h->temperature > 0.f) || !(h->temperature < INFINITY))) return NIF_ERR_INVALID_ARG;
+  }
+  return NIF_OK;
+}
+
+}  // namespace nif
+
+extern "C" size_t nif_head_state_bytes(const nif_head_desc* h) {
+  nif::Plan p;
+  return nif::make_plan(h, p) ? p.state : 0;
+}
+
+extern "C" size_t nif_head_forward_workspace_bytes(const nif_head_desc* h) {
+  nif::Plan p;
+  return nif::make_plan(h, p) ? nif::forward_space(p).bytes + (size_t)p.cap * 4 : 0;
+}
+
+extern "C" size_t nif_head_backward_workspace_bytes(const nif_head_desc* h) {
+  nif::Plan p;
+  return nif::make_plan(h, p) ? nif::backward_space(p).bytes : 0;
+}
+
+extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state, size_t state_bytes, void* ws, size_t ws_bytes,
+                                void* stream) {
+  nif::Range nif_range_("nif_head_forward");
+  using namespace nif;
+  Plan p;
+  const int rc = check_desc(h, p);
+  if (rc != NIF_OK) return rc;
+  if (!loss && (h->rows > 0 || h->reduction != NIF_REDUCE_NONE)) return NIF_ERR_INVALID_ARG;
+  if (!state || state_bytes < nif_head_state_bytes(h) || !ws || ws_bytes < nif_head_forward_workspace_bytes(h)) return NIF_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  char* s = (char*)state;
+  const FwdSpace f = forward_space(p);
+  clear_err();
+  int* rows = (int*)(s + p.s_rows);
+  int* inv = (int*)(s + p.s_inv);
+  int* count = (int*)(s + p.s_count);
+  float* row_loss = h->reduction == NIF_REDUCE_NONE ? loss : (float*)((char*)ws + f.bytes);
+  if (p.n > 0) {
+    const Targets tg = targets_of(h, p, s);
+    launch_targets(h->labels, h->ignore_index, h->top_indices, h->top_values, h->top_lse, p.n, p.k, p.v, tg, st);
+    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, tg.P, p.n, rows, inv, count, (int*)(s + p.s_zero));
+    hipLaunchKernelGGL(head_clear_loss_kernel, dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, st, inv, p.n, row_loss);
+    if (h->dtype == NIF_F32)
+      hipLaunchKernelGGL(head_pack_kernel<true>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d, rows, count, p.n,
+                         (short*)(s + p.s_h), p.cap * p.ldd, p.ldd);
+    else
+      hipLaunchKernelGGL(head_pack_kernel<false>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d, rows, count, p.n,
+                         (short*)(s + p.s_h), p.cap * p.ldd, p.ldd);
+    int tiles = 0;
+    if (h->dtype == NIF_F32)
+      forward_products<F32>(h, p, s, (char*)ws, f, tiles, st);
+    else if (h->dtype == NIF_BF16)
+      forward_products<Bf16>(h, p, s, (char*)ws, f, tiles, st);
+    else
+      forward_products<F16>(h, p, s, (char*)ws, f, tiles, st);
+    const float2* stats = (const float2*)((char*)ws + f.stats);
+    if (h->dtype == NIF_F32)
+      finish<NIF_F32>(h, p, s, stats, tiles, row_loss, st);
+    else if (h->dtype == NIF_BF16)
+      finish<NIF_BF16>(h, p, s, stats, tiles, row_loss, st);
+    else
+      finish<NIF_F16>(h, p, s, stats, tiles, row_loss, st);
+  } else {
+    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, rows, inv, count, (int*)(s + p.s_zero));
+  }
+  if (h->reduction != NIF_REDUCE_NONE)
+    hipLaunchKernelGGL(head_reduce_kernel, dim3(1), dim3(1024), 0, st, row_loss, p.n, count, h->reduction == NIF_REDUCE_MEAN, loss);
+  return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
+}
+
+extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss, const void* state, size_t state_bytes, void* dhidden,
+                                 int64_t lddh, void* dweight, int64_t lddw, void* dbias, void* ws, size_t ws_bytes, void* stream) {
+  nif::Range nif_range_("nif_head_backward");
+  using namespace nif;
+  Plan p;
+  const int rc = check_desc(h, p);
+  if (rc != NIF_OK) return rc;
+  if ((p.n > 0 && !grad_loss) || (dhidden && lddh < h->features) || (dweight && lddw < h->features)) return NIF_ERR_INVALID_ARG;
+  if (!state || state_bytes < nif_head_state_bytes(h) || !ws || ws_bytes < nif_head_backward_workspace_bytes(h)) return NIF_ERR_WORKSPACE;
+  if (!dhidden && !dweight && !dbias) return NIF_OK;
+  hipStream_t st = (hipStream_t)stream;
+  const char* s = (const char*)state;
+  const BwdSpace b = backward_space(p);
+  clear_err();
+  hipLaunchKernelGGL(head_coef_kernel, dim3(1), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
+                     h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_count),
+                     h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp), (float*)((char*)ws + b.scale));
+  if (dhidden && p.n > 0) {
+    if (h->dtype == NIF_F32)
+      hipLaunchKernelGGL(head_clear_rows_kernel<float>, dim3((unsigned)p.n), dim3(256), 0, st, (const int*)(s + p.s_inv), (float*)dhidden,
+                         lddh, p.d);
+    else
+      hipLaunchKernelGGL(head_clear_rows_kernel<short>, dim3((unsigned)p.n), dim3(256), 0, st, (const int*)(s + p.s_inv), (short*)dhidden,
+                         lddh, p.d);
+  }
+  if (h->dtype == NIF_F32)
+    backward_products<F32>(h, p, s, (char*)ws, b, dhidden, lddh, dweight, lddw, dbias, st);
+  else if (h->dtype == NIF_BF16)
+    backward_products<Bf16>(h, p, s, (char*)ws, b, dhidden, lddh, dweight, lddw, dbias, st);
+  else
+    backward_products<F16>(h, p, s, (char*)ws, b, dhidden, lddh, dweight, lddw, dbias, st);
+  return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
+}
