@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void label_targets_kernel(const int64_t* __res
 
 // p_k = exp(t_k / tau - L), L = lse of the teacher's row where given, else over the row's entries.  Entries of a
 // negative class or of value -inf carry nothing; a class that does not exist makes the row NaN.  One wave per row.
-__device__ __forceinline__ void top_targets(const int32_t* __restrict__ indices, const float* __restrict__ values,
+__device__ __forceinline__ float top_targets(const int32_t* __restrict__ indices, const float* __restrict__ values,
                                             const float* __restrict__ lse, int64_t row, int classes, const Targets& t, int lane) {
   const int32_t* at = indices + row * t.k;
   const float* val = values + row * t.k;
@@ -62,7 +62,9 @@ __device__ __forceinline__ void top_targets(const int32_t* __restrict__ indices,
     P += p;
   }
   P = wave_sum_f32(P);
-  if (lane == 0) t.P[row] = live ? P : NO_TARGET;
+  P = live ? P : NO_TARGET;
+  if (lane == 0) t.P[row] = P;
+  return P;
 }
 
 __global__ __launch_bounds__(256) void top_targets_kernel(const int32_t* __restrict__ indices, const float* __restrict__ values,
@@ -82,45 +84,145 @@ void launch_targets(const int64_t* labels, int64_t ignore, const int32_t* indice
 
 // ---- distillation of given logits ---------------------------------------------------------------------------
 
-// One block per row: (max, sum of exponentials) in one pass, the targets' terms, the row's loss.
+// A row as 16-byte vectors: [0, head) and [tail, n) are the elements before the first and behind the last whole one.
 template <int DT>
-__global__ __launch_bounds__(256) void distill_rows_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
-                                                           float* __restrict__ lse_out, float* __restrict__ loss) {
-  __shared__ float sh_top[4], sh_sum[4];
-  __shared__ double sh_loss[4];
+struct RowView {
+  const typename Elem<DT>::t* z;
+  int n, head, vecs;
+  __device__ __forceinline__ RowView(const void* base, int64_t at, int classes) {
+    constexpr int V = Elem<DT>::PER16;
+    z = (const typename Elem<DT>::t*)base + at;
+    n = classes;
+    head = min(n, (int)((16 - ((uintptr_t)z & 15)) & 15) / (16 / V));
+    vecs = (n - head) / V;
+  }
+  __device__ __forceinline__ int tail() const { return head + vecs * Elem<DT>::PER16; }
+  __device__ __forceinline__ vec4f vec(int i) const { return ((const vec4f*)(z + head))[i]; }
+  // loose element j = 0 .. loose() - 1: the head's, then the tail's
+  __device__ __forceinline__ int loose() const { return head + (n - tail()); }
+  __device__ __forceinline__ int loose_at(int j) const { return j < head ? j : tail() + (j - head); }
+};
+
+// 2^x. 16-bit inputs: the hardware's (2^-22 relative); f32: the library's exponential of the natural argument.
+template <int DT>
+__device__ __forceinline__ float exp_of(float x, float scale, float shift) {
+  return DT == NIF_F32 ? expf(fmaf(x, scale, -shift)) : __builtin_amdgcn_exp2f(fmaf(x, scale, -shift));
+}
+// what logits are multiplied with before exp_of: 1 / tau, and log2(e) where the hardware's exponential is used
+template <int DT>
+__device__ __forceinline__ float exp_scale(float inv_tau) {
+  return DT == NIF_F32 ? inv_tau : inv_tau * 1.4426950408889634f;
+}
+
+// Running (maximum, sum of exponentials) of scaled logits: one rescaling per batch of elements.
+template <int DT>
+struct Running {
+  float top, sum;  // top in the logits' own units
+  __device__ __forceinline__ void init() { top = -INFINITY, sum = 0.f; }
+  template <int N>
+  __device__ __forceinline__ float add(const float (&x)[N], float scale) {  // returns the batch's maximum
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) m = fmaxf(m, x[e]);
+    const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.f : now * scale;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += exp_of<DT>(x[e], scale, ref);
+    sum = sum * exp_of<DT>(top, scale, ref) + s;
+    top = now;
+    return m;
+  }
+  // the block's lse in natural units; every thread gets it.  sh: 2 * waves floats
+  template <int NT>
+  __device__ __forceinline__ float lse(float scale, float inv_tau, float* sh) {
+    const float wtop = wave_max_f32(top), ref = wtop == -INFINITY ? 0.f : wtop * scale;
+    const float wsum = wave_sum_f32(sum * exp_of<DT>(top, scale, ref));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane == 0) sh[2 * wave] = wtop, sh[2 * wave + 1] = wsum;
+    __syncthreads();
+    float t = sh[0] * inv_tau, s = sh[1];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) join(t, s, sh[2 * w] * inv_tau, sh[2 * w + 1]);
+    return t + logf(s);
+  }
+};
+
+// Streams a row through `f(x[batch], first element's column or -1 for the row's loose ends, vector of elements e ->
+// column + e)` in batches of U vectors a thread; the next batch's loads are in flight while one is worked on.
+template <int DT, int NT, int U, class F>
+__device__ __forceinline__ void stream_row(const RowView<DT>& r, F&& f) {
+  constexpr int V = Elem<DT>::PER16;
+  vec4f next[U];
+  const auto fetch = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = base + u * NT + (int)threadIdx.x;
+      if (i < r.vecs) next[u] = r.vec(i);
+    }
+  };
+  fetch(0);
+  for (int base = 0; base < r.vecs; base += U * NT) {
+    vec4f raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
+    fetch(base + U * NT);
+    float x[U * V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float y[V];
+      unpack16<DT>(raw[u], y);
+      const bool have = base + u * NT + (int)threadIdx.x < r.vecs;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[u * V + e] = have ? y[e] : -INFINITY;
+    }
+    f(x, base);
+  }
+}
+
+// One block per row: the targets' probabilities, (max, sum of exponentials) in one pass over the logits, the targets'
+// terms and the row's loss.  Bound by the read of the logits.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
+                                                          const int32_t* __restrict__ indices, const float* __restrict__ values,
+                                                          const float* __restrict__ top_lse, float* __restrict__ lse_out,
+                                                          float* __restrict__ loss) {
+  __shared__ float sh[2 * NT / 64], sh_P;
+  __shared__ double sh_loss[NT / 64];
   const int64_t row = blockIdx.x;
-  const float P = t.P[row];
-  if (P == NO_TARGET) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (wave == 0) {
+    const float P = top_targets(indices, values, top_lse, row, classes, t, lane);
+    if (lane == 0) sh_P = P;
+  }
+  __syncthreads();
+  if (sh_P == NO_TARGET) {
     if (threadIdx.x == 0) loss[row] = 0.f, lse_out[row] = 0.f;
     return;
   }
-  const typename Elem<DT>::t* z = (const typename Elem<DT>::t*)logits + row * ld;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float top = -INFINITY, sum = 0.f;
-  for (int c = threadIdx.x; c < classes; c += 256) {
-    const float u = (float)z[c] * t.inv_tau;
-    const float m = fmaxf(top, u), ref = m == -INFINITY ? 0.f : m;
-    sum = sum * expf(top - ref) + expf(u - ref);
-    top = m;
+  const RowView<DT> r(logits, row * ld, classes);
+  const float scale = exp_scale<DT>(t.inv_tau);
+  Running<DT> run;
+  run.init();
+  if ((int)threadIdx.x < r.loose()) {
+    const float x[1] = {(float)r.z[r.loose_at(threadIdx.x)]};
+    run.add(x, scale);
   }
-  const float wtop = wave_max_f32(top), ref = wtop == -INFINITY ? 0.f : wtop;
-  sum = wave_sum_f32(sum * expf(top - ref));
-  if (lane == 0) sh_top[wave] = wtop, sh_sum[wave] = sum;
-  __syncthreads();
-  top = sh_top[0], sum = sh_sum[0];
-  for (int w = 1; w < 4; ++w) join(top, sum, sh_top[w], sh_sum[w]);
-  const float lse = top + logf(sum);
+  constexpr int U = DT == NIF_F32 ? 4 : 2;
+  stream_row<DT, NT, U>(r, [&](const float (&x)[U * Elem<DT>::PER16], int) { run.add(x, scale); });
+  const float lse = run.template lse<NT>(scale, t.inv_tau, sh);
   double s = 0.0;
-  for (int k = threadIdx.x; k < t.k; k += 256) {
+  for (int k = threadIdx.x; k < t.k; k += NT) {
     const int at = t.at[row * t.k + k];
-    if (at >= 0) s += target_term(t, row, k, (float)z[at] * t.inv_tau, lse);
+    if (at >= 0) s += target_term(t, row, k, (float)r.z[at] * t.inv_tau, lse);
   }
   s = wave_sum_f64(s);
   if (lane == 0) sh_loss[wave] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < NT / 64; ++w) s += sh_loss[w];
     lse_out[row] = lse;
-    loss[row] = (float)(((sh_loss[0] + sh_loss[1]) + (sh_loss[2] + sh_loss[3])) * t.tau2);
+    loss[row] = (float)(s * t.tau2);
   }
 }
 
@@ -146,24 +248,62 @@ __global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* __res
   }
 }
 
-// One block per row and stretch of classes.  The targets' entries are stored again after the block's other stores.
+// One block per row and stretch of classes, the rows in reverse: the last ones read by the loss are the likeliest to be
+// in the cache still.  The targets' entries are stored again after the block's other stores.  Bound by memory: 16-byte
+// loads and stores, also where the row starts off a 16-byte border (the output's rows then start alike, or go by element).
 template <int DT>
 __global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
                                                            const float* __restrict__ lse, const float* __restrict__ grad, int per_row,
                                                            const float* __restrict__ count, void* __restrict__ out, int64_t ldo,
                                                            int stretch) {
   typedef typename Elem<DT>::t E;
-  const int64_t row = blockIdx.x;
-  const int c0 = blockIdx.y * stretch, c1 = min(classes, c0 + stretch);
-  const E* z = (const E*)logits + row * ld;
+  constexpr int V = Elem<DT>::PER16, U = 4;
+  const int64_t row = (int64_t)gridDim.x - 1 - blockIdx.x;
+  const RowView<DT> r(logits, row * ld, classes);
   E* o = (E*)out + row * ldo;
   const float P = t.P[row];
-  if (P == NO_TARGET) {
-    for (int c = c0 + threadIdx.x; c < c1; c += 256) o[c] = (E)0.f;
-    return;
+  const bool live = P != NO_TARGET;
+  const float coef = live ? (per_row ? grad[row] : count ? grad[0] / *count : grad[0]) * t.tau : 0.f;
+  const float cp = live ? coef * P : 0.f, l = lse[row];
+  const float scale = exp_scale<DT>(t.inv_tau), shift = DT == NIF_F32 ? l : l * 1.4426950408889634f;
+  const auto dz = [&](float x) { return live ? cp * exp_of<DT>(x, scale, shift) : 0.f; };
+  int c0, c1;  // this block's columns
+  if (((uintptr_t)r.z & 15) == ((uintptr_t)o & 15)) {
+    const int v0 = min(r.vecs, (int)blockIdx.y * (stretch / V)), v1 = min(r.vecs, v0 + stretch / V);
+    vec4f* ov = (vec4f*)(o + r.head);
+    const auto one = [&](vec4f raw) {
+      float x[V];
+      unpack16<DT>(raw, x);
+      E y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = (E)dz(x[e]);
+      vec4f w;
+      __builtin_memcpy(&w, y, 16);
+      return w;
+    };
+    int i = v0 + threadIdx.x;
+    for (; i + (U - 1) * 256 < v1; i += U * 256) {
+      vec4f raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = r.vec(i + u * 256);
+#pragma unroll
+      for (int u = 0; u < U; ++u) __builtin_nontemporal_store(one(raw[u]), ov + i + u * 256);
+    }
+    for (; i < v1; i += 256) ov[i] = one(r.vec(i));
+    c0 = r.head + v0 * V, c1 = r.head + v1 * V;
+    if (blockIdx.y == 0) {
+      c0 = 0;
+      if ((int)threadIdx.x < r.head) o[threadIdx.x] = (E)dz((float)r.z[threadIdx.x]);
+    }
+    if (blockIdx.y == gridDim.y - 1) {
+      c1 = classes;
+      if (r.tail() + (int)threadIdx.x < classes) o[r.tail() + threadIdx.x] = (E)dz((float)r.z[r.tail() + threadIdx.x]);
+    }
+  } else {
+    c0 = blockIdx.y * stretch, c1 = blockIdx.y == gridDim.y - 1 ? classes : min(classes, c0 + stretch);
+    for (int c = c0 + threadIdx.x; c < c1; c += 256) o[c] = (E)dz((float)r.z[c]);
   }
-  const float coef = (per_row ? grad[row] : count ? grad[0] / *count : grad[0]) * t.tau, cp = coef * P, l = lse[row];
-  for (int c = c0 + threadIdx.x; c < c1; c += 256) o[c] = (E)(cp * expf((float)z[c] * t.inv_tau - l));
+  if (!live) return;
   __syncthreads();  // the block's stores are done
   for (int k = threadIdx.x; k < t.k; k += 256) {
     const int v = t.at[row * t.k + k];
@@ -175,7 +315,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restric
         first &= q >= k;
         sum += t.p[row * t.k + q];
       }
-    if (first) o[v] = (E)(cp * expf((float)z[v] * t.inv_tau - l) - coef * sum);
+    if (first) o[v] = (E)(dz((float)r.z[v]) - coef * sum);
   }
 }
 
@@ -189,53 +329,176 @@ __device__ __forceinline__ unsigned order_of(float x) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-// One block per row, one pass per entry: the largest key below the last one.  With the log-sum-exp of the row.
-template <int DT>
-__global__ __launch_bounds__(256) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,
-                                                         void* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse) {
-  typedef typename Elem<DT>::t E;
-  __shared__ unsigned long long sh_key[4];
-  __shared__ float sh_top[4], sh_sum[4];
-  const int64_t row = blockIdx.x;
-  const E* z = (const E*)logits + row * ld;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float top = -INFINITY, sum = 0.f;
-  for (int c = threadIdx.x; c < classes; c += 256) {
-    const float u = (float)z[c] * inv_tau;
-    const float m = fmaxf(top, u), ref = m == -INFINITY ? 0.f : m;
-    sum = sum * expf(top - ref) + expf(u - ref);
-    top = m;
-  }
-  const float wtop = wave_max_f32(top), ref = wtop == -INFINITY ? 0.f : wtop;
-  sum = wave_sum_f32(sum * expf(top - ref));
-  if (lane == 0) sh_top[wave] = wtop, sh_sum[wave] = sum;
+__device__ __forceinline__ unsigned long long key_of(float x, int c) {
+  return ((unsigned long long)order_of(x) << 32) | (0xfffffffeu - (unsigned)c);
+}
+
+// n keys (a power of two) in descending order
+template <int NT>
+__device__ __forceinline__ void sort_keys(unsigned long long* key, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += NT) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const unsigned long long a = key[lo], b = key[hi];
+        if ((a < b) == ((lo & size) == 0)) key[lo] = b, key[hi] = a;
+      }
+    }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    top = sh_top[0], sum = sh_sum[0];
-    for (int w = 1; w < 4; ++w) join(top, sum, sh_top[w], sh_sum[w]);
-    lse[row] = top + logf(sum);
+}
+
+// The k-th largest of the block's NT values (1 <= k <= NT), one a thread: sorted with wave shuffles, the three or more
+// steps wider than a wave through LDS.
+template <int NT>
+__device__ __forceinline__ float kth_largest(float x, int k, float* sh) {
+  for (int size = 2; size <= NT; size <<= 1)
+    for (int step = size >> 1; step; step >>= 1) {
+      float y;
+      if (step >= 64) {
+        __syncthreads();
+        sh[threadIdx.x] = x;
+        __syncthreads();
+        y = sh[threadIdx.x ^ step];
+      } else {
+        y = __shfl_xor(x, step, 64);
+      }
+      const bool want_max = ((threadIdx.x & step) == 0) == ((threadIdx.x & size) == 0);
+      x = want_max ? fmaxf(x, y) : fminf(x, y);
+    }
+  __syncthreads();
+  sh[threadIdx.x] = x;
+  __syncthreads();
+  x = sh[k - 1];
+  __syncthreads();
+  return x;
+}
+
+constexpr int TOP_LIST = 2048;
+
+// Any row: the k-th largest order by four passes of eight bits each, then everything above it and the first of its
+// equals by class.  `key` ends with the k entries, unordered beyond that.
+template <int DT, int NT>
+__device__ __forceinline__ void select_by_digits(const typename Elem<DT>::t* z, int classes, int k, unsigned long long* key, unsigned* hist,
+                                                 int* sh_n) {
+  unsigned prefix = 0, mask = 0;
+  int need = k;  // entries still wanted among those that match the prefix
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += NT) hist[i] = 0;
+    __syncthreads();
+    for (int c = threadIdx.x; c < classes; c += NT) {
+      const unsigned o = order_of((float)z[c]);
+      if ((o & mask) == prefix) atomicAdd(&hist[o >> shift & 255], 1u);
+    }
+    __syncthreads();
+    int d = 255, left = need;
+    while (d > 0 && (int)hist[d] < left) left -= (int)hist[d--];
+    need = left;
+    prefix |= (unsigned)d << shift;
+    mask |= 255u << shift;
+    __syncthreads();
   }
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < k; ++j) {
-    unsigned long long best = 0;
-    for (int c = threadIdx.x; c < classes; c += 256) {
-      const unsigned long long key = ((unsigned long long)order_of((float)z[c]) << 32) | (0xfffffffeu - (unsigned)c);
-      if (key < last && key > best) best = key;
+  if (threadIdx.x == 0) *sh_n = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int taken = 0;  // equals before this stretch
+  for (int c0 = 0; c0 < classes; c0 += NT) {
+    const int c = c0 + threadIdx.x;
+    const unsigned o = c < classes ? order_of((float)z[c]) : 0u;
+    const bool equal = c < classes && o == prefix;
+    const unsigned long long m = __ballot(equal);
+    if (lane == 0) hist[wave] = __popcll(m);
+    __syncthreads();
+    int before = taken + __popcll(m & ((1ull << lane) - 1)), all = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+      if (w < wave) before += hist[w];
+      all += hist[w];
     }
-    for (int o = 32; o; o >>= 1) {
-      const unsigned long long x = __shfl_xor(best, o, 64);
-      best = x > best ? x : best;
+    if ((c < classes && o > prefix) || (equal && before < need)) key[atomicAdd(sh_n, 1)] = ((unsigned long long)o << 32) | (0xfffffffeu - (unsigned)c);
+    taken += all;
+    __syncthreads();
+  }
+}
+
+// One block per row, one pass over it: a threshold that k elements of the first stretch reach (the k-th largest of the
+// threads' maxima) keeps all but about k of each stretch out of a list in LDS; when the list grows it is sorted, cut to k
+// and its last entry becomes the threshold.  Rows that this does not fit (more ties at the threshold than the list
+// holds, NaN) are selected by digits instead.  The log-sum-exp goes along.  Bound by the read of the logits.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,
+                                                        void* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse) {
+  typedef typename Elem<DT>::t E;
+  constexpr int V = Elem<DT>::PER16, U = DT == NIF_F32 ? 4 : 2;
+  __shared__ unsigned long long key[TOP_LIST];
+  __shared__ float sh[NT];
+  __shared__ int sh_n;
+  const int64_t row = blockIdx.x;
+  const RowView<DT> r(logits, row * ld, classes);
+  const float scale = exp_scale<DT>(inv_tau);
+  if (threadIdx.x == 0) sh_n = 0;
+  __syncthreads();
+  Running<DT> run;
+  run.init();
+  const auto put = [&](float x, int c) {
+    const int at = atomicAdd(&sh_n, 1);
+    if (at < TOP_LIST) key[at] = key_of(x, c);
+  };
+  // Sorts the list and cuts it to k; the first absent key is 0.
+  const auto cut = [&](int n) {
+    int p = 64;
+    while (p < n) p <<= 1;
+    for (int i = n + threadIdx.x; i < p; i += NT) key[i] = 0;
+    sort_keys<NT>(key, p);
+  };
+  if ((int)threadIdx.x < r.loose()) {
+    const float x[1] = {(float)r.z[r.loose_at(threadIdx.x)]};
+    run.add(x, scale);
+  }
+  float bar = -INFINITY;  // k entries of lower classes than any element to come reach it: those must exceed it
+  bool first = true, over = k > NT;
+  stream_row<DT, NT, U>(r, [&](const float (&x)[U * V], int base) {
+    const float m = run.add(x, scale);
+    if (over) return;
+    if (first) bar = kth_largest<NT>(m, k, sh);
+    if (first ? m >= bar : m > bar) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = base + u * NT + (int)threadIdx.x;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if ((first ? x[u * V + e] >= bar : x[u * V + e] > bar) && i < r.vecs) put(x[u * V + e], r.head + i * V + e);
+      }
+    }
+    first = false;
+    __syncthreads();
+    const int n = sh_n;
+    over = n > TOP_LIST - 16;
+    if (!over && n > TOP_LIST / 2 - 256 && n > k) {
+      cut(n);
+      const unsigned o = (unsigned)(key[k - 1] >> 32);
+      bar = __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
+      __syncthreads();
+      if (threadIdx.x == 0) sh_n = k;
     }
     __syncthreads();
-    if (lane == 0) sh_key[wave] = best;
+  });
+  const float l = run.template lse<NT>(scale, inv_tau, sh);
+  __syncthreads();
+  if (threadIdx.x == 0) lse[row] = l;
+  // the row's loose ends (fewer than 16), whatever they are
+  if (!over && (int)threadIdx.x < r.loose()) put((float)r.z[r.loose_at(threadIdx.x)], r.loose_at(threadIdx.x));
+  __syncthreads();
+  int n = sh_n;
+  if (over || l != l || n < k) {  // l is NaN where the row holds NaN or +inf, which the comparisons above do not order
     __syncthreads();
-    for (int w = 0; w < 4; ++w) best = sh_key[w] > best ? sh_key[w] : best;
-    last = best;
-    if (threadIdx.x == 0) {
-      const int c = (int)(0xfffffffeu - (unsigned)best);
-      indices[row * k + j] = c;
-      ((E*)values)[row * k + j] = z[c];
-    }
+    select_by_digits<DT, NT>(r.z, classes, k, key, (unsigned*)sh, &sh_n);
+    n = k;
+  }
+  cut(n);
+  for (int j = threadIdx.x; j < k; j += NT) {
+    const int c = (int)(0xfffffffeu - (unsigned)key[j]);
+    indices[row * k + j] = c;
+    ((E*)values)[row * k + j] = r.z[c];
   }
 }
 
@@ -317,9 +580,13 @@ extern "C" int nif_distill_forward(const void* logits, int64_t ld, int64_t rows,
   float* row_loss = reduction == NIF_REDUCE_NONE ? loss : (float*)ws;
   clear_err();
   if (rows > 0) {
-    launch_targets(nullptr, 0, top_indices, top_values, top_lse, rows, top, classes, t, st);
-    NIF_BY_TYPE(dtype, hipLaunchKernelGGL(distill_rows_kernel<D>, dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, t,
-                                          (float*)((char*)state + s.lse), row_loss));
+    // a block of 1024 where rows alone do not fill the machine and are long
+    if (rows < 1024 && classes >= 8192)
+      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, logits, ld, classes,
+                                            t, top_indices, top_values, top_lse, (float*)((char*)state + s.lse), row_loss));
+    else
+      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, t,
+                                            top_indices, top_values, top_lse, (float*)((char*)state + s.lse), row_loss));
   }
   hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, row_loss, t.P, rows, reduction == NIF_REDUCE_MEAN,
                      (float*)((char*)state + s.count), reduction == NIF_REDUCE_NONE ? nullptr : loss);
@@ -357,7 +624,11 @@ extern "C" int nif_top_logits(const void* logits, int64_t ld, int64_t rows, int 
   if (rows == 0) return NIF_OK;
   hipStream_t st = (hipStream_t)stream;
   clear_err();
-  NIF_BY_TYPE(dtype, hipLaunchKernelGGL(top_logits_kernel<D>, dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, top,
-                                        1.f / temperature, values, indices, lse));
+  if (rows < 1024 && classes >= 8192)
+    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, logits, ld, classes, top,
+                                          1.f / temperature, values, indices, lse));
+  else
+    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, top,
+                                          1.f / temperature, values, indices, lse));
   return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
 }
