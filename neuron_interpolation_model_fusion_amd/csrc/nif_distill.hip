@@ -17,54 +17,10 @@ namespace nif {
 
 // ---- targets ------------------------------------------------------------------------------------------------
 
-// a label outside the classes that is not the ignored one has p = NaN: its row's loss and gradients are NaN
 __global__ __launch_bounds__(256) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t n, int classes,
                                                             Targets t) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int64_t y = labels[i];
-  const bool live = y != ignore, good = y >= 0 && y < classes;
-  t.at[i] = !live ? -1 : good ? (int)y : 0;
-  t.p[i] = !live ? 0.f : good ? 1.f : NAN;
-  t.P[i] = !live ? NO_TARGET : good ? 1.f : NAN;
-}
-
-// p_k = exp(t_k / tau - L), L = lse of the teacher's row where given, else over the row's entries.  Entries of a
-// negative class or of value -inf carry nothing; a class that does not exist makes the row NaN.  One wave per row.
-__device__ __forceinline__ float top_targets(const int32_t* __restrict__ indices, const float* __restrict__ values,
-                                            const float* __restrict__ lse, int64_t row, int classes, const Targets& t, int lane) {
-  const int32_t* at = indices + row * t.k;
-  const float* val = values + row * t.k;
-  float top = -INFINITY;
-  bool any = false;
-  for (int k = lane; k < t.k; k += 64) {
-    const bool have = at[k] >= 0 && val[k] != -INFINITY;
-    any |= have;
-    if (have) top = fmaxf(top, val[k] * t.inv_tau);
-  }
-  const bool live = __any(any);
-  top = wave_max_f32(top);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int k = lane; k < t.k; k += 64)
-    if (at[k] >= 0 && val[k] != -INFINITY) sum += expf(val[k] * t.inv_tau - ref);
-  sum = wave_sum_f32(sum);
-  const float L = lse ? lse[row] : ref + logf(sum);
-  float P = 0.f;
-  for (int k = lane; k < t.k; k += 64) {
-    const bool have = at[k] >= 0 && val[k] != -INFINITY;
-    const bool good = at[k] < classes;
-    // without lse: exp(. - ref) / sum, which adds up to one to rounding
-    const float e = lse ? expf(val[k] * t.inv_tau - L) : expf(val[k] * t.inv_tau - ref) / sum;
-    const float p = !have ? 0.f : good ? e : NAN;
-    t.at[row * t.k + k] = !have ? -1 : good ? at[k] : 0;
-    t.p[row * t.k + k] = p;
-    P += p;
-  }
-  P = wave_sum_f32(P);
-  P = live ? P : NO_TARGET;
-  if (lane == 0) t.P[row] = P;
-  return P;
+  if (i < n) label_target(labels[i], ignore, classes, t.p[i], t.at[i], t.P[i]);
 }
 
 __global__ __launch_bounds__(256) void top_targets_kernel(const int32_t* __restrict__ indices, const float* __restrict__ values,
@@ -226,13 +182,14 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict
   }
 }
 
-__global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* __restrict__ rows, const float* __restrict__ P, int64_t n,
+// sum or mean over the rows that count, in a fixed order and 64 bits; rows without a target hold 0
+__global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restrict__ rows, const float* __restrict__ P, int64_t n,
                                                               int mean, float* __restrict__ count, float* __restrict__ loss) {
   __shared__ double sh[16];
   __shared__ int sc[16];
   double s = 0.0;
   int c = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
     s += (double)rows[i];
     c += P[i] != NO_TARGET;
   }
@@ -242,10 +199,14 @@ __global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* __res
   __syncthreads();
   if (threadIdx.x == 0) {
     s = 0.0, c = 0;
-    for (int w = 0; w < 16; ++w) s += sh[w], c += sc[w];
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) s += sh[w], c += sc[w];
     *count = (float)(c > 0 ? c : 1);
-    if (loss) loss[0] = (float)(mean ? s / (c > 0 ? c : 1) : s);
+    loss[0] = (float)(mean ? s / (c > 0 ? c : 1) : s);
   }
+}
+
+void launch_reduce(const float* row_loss, const float* P, int64_t n, bool mean, float* count, float* loss, hipStream_t st) {
+  hipLaunchKernelGGL(reduce_rows_kernel, dim3(1), dim3(n <= 4096 ? 256 : 1024), 0, st, row_loss, P, n, mean, count, loss);
 }
 
 // One block per row and stretch of classes, the rows in reverse: the last ones read by the loss are the likeliest to be
@@ -588,8 +549,8 @@ extern "C" int nif_distill_forward(const void* logits, int64_t ld, int64_t rows,
       NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, t,
                                             top_indices, top_values, top_lse, (float*)((char*)state + s.lse), row_loss));
   }
-  hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, row_loss, t.P, rows, reduction == NIF_REDUCE_MEAN,
-                     (float*)((char*)state + s.count), reduction == NIF_REDUCE_NONE ? nullptr : loss);
+  if (reduction != NIF_REDUCE_NONE)
+    launch_reduce(row_loss, t.P, rows, reduction == NIF_REDUCE_MEAN, (float*)((char*)state + s.count), loss, st);
   return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
 }
 

@@ -504,22 +504,6 @@ __global__ __launch_bounds__(256) void head_finish_kernel(const void* __restrict
   }
 }
 
-// sum or mean over the rows that count, in a fixed order and 64 bits; rows without a target hold 0
-__global__ __launch_bounds__(1024) void head_reduce_kernel(const float* __restrict__ row_loss, int64_t n, const int* __restrict__ count,
-                                                           int mean, float* __restrict__ loss) {
-  __shared__ double sh[16];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)row_loss[i];
-  s = wave_sum_f64(s);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s = 0.0;
-    for (int w = 0; w < 16; ++w) s += sh[w];
-    loss[0] = (float)(mean ? s / max(1, *count) : s);
-  }
-}
-
 // rows without a target: loss 0 (before the finish kernel), gradient 0
 __global__ __launch_bounds__(256) void head_clear_loss_kernel(const int* __restrict__ inv, int64_t n, float* __restrict__ loss) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -647,6 +631,164 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
   }
 }
 
+// ---- small heads ----------------------------------------------------------------------------------------------
+// A batch of a classifier's level fit (32 rows, 10 to 200 classes, 400 features) costs launches, not arithmetic: forward
+// one block per row, which keeps the row's dz (n x classes f32, at most 2 MiB) for the backward pass, a single launch of
+// dot products.  Sums in 32 bits, the row's loss in 64.
+constexpr int SMALL_V = 1024;
+
+template <int DT>
+__global__ __launch_bounds__(256) void head_small_forward_kernel(nif_head_desc h, Targets t, float* __restrict__ dz,
+                                                                 float* __restrict__ row_loss) {
+  typedef typename Elem<DT>::t E;
+  constexpr int V = Elem<DT>::PER16, Q = 4;
+  __shared__ float u[SMALL_V], sh[8];
+  __shared__ double sh_loss[4];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int classes = h.classes, d = h.features;
+  __shared__ float sh_P;
+  if (wave == 0) {
+    if (h.labels) {
+      if (lane == 0) label_target(h.labels[row], h.ignore_index, classes, t.p[row], t.at[row], sh_P), t.P[row] = sh_P;
+    } else {
+      const float P = top_targets(h.top_indices, h.top_values, h.top_lse, row, classes, t, lane);
+      if (lane == 0) sh_P = P;
+    }
+  }
+  __syncthreads();
+  const float P = sh_P;
+  if (P == NO_TARGET) {
+    if (threadIdx.x == 0) row_loss[row] = 0.f;
+    return;
+  }
+  const E* x = (const E*)h.hidden + row * h.ldh;
+  const E* w = (const E*)h.weight;
+  const bool vec = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && h.ldw % V == 0;
+  for (int v0 = wave * Q; v0 < classes; v0 += 4 * Q) {
+    float s[Q];
+    const E* wr[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) s[q] = 0.f, wr[q] = w + (int64_t)min(v0 + q, classes - 1) * h.ldw;
+    int c = vec ? lane * V : d;
+    for (; c + V <= d; c += 64 * V) {
+      float a[V];
+      unpack16<DT>(*(const vec4f*)(x + c), a);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        float b[V];
+        unpack16<DT>(*(const vec4f*)(wr[q] + c), b);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[q] = fmaf(a[e], b[e], s[q]);
+      }
+    }
+    for (c = (vec ? d / V * V : 0) + lane; c < d; c += 64)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) s[q] = fmaf((float)x[c], (float)wr[q][c], s[q]);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      s[q] = wave_sum_f32(s[q]);
+      if (lane == 0 && v0 + q < classes) u[v0 + q] = (s[q] + (h.bias ? Elem<DT>::load(h.bias, v0 + q) : 0.f)) * t.inv_tau;
+    }
+  }
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+  for (int v = threadIdx.x; v < classes; v += 256) top = fmaxf(top, u[v]);
+  top = wave_max_f32(top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  for (int v = threadIdx.x; v < classes; v += 256) sum += expf(u[v] - ref);
+  sum = wave_sum_f32(sum);
+  if (lane == 0) sh[2 * wave] = top, sh[2 * wave + 1] = sum;
+  __syncthreads();
+  top = sh[0], sum = sh[1];
+  for (int q = 1; q < 4; ++q) join(top, sum, sh[2 * q], sh[2 * q + 1]);
+  const float lse = top + logf(sum);
+  double loss = 0.0;
+  for (int k = threadIdx.x; k < t.k; k += 256) {
+    const int at = t.at[row * t.k + k];
+    if (at >= 0) loss += target_term(t, row, k, u[at], lse);
+  }
+  loss = wave_sum_f64(loss);
+  if (lane == 0) sh_loss[wave] = loss;
+  __syncthreads();
+  if (threadIdx.x == 0) row_loss[row] = (float)(((sh_loss[0] + sh_loss[1]) + (sh_loss[2] + sh_loss[3])) * t.tau2);
+  for (int v = threadIdx.x; v < classes; v += 256) u[v] = t.tau * P * expf(u[v] - lse);
+  __syncthreads();
+  for (int k = threadIdx.x; k < t.k; k += 256) {
+    const int v = t.at[row * t.k + k];
+    if (v < 0) continue;
+    float p = 0.f;
+    bool first = true;
+    for (int q = 0; q < t.k; ++q)
+      if (t.at[row * t.k + q] == v) {
+        first &= q >= k;
+        p += t.p[row * t.k + q];
+      }
+    if (first) u[v] -= t.tau * p;
+  }
+  __syncthreads();
+  for (int v = threadIdx.x; v < classes; v += 256) dz[row * classes + v] = u[v];
+}
+
+// Blocks of 64 columns x 4 parts of a sum: first those of dhidden (a row each), then those of dweight (4 classes each).
+template <int DT>
+__global__ __launch_bounds__(256) void head_small_backward_kernel(nif_head_desc h, const float* __restrict__ P, const float* __restrict__ dz,
+                                                                  const float* __restrict__ count, const float* __restrict__ grad,
+                                                                  void* __restrict__ dhidden, int64_t lddh, void* __restrict__ dweight,
+                                                                  int64_t lddw, void* __restrict__ dbias, int hidden_blocks, int stretches) {
+  typedef typename Elem<DT>::t E;
+  __shared__ float sh[4][4][64], shb[4][4];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const int n = (int)h.rows, classes = h.classes, d = h.features;
+  const bool per_row = h.reduction == NIF_REDUCE_NONE;
+  const float share = h.reduction == NIF_REDUCE_MEAN ? 1.f / *count : 1.f;
+  const int block = (int)blockIdx.x < hidden_blocks ? blockIdx.x : blockIdx.x - hidden_blocks;
+  const int c = block % stretches * 64 + lane;
+  if ((int)blockIdx.x < hidden_blocks) {
+    const int64_t row = block / stretches;
+    E* out = (E*)dhidden + row * lddh;
+    if (P[row] == NO_TARGET) {
+      if (part == 0 && c < d) out[c] = (E)0.f;
+      return;
+    }
+    const float coef = grad[per_row ? row : 0] * share;
+    const E* w = (const E*)h.weight + min(c, d - 1);
+    const float* z = dz + row * classes;
+    float s = 0.f;
+#pragma unroll 8
+    for (int v = part; v < classes; v += 4) s = fmaf(z[v], (float)w[v * h.ldw], s);
+    sh[0][part][lane] = s;
+    __syncthreads();
+    if (part == 0 && c < d) out[c] = (E)(coef * ((sh[0][0][lane] + sh[0][1][lane]) + (sh[0][2][lane] + sh[0][3][lane])));
+    return;
+  }
+  const int v0 = block / stretches * 4;
+  const bool bias = dbias && block % stretches == 0;
+  const E* x = (const E*)h.hidden + min(c, d - 1);
+  float s[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int r = part; r < n; r += 4) {
+    if (P[r] == NO_TARGET) continue;  // whatever such a row holds
+    const float coef = grad[per_row ? r : 0] * share, a = dweight ? (float)x[r * h.ldh] : 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float g = coef * dz[(int64_t)r * classes + min(v0 + q, classes - 1)];
+      s[q] = fmaf(g, a, s[q]);
+      sb[q] += g;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    sh[q][part][lane] = s[q];
+    if (lane == 0) shb[q][part] = sb[q];
+  }
+  __syncthreads();
+  const int v = v0 + part;  // each wave writes one of the four classes
+  if (v >= classes) return;
+  if (dweight && c < d) ((E*)dweight)[v * lddw + c] = (E)((sh[part][0][lane] + sh[part][1][lane]) + (sh[part][2][lane] + sh[part][3][lane]));
+  if (bias && lane == 0) ((E*)dbias)[v] = (E)((shb[part][0] + shb[part][1]) + (shb[part][2] + shb[part][3]));
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------
 
 static inline int64_t round_up(int64_t x, int64_t q) { return (x + q - 1) / q * q; }
@@ -655,9 +797,10 @@ struct Plan {
   int64_t n, cap;
   int d, ldd, v, planes, k;
   bool pack_w;       // the weight is copied by pieces: f32, or rows that 16-byte loads cannot take
+  bool small;        // the small heads' kernels
   int piece;         // classes per piece (multiple of 256, or all)
   // state: what the backward pass reads
-  size_t s_p, s_at, s_P, s_rows, s_inv, s_count, s_zero, s_lse, s_uk, s_h, state;
+  size_t s_p, s_at, s_P, s_dz, s_fcount, s_rows, s_inv, s_count, s_zero, s_lse, s_uk, s_h, state;
 };
 
 static constexpr size_t PIECE_BYTES = (size_t)256 << 20;
@@ -685,13 +828,23 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   if (c < 1024) c = 1024;
   if (c > p.v) c = p.v;
   p.piece = (int)c;
+  // Small: the weight fits a CU's reach many times over (each row's block reads it whole, from L2), and the whole product
+  // is too little for tiles of 128.
+  p.small = p.n <= 512 && p.v <= SMALL_V && (int64_t)p.v * p.d <= (1 << 19) && p.n * p.v * p.d <= (1 << 25);
   size_t at = 0;
   p.s_p = take(at, (size_t)p.n * p.k * 4);
   p.s_at = take(at, (size_t)p.n * p.k * 4);
   p.s_P = take(at, (size_t)p.n * 4);
+  p.s_count = take(at, 4);
+  p.s_dz = 0;
+  if (p.small) {
+    p.s_dz = take(at, (size_t)p.n * p.v * 4);
+    p.state = at;
+    return true;
+  }
+  p.s_fcount = take(at, 4);
   p.s_rows = take(at, (size_t)p.cap * 4);
   p.s_inv = take(at, (size_t)p.cap * 4);
-  p.s_count = take(at, 4);
   p.s_zero = take(at, 16);
   p.s_lse = take(at, (size_t)p.cap * 4);
   p.s_uk = take(at, (size_t)p.cap * p.k * 4);
@@ -966,12 +1119,12 @@ extern "C" size_t nif_head_state_bytes(const nif_head_desc* h) {
 
 extern "C" size_t nif_head_forward_workspace_bytes(const nif_head_desc* h) {
   nif::Plan p;
-  return nif::make_plan(h, p) ? nif::forward_space(p).bytes + (size_t)p.cap * 4 : 0;
+  return nif::make_plan(h, p) ? (p.small ? 0 : nif::forward_space(p).bytes) + (size_t)p.cap * 4 : 0;
 }
 
 extern "C" size_t nif_head_backward_workspace_bytes(const nif_head_desc* h) {
   nif::Plan p;
-  return nif::make_plan(h, p) ? nif::backward_space(p).bytes : 0;
+  return !nif::make_plan(h, p) ? 0 : p.small ? 256 : nif::backward_space(p).bytes;
 }
 
 extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state, size_t state_bytes, void* ws, size_t ws_bytes,
@@ -985,8 +1138,24 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
   if (!state || state_bytes < nif_head_state_bytes(h) || !ws || ws_bytes < nif_head_forward_workspace_bytes(h)) return NIF_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
   char* s = (char*)state;
-  const FwdSpace f = forward_space(p);
   clear_err();
+  if (p.small) {
+    Targets tg = targets_of(h, p, s);
+    float* row_loss = h->reduction == NIF_REDUCE_NONE ? loss : (float*)ws;
+    float* dz = (float*)(s + p.s_dz);
+    if (p.n > 0) {
+      if (h->dtype == NIF_F32)
+        hipLaunchKernelGGL(head_small_forward_kernel<NIF_F32>, dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+      else if (h->dtype == NIF_BF16)
+        hipLaunchKernelGGL(head_small_forward_kernel<NIF_BF16>, dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+      else
+        hipLaunchKernelGGL(head_small_forward_kernel<NIF_F16>, dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+    }
+    if (h->reduction != NIF_REDUCE_NONE)
+      launch_reduce(row_loss, tg.P, p.n, h->reduction == NIF_REDUCE_MEAN, (float*)(s + p.s_count), loss, st);
+    return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
+  }
+  const FwdSpace f = forward_space(p);
   int* rows = (int*)(s + p.s_rows);
   int* inv = (int*)(s + p.s_inv);
   int* count = (int*)(s + p.s_count);
@@ -1020,7 +1189,7 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
     hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, rows, inv, count, (int*)(s + p.s_zero));
   }
   if (h->reduction != NIF_REDUCE_NONE)
-    hipLaunchKernelGGL(head_reduce_kernel, dim3(1), dim3(1024), 0, st, row_loss, p.n, count, h->reduction == NIF_REDUCE_MEAN, loss);
+    launch_reduce(row_loss, (const float*)(s + p.s_P), p.n, h->reduction == NIF_REDUCE_MEAN, (float*)(s + p.s_fcount), loss, st);
   return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
 }
 
@@ -1036,8 +1205,28 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
   if (!dhidden && !dweight && !dbias) return NIF_OK;
   hipStream_t st = (hipStream_t)stream;
   const char* s = (const char*)state;
-  const BwdSpace b = backward_space(p);
   clear_err();
+  if (p.small) {
+    const int stretches = (p.d + 63) / 64;
+    const int hb = dhidden ? (int)p.n * stretches : 0, wb = dweight ? (p.v + 3) / 4 * stretches : 0;
+    const int bb = !dweight && dbias ? (p.v + 3) / 4 * stretches : 0;
+    if (hb + wb + bb == 0) return NIF_OK;
+    const float* P = (const float*)(s + p.s_P);
+    const float* dz = (const float*)(s + p.s_dz);
+    const float* count = (const float*)(s + p.s_count);
+    const dim3 grid((unsigned)(hb + wb + bb));
+    if (h->dtype == NIF_F32)
+      hipLaunchKernelGGL(head_small_backward_kernel<NIF_F32>, grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh, dweight,
+                         lddw, dbias, hb, stretches);
+    else if (h->dtype == NIF_BF16)
+      hipLaunchKernelGGL(head_small_backward_kernel<NIF_BF16>, grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh, dweight,
+                         lddw, dbias, hb, stretches);
+    else
+      hipLaunchKernelGGL(head_small_backward_kernel<NIF_F16>, grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh, dweight,
+                         lddw, dbias, hb, stretches);
+    return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
+  }
+  const BwdSpace b = backward_space(p);
   hipLaunchKernelGGL(head_coef_kernel, dim3(1), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
                      h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_count),
                      h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp), (float*)((char*)ws + b.scale));

@@ -106,9 +106,58 @@ __device__ __forceinline__ double target_term(const Targets& t, int64_t row, int
   return (double)p * ((double)logf(p) - (double)u + (double)lse);
 }
 
+// p_k = exp(t_k / tau - L), L = lse of the teacher's row where given, else over the row's entries.  Entries of a
+// negative class or of value -inf carry nothing; a class that does not exist makes the row NaN.  One wave per row.
+__device__ __forceinline__ float top_targets(const int32_t* __restrict__ indices, const float* __restrict__ values,
+                                            const float* __restrict__ lse, int64_t row, int classes, const Targets& t, int lane) {
+  const int32_t* at = indices + row * t.k;
+  const float* val = values + row * t.k;
+  float top = -INFINITY;
+  bool any = false;
+  for (int k = lane; k < t.k; k += 64) {
+    const bool have = at[k] >= 0 && val[k] != -INFINITY;
+    any |= have;
+    if (have) top = fmaxf(top, val[k] * t.inv_tau);
+  }
+  const bool live = __any(any);
+  top = wave_max_f32(top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int k = lane; k < t.k; k += 64)
+    if (at[k] >= 0 && val[k] != -INFINITY) sum += expf(val[k] * t.inv_tau - ref);
+  sum = wave_sum_f32(sum);
+  const float L = lse ? lse[row] : ref + logf(sum);
+  float P = 0.f;
+  for (int k = lane; k < t.k; k += 64) {
+    const bool have = at[k] >= 0 && val[k] != -INFINITY;
+    const bool good = at[k] < classes;
+    // without lse: exp(. - ref) / sum, which adds up to one to rounding
+    const float e = lse ? expf(val[k] * t.inv_tau - L) : expf(val[k] * t.inv_tau - ref) / sum;
+    const float p = !have ? 0.f : good ? e : NAN;
+    t.at[row * t.k + k] = !have ? -1 : good ? at[k] : 0;
+    t.p[row * t.k + k] = p;
+    P += p;
+  }
+  P = wave_sum_f32(P);
+  P = live ? P : NO_TARGET;
+  if (lane == 0) t.P[row] = P;
+  return P;
+}
+
+// a label outside the classes that is not the ignored one has p = NaN: its row's loss and gradients are NaN
+__device__ __forceinline__ void label_target(int64_t y, int64_t ignore, int classes, float& p, int& at, float& P) {
+  const bool live = y != ignore, good = y >= 0 && y < classes;
+  at = !live ? -1 : good ? (int)y : 0;
+  p = !live ? 0.f : good ? 1.f : NAN;
+  P = !live ? NO_TARGET : p;
+}
+
 // Fills p, at and P of n rows from labels or from top logits (nif_distill.hip).
 void launch_targets(const int64_t* labels, int64_t ignore, const int32_t* indices, const float* values, const float* lse, int64_t n, int k,
                     int classes, const Targets& t, hipStream_t st);
+
+// loss = sum or mean of the rows' losses over the rows that count; count = their number, at least 1 (nif_distill.hip).
+void launch_reduce(const float* row_loss, const float* P, int64_t n, bool mean, float* count, float* loss, hipStream_t st);
 
 }  // namespace nif
 

@@ -991,15 +991,30 @@ _HEAD_DT = {torch.float32: _lib.NIF_F32, torch.bfloat16: _lib.NIF_BF16, torch.fl
 _REDUCTIONS = {'none': _lib.NIF_REDUCE_NONE, 'mean': _lib.NIF_REDUCE_MEAN, 'sum': _lib.NIF_REDUCE_SUM}
 
 
+# A head of a level fit is a handful of launches of a few microseconds, and its backward pass runs in autograd's own
+# thread: device guard, stream and addresses are taken the short way here.
+
+def _on(t):
+    return torch.cuda._DeviceGuard(t.device.index)
+
+
+def _stream_of(t):
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _bytes(n, device):
-    return torch.empty(max(int(n), 1), dtype=torch.uint8, device=device)
+    return torch.empty(n or 1, dtype=torch.uint8, device=device)
 
 
-def _same_device(what, *ts):
-    _need_gpu(*ts)
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f'{what}: tensors are on different devices: {sorted(map(str, devices))}')
+def _same_device(what, first, *ts):
+    _need_gpu(first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f'{what}: tensors are on different devices: {first.device} and {t.device}')
 
 
 def _reduction(what, reduction):
@@ -1009,9 +1024,9 @@ def _reduction(what, reduction):
 
 
 def _head_type(what, *ts):
-    types = {t.dtype for t in ts if t is not None}
-    if len(types) != 1 or next(iter(types)) not in _HEAD_DT:
-        raise TypeError(f'{what} needs matching float32, bfloat16 or float16 inputs, got {sorted(map(str, types))}')
+    if ts[0].dtype not in _HEAD_DT or any(t is not None and t.dtype != ts[0].dtype for t in ts):
+        raise TypeError(f'{what} needs matching float32, bfloat16 or float16 inputs, got '
+                        f'{[str(t.dtype) for t in ts if t is not None]}')
 
 
 def _temperature(what, temperature):
@@ -1046,14 +1061,9 @@ def _top_targets(values, indices, lse):
 
 def _head_desc(hidden, weight, bias, labels, indices, values, lse, settings):
     temperature, ignore_index, reduction = settings
-    d = _lib.HeadDesc()
-    d.hidden, d.ldh, d.weight, d.ldw, d.bias = _ptr(hidden), _ld(hidden), _ptr(weight), _ld(weight), _ptr(bias)
-    d.rows, d.features, d.classes = hidden.shape[0], hidden.shape[1], weight.shape[0]
-    d.dtype, d.reduction = _HEAD_DT[hidden.dtype], reduction
-    d.labels, d.ignore_index = _ptr(labels), ignore_index
-    d.top_indices, d.top_values, d.top_lse = _ptr(indices), _ptr(values), _ptr(lse)
-    d.top, d.temperature = 0 if indices is None else indices.shape[1], temperature
-    return ctypes.byref(d)
+    return _lib.HeadDesc(hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight), _addr(bias), hidden.shape[0],
+                         hidden.shape[1], weight.shape[0], _HEAD_DT[hidden.dtype], reduction, _addr(labels), ignore_index,
+                         _addr(indices), _addr(values), _addr(lse), 0 if indices is None else indices.shape[1], temperature)
 
 
 class _LinearHead(torch.autograd.Function):
@@ -1061,13 +1071,13 @@ class _LinearHead(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, labels, indices, values, lse, settings):
         dev = hidden.device
         d = _head_desc(hidden, weight, bias, labels, indices, values, lse, settings)
-        with torch.cuda.device(dev):
+        with _on(hidden):
             per_row = settings[2] == _lib.NIF_REDUCE_NONE
             loss = torch.empty((hidden.shape[0],) if per_row else (), dtype=torch.float32, device=dev)
-            state = _bytes(lib.nif_head_state_bytes(d), dev)
-            ws = _bytes(lib.nif_head_forward_workspace_bytes(d), dev)
-            check(lib.nif_head_forward(d, _ptr(loss), _ptr(state), state.numel(), _ptr(ws), ws.numel(), _stream()),
-                  'nif_head_forward')
+            state_bytes, ws_bytes = lib.nif_head_state_bytes(d), lib.nif_head_forward_workspace_bytes(d)
+            state, ws = _bytes(state_bytes, dev), _bytes(ws_bytes, dev)
+            check(lib.nif_head_forward(d, loss.data_ptr(), state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes,
+                                       _stream_of(hidden)), 'nif_head_forward')
         ctx.save_for_backward(hidden, weight, bias, labels, indices, values, lse, state)
         ctx.settings = settings
         return loss
@@ -1078,13 +1088,15 @@ class _LinearHead(torch.autograd.Function):
         hidden, weight, bias, labels, indices, values, lse, state = ctx.saved_tensors
         dev = hidden.device
         d = _head_desc(hidden, weight, bias, labels, indices, values, lse, ctx.settings)
-        grad_out = grad_out.to(torch.float32).contiguous()
-        with torch.cuda.device(dev):
+        grad_out = grad_out.contiguous()
+        with _on(hidden):
             dh, dw, db = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
                           for t, need in zip((hidden, weight, bias), ctx.needs_input_grad))
-            ws = _bytes(lib.nif_head_backward_workspace_bytes(d), dev)
-            check(lib.nif_head_backward(d, _ptr(grad_out), _ptr(state), state.numel(), _ptr(dh), hidden.shape[1], _ptr(dw),
-                                        weight.shape[1], _ptr(db), _ptr(ws), ws.numel(), _stream()), 'nif_head_backward')
+            ws_bytes = lib.nif_head_backward_workspace_bytes(d)
+            ws = _bytes(ws_bytes, dev)
+            check(lib.nif_head_backward(d, grad_out.data_ptr(), state.data_ptr(), state.numel(), _addr(dh), hidden.shape[1],
+                                        _addr(dw), weight.shape[1], _addr(db), ws.data_ptr(), ws_bytes, _stream_of(hidden)),
+                  'nif_head_backward')
         return dh, dw, db, None, None, None, None, None
 
 
@@ -1143,14 +1155,14 @@ class _Distill(torch.autograd.Function):
         temperature, reduction = settings
         n, classes = logits.shape
         k, dev = indices.shape[1], logits.device
-        with torch.cuda.device(dev):
-            per_row = reduction == _lib.NIF_REDUCE_NONE
-            loss = torch.empty((n,) if per_row else (), dtype=torch.float32, device=dev)
-            state = _bytes(lib.nif_distill_state_bytes(n, k), dev)
-            ws = _bytes(lib.nif_distill_workspace_bytes(n), dev)
-            check(lib.nif_distill_forward(_ptr(logits), _ld(logits), n, classes, _HEAD_DT[logits.dtype], _ptr(indices),
-                                          _ptr(values), _ptr(lse), k, temperature, reduction, _ptr(loss), _ptr(state),
-                                          state.numel(), _ptr(ws), ws.numel(), _stream()), 'nif_distill_forward')
+        with _on(logits):
+            loss = torch.empty((n,) if reduction == _lib.NIF_REDUCE_NONE else (), dtype=torch.float32, device=dev)
+            state_bytes, ws_bytes = lib.nif_distill_state_bytes(n, k), lib.nif_distill_workspace_bytes(n)
+            state, ws = _bytes(state_bytes, dev), _bytes(ws_bytes, dev)
+            check(lib.nif_distill_forward(logits.data_ptr(), _ld(logits), n, classes, _HEAD_DT[logits.dtype],
+                                          indices.data_ptr(), values.data_ptr(), _addr(lse), k, temperature, reduction,
+                                          loss.data_ptr(), state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes,
+                                          _stream_of(logits)), 'nif_distill_forward')
         ctx.save_for_backward(logits, state)
         ctx.settings = settings + (k,)
         return loss
@@ -1161,12 +1173,12 @@ class _Distill(torch.autograd.Function):
         logits, state = ctx.saved_tensors
         temperature, reduction, k = ctx.settings
         n, classes = logits.shape
-        grad_out = grad_out.to(torch.float32).contiguous()
-        with torch.cuda.device(logits.device):
+        grad_out = grad_out.contiguous()
+        with _on(logits):
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            check(lib.nif_distill_backward(_ptr(logits), _ld(logits), n, classes, _HEAD_DT[logits.dtype], k, temperature,
-                                           reduction, _ptr(grad_out), _ptr(state), state.numel(), _ptr(grad), classes,
-                                           _stream()), 'nif_distill_backward')
+            check(lib.nif_distill_backward(logits.data_ptr(), _ld(logits), n, classes, _HEAD_DT[logits.dtype], k, temperature,
+                                           reduction, grad_out.data_ptr(), state.data_ptr(), state.numel(), grad.data_ptr(),
+                                           classes, _stream_of(logits)), 'nif_distill_backward')
         return grad, None, None, None, None
 
 
@@ -1206,12 +1218,12 @@ def top_logits(logits, k, *, temperature=1.0):
     lead = logits.shape[:-1]
     z = _mat(logits.detach().reshape(-1, logits.shape[-1]), 'logits')
     n, dev = z.shape[0], z.device
-    with torch.cuda.device(dev):
+    with _on(z):
         values = torch.empty((n, k), dtype=z.dtype, device=dev)
         indices = torch.empty((n, k), dtype=torch.int32, device=dev)
         lse = torch.empty((n,), dtype=torch.float32, device=dev)
-        check(lib.nif_top_logits(_ptr(z), _ld(z), n, z.shape[1], _HEAD_DT[z.dtype], k, temperature, _ptr(values), _ptr(indices),
-                                 _ptr(lse), _stream()), 'nif_top_logits')
+        check(lib.nif_top_logits(z.data_ptr(), _ld(z), n, z.shape[1], _HEAD_DT[z.dtype], k, temperature, values.data_ptr(),
+                                 indices.data_ptr(), lse.data_ptr(), _stream_of(z)), 'nif_top_logits')
     return values.reshape(*lead, k), indices.reshape(*lead, k), lse.reshape(lead)
 
 
