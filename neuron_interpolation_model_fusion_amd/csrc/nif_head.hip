@@ -20,6 +20,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/nif.h"
 #include "nif_common.h"
 #include "nif_target.h"
@@ -117,47 +119,70 @@ __device__ __forceinline__ void tile_of(int id, int total, int mt, int nt, int& 
   tn = first + in % width;
 }
 
-// Copies a 64-deep tile of one side into LDS with direct 16-byte loads.  Plain: [BT rows][8 units of 16 bytes], unit
-// u of row r at u ^ (r & 7).  Transposed: [64 k][BT / 8 units], pairs of units xor-ed with (k & 3) | (k >> 3 & 1) << 2:
-// both keep the fragment reads free of bank conflicts.
+// Copies a 32-deep tile of one side into LDS with direct 16-byte loads.  Plain: [BT rows][4 units of 16 bytes], unit u of
+// row r at u ^ row_swizzle(r): 16-byte reads go 16 lanes at a time, lanes 0-3, 12-15, 20-23, 24-27 together, then 4-11,
+// 16-19, 28-31, and so on (u ^ (r >> 2 & 3) measured two cycles for one).  Transposed: [32 k][BT / 8 units], pairs of units xor-ed with (k & 3) | (k >> 3 & 1) << 2.
+// Both keep the fragment reads free of bank conflicts.
+constexpr int BK = 32;
+constexpr int64_t HEAD_MAX_LD = 1 << 20;
+
+__device__ __forceinline__ int row_swizzle(int row) { return 0x78 >> (row >> 2 & 3) * 2 & 3; }  // 0, 2, 3, 1
+
+__device__ __forceinline__ unsigned lds_offset(const void* p) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
+
+// Direct loads into LDS, 16 bytes a lane, lane i to dst + 16 i.  In assembly because the compiler, which cannot tell the
+// stages apart, would have every LDS read wait for all of them; step_barrier waits instead.  They write no register.
+__device__ __forceinline__ void load_lds16(const void* base, unsigned off, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds16(const void* at, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(at) : "memory");
+}
+
 template <int BT, int NW, bool TR>
 struct Stager {
-  static constexpr int CW = BT / 8 / NW;  // 1 KiB pieces per wave
+  static constexpr int PIECES = BT / 16;                          // of 1 KiB
+  static constexpr int CW = PIECES > NW ? PIECES / NW : 1;        // pieces per wave (some twice where waves outnumber them)
   static constexpr int U = BT / 8;
-  const char* p[CW];
-  int64_t step;
-  int k_of[CW];
+  const char* base;    // of the tile at k = 0 (the same for every lane)
+  unsigned piece[CW];  // where this wave's pieces go in a stage
+  unsigned off[CW];    // bytes from there to this lane's 16, 32 bits (leading dimensions are at most HEAD_MAX_LD)
+  int k_of;            // of this lane's first 16 bytes; transposed: 64 / U more for each piece
   __device__ __forceinline__ void init(const Side& s, int r0, int wave, int lane) {
+    base = (const char*)(TR ? s.base : s.base + (int64_t)r0 * s.ld);
 #pragma unroll
     for (int q = 0; q < CW; ++q) {
-      const int c = wave * CW + q;
+      const int c = (wave * CW + q) % PIECES;
+      piece[q] = c * 1024;
       if (!TR) {
-        const int row = 8 * c + (lane >> 3);
-        const int64_t r = min(r0 + row, s.rlim - 1);
-        k_of[q] = ((lane & 7) ^ (row & 7)) * 8;
-        p[q] = (const char*)(s.base + r * s.ld + k_of[q]);
+        const int row = 16 * c + (lane >> 2);
+        k_of = ((lane & 3) ^ row_swizzle(row)) * 8;
+        off[q] = (unsigned)min(row, s.rlim - 1 - r0) * (unsigned)s.ld * 2 + k_of * 2;
       } else {
         const int k = c * (64 / U) + lane / U, d = lane % U;
         const int f = ((k & 3) | ((k >> 3 & 1) << 2)) & (U / 2 - 1);
-        const int unit = min(r0 / 8 + (d ^ (f << 1)), s.rlim / 8 - 1);
-        k_of[q] = k;
-        p[q] = (const char*)(s.base + (int64_t)unit * 8);
+        if (q == 0) k_of = k;
+        off[q] = (unsigned)k * (unsigned)s.ld * 2 + (unsigned)min(r0 / 8 + (d ^ (f << 1)), s.rlim / 8 - 1) * 16;
       }
     }
   }
-  __device__ __forceinline__ void issue(const Side& s, const char* zero, int plane, int64_t k0, char* lds, int wave) const {
-    const int64_t po = (int64_t)plane * s.plane * 2;
+  // the tile at `at` = base + its k (and plane); `tail`: k that exist from there on, where that is less than BK
+  __device__ __forceinline__ void issue(const Side& s, const char* zero, const char* at, int tail, unsigned dst) const {
+    if (tail >= BK) {
 #pragma unroll
-    for (int q = 0; q < CW; ++q) {
-      const char* a;
-      if (!TR) {
-        a = k0 + k_of[q] < s.klim ? p[q] + po + k0 * 2 : zero;
-      } else {
-        const int64_t k = min(k0 + k_of[q], s.klim - 1);
-        a = p[q] + po + k * s.ld * 2;
+      for (int q = 0; q < CW; ++q) load_lds16(at, off[q], dst + piece[q]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < CW; ++q) {
+        const char* a = at + off[q];
+        if (!TR)
+          a = k_of < tail ? a : zero;
+        else
+          a -= (int64_t)max(0, k_of + q * (64 / U) - (tail - 1)) * s.ld * 2;
+        load_lds16(a, dst + piece[q]);
       }
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)a,
-                                       (__attribute__((address_space(3))) void*)(lds + (wave * CW + q) * 1024), 16, 0, 0);
     }
   }
 };
@@ -167,20 +192,19 @@ struct Reader {
   int base, lane_f;
   __device__ __forceinline__ void init(int w0, int lane) {
     if (!TR) {
-      base = (w0 + (lane & 15)) * 128;
-      lane_f = (lane >> 4) ^ (lane & 7);
+      base = (w0 + (lane & 15)) * 64 + ((lane >> 4) ^ row_swizzle(lane)) * 16;
     } else {
       const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
       lane_f = (q | ((g & 1) << 2)) & (BT / 16 - 1);
       base = (8 * g + q) * (BT * 2) + pp * 8;
     }
   }
-  // fragment i (16 rows from w0 + 16 i) of k step ks (32 deep)
-  __device__ __forceinline__ s16x8 get(const char* lds, int w0, int i, int ks) const {
+  // fragment i: 16 rows from w0 + 16 i, 32 k
+  __device__ __forceinline__ s16x8 get(const char* lds, int w0, int i) const {
     if (!TR) {
-      return *(const s16x8*)(lds + base + i * 2048 + ((lane_f ^ (ks * 4)) << 4));
+      return *(const s16x8*)(lds + base + i * 1024);
     } else {
-      const char* a = lds + base + ks * 32 * BT * 2 + (((w0 / 16 + i) ^ lane_f) << 5);
+      const char* a = lds + base + (((w0 / 16 + i) ^ lane_f) << 5);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * BT * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -191,8 +215,8 @@ struct Reader {
 template <class T, int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
-  __shared__ __attribute__((aligned(1024))) char lds_a[2][BM * 128];
-  __shared__ __attribute__((aligned(1024))) char lds_b[2][BN * 128];
+  __shared__ __attribute__((aligned(1024))) char lds_a[4][BM * 64];
+  __shared__ __attribute__((aligned(1024))) char lds_b[4][BN * 64];
   const int split = blockIdx.x / (g.mt * g.nt);
   int tm, tn;
   tile_of(blockIdx.x % (g.mt * g.nt), g.mt * g.nt, g.mt, g.nt, tm, tn);
@@ -201,7 +225,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   // dz is the next products' operand in steps of 64 rows: rows up to there are written as zeros
   if (n0 >= (EPI == EPI_DZ ? (N + 63) / 64 * 64 : N)) return;
   const int64_t K = g.k_dev ? min(g.K, (int64_t)*g.k_dev) : g.K;
-  const int ktiles = (int)((K + 63) / 64);
+  const int ktiles = (int)((K + BK - 1) / BK);
   const int total = ktiles * (T::PLANES == 3 ? 6 : 1);
   const int per = (total + g.splits - 1) / g.splits;
   const int t0 = min(split * per, total), t1 = min(t0 + per, total);
@@ -225,30 +249,96 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // plane pairs, smallest products first: (l, h) (h, l) (m, m) (m, h) (h, m) (h, h)
-  auto issue = [&](int t, int buf) {
-    const int pair = t / ktiles;
-    const int64_t k0 = (int64_t)(t - pair * ktiles) * 64;
+  // The tiles are issued in order: `at_a`, `at_b` walk along k, then to the next pair of planes.
+  const int64_t step_a = BK * 2 * (TRA ? g.A.ld : 1), step_b = BK * 2 * (TRB ? g.B.ld : 1);
+  int pair = T::PLANES == 3 ? t0 / max(1, ktiles) : 0, kt = t0 - pair * ktiles;
+  const char *at_a = nullptr, *at_b = nullptr;
+  const auto aim = [&] {
     const int pa = T::PLANES == 3 ? (0x001102 >> (4 * pair)) & 3 : 0;
     const int pb = T::PLANES == 3 ? (0x010120 >> (4 * pair)) & 3 : 0;
-    sa.issue(g.A, zero, pa, k0, lds_a[buf], wave);
-    sb.issue(g.B, zero, pb, k0, lds_b[buf], wave);
+    at_a = sa.base + pa * g.A.plane * 2 + kt * step_a;
+    at_b = sb.base + pb * g.B.plane * 2 + kt * step_b;
   };
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    __syncthreads();  // the tile has landed for every wave, and every wave is done with the other buffer
-    if (t + 1 < t1) issue(t + 1, buf ^ 1);
+  aim();
+  const unsigned dst_a = lds_offset(lds_a), dst_b = lds_offset(lds_b);
+  int stage = 0;
+  const auto issue_a = [&] { sa.issue(g.A, zero, at_a, (int)min((int64_t)BK, g.A.klim - (int64_t)kt * BK), dst_a + stage * BM * 64); };
+  const auto issue_b = [&] {
+    sb.issue(g.B, zero, at_b, (int)min((int64_t)BK, g.B.klim - (int64_t)kt * BK), dst_b + stage * BN * 64);
+    stage = (stage + 1) & 3;
+    at_a += step_a;
+    at_b += step_b;
+    if (++kt == ktiles && T::PLANES == 3) {
+      kt = 0;
+      ++pair;
+      aim();
+    }
+  };
+  // Four stages of 32 k: while a step's matrix instructions run on fragments that are in registers, the next step's
+  // fragments are read from LDS and the loads of the third step from now are in flight.  One barrier a step: behind it
+  // the tile after next has landed for every wave, and nobody still reads the stage that the next loads overwrite.
+  constexpr int LOADS = Stager<BM, NW, TRA>::CW + Stager<BN, NW, TRB>::CW;
+  s16x8 a0[FI], b0[FJ], a1[FI], b1[FJ];
+  auto fetch = [&](int t, s16x8(&a)[FI], s16x8(&b)[FJ]) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      s16x8 a[FI], b[FJ];
+    for (int i = 0; i < FI; ++i) a[i] = ra.get(lds_a[(t - t0) & 3], wm * WTM, i);
 #pragma unroll
-      for (int i = 0; i < FI; ++i) a[i] = ra.get(lds_a[buf], wm * WTM, i, ks);
+    for (int j = 0; j < FJ; ++j) b[j] = rb.get(lds_b[(t - t0) & 3], wn * WTN, j);
+  };
+  // all loads but the newest step's have landed, all LDS reads are done, in every wave; nothing moves across
+  auto step_barrier = [&](bool newer) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (newer)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto multiply = [&](int i0, int i1, const s16x8(&a)[FI], const s16x8(&b)[FJ]) {
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) b[j] = rb.get(lds_b[buf], wn * WTN, j, ks);
+    for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int i = 0; i < FI; ++i)
+      for (int j = 0; j < FJ; ++j)
+        if (i >= i0 && i < i1) acc[i][j] = T::mfma(a[i], b[j], acc[i][j]);
+  };
+  // `steady`: the loads of step t + 3 exist.  The reads go between the first half of the matrix instructions, the loads
+  // (and their address arithmetic) into the second: at the head of the step they would hold up both waves of a SIMD.
+  auto step = [&](auto steady, int t, const s16x8(&a)[FI], const s16x8(&b)[FJ], s16x8(&an)[FI], s16x8(&bn)[FJ]) {
+    if (steady || t + 1 < t1) fetch(t + 1, an, bn);
+    multiply(0, FI / 2, a, b);
+    if (steady) {
+      constexpr int READS = FI * (TRA ? 2 : 1) + FJ * (TRB ? 2 : 1), HALF = FI / 2 * FJ, EACH = (READS + HALF - 1) / HALF;
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = T::mfma(a[i], b[j], acc[i][j]);
+      for (int r = 0; r < HALF; ++r) {
+        __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (steady) issue_a();
+    multiply(FI / 2, FI / 2 + FI / 4, a, b);
+    __builtin_amdgcn_sched_barrier(0);
+    if (steady) issue_b();
+    multiply(FI / 2 + FI / 4, FI, a, b);
+    step_barrier(steady);
+  };
+  if (t0 < t1) {
+    for (int t = t0; t < min(t0 + 3, t1); ++t) issue_a(), issue_b();
+    step_barrier(t0 + 2 < t1);
+    fetch(t0, a0, b0);
+    int t = t0;
+    for (; t + 4 < t1; t += 2) {
+      step(std::true_type(), t, a0, b0, a1, b1);
+      step(std::true_type(), t + 1, a1, b1, a0, b0);
+    }
+    if (t + 3 < t1) {  // four steps are left, else one to three
+      step(std::true_type(), t, a0, b0, a1, b1);
+      step(std::false_type(), t + 1, a1, b1, a0, b0);
+      t += 2;
+    }
+    for (; t < t1; t += 2) {
+      step(std::false_type(), t, a0, b0, a1, b1);
+      if (t + 1 < t1) step(std::false_type(), t + 1, a1, b1, a0, b0);
     }
   }
 
@@ -822,7 +912,8 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.v = h->classes;
   p.k = h->top > 0 ? h->top : 1;
   p.planes = h->dtype == NIF_F32 ? 3 : 1;
-  p.pack_w = h->dtype == NIF_F32 || p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0;
+  p.pack_w = h->dtype == NIF_F32 || p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0 ||
+             h->ldw > HEAD_MAX_LD;
   const int64_t per = (p.pack_w && p.ldd > p.cap ? (int64_t)p.ldd : p.cap) * 2 * p.planes;  // bytes of one class of a piece
   int64_t c = (int64_t)(PIECE_BYTES / per) / 256 * 256;
   if (c < 1024) c = 1024;
@@ -870,8 +961,8 @@ struct Shape {
 };
 // tile of a product with extents m x n
 static Shape shape_of(int64_t m, int64_t n) {
-  (void)m;
   if (n <= 32) return {128, 32, 4};
+  if (m >= 1024 && n >= 1024) return {256, 256, 2};
   return {128, 128, 2};
 }
 
@@ -883,6 +974,8 @@ static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
   if (grid.x == 0) return;
   if (s.bn == 32)
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 32, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+  else if (s.bn == 256)
+    hipLaunchKernelGGL((head_gemm_kernel<T, 256, 256, 2, 4, TRA, TRB, EPI>), grid, dim3(512), 0, st, g);
   else
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
 }

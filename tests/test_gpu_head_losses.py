@@ -142,6 +142,12 @@ def test_distillation_of_a_head_and_gradients(ops, dt, n, d, v, k):
 
 
 @pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, d, v, k', [(1030, 1048, 1300, None), (1290, 1025, 1543, 20), (1024, 1536, 2048, None)])
+def test_sizes_of_the_large_tiles(ops, dt, n, d, v, k):
+    _check_head(ops, dt, n, d, v, k=k, tau=2.0 if k else 1.0, bias=n % 4 == 2, empty=0.01, seed=n)
+
+
+@pytest.mark.parametrize('dt', TYPES)
 @pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
 def test_reductions(ops, dt, reduction):
     _check_head(ops, dt, 70, 40, 90, reduction=reduction, empty=0.4, seed=1)
