@@ -32,15 +32,16 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+// The matrix instructions are written out so that the accumulators stay where they are, in accumulation registers: left
+// to itself the compiler moves them through spare vector registers, of which a 256 x 256 tile leaves none.  Volatile, so
+// that they keep their order against the loads between them; mfma_done() before the results are read.
 struct Bf16 {
   typedef __bf16 t;
   static constexpr int PLANES = 1;
-  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  static __device__ __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
 struct F32 : Bf16 {  // as three bf16 planes
@@ -49,10 +50,19 @@ struct F32 : Bf16 {  // as three bf16 planes
 struct F16 {
   typedef _Float16 t;
   static constexpr int PLANES = 1;
-  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  static __device__ __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
+// the compiler does not know that the results take a few cycles more
+template <int FI, int FJ>
+__device__ __forceinline__ void mfma_done(f32x4 (&acc)[FI][FJ]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
 
 template <class T>
 __device__ __forceinline__ short to16(float x) {
@@ -65,15 +75,18 @@ __device__ __forceinline__ float head_exp(float x) {
   return T::PLANES == 3 ? expf(x) : __expf(x);
 }
 
+constexpr int K_PAD = 128;     // contractions run in whole groups of four steps of 32
 constexpr int HEAD_PAD = 256;  // packed rows are padded to a multiple of the largest tile
 
-// One side of a product.  Plain side: element (r, k) at base[r * ld + k]; transposed side: base[k * ld + r].
+// One side of a product.  Plain side: element (r, k) at base[r * ld + k]; transposed side: base[k * ld + r].  Rows behind
+// rlim are read as the last one (their results are not stored), and so are k behind klim: there the other side, which
+// is always a packed one, holds zeros up to the next multiple of K_PAD.
 struct Side {
   const short* base;
   int64_t plane;  // elements between the planes of a split f32 operand
   int64_t ld;
-  int rlim;       // rows that exist (plain) / row extent rounded up to 8 (transposed); reads behind are clamped
-  int64_t klim;   // k that exist: plain: multiple of 8, zeros are read behind it; transposed: clamped
+  int rlim;       // transposed: a multiple of 8
+  int klim;       // plain: a multiple of 8
 };
 
 enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
@@ -81,10 +94,9 @@ enum { OUT_F32 = 0, OUT_ADD = 1, OUT_FINAL = 2 };
 
 struct GemmArgs {
   Side A, B;
-  const short* zero;    // 16 bytes of zeros
   int M, N;             // extents that are computed (N: at most *n_dev when given)
   const int* n_dev;
-  int64_t K;            // contraction length (at most *k_dev when given)
+  int K;                // contraction length (at most *k_dev when given)
   const int* k_dev;
   int mt, nt, splits;
   // EPI_STATS / EPI_DZ: the logit's last steps
@@ -134,28 +146,25 @@ __device__ __forceinline__ unsigned lds_offset(const void* p) {
 
 // Direct loads into LDS, 16 bytes a lane, lane i to dst + 16 i.  In assembly because the compiler, which cannot tell the
 // stages apart, would have every LDS read wait for all of them; step_barrier waits instead.  They write no register.
-__device__ __forceinline__ void load_lds16(const void* base, unsigned off, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+__device__ __forceinline__ void load_lds16(const void* base, unsigned off, unsigned dst, unsigned more) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(dst), "i"(more), "v"(off), "s"(base)
+               : "memory", "scc");
 }
-__device__ __forceinline__ void load_lds16(const void* at, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(at) : "memory");
-}
-
 template <int BT, int NW, bool TR>
 struct Stager {
   static constexpr int PIECES = BT / 16;                          // of 1 KiB
   static constexpr int CW = PIECES > NW ? PIECES / NW : 1;        // pieces per wave (some twice where waves outnumber them)
   static constexpr int U = BT / 8;
   const char* base;    // of the tile at k = 0 (the same for every lane)
-  unsigned piece[CW];  // where this wave's pieces go in a stage
+  unsigned piece[CW];  // where this wave's pieces go in the first stage (LDS bytes)
   unsigned off[CW];    // bytes from there to this lane's 16, 32 bits (leading dimensions are at most HEAD_MAX_LD)
   int k_of;            // of this lane's first 16 bytes; transposed: 64 / U more for each piece
-  __device__ __forceinline__ void init(const Side& s, int r0, int wave, int lane) {
+  __device__ __forceinline__ void init(const Side& s, int r0, const void* lds, int wave, int lane) {
     base = (const char*)(TR ? s.base : s.base + (int64_t)r0 * s.ld);
 #pragma unroll
     for (int q = 0; q < CW; ++q) {
       const int c = (wave * CW + q) % PIECES;
-      piece[q] = c * 1024;
+      piece[q] = lds_offset(lds) + c * 1024;
       if (!TR) {
         const int row = 16 * c + (lane >> 2);
         k_of = ((lane & 3) ^ row_swizzle(row)) * 8;
@@ -168,47 +177,55 @@ struct Stager {
       }
     }
   }
-  // the tile at `at` = base + its k (and plane); `tail`: k that exist from there on, where that is less than BK
-  __device__ __forceinline__ void issue(const Side& s, const char* zero, const char* at, int tail, unsigned dst) const {
-    if (tail >= BK) {
+  // the tile at `at` = base + its k (and plane), into stage STAGE
+  template <int STAGE>
+  __device__ __forceinline__ void issue(const char* at) const {
 #pragma unroll
-      for (int q = 0; q < CW; ++q) load_lds16(at, off[q], dst + piece[q]);
-    } else {
+    for (int q = 0; q < CW; ++q) load_lds16(at, off[q], piece[q], STAGE * BT * 64);
+  }
+  // a tile of which only `have` k exist (0 or fewer: none): the last ones again in the place of the others.  The base goes
+  // back to where the tile holds one, so that the lanes' offsets, which only shrink, never fall below zero.
+  template <int STAGE>
+  __device__ __forceinline__ void issue_ragged(const Side& s, const char* at, int have) const {
+    constexpr int LEAST = TR ? 1 : 8;
+    const int64_t ld = TR ? s.ld : 1;
+    if (have < LEAST) at -= (LEAST - have) * ld * 2, have = LEAST;
 #pragma unroll
-      for (int q = 0; q < CW; ++q) {
-        const char* a = at + off[q];
-        if (!TR)
-          a = k_of < tail ? a : zero;
-        else
-          a -= (int64_t)max(0, k_of + q * (64 / U) - (tail - 1)) * s.ld * 2;
-        load_lds16(a, dst + piece[q]);
-      }
+    for (int q = 0; q < CW; ++q) {
+      const int behind = k_of + (TR ? q * (64 / U) : 0) + LEAST - have;
+      load_lds16(at, off[q] - (unsigned)max(0, behind) * (unsigned)ld * 2, piece[q], STAGE * BT * 64);
     }
   }
 };
 
+typedef __attribute__((address_space(3))) const s16x8 lds_s16x8;
+
 template <int BT, bool TR>
 struct Reader {
-  int base, lane_f;
-  __device__ __forceinline__ void init(int w0, int lane) {
+  unsigned at;  // LDS bytes of this lane's share of fragment 0 in the first stage
+  __device__ __forceinline__ void init(const void* lds, int w0, int lane) {
     if (!TR) {
-      base = (w0 + (lane & 15)) * 64 + ((lane >> 4) ^ row_swizzle(lane)) * 16;
+      at = (w0 + (lane & 15)) * 64 + ((lane >> 4) ^ row_swizzle(lane)) * 16;
     } else {
-      const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
-      lane_f = (q | ((g & 1) << 2)) & (BT / 16 - 1);
-      base = (8 * g + q) * (BT * 2) + pp * 8;
+      const int g = lane >> 4, q = (lane & 15) >> 2, f = (q | ((g & 1) << 2)) & (BT / 16 - 1);
+      at = (8 * g + q) * (BT * 2) + (((w0 / 16) ^ f) << 5) + (lane & 3) * 8;
     }
+    at += lds_offset(lds);
+    asm("" : "+v"(at));  // one register: the reads' own offsets reach all stages
   }
   // fragment i: 16 rows from w0 + 16 i, 32 k
-  __device__ __forceinline__ s16x8 get(const char* lds, int w0, int i) const {
+  __device__ __forceinline__ s16x8 get(int stage, int i) const {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"
     if (!TR) {
-      return *(const s16x8*)(lds + base + i * 1024);
+      return *(lds_s16x8*)(at + stage * BT * 64 + i * 1024);
     } else {
-      const char* a = lds + base + (((w0 / 16 + i) ^ lane_f) << 5);
+      const unsigned a = (at ^ (i << 5)) + stage * BT * 64;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * BT * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+#pragma clang diagnostic pop
   }
 };
 
@@ -222,31 +239,31 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   tile_of(blockIdx.x % (g.mt * g.nt), g.mt * g.nt, g.mt, g.nt, tm, tn);
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
   const int m0 = tm * BM, n0 = tn * BN;
-  // dz is the next products' operand in steps of 64 rows: rows up to there are written as zeros
-  if (n0 >= (EPI == EPI_DZ ? (N + 63) / 64 * 64 : N)) return;
-  const int64_t K = g.k_dev ? min(g.K, (int64_t)*g.k_dev) : g.K;
-  const int ktiles = (int)((K + BK - 1) / BK);
+  // dz is an operand of the next products: rows up to a multiple of K_PAD are written, as zeros
+  if (n0 >= (EPI == EPI_DZ ? (N + K_PAD - 1) / K_PAD * K_PAD : N)) return;
+  const int K = g.k_dev ? min(g.K, *g.k_dev) : g.K;
+  const int ktiles = (K + K_PAD - 1) / K_PAD * (K_PAD / BK);
   const int total = ktiles * (T::PLANES == 3 ? 6 : 1);
-  const int per = (total + g.splits - 1) / g.splits;
+  const int per = (total / 4 + g.splits - 1) / g.splits * 4;
   const int t0 = min(split * per, total), t1 = min(t0 + per, total);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const char* zero = (const char*)g.zero;
   Stager<BM, NW, TRA> sa;
   Stager<BN, NW, TRB> sb;
-  sa.init(g.A, m0, wave, lane);
-  sb.init(g.B, n0, wave, lane);
+  sa.init(g.A, m0, lds_a, wave, lane);
+  sb.init(g.B, n0, lds_b, wave, lane);
   Reader<BM, TRA> ra;
   Reader<BN, TRB> rb;
-  ra.init(wm * WTM, lane);
-  rb.init(wn * WTN, lane);
+  ra.init(lds_a, wm * WTM, lane);
+  rb.init(lds_b, wn * WTN, lane);
 
   f32x4 acc[FI][FJ];
 #pragma unroll
   for (int i = 0; i < FI; ++i)
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  mfma_done(acc);  // written, before the first matrix instruction reads them
 
   // plane pairs, smallest products first: (l, h) (h, l) (m, m) (m, h) (h, m) (h, h)
   // The tiles are issued in order: `at_a`, `at_b` walk along k, then to the next pair of planes.
@@ -260,87 +277,79 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
     at_b = sb.base + pb * g.B.plane * 2 + kt * step_b;
   };
   aim();
-  const unsigned dst_a = lds_offset(lds_a), dst_b = lds_offset(lds_b);
-  int stage = 0;
-  const auto issue_a = [&] { sa.issue(g.A, zero, at_a, (int)min((int64_t)BK, g.A.klim - (int64_t)kt * BK), dst_a + stage * BM * 64); };
-  const auto issue_b = [&] {
-    sb.issue(g.B, zero, at_b, (int)min((int64_t)BK, g.B.klim - (int64_t)kt * BK), dst_b + stage * BN * 64);
-    stage = (stage + 1) & 3;
-    at_a += step_a;
-    at_b += step_b;
-    if (++kt == ktiles && T::PLANES == 3) {
-      kt = 0;
-      ++pair;
-      aim();
+  int left = t1 - t0;  // tiles that are still to be issued; behind the last one it is issued again, for the count of loads
+  const auto issue = [&](auto stage) {
+    if (kt * BK + BK <= g.A.klim)
+      sa.template issue<stage>(at_a);
+    else
+      sa.template issue_ragged<stage>(g.A, at_a, g.A.klim - kt * BK);
+    sb.template issue<stage>(at_b);
+    if (--left > 0) {
+      at_a += step_a;
+      at_b += step_b;
+      if (++kt == ktiles && T::PLANES == 3) {
+        kt = 0;
+        ++pair;
+        aim();
+      }
     }
   };
   // Four stages of 32 k: while a step's matrix instructions run on fragments that are in registers, the next step's
-  // fragments are read from LDS and the loads of the third step from now are in flight.  One barrier a step: behind it
-  // the tile after next has landed for every wave, and nobody still reads the stage that the next loads overwrite.
+  // fragments are read from LDS, two more tiles are in flight and the loads of the fourth go into the stage that the
+  // step's own fragments came from.  One barrier a step: behind it the tile after next has landed for every wave, and
+  // nobody still reads the stage that the next loads overwrite.
   constexpr int LOADS = Stager<BM, NW, TRA>::CW + Stager<BN, NW, TRB>::CW;
   s16x8 a0[FI], b0[FJ], a1[FI], b1[FJ];
-  auto fetch = [&](int t, s16x8(&a)[FI], s16x8(&b)[FJ]) {
-#pragma unroll
-    for (int i = 0; i < FI; ++i) a[i] = ra.get(lds_a[(t - t0) & 3], wm * WTM, i);
-#pragma unroll
-    for (int j = 0; j < FJ; ++j) b[j] = rb.get(lds_b[(t - t0) & 3], wn * WTN, j);
-  };
-  // all loads but the newest step's have landed, all LDS reads are done, in every wave; nothing moves across
-  auto step_barrier = [&](bool newer) {
-    __builtin_amdgcn_sched_barrier(0);
-    if (newer)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  const auto multiply = [&](int i0, int i1, const s16x8(&a)[FI], const s16x8(&b)[FJ]) {
-#pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-      for (int j = 0; j < FJ; ++j)
-        if (i >= i0 && i < i1) acc[i][j] = T::mfma(a[i], b[j], acc[i][j]);
-  };
-  // `steady`: the loads of step t + 3 exist.  The reads go between the first half of the matrix instructions, the loads
-  // (and their address arithmetic) into the second: at the head of the step they would hold up both waves of a SIMD.
-  auto step = [&](auto steady, int t, const s16x8(&a)[FI], const s16x8(&b)[FJ], s16x8(&an)[FI], s16x8(&bn)[FJ]) {
-    if (steady || t + 1 < t1) fetch(t + 1, an, bn);
-    multiply(0, FI / 2, a, b);
-    if (steady) {
-      constexpr int READS = FI * (TRA ? 2 : 1) + FJ * (TRB ? 2 : 1), HALF = FI / 2 * FJ, EACH = (READS + HALF - 1) / HALF;
-#pragma unroll
-      for (int r = 0; r < HALF; ++r) {
-        __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      }
+  // Fragments of the next tile are read in the order b, the last two rows of a, the other rows of a: those go into the
+  // registers of rows that are done with.
+  constexpr int FRAGS = FI + FJ, PER_ROW = FI > 1 ? (FRAGS + FI - 2) / (FI - 1) : FRAGS;
+  const auto fetch = [&](int f, int stage, s16x8(&a)[FI], s16x8(&b)[FJ]) {
+    if (f < FJ) {
+      b[f] = rb.get(stage, f);
+    } else {
+      const int i = FI < 3 ? f - FJ : f - FJ < 2 ? FI - 1 - (f - FJ) : f - FJ - 2;
+      a[i] = ra.get(stage, i);
     }
+  };
+  // all loads but the newest two tiles' have landed, all LDS reads are done, in every wave; nothing moves across
+  const auto step_barrier = [&] {
     __builtin_amdgcn_sched_barrier(0);
-    if (steady) issue_a();
-    multiply(FI / 2, FI / 2 + FI / 4, a, b);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
     __builtin_amdgcn_sched_barrier(0);
-    if (steady) issue_b();
-    multiply(FI / 2 + FI / 4, FI, a, b);
-    step_barrier(steady);
+  };
+  // Each row of matrix instructions takes its share of the next tile's reads along; nothing moves across rows, so that
+  // neither the reads nor the loads hold up both waves of a SIMD at once.
+  const auto step = [&](auto stage, const s16x8(&a)[FI], const s16x8(&b)[FJ], s16x8(&an)[FI], s16x8(&bn)[FJ]) {
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f)
+        if (f / PER_ROW == i) fetch(f, (stage + 1) & 3, an, bn);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) T::mfma(acc[i][j], a[i], b[j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i == 0) issue(stage);
+    }
+    step_barrier();
   };
   if (t0 < t1) {
-    for (int t = t0; t < min(t0 + 3, t1); ++t) issue_a(), issue_b();
-    step_barrier(t0 + 2 < t1);
-    fetch(t0, a0, b0);
-    int t = t0;
-    for (; t + 4 < t1; t += 2) {
-      step(std::true_type(), t, a0, b0, a1, b1);
-      step(std::true_type(), t + 1, a1, b1, a0, b0);
+    issue(std::integral_constant<int, 0>());
+    issue(std::integral_constant<int, 1>());
+    issue(std::integral_constant<int, 2>());
+    issue(std::integral_constant<int, 3>());
+    step_barrier();
+#pragma unroll
+    for (int f = 0; f < FRAGS; ++f) fetch(f, 0, a0, b0);
+    step_barrier();  // every wave has read the first stage, which the first step overwrites
+    for (int t = t0; t < t1; t += 4) {
+      step(std::integral_constant<int, 0>(), a0, b0, a1, b1);
+      step(std::integral_constant<int, 1>(), a1, b1, a0, b0);
+      step(std::integral_constant<int, 2>(), a0, b0, a1, b1);
+      step(std::integral_constant<int, 3>(), a1, b1, a0, b0);
     }
-    if (t + 3 < t1) {  // four steps are left, else one to three
-      step(std::true_type(), t, a0, b0, a1, b1);
-      step(std::false_type(), t + 1, a1, b1, a0, b0);
-      t += 2;
-    }
-    for (; t < t1; t += 2) {
-      step(std::false_type(), t, a0, b0, a1, b1);
-      if (t + 1 < t1) step(std::false_type(), t + 1, a1, b1, a0, b0);
-    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles issued again
   }
+  mfma_done(acc);
 
   // acc[i][j][r]: m = .. + 16 i + 4 (lane / 16) + r, n = .. + 16 j + lane % 16 -- a lane holds four neighbours along m
   const int mw = m0 + wm * WTM + 4 * (lane >> 4), nw = n0 + wn * WTN + (lane & 15);
@@ -452,12 +461,11 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
 }
 
 // ---- the rows that count ------------------------------------------------------------------------------
-// One workgroup: rows[i] = i-th row with a target, inv[r] = its place or -1, count; also 16 zero bytes.
+// One workgroup: rows[i] = i-th row with a target, inv[r] = its place or -1, count.
 __global__ __launch_bounds__(1024) void head_rows_kernel(const float* __restrict__ P, int64_t n, int* __restrict__ rows,
-                                                         int* __restrict__ inv, int* __restrict__ count, int* __restrict__ zero) {
+                                                         int* __restrict__ inv, int* __restrict__ count) {
   __shared__ int sh[17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x < 4) zero[threadIdx.x] = 0;
   int base = 0;
   for (int64_t r0 = 0; r0 < n; r0 += 1024) {
     const int64_t r = r0 + threadIdx.x;
@@ -890,7 +898,7 @@ struct Plan {
   bool small;        // the small heads' kernels
   int piece;         // classes per piece (multiple of 256, or all)
   // state: what the backward pass reads
-  size_t s_p, s_at, s_P, s_dz, s_fcount, s_rows, s_inv, s_count, s_zero, s_lse, s_uk, s_h, state;
+  size_t s_p, s_at, s_P, s_dz, s_fcount, s_rows, s_inv, s_count, s_lse, s_uk, s_h, state;
 };
 
 static constexpr size_t PIECE_BYTES = (size_t)256 << 20;
@@ -908,7 +916,7 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.n = h->rows;
   p.cap = round_up(p.n > 0 ? p.n : 1, HEAD_PAD);
   p.d = h->features;
-  p.ldd = (int)round_up(p.d, 64);
+  p.ldd = (int)round_up(p.d, K_PAD);
   p.v = h->classes;
   p.k = h->top > 0 ? h->top : 1;
   p.planes = h->dtype == NIF_F32 ? 3 : 1;
@@ -936,7 +944,6 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.s_fcount = take(at, 4);
   p.s_rows = take(at, (size_t)p.cap * 4);
   p.s_inv = take(at, (size_t)p.cap * 4);
-  p.s_zero = take(at, 16);
   p.s_lse = take(at, (size_t)p.cap * 4);
   p.s_uk = take(at, (size_t)p.cap * p.k * 4);
   p.s_h = take(at, (size_t)p.cap * p.ldd * 2 * p.planes);
@@ -1035,7 +1042,6 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
     GemmArgs g = {};
     g.A = weight_side(h, p, v0, vc, (short*)(ws + f.w), st);
     g.B = Side{(const short*)(state + p.s_h), p.cap * p.ldd, p.ldd, (int)p.cap, p.ldd};
-    g.zero = (const short*)(state + p.s_zero);
     g.M = vc;
     g.N = (int)p.n;
     g.n_dev = (const int*)(state + p.s_count);
@@ -1065,7 +1071,7 @@ struct BwdSpace {
 };
 static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
-  b.ldz = round_up(p.piece, 64);
+  b.ldz = round_up(p.piece, K_PAD);
   b.dh_ld = round_up(p.d, 4);
   b.dh = shape_of(p.d, p.n);
   b.dw = shape_of(p.d, p.piece);
@@ -1107,14 +1113,13 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     const int vc = p.v - v0 < p.piece ? p.v - v0 : p.piece;
     const bool first = v0 == 0, last = v0 + vc == p.v;
     const Side w = weight_side(h, p, v0, vc, (short*)(ws + b.w), st);
-    const int64_t kz = round_up(vc, 64);  // columns of dz that are written
+    const int kz = (int)round_up(vc, K_PAD);  // columns of dz that are written
     {
       GemmArgs g = {};
       g.A = w;
       g.B = Side{hp, p.cap * p.ldd, p.ldd, (int)p.cap, p.ldd};
-      g.zero = (const short*)(state + p.s_zero);
       g.M = vc;
-      g.N = (int)round_up(p.n, 64);
+      g.N = (int)round_up(p.n, K_PAD);
       g.n_dev = count;
       g.K = p.ldd;
       g.splits = 1;
@@ -1135,12 +1140,11 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
                          (char*)dbias + (size_t)v0 * (f32 ? 4 : 2), f32);
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
       GemmArgs g = {};
-      g.A = Side{hp, p.cap * p.ldd, p.ldd, p.ldd, p.cap};
-      g.B = Side{dz, dz_plane, b.ldz, (int)kz, p.cap};
-      g.zero = (const short*)(state + p.s_zero);
+      g.A = Side{hp, p.cap * p.ldd, p.ldd, p.ldd, (int)p.cap};
+      g.B = Side{dz, dz_plane, b.ldz, kz, (int)p.cap};
       g.M = p.d;
       g.N = vc;
-      g.K = p.cap;
+      g.K = (int)p.cap;
       g.k_dev = count;
       g.splits = b.dw_splits;
       g.out = (char*)dweight + (size_t)v0 * lddw * (f32 ? 4 : 2);
@@ -1164,7 +1168,6 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.A.klim = w.rlim;
       g.A.rlim = p.pack_w ? p.ldd : p.d;
       g.B = Side{dz, dz_plane, b.ldz, (int)p.cap, kz};
-      g.zero = (const short*)(state + p.s_zero);
       g.M = p.d;
       g.N = (int)p.n;
       g.n_dev = count;
@@ -1256,7 +1259,7 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
   if (p.n > 0) {
     const Targets tg = targets_of(h, p, s);
     launch_targets(h->labels, h->ignore_index, h->top_indices, h->top_values, h->top_lse, p.n, p.k, p.v, tg, st);
-    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, tg.P, p.n, rows, inv, count, (int*)(s + p.s_zero));
+    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, tg.P, p.n, rows, inv, count);
     hipLaunchKernelGGL(head_clear_loss_kernel, dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, st, inv, p.n, row_loss);
     if (h->dtype == NIF_F32)
       hipLaunchKernelGGL(head_pack_kernel<true>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d, rows, count, p.n,
@@ -1279,7 +1282,7 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
     else
       finish<NIF_F16>(h, p, s, stats, tiles, row_loss, st);
   } else {
-    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, rows, inv, count, (int*)(s + p.s_zero));
+    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, rows, inv, count);
   }
   if (h->reduction != NIF_REDUCE_NONE)
     launch_reduce(row_loss, (const float*)(s + p.s_P), p.n, h->reduction == NIF_REDUCE_MEAN, (float*)(s + p.s_fcount), loss, st);
