@@ -69,10 +69,10 @@ __device__ __forceinline__ short to16(float x) {
   return __builtin_bit_cast(short, (typename T::t)x);  // round to nearest even
 }
 
-// 16-bit outputs: the hardware's exponential (about 2^-21 relative); f32: the library's
+// 16-bit types: 2^x by the hardware (2^-22 relative); f32: the library's e^x
 template <class T>
 __device__ __forceinline__ float head_exp(float x) {
-  return T::PLANES == 3 ? expf(x) : __expf(x);
+  return T::PLANES == 3 ? expf(x) : __builtin_amdgcn_exp2f(x);
 }
 
 constexpr int K_PAD = 128;     // contractions run in whole groups of four steps of 32
@@ -132,13 +132,13 @@ __device__ __forceinline__ void tile_of(int id, int total, int mt, int nt, int& 
 }
 
 // Copies a 32-deep tile of one side into LDS with direct 16-byte loads.  Plain: [BT rows][4 units of 16 bytes], unit u of
-// row r at u ^ row_swizzle(r): 16-byte reads go 16 lanes at a time, lanes 0-3, 12-15, 20-23, 24-27 together, then 4-11,
+// row r at u ^ row_swizzle(r / 4) (r / 8: EIGHT): 16-byte reads go 16 lanes at a time, lanes 0-3, 12-15, 20-23, 24-27 together, then 4-11,
 // 16-19, 28-31, and so on (u ^ (r >> 2 & 3) measured two cycles for one).  Transposed: [32 k][BT / 8 units], pairs of units xor-ed with (k & 3) | (k >> 3 & 1) << 2.
 // Both keep the fragment reads free of bank conflicts.
 constexpr int BK = 32;
 constexpr int64_t HEAD_MAX_LD = 1 << 20;
 
-__device__ __forceinline__ int row_swizzle(int row) { return 0x78 >> (row >> 2 & 3) * 2 & 3; }  // 0, 2, 3, 1
+__device__ __forceinline__ int row_swizzle(int row) { return 0x78 >> (row & 3) * 2 & 3; }  // 0, 2, 3, 1
 
 __device__ __forceinline__ unsigned lds_offset(const void* p) {
   return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
@@ -150,7 +150,9 @@ __device__ __forceinline__ void load_lds16(const void* base, unsigned off, unsig
   asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(dst), "i"(more), "v"(off), "s"(base)
                : "memory", "scc");
 }
-template <int BT, int NW, bool TR>
+// EIGHT: the fragments of a plain side take their 16 rows as 4 of each 8, two fragments sharing 32 rows, so that a lane's
+// results of such a pair are eight neighbours.
+template <int BT, int NW, bool TR, bool EIGHT>
 struct Stager {
   static constexpr int PIECES = BT / 16;                          // of 1 KiB
   static constexpr int CW = PIECES > NW ? PIECES / NW : 1;        // pieces per wave (some twice where waves outnumber them)
@@ -158,7 +160,7 @@ struct Stager {
   const char* base;    // of the tile at k = 0 (the same for every lane)
   unsigned piece[CW];  // where this wave's pieces go in the first stage (LDS bytes)
   unsigned off[CW];    // bytes from there to this lane's 16, 32 bits (leading dimensions are at most HEAD_MAX_LD)
-  int k_of;            // of this lane's first 16 bytes; transposed: 64 / U more for each piece
+  int k_of[CW];        // the (first) k of those
   __device__ __forceinline__ void init(const Side& s, int r0, const void* lds, int wave, int lane) {
     base = (const char*)(TR ? s.base : s.base + (int64_t)r0 * s.ld);
 #pragma unroll
@@ -167,12 +169,12 @@ struct Stager {
       piece[q] = lds_offset(lds) + c * 1024;
       if (!TR) {
         const int row = 16 * c + (lane >> 2);
-        k_of = ((lane & 3) ^ row_swizzle(row)) * 8;
-        off[q] = (unsigned)min(row, s.rlim - 1 - r0) * (unsigned)s.ld * 2 + k_of * 2;
+        k_of[q] = ((lane & 3) ^ row_swizzle(row >> (EIGHT ? 3 : 2))) * 8;
+        off[q] = (unsigned)min(row, s.rlim - 1 - r0) * (unsigned)s.ld * 2 + k_of[q] * 2;
       } else {
         const int k = c * (64 / U) + lane / U, d = lane % U;
         const int f = ((k & 3) | ((k >> 3 & 1) << 2)) & (U / 2 - 1);
-        if (q == 0) k_of = k;
+        k_of[q] = k;
         off[q] = (unsigned)k * (unsigned)s.ld * 2 + (unsigned)min(r0 / 8 + (d ^ (f << 1)), s.rlim / 8 - 1) * 16;
       }
     }
@@ -192,7 +194,7 @@ struct Stager {
     if (have < LEAST) at -= (LEAST - have) * ld * 2, have = LEAST;
 #pragma unroll
     for (int q = 0; q < CW; ++q) {
-      const int behind = k_of + (TR ? q * (64 / U) : 0) + LEAST - have;
+      const int behind = k_of[q] + LEAST - have;
       load_lds16(at, off[q] - (unsigned)max(0, behind) * (unsigned)ld * 2, piece[q], STAGE * BT * 64);
     }
   }
@@ -200,12 +202,13 @@ struct Stager {
 
 typedef __attribute__((address_space(3))) const s16x8 lds_s16x8;
 
-template <int BT, bool TR>
+template <int BT, bool TR, bool EIGHT>
 struct Reader {
   unsigned at;  // LDS bytes of this lane's share of fragment 0 in the first stage
   __device__ __forceinline__ void init(const void* lds, int w0, int lane) {
     if (!TR) {
-      at = (w0 + (lane & 15)) * 64 + ((lane >> 4) ^ row_swizzle(lane)) * 16;
+      const int r = lane & 15;
+      at = (w0 + (EIGHT ? (r >> 2) * 8 + (r & 3) : r)) * 64 + ((lane >> 4) ^ row_swizzle(r >> 2)) * 16;
     } else {
       const int g = lane >> 4, q = (lane & 15) >> 2, f = (q | ((g & 1) << 2)) & (BT / 16 - 1);
       at = (8 * g + q) * (BT * 2) + (((w0 / 16) ^ f) << 5) + (lane & 3) * 8;
@@ -213,12 +216,12 @@ struct Reader {
     at += lds_offset(lds);
     asm("" : "+v"(at));  // one register: the reads' own offsets reach all stages
   }
-  // fragment i: 16 rows from w0 + 16 i, 32 k
+  // fragment i: 16 rows from w0 + 16 i (EIGHT: of the 32 from w0 + 32 (i / 2)), 32 k
   __device__ __forceinline__ s16x8 get(int stage, int i) const {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"
     if (!TR) {
-      return *(lds_s16x8*)(at + stage * BT * 64 + i * 1024);
+      return *(lds_s16x8*)(at + stage * BT * 64 + (EIGHT ? (i >> 1) * 2048 + (i & 1) * 256 : i * 1024));
     } else {
       const unsigned a = (at ^ (i << 5)) + stage * BT * 64;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
@@ -249,12 +252,13 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  Stager<BM, NW, TRA> sa;
-  Stager<BN, NW, TRB> sb;
+  constexpr bool EIGHT = !TRA && FI % 2 == 0;
+  Stager<BM, NW, TRA, EIGHT> sa;
+  Stager<BN, NW, TRB, false> sb;
   sa.init(g.A, m0, lds_a, wave, lane);
   sb.init(g.B, n0, lds_b, wave, lane);
-  Reader<BM, TRA> ra;
-  Reader<BN, TRB> rb;
+  Reader<BM, TRA, EIGHT> ra;
+  Reader<BN, TRB, false> rb;
   ra.init(lds_a, wm * WTM, lane);
   rb.init(lds_b, wn * WTN, lane);
 
@@ -298,7 +302,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   // fragments are read from LDS, two more tiles are in flight and the loads of the fourth go into the stage that the
   // step's own fragments came from.  One barrier a step: behind it the tile after next has landed for every wave, and
   // nobody still reads the stage that the next loads overwrite.
-  constexpr int LOADS = Stager<BM, NW, TRA>::CW + Stager<BN, NW, TRB>::CW;
+  constexpr int LOADS = sa.CW + sb.CW;
   s16x8 a0[FI], b0[FJ], a1[FI], b1[FJ];
   // Fragments of the next tile are read in the order b, the last two rows of a, the other rows of a: those go into the
   // registers of rows that are done with.
@@ -351,17 +355,27 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   }
   mfma_done(acc);
 
-  // acc[i][j][r]: m = .. + 16 i + 4 (lane / 16) + r, n = .. + 16 j + lane % 16 -- a lane holds four neighbours along m
-  const int mw = m0 + wm * WTM + 4 * (lane >> 4), nw = n0 + wn * WTN + (lane & 15);
+  // acc[i][j][r]: n = .. + 16 j + lane % 16, m = .. + 16 i + 4 (lane / 16) + r (EIGHT: .. + 32 (i / 2) + 8 (lane / 16) +
+  // 4 (i % 2) + r) -- a lane holds four or eight neighbours along m
+  const int mw = m0 + wm * WTM + (EIGHT ? 8 : 4) * (lane >> 4), nw = n0 + wn * WTN + (lane & 15);
+  const auto m_of = [&](int i) { return mw + (EIGHT ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i); };
   if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
-    float bias[FI][4];
+    // in units of the exponential: natural for f32, of two for the 16-bit types
+    const float unit = T::PLANES == 3 ? 1.f : 1.4426950408889634f, scale = g.inv_tau * unit;
+    float bias[FI][4];  // times scale; -inf behind the last class
 #pragma unroll
     for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = min(mw + 16 * i + r, g.M - 1);
-        bias[i][r] = !g.bias ? 0.f : T::PLANES == 3 ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m];
-      }
+      for (int r = 0; r < 4; ++r) bias[i][r] = m_of(i) + r < g.M ? 0.f : -INFINITY;
+    if (g.bias) {
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = min(m_of(i) + r, g.M - 1);
+          bias[i][r] += scale * (T::PLANES == 3 ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m]);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
       const int n = nw + 16 * j;
@@ -371,10 +385,8 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
         for (int i = 0; i < FI; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float u = (acc[i][j][r] + bias[i][r]) * g.inv_tau;
-            u = mw + 16 * i + r < g.M ? u : -INFINITY;
-            acc[i][j][r] = u;
-            top = fmaxf(top, u);
+            acc[i][j][r] = fmaf(acc[i][j][r], scale, bias[i][r]);
+            top = fmaxf(top, acc[i][j][r]);
           }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -386,30 +398,31 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
           for (int r = 0; r < 4; ++r) sum += head_exp<T>(acc[i][j][r] - ref);  // a NaN stays in the sum
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        if (lane < 16 && n < N) g.stats[(int64_t)(tm * WM + wm) * g.stat_ld + n] = make_float2(top, sum);
-      } else {
+        if (lane < 16 && n < N) g.stats[(int64_t)(tm * WM + wm) * g.stat_ld + n] = make_float2(top / unit, sum);
+      } else if (m0 + wm * WTM < g.ldz) {  // all or nothing of a wave's columns: ldz is a multiple of K_PAD
         const bool live = n < N;
-        const float lse = live ? g.lse[n] : 0.f, cp = live ? g.cp[n] : 0.f;
+        const float lse = live ? g.lse[n] * unit : 0.f, cp = live ? g.cp[n] : 0.f;
+        short* out = g.dz + (int64_t)n * g.ldz;
+        constexpr int GROUP = EIGHT ? 2 : 1;
 #pragma unroll
-        for (int i = 0; i < FI; ++i) {
-          const int m = mw + 16 * i;
-          s16x4 w[T::PLANES];
+        for (int i0 = 0; i0 < FI; i0 += GROUP) {
+          short w[T::PLANES][4 * GROUP];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float u = (acc[i][j][r] + bias[i][r]) * g.inv_tau;
+          for (int e = 0; e < 4 * GROUP; ++e) {
+            const int i = i0 + e / 4, r = e % 4;
             // Rounded to the 16-bit type (half a step, 2^-8 bf16 / 2^-11 f16, of each element; f16 after scaling by a
             // power of two): the size of the rounding that the gradients themselves get.  f32: three exact planes.
-            float x = live && m + r < g.M ? cp * head_exp<T>(u - lse) : 0.f;
+            float x = cp * head_exp<T>(fmaf(acc[i][j][r], scale, bias[i][r]) - lse);
+            x = live ? x : 0.f;
 #pragma unroll
             for (int pl = 0; pl < T::PLANES; ++pl) {
               const short h = to16<T>(x);
-              w[pl][r] = h;
+              w[pl][e] = h;
               x -= (float)__builtin_bit_cast(typename T::t, h);
             }
           }
-          if (m < g.ldz)
 #pragma unroll
-            for (int pl = 0; pl < T::PLANES; ++pl) *(s16x4*)(g.dz + pl * g.dz_plane + (int64_t)n * g.ldz + m) = w[pl];
+          for (int pl = 0; pl < T::PLANES; ++pl) __builtin_memcpy(out + pl * g.dz_plane + m_of(i0), w[pl], 8 * GROUP);
         }
       }
     }
@@ -423,7 +436,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
       const int64_t orow = (int64_t)(g.rowmap ? g.rowmap[n] : n) * g.out_ld;
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
-        const int m = mw + 16 * i;
+        const int m = m_of(i);
         f32x4 x = acc[i][j];
         if (m >= g.M) continue;
         if (g.out_kind != OUT_FINAL) {  // acc rows are padded to a multiple of 4
