@@ -179,24 +179,20 @@ struct Stager {
       }
     }
   }
-  // the tile at `at` = base + its k (and plane), into stage STAGE
+  // piece q of the tile at `at` = base + its k (and plane), into stage STAGE
   template <int STAGE>
-  __device__ __forceinline__ void issue(const char* at) const {
-#pragma unroll
-    for (int q = 0; q < CW; ++q) load_lds16(at, off[q], piece[q], STAGE * BT * 64);
+  __device__ __forceinline__ void issue(const char* at, int q) const {
+    load_lds16(at, off[q], piece[q], STAGE * BT * 64);
   }
-  // a tile of which only `have` k exist (0 or fewer: none): the last ones again in the place of the others.  The base goes
-  // back to where the tile holds one, so that the lanes' offsets, which only shrink, never fall below zero.
+  // of a tile of which only `have` k exist (0 or fewer: none): the last ones again in the place of the others.  The base
+  // goes back to where the tile holds one, so that the lanes' offsets, which only shrink, never fall below zero.
   template <int STAGE>
-  __device__ __forceinline__ void issue_ragged(const Side& s, const char* at, int have) const {
+  __device__ __forceinline__ void issue_ragged(const Side& s, const char* at, int have, int q) const {
     constexpr int LEAST = TR ? 1 : 8;
     const int64_t ld = TR ? s.ld : 1;
     if (have < LEAST) at -= (LEAST - have) * ld * 2, have = LEAST;
-#pragma unroll
-    for (int q = 0; q < CW; ++q) {
-      const int behind = k_of[q] + LEAST - have;
-      load_lds16(at, off[q] - (unsigned)max(0, behind) * (unsigned)ld * 2, piece[q], STAGE * BT * 64);
-    }
+    const int behind = k_of[q] + LEAST - have;
+    load_lds16(at, off[q] - (unsigned)max(0, behind) * (unsigned)ld * 2, piece[q], STAGE * BT * 64);
   }
 };
 
@@ -282,13 +278,14 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   };
   aim();
   int left = t1 - t0;  // tiles that are still to be issued; behind the last one it is issued again, for the count of loads
-  const auto issue = [&](auto stage) {
-    if (kt * BK + BK <= g.A.klim)
-      sa.template issue<stage>(at_a);
+  const auto issue = [&](auto stage, int q) {
+    if (q >= sa.CW)
+      sb.template issue<stage>(at_b, q - sa.CW);
+    else if (kt * BK + BK <= g.A.klim)
+      sa.template issue<stage>(at_a, q);
     else
-      sa.template issue_ragged<stage>(g.A, at_a, g.A.klim - kt * BK);
-    sb.template issue<stage>(at_b);
-    if (--left > 0) {
+      sa.template issue_ragged<stage>(g.A, at_a, g.A.klim - kt * BK, q);
+    if (q == sa.CW + sb.CW - 1 && --left > 0) {
       at_a += step_a;
       at_b += step_b;
       if (++kt == ktiles && T::PLANES == 3) {
@@ -297,6 +294,10 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
         aim();
       }
     }
+  };
+  const auto issue_all = [&](auto stage) {
+#pragma unroll
+    for (int q = 0; q < sa.CW + sb.CW; ++q) issue(stage, q);
   };
   // Four stages of 32 k: while a step's matrix instructions run on fragments that are in registers, the next step's
   // fragments are read from LDS, two more tiles are in flight and the loads of the fourth go into the stage that the
@@ -321,8 +322,8 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // Each row of matrix instructions takes its share of the next tile's reads along; nothing moves across rows, so that
-  // neither the reads nor the loads hold up both waves of a SIMD at once.
+  // Each row of matrix instructions takes its share of the next tile's reads and of the loads along, and nothing moves
+  // across rows: all waves' loads in one place would queue up (16 cycles each) with the matrix units idle behind them.
   const auto step = [&](auto stage, const s16x8(&a)[FI], const s16x8(&b)[FJ], s16x8(&an)[FI], s16x8(&bn)[FJ]) {
 #pragma unroll
     for (int i = 0; i < FI; ++i) {
@@ -332,15 +333,17 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
 #pragma unroll
       for (int j = 0; j < FJ; ++j) T::mfma(acc[i][j], a[i], b[j]);
       __builtin_amdgcn_sched_barrier(0);
-      if (i == 0) issue(stage);
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q)
+        if (q * FI / LOADS == i) issue(stage, q);
     }
     step_barrier();
   };
   if (t0 < t1) {
-    issue(std::integral_constant<int, 0>());
-    issue(std::integral_constant<int, 1>());
-    issue(std::integral_constant<int, 2>());
-    issue(std::integral_constant<int, 3>());
+    issue_all(std::integral_constant<int, 0>());
+    issue_all(std::integral_constant<int, 1>());
+    issue_all(std::integral_constant<int, 2>());
+    issue_all(std::integral_constant<int, 3>());
     step_barrier();
 #pragma unroll
     for (int f = 0; f < FRAGS; ++f) fetch(f, 0, a0, b0);
