@@ -75,7 +75,8 @@ __device__ __forceinline__ float head_exp(float x) {
   return T::PLANES == 3 ? expf(x) : __builtin_amdgcn_exp2f(x);
 }
 
-constexpr int K_PAD = 128;     // contractions run in whole groups of four steps of 32
+constexpr int K_PAD = 64;      // packed operands hold zeros up to a multiple of this along the contraction
+constexpr int DZ_PAD = 128;    // rows of dz
 constexpr int HEAD_PAD = 256;  // packed rows are padded to a multiple of the largest tile
 
 // One side of a product.  Plain side: element (r, k) at base[r * ld + k]; transposed side: base[k * ld + r].  Rows behind
@@ -241,9 +242,9 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   // dz is an operand of the next products: rows up to a multiple of K_PAD are written, as zeros
   if (n0 >= (EPI == EPI_DZ ? (N + K_PAD - 1) / K_PAD * K_PAD : N)) return;
   const int K = g.k_dev ? min(g.K, *g.k_dev) : g.K;
-  const int ktiles = (K + K_PAD - 1) / K_PAD * (K_PAD / BK);
+  const int ktiles = (K + BK - 1) / BK;
   const int total = ktiles * (T::PLANES == 3 ? 6 : 1);
-  const int per = (total / 4 + g.splits - 1) / g.splits * 4;
+  const int per = (total + g.splits - 1) / g.splits;
   const int t0 = min(split * per, total), t1 = min(t0 + per, total);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -348,11 +349,15 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
 #pragma unroll
     for (int f = 0; f < FRAGS; ++f) fetch(f, 0, a0, b0);
     step_barrier();  // every wave has read the first stage, which the first step overwrites
-    for (int t = t0; t < t1; t += 4) {
+    for (int t = t0;; t += 4) {
       step(std::integral_constant<int, 0>(), a0, b0, a1, b1);
+      if (t + 1 >= t1) break;
       step(std::integral_constant<int, 1>(), a1, b1, a0, b0);
+      if (t + 2 >= t1) break;
       step(std::integral_constant<int, 2>(), a0, b0, a1, b1);
+      if (t + 3 >= t1) break;
       step(std::integral_constant<int, 3>(), a1, b1, a0, b0);
+      if (t + 4 >= t1) break;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles issued again
   }
@@ -362,6 +367,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   // 4 (i % 2) + r) -- a lane holds four or eight neighbours along m
   const int mw = m0 + wm * WTM + (EIGHT ? 8 : 4) * (lane >> 4), nw = n0 + wn * WTN + (lane & 15);
   const auto m_of = [&](int i) { return mw + (EIGHT ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i); };
+  static_assert(DZ_PAD % WTM == 0);
   if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
     // in units of the exponential: natural for f32, of two for the 16-bit types
     const float unit = T::PLANES == 3 ? 1.f : 1.4426950408889634f, scale = g.inv_tau * unit;
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
         if (lane < 16 && n < N) g.stats[(int64_t)(tm * WM + wm) * g.stat_ld + n] = make_float2(top / unit, sum);
-      } else if (m0 + wm * WTM < g.ldz) {  // all or nothing of a wave's columns: ldz is a multiple of K_PAD
+      } else if (m0 + wm * WTM < g.ldz) {  // all or nothing of a wave's columns, of which DZ_PAD is a multiple
         const bool live = n < N;
         const float lse = live ? g.lse[n] * unit : 0.f, cp = live ? g.cp[n] : 0.f;
         short* out = g.dz + (int64_t)n * g.ldz;
@@ -564,57 +570,92 @@ __global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__
 }
 
 // ---- the loss of each row -------------------------------------------------------------------------------
-// One block per 16 packed rows: joins the tiles' (maximum, sum) pairs into lse, takes the targets' logits as dot
-// products of the inputs (32-bit accumulation), and writes the row's loss to its own place.
+// The targets' logits u = (hidden . weight[at] + bias) / tau as dot products of the inputs, in 32 bits: a wave for eight
+// targets of a packed row, their weight rows in flight together.  Bound by the gathered rows' bytes.
+constexpr int DOTS = 8;
 template <int DT>
-__global__ __launch_bounds__(256) void head_finish_kernel(const void* __restrict__ hidden, int64_t ldh, const void* __restrict__ weight,
-                                                          int64_t ldw, const void* __restrict__ bias, int d,
-                                                          const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
-                                                          const int* __restrict__ rows, const int* __restrict__ count,
-                                                          float* __restrict__ lse, float* __restrict__ uk, float* __restrict__ loss) {
-  __shared__ float sh_top[16][17], sh_sum[16][17], sh_lse[16];
+__global__ __launch_bounds__(256) void head_dots_kernel(const void* __restrict__ hidden, int64_t ldh, const void* __restrict__ weight,
+                                                        int64_t ldw, const void* __restrict__ bias, int d, Targets tg, int groups,
+                                                        const int* __restrict__ rows, const int* __restrict__ count,
+                                                        float* __restrict__ uk) {
+  typedef typename Elem<DT>::t E;
+  constexpr int V = Elem<DT>::PER16;
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int i = unit / groups, k0 = unit % groups * DOTS;
+  if (i >= *count) return;
+  const int64_t src = rows[i];
+  const E* h = (const E*)hidden + src * ldh;
+  const E* w[DOTS];
+  float s[DOTS];
+  bool vec = (((uintptr_t)h | (uintptr_t)weight) & 15) == 0 && ldw % V == 0, any = false;
+#pragma unroll
+  for (int q = 0; q < DOTS; ++q) {
+    const int at = k0 + q < tg.k ? tg.at[src * tg.k + k0 + q] : -1;
+    any |= at >= 0;
+    w[q] = (const E*)weight + (int64_t)max(at, 0) * ldw;
+    s[q] = 0.f;
+  }
+  if (any) {
+    int c = vec ? lane * V : d;
+    for (; c + V <= d; c += 64 * V) {
+      float x[V];
+      unpack16<DT>(*(const vec4f*)(h + c), x);
+#pragma unroll
+      for (int q = 0; q < DOTS; ++q) {
+        if (k0 + q >= tg.k) break;
+        float y[V];
+        unpack16<DT>(*(const vec4f*)(w[q] + c), y);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[q] = fmaf(x[e], y[e], s[q]);
+      }
+    }
+    for (c = (vec ? d / V * V : 0) + lane; c < d; c += 64)
+      for (int q = 0; q < DOTS && k0 + q < tg.k; ++q) s[q] = fmaf((float)h[c], (float)w[q][c], s[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < DOTS; ++q) {
+    if (k0 + q >= tg.k) break;
+    const float u = wave_sum_f32(s[q]);
+    const int at = tg.at[src * tg.k + k0 + q];
+    if (lane == 0) uk[(int64_t)i * tg.k + k0 + q] = at < 0 ? 0.f : (u + (bias ? Elem<DT>::load(bias, at) : 0.f)) * tg.inv_tau;
+  }
+}
+
+// 16 packed rows a block: joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.
+constexpr int FINISH_NT = 1024;
+__global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
+                                                                const int* __restrict__ rows, const int* __restrict__ count,
+                                                                float* __restrict__ lse, const float* __restrict__ uk,
+                                                                float* __restrict__ loss) {
+  constexpr int PARTS = FINISH_NT / 16;
+  __shared__ float sh_top[16][PARTS + 1], sh_sum[16][PARTS + 1];
   const int i0 = blockIdx.x * 16, n = *count;
   if (i0 >= n) return;
   const int r = threadIdx.x & 15, part = threadIdx.x >> 4;
   float top = -INFINITY, sum = 0.f;
   if (i0 + r < n)
-    for (int t = part; t < tiles; t += 16) {
+#pragma unroll 4
+    for (int t = part; t < tiles; t += PARTS) {
       const float2 x = stats[(int64_t)t * stat_ld + i0 + r];
       join(top, sum, x.x, x.y);
     }
   sh_top[r][part] = top;
   sh_sum[r][part] = sum;
   __syncthreads();
-  if (threadIdx.x < 16) {
-    top = sh_top[threadIdx.x][0], sum = sh_sum[threadIdx.x][0];
-    for (int p = 1; p < 16; ++p) join(top, sum, sh_top[threadIdx.x][p], sh_sum[threadIdx.x][p]);
-    const float l = top + logf(sum);
-    sh_lse[threadIdx.x] = l;
-    if (i0 + (int)threadIdx.x < n) lse[i0 + threadIdx.x] = l;
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rn = min(16, n - i0);
-  for (int q = wave; q < rn * tg.k; q += 4) {
-    const int i = i0 + q / tg.k, k = q % tg.k;
-    const int64_t src = rows[i];
-    const int at = tg.at[src * tg.k + k];
-    float u = 0.f;
-    if (at >= 0) {
-      u = wave_dot<DT>(hidden, src * ldh, weight, (int64_t)at * ldw, d, lane);
-      if (bias) u += Elem<DT>::load(bias, at);
-      u *= tg.inv_tau;
-    }
-    if (lane == 0) uk[(int64_t)i * tg.k + k] = u;
-  }
-  __syncthreads();
-  for (int q = wave; q < rn; q += 4) {
-    const int i = i0 + q;
-    const int64_t src = rows[i];
-    double s = 0.0;
-    for (int k = lane; k < tg.k; k += 64) s += target_term(tg, src, k, uk[(int64_t)i * tg.k + k], sh_lse[q]);
-    s = wave_sum_f64(s);
-    if (lane == 0) loss[src] = (float)(s * tg.tau2);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;  // a wave a row
+  const int i = i0 + wave;
+  if (i >= n) return;
+  top = sh_top[wave][lane], sum = sh_sum[wave][lane];
+  const float all = wave_max_f32(top), ref = all == -INFINITY ? 0.f : all;
+  sum = wave_sum_f32(sum * expf(top - ref));
+  const float l = all + logf(sum);
+  const int64_t src = rows[i];
+  double s = 0.0;
+  for (int k = lane; k < tg.k; k += 64) s += target_term(tg, src, k, uk[(int64_t)i * tg.k + k], l);
+  s = wave_sum_f64(s);
+  if (lane == 0) {
+    lse[i] = l;
+    loss[src] = (float)(s * tg.tau2);
   }
 }
 
@@ -699,28 +740,49 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int
   }
 }
 
-// dbias of a piece: column sums of dz over the packed rows; 64 columns a block, 4 waves over the rows
+// dbias of a piece: column sums of dz over stretches of BIAS_ROWS packed rows (256 columns a block, 8 a thread), joined in
+// order by head_bias_join_kernel.  Bound by the read of dz.
+constexpr int BIAS_ROWS = 256;
 template <class T>
-__global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int planes,
-                                                        const int* __restrict__ count, int cols, const float* __restrict__ inv_scale,
-                                                        void* __restrict__ out, int out_f32) {
-  __shared__ float sh[4][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
-  const int n = *count;
-  float s = 0.f;
-  if (c < cols)
-    for (int i = part; i < n; i += 4)
-      for (int pl = 0; pl < planes; ++pl)
-        s += (float)__builtin_bit_cast(typename T::t, dz[pl * dz_plane + (int64_t)i * ldz + c]);
-  sh[part][threadIdx.x & 63] = s;
+__global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int cols,
+                                                        const int* __restrict__ count, float* __restrict__ part) {
+  __shared__ float sh[8][256 + 8];
+  const int c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8, group = threadIdx.x >> 5;
+  const int r0 = blockIdx.y * BIAS_ROWS, r1 = min(*count, r0 + BIAS_ROWS);
+  if (r0 >= r1) return;
+  float s[8] = {};
+  if (c0 < ldz)
+#pragma unroll 4
+    for (int r = r0 + group; r < r1; r += 8)
+#pragma unroll
+      for (int pl = 0; pl < T::PLANES; ++pl) {
+        const s16x8 x = *(const s16x8*)(dz + pl * dz_plane + (int64_t)r * ldz + c0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += (float)__builtin_bit_cast(typename T::t, (short)x[e]);
+      }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sh[group][(threadIdx.x & 31) * 8 + e] = s[e];
   __syncthreads();
-  if (part == 0 && c < cols) {
-    s = ((sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x])) * *inv_scale;
-    if (out_f32)
-      ((float*)out)[c] = s;
-    else
-      ((short*)out)[c] = to16<T>(s);
-  }
+  float sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sum += sh[q][threadIdx.x];
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < cols) part[(int64_t)blockIdx.y * cols + c] = sum;
+}
+template <class T>
+__global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __restrict__ part, int cols, const int* __restrict__ count,
+                                                             const float* __restrict__ inv_scale, void* __restrict__ out) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  const int stretches = (*count + BIAS_ROWS - 1) / BIAS_ROWS;
+  float s = 0.f;
+#pragma unroll 8
+  for (int q = 0; q < stretches; ++q) s += part[(int64_t)q * cols + c];
+  s *= *inv_scale;
+  if (T::PLANES == 3)
+    ((float*)out)[c] = s;
+  else
+    ((short*)out)[c] = to16<T>(s);
 }
 
 // out = (sum of the splits' partial sums, in order, + acc) * inv_scale, or acc = that sum
@@ -1074,9 +1136,15 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
 
 template <int DT>
 static void finish(const nif_head_desc* h, const Plan& p, char* state, const float2* stats, int tiles, float* row_loss, hipStream_t st) {
-  hipLaunchKernelGGL(head_finish_kernel<DT>, dim3((unsigned)((p.n + 15) / 16)), dim3(256), 0, st, h->hidden, h->ldh, h->weight, h->ldw,
-                     h->bias, p.d, stats, p.cap, tiles, targets_of(h, p, state), (const int*)(state + p.s_rows),
-                     (const int*)(state + p.s_count), (float*)(state + p.s_lse), (float*)(state + p.s_uk), row_loss);
+  const Targets tg = targets_of(h, p, state);
+  const int* rows = (const int*)(state + p.s_rows);
+  const int* count = (const int*)(state + p.s_count);
+  float* uk = (float*)(state + p.s_uk);
+  const int groups = (p.k + DOTS - 1) / DOTS;
+  hipLaunchKernelGGL(head_dots_kernel<DT>, dim3((unsigned)((p.n * groups + 3) / 4)), dim3(256), 0, st, h->hidden, h->ldh, h->weight, h->ldw,
+                     h->bias, p.d, tg, groups, rows, count, uk);
+  hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg, rows, count,
+                     (float*)(state + p.s_lse), uk, row_loss);
 }
 
 struct BwdSpace {
@@ -1087,7 +1155,7 @@ struct BwdSpace {
 };
 static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
-  b.ldz = round_up(p.piece, K_PAD);
+  b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
   b.dh = shape_of(p.d, p.n);
   b.dw = shape_of(p.d, p.piece);
@@ -1103,7 +1171,9 @@ static BwdSpace backward_space(const Plan& p) {
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
   const size_t part_h = b.dh_splits > 1 ? (size_t)b.dh_splits * p.cap * b.dh_ld * 4 : 0;
   const size_t part_w = b.dw_splits > 1 ? (size_t)b.dw_splits * p.piece * b.dh_ld * 4 : 0;
-  b.part = take(at, part_h > part_w ? part_h : part_w);
+  const size_t part_b = (size_t)((p.n + BIAS_ROWS - 1) / BIAS_ROWS) * p.piece * 4;
+  const size_t part = part_h > part_w ? part_h : part_w;
+  b.part = take(at, part > part_b ? part : part_b);
   b.bytes = at;
   return b;
 }
@@ -1151,9 +1221,13 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     if (p.n > 0)
       hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
                        v0 + vc, dz, dz_plane, b.ldz, p.planes);
-    if (dbias)
-      hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 63) / 64), dim3(256), 0, st, dz, dz_plane, b.ldz, p.planes, count, vc, inv_scale,
-                         (char*)dbias + (size_t)v0 * (f32 ? 4 : 2), f32);
+    if (dbias) {
+      if (p.n > 0)
+        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, (unsigned)((p.n + BIAS_ROWS - 1) / BIAS_ROWS)), dim3(256), 0, st, dz,
+                           dz_plane, b.ldz, vc, count, part);
+      hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, inv_scale,
+                         (char*)dbias + (size_t)v0 * (f32 ? 4 : 2));
+    }
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
       GemmArgs g = {};
       g.A = Side{hp, p.cap * p.ldd, p.ldd, p.ldd, (int)p.cap};

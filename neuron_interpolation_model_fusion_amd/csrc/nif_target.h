@@ -75,30 +75,6 @@ __device__ __forceinline__ float wave_sum_f32(float x) {
   return x;
 }
 
-// a . b over d elements by one wave, in 32 bits
-template <int DT>
-__device__ __forceinline__ float wave_dot(const void* a, int64_t ao, const void* b, int64_t bo, int d, int lane) {
-  constexpr int V = Elem<DT>::PER16;
-  typedef typename Elem<DT>::t t;
-  const t* pa = (const t*)a + ao;
-  const t* pb = (const t*)b + bo;
-  float s = 0.f;
-  if ((((uintptr_t)pa | (uintptr_t)pb) & 15) == 0) {
-    int c = lane * V;
-    for (; c + V <= d; c += 64 * V) {
-      float x[V], y[V];
-      unpack16<DT>(*(const vec4f*)(pa + c), x);
-      unpack16<DT>(*(const vec4f*)(pb + c), y);
-#pragma unroll
-      for (int e = 0; e < V; ++e) s = fmaf(x[e], y[e], s);
-    }
-    for (int e = 0; e < V && c + e < d; ++e) s = fmaf((float)pa[c + e], (float)pb[c + e], s);
-  } else {
-    for (int c = lane; c < d; c += 64) s = fmaf((float)pa[c], (float)pb[c], s);
-  }
-  return wave_sum_f32(s);
-}
-
 // one target's term of a row's loss / tau^2; an entry of no weight adds nothing, whatever its logit is
 __device__ __forceinline__ double target_term(const Targets& t, int64_t row, int k, float u, float lse) {
   const float p = t.p[row * t.k + k];
