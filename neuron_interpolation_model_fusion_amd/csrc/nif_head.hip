@@ -119,11 +119,14 @@ struct GemmArgs {
   const float* inv_scale;
 };
 
-// blockIdx -> tile: blocks b and b + 8 share an XCD (and its L2), so each XCD takes a contiguous range of ids; inside,
-// tiles go in groups of 8 along n for each step along m, so that the blocks in flight on an XCD share their panels.
-__device__ __forceinline__ void tile_of(int id, int total, int mt, int nt, int& tm, int& tn) {
+// blockIdx -> split and tile: blocks b and b + 8 share an XCD (and its L2), so each XCD takes a contiguous range of ids --
+// with eight splits, a stretch of the contraction of its own.  Inside, tiles go in groups of 8 along n for each step along
+// m, so that the blocks in flight on an XCD share their panels.
+__device__ __forceinline__ void tile_of(int id, int total, int mt, int nt, int& split, int& tm, int& tn) {
   const int q = total >> 3, rr = total & 7, xcd = id & 7;
-  const int wg = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + (id >> 3);
+  int wg = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + (id >> 3);
+  split = wg / (mt * nt);
+  wg -= split * mt * nt;
   const int G = 8;
   const int group = wg / (G * mt), first = group * G;
   const int width = min(G, nt - first);
@@ -234,9 +237,8 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
   __shared__ __attribute__((aligned(1024))) char lds_a[4][BM * 64];
   __shared__ __attribute__((aligned(1024))) char lds_b[4][BN * 64];
-  const int split = blockIdx.x / (g.mt * g.nt);
-  int tm, tn;
-  tile_of(blockIdx.x % (g.mt * g.nt), g.mt * g.nt, g.mt, g.nt, tm, tn);
+  int split, tm, tn;
+  tile_of(blockIdx.x, gridDim.x, g.mt, g.nt, split, tm, tn);
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
   const int m0 = tm * BM, n0 = tn * BN;
   // dz is an operand of the next products: rows up to a multiple of K_PAD are written, as zeros
@@ -1041,14 +1043,35 @@ static Targets targets_of(const nif_head_desc* h, const Plan& p, char* state) {
   return t;
 }
 
+// Tile and split of a product, by what it would take: `rounds` of blocks that run at once, each its share of the k steps
+// (us a step, measured in the middle of long products with that many blocks on each CU) and a prologue and epilogue; a
+// split writes and reads its partial sums (f32, 4 TB/s).
 struct Shape {
-  int bm, bn, wm;
+  int bm, bn, wm, splits;
 };
-// tile of a product with extents m x n
-static Shape shape_of(int64_t m, int64_t n) {
-  if (n <= 32) return {128, 32, 4};
-  if (m >= 1024 && n >= 1024) return {256, 256, 2};
-  return {128, 128, 2};
+struct Tile {
+  int bm, bn, wm, slots;
+  float step, fixed;
+};
+static const Tile TILES[] = {
+    {256, 256, 2, 256, 0.85f, 8.f},
+    {128, 128, 2, 512, 0.52f, 5.f},
+    {128, 32, 4, 1024, 0.40f, 4.f},
+};
+static Shape shape_of(int64_t m, int64_t n, int64_t ksteps, bool may_split) {
+  Shape best = {128, 128, 2, 1};
+  float least = INFINITY;
+  for (const Tile& t : TILES) {
+    const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+    for (int splits = 1; splits <= (may_split ? 32 : 1); splits *= 2) {
+      if (splits > 1 && ksteps / splits < 8) break;
+      const float rounds = (float)((tiles * splits + t.slots - 1) / t.slots);
+      const float us = rounds * ((float)((ksteps + splits - 1) / splits) * t.step + t.fixed) +
+                       (splits > 1 ? 5.f + (float)splits * (float)m * (float)n * 8e-6f / 4.f : 0.f);
+      if (us < least) least = us, best = {t.bm, t.bn, t.wm, splits};
+    }
+  }
+  return best;
 }
 
 template <class T, bool TRA, bool TRB, int EPI>
@@ -1065,13 +1088,9 @@ static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
 }
 
-static int splits_for(const Shape& s, int64_t m, int64_t n, int64_t ktiles) {
-  const int64_t tiles = ((m + s.bm - 1) / s.bm) * ((n + s.bn - 1) / s.bn);
-  int64_t q = 512 / (tiles > 0 ? tiles : 1);  // no rows: no tiles
-  if (q > ktiles / 4) q = ktiles / 4;
-  if (q > 32) q = 32;
-  return (int)(q < 1 ? 1 : q);
-}
+static int pairs_of(const Plan& p) { return p.planes == 3 ? 6 : 1; }
+// of the products that make logits of a piece of `classes`
+static Shape logit_shape(const Plan& p, int classes) { return shape_of(classes, p.n, (p.d + BK - 1) / BK * pairs_of(p), false); }
 
 struct FwdSpace {
   size_t stats, w, bytes;
@@ -1079,7 +1098,7 @@ struct FwdSpace {
 static FwdSpace forward_space(const Plan& p) {
   FwdSpace f;
   size_t at = 0;
-  const Shape s = shape_of(p.v, p.n);
+  const Shape s = logit_shape(p, p.pack_w ? p.piece : p.v);
   const int64_t tiles = (p.v / s.bm + p.v / p.piece + 2) * s.wm;
   f.stats = take(at, (size_t)tiles * p.cap * 8);
   f.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * 2 * p.planes : 0);
@@ -1113,7 +1132,7 @@ static const void* bias_at(const nif_head_desc* h, int v0) {
 
 template <class T>
 static void forward_products(const nif_head_desc* h, const Plan& p, char* state, char* ws, const FwdSpace& f, int& tiles, hipStream_t st) {
-  const Shape s = shape_of(p.v, p.n);
+  const Shape s = logit_shape(p, p.pack_w ? p.piece : p.v);
   tiles = 0;
   for (int v0 = 0; v0 < p.v; v0 += p.pack_w ? p.piece : p.v) {
     const int vc = p.pack_w ? (p.v - v0 < p.piece ? p.v - v0 : p.piece) : p.v;
@@ -1150,18 +1169,14 @@ static void finish(const nif_head_desc* h, const Plan& p, char* state, const flo
 struct BwdSpace {
   size_t coef, cp, scale, dz, w, acc, part, bytes;
   int64_t ldz, dh_ld;
-  int dh_splits, dw_splits;
   Shape dh, dw;
 };
 static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
   b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
-  b.dh = shape_of(p.d, p.n);
-  b.dw = shape_of(p.d, p.piece);
-  const int pairs = p.planes == 3 ? 6 : 1;
-  b.dh_splits = splits_for(b.dh, p.d, p.n, b.ldz / 64 * pairs);
-  b.dw_splits = splits_for(b.dw, p.d, p.piece, (p.cap / 64) * pairs);
+  b.dh = shape_of(p.d, p.n, (p.piece + BK - 1) / BK * pairs_of(p), true);
+  b.dw = shape_of(p.d, p.piece, (p.n + BK - 1) / BK * pairs_of(p), true);
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
@@ -1169,8 +1184,8 @@ static BwdSpace backward_space(const Plan& p) {
   b.dz = take(at, (size_t)p.cap * b.ldz * 2 * p.planes);
   b.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * 2 * p.planes : 0);
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
-  const size_t part_h = b.dh_splits > 1 ? (size_t)b.dh_splits * p.cap * b.dh_ld * 4 : 0;
-  const size_t part_w = b.dw_splits > 1 ? (size_t)b.dw_splits * p.piece * b.dh_ld * 4 : 0;
+  const size_t part_h = b.dh.splits > 1 ? (size_t)b.dh.splits * p.cap * b.dh_ld * 4 : 0;
+  const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
   const size_t part_b = (size_t)((p.n + BIAS_ROWS - 1) / BIAS_ROWS) * p.piece * 4;
   const size_t part = part_h > part_w ? part_h : part_w;
   b.part = take(at, part > part_b ? part : part_b);
@@ -1216,7 +1231,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.dz = dz;
       g.dz_plane = dz_plane;
       g.ldz = b.ldz;
-      run_gemm<T, false, false, EPI_DZ>(shape_of(vc, p.n), g, st);
+      run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc), g, st);
     }
     if (p.n > 0)
       hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
@@ -1236,7 +1251,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.N = vc;
       g.K = (int)p.cap;
       g.k_dev = count;
-      g.splits = b.dw_splits;
+      g.splits = b.dw.splits;
       g.out = (char*)dweight + (size_t)v0 * lddw * (f32 ? 4 : 2);
       g.out_ld = lddw;
       g.inv_scale = inv_scale;
@@ -1262,7 +1277,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.N = (int)p.n;
       g.n_dev = count;
       g.K = kz;
-      g.splits = b.dh_splits;
+      g.splits = b.dh.splits;
       g.out = dhidden;
       g.out_ld = lddh;
       g.rowmap = rows;
