@@ -381,12 +381,13 @@ __device__ __forceinline__ void select_by_digits(const typename Elem<DT>::t* z, 
   }
 }
 
-// One block per row, one pass over it: a threshold that k elements of the first stretch reach (the k-th largest of the
-// threads' maxima) keeps all but about k of each stretch out of a list in LDS; when the list grows it is sorted, cut to k
-// and its last entry becomes the threshold.  Rows that this does not fit (more ties at the threshold than the list
-// holds, NaN) are selected by digits instead.  The log-sum-exp goes along.  Bound by the read of the logits.
+// One block per row, one pass over it.  The k-th largest of the threads' maxima so far is a bar that k elements reach, so
+// whatever comes later must exceed it; it is taken anew after 1, 2, 4, 8, .. stretches, which leaves about 6 k elements
+// of a row of 131072 (k log2 of the stretches) in a list in LDS.  The last bar cuts the list to little more than k, which are sorted.  Rows that
+// this does not fit (more than the list holds: ties at the bar, rising rows; NaN) are selected by digits instead.  The
+// log-sum-exp goes along.  Bound by the read of the logits and the exponentials.
 template <int DT, int NT>
-__global__ __launch_bounds__(NT) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,
+__global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,
                                                         void* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16, U = DT == NIF_F32 ? 4 : 2;
@@ -404,58 +405,62 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const void* __restrict__
     const int at = atomicAdd(&sh_n, 1);
     if (at < TOP_LIST) key[at] = key_of(x, c);
   };
-  // Sorts the list and cuts it to k; the first absent key is 0.
-  const auto cut = [&](int n) {
-    int p = 64;
-    while (p < n) p <<= 1;
-    for (int i = n + threadIdx.x; i < p; i += NT) key[i] = 0;
-    sort_keys<NT>(key, p);
-  };
   if ((int)threadIdx.x < r.loose()) {
     const float x[1] = {(float)r.z[r.loose_at(threadIdx.x)]};
     run.add(x, scale);
   }
-  float bar = -INFINITY;  // k entries of lower classes than any element to come reach it: those must exceed it
-  bool first = true, over = k > NT;
+  float bar = -INFINITY, mine = -INFINITY;
+  int stretch = 0;
   stream_row<DT, NT, U>(r, [&](const float (&x)[U * V], int base) {
     const float m = run.add(x, scale);
-    if (over) return;
-    if (first) bar = kth_largest<NT>(m, k, sh);
-    if (first ? m >= bar : m > bar) {
+    mine = fmaxf(mine, m);
+    const bool anew = k <= NT && (stretch & (stretch + 1)) == 0;
+    if (anew) bar = kth_largest<NT>(mine, k, sh);
+    // elements of this stretch may be among the k that reach a new bar; those behind it must exceed it
+    if (anew ? m >= bar : m > bar) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = base + u * NT + (int)threadIdx.x;
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if ((first ? x[u * V + e] >= bar : x[u * V + e] > bar) && i < r.vecs) put(x[u * V + e], r.head + i * V + e);
+          if ((anew ? x[u * V + e] >= bar : x[u * V + e] > bar) && i < r.vecs) put(x[u * V + e], r.head + i * V + e);
       }
     }
-    first = false;
-    __syncthreads();
-    const int n = sh_n;
-    over = n > TOP_LIST - 16;
-    if (!over && n > TOP_LIST / 2 - 256 && n > k) {
-      cut(n);
-      const unsigned o = (unsigned)(key[k - 1] >> 32);
-      bar = __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
-      __syncthreads();
-      if (threadIdx.x == 0) sh_n = k;
-    }
-    __syncthreads();
+    ++stretch;
   });
   const float l = run.template lse<NT>(scale, inv_tau, sh);
   __syncthreads();
   if (threadIdx.x == 0) lse[row] = l;
   // the row's loose ends (fewer than 16), whatever they are
-  if (!over && (int)threadIdx.x < r.loose()) put((float)r.z[r.loose_at(threadIdx.x)], r.loose_at(threadIdx.x));
+  if ((int)threadIdx.x < r.loose()) put((float)r.z[r.loose_at(threadIdx.x)], r.loose_at(threadIdx.x));
+  if (k <= NT && stretch > 0) bar = kth_largest<NT>(mine, k, sh);
   __syncthreads();
   int n = sh_n;
-  if (over || l != l || n < k) {  // l is NaN where the row holds NaN or +inf, which the comparisons above do not order
+  if (k > NT || n > TOP_LIST || l != l || n < k) {  // l is NaN where the row holds NaN or +inf, which floats do not order
     __syncthreads();
     select_by_digits<DT, NT>(r.z, classes, k, key, (unsigned*)sh, &sh_n);
     n = k;
+  } else if (n > 2 * k) {
+    unsigned long long mykeys[TOP_LIST / NT];
+    const unsigned long long least = (unsigned long long)order_of(bar) << 32;
+#pragma unroll
+    for (int q = 0; q < TOP_LIST / NT; ++q) {
+      const int at = q * NT + threadIdx.x;
+      mykeys[q] = at < n ? key[at] : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sh_n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < TOP_LIST / NT; ++q)
+      if (q * NT < n && mykeys[q] > least) key[atomicAdd(&sh_n, 1)] = mykeys[q];  // no key is `least` itself: classes end below
+    __syncthreads();
+    n = sh_n;
   }
-  cut(n);
+  int p = 64;
+  while (p < n) p <<= 1;
+  for (int i = n + threadIdx.x; i < p; i += NT) key[i] = 0;
+  sort_keys<NT>(key, p);
   for (int j = threadIdx.x; j < k; j += NT) {
     const int c = (int)(0xfffffffeu - (unsigned)key[j]);
     indices[row * k + j] = c;
