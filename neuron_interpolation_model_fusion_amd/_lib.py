@@ -1,10 +1,11 @@
-"""ctypes binding of libnif.so (the C ABI declared in include/nif.h).
+"""ctypes binding of libnif.so (the C ABI declared in include/nif.h), and nif_torch.so, the autograd functions over it.
 
 The library is built in-tree (``csrc/libnif.so``, see ``__graft_entry__.build``).
 There is no fallback: if the shared object is missing or a symbol is absent the
 import fails loudly, and every op raises on a non-zero status.
 """
 import ctypes
+import importlib.util
 import os
 
 # torch first: libnif.so must bind to the HIP runtime torch has already loaded.  Loading the
@@ -14,6 +15,7 @@ import torch  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libnif.so')
+TORCH_PATH = os.path.join(_HERE, 'csrc', 'nif_torch.so')
 
 NIF_F32, NIF_F64, NIF_BF16, NIF_F16 = 0, 1, 2, 3
 NIF_REDUCE_NONE, NIF_REDUCE_MEAN, NIF_REDUCE_SUM = 0, 1, 2
@@ -140,10 +142,11 @@ class NifError(RuntimeError):
 
 
 def _load():
-    if not os.path.exists(LIB_PATH):
-        raise ImportError(
-            f'{LIB_PATH} is missing: build it with `python -c "import __graft_entry__ as g; g.build()"` '
-            f'or `make -C {os.path.dirname(LIB_PATH)}`. There is no CPU fallback.')
+    for path in (LIB_PATH, TORCH_PATH):
+        if not os.path.exists(path):
+            raise ImportError(
+                f'{path} is missing: build it with `python -c "import __graft_entry__ as g; g.build()"` '
+                f'or `make -C {os.path.dirname(path)}`. There is no CPU fallback.')
     lib = ctypes.CDLL(LIB_PATH)
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is absent
@@ -152,7 +155,16 @@ def _load():
     return lib
 
 
+def _load_torch():
+    spec = importlib.util.spec_from_file_location('nif_torch', TORCH_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)  # finds libnif.so, loaded above, beside itself
+    module.set_error(NifError)
+    return module
+
+
 lib = _load()
+nif_torch = _load_torch()
 
 
 def check(status, what):

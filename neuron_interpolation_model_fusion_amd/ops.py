@@ -987,27 +987,8 @@ def weighted_mse(pred, truth, w=None):
 
 # ---- losses of a head over many classes ----------------------------------------------------------------
 
-_HEAD_DT = {torch.float32: _lib.NIF_F32, torch.bfloat16: _lib.NIF_BF16, torch.float16: _lib.NIF_F16}
+_HEAD_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _REDUCTIONS = {'none': _lib.NIF_REDUCE_NONE, 'mean': _lib.NIF_REDUCE_MEAN, 'sum': _lib.NIF_REDUCE_SUM}
-
-
-# A head of a level fit is a handful of launches of a few microseconds, and its backward pass runs in autograd's own
-# thread: device guard, stream and addresses are taken the short way here.
-
-def _on(t):
-    return torch.cuda._DeviceGuard(t.device.index)
-
-
-def _stream_of(t):
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _bytes(n, device):
-    return torch.empty(n or 1, dtype=torch.uint8, device=device)
 
 
 def _same_device(what, first, *ts):
@@ -1024,7 +1005,7 @@ def _reduction(what, reduction):
 
 
 def _head_type(what, *ts):
-    if ts[0].dtype not in _HEAD_DT or any(t is not None and t.dtype != ts[0].dtype for t in ts):
+    if ts[0].dtype not in _HEAD_TYPES or any(t is not None and t.dtype != ts[0].dtype for t in ts):
         raise TypeError(f'{what} needs matching float32, bfloat16 or float16 inputs, got '
                         f'{[str(t.dtype) for t in ts if t is not None]}')
 
@@ -1059,47 +1040,6 @@ def _top_targets(values, indices, lse):
     return indices, values, None if lse is None else lse.detach().float().reshape(-1).contiguous()
 
 
-def _head_desc(hidden, weight, bias, labels, indices, values, lse, settings):
-    temperature, ignore_index, reduction = settings
-    return _lib.HeadDesc(hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight), _addr(bias), hidden.shape[0],
-                         hidden.shape[1], weight.shape[0], _HEAD_DT[hidden.dtype], reduction, _addr(labels), ignore_index,
-                         _addr(indices), _addr(values), _addr(lse), 0 if indices is None else indices.shape[1], temperature)
-
-
-class _LinearHead(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, labels, indices, values, lse, settings):
-        dev = hidden.device
-        d = _head_desc(hidden, weight, bias, labels, indices, values, lse, settings)
-        with _on(hidden):
-            per_row = settings[2] == _lib.NIF_REDUCE_NONE
-            loss = torch.empty((hidden.shape[0],) if per_row else (), dtype=torch.float32, device=dev)
-            state_bytes, ws_bytes = lib.nif_head_state_bytes(d), lib.nif_head_forward_workspace_bytes(d)
-            state, ws = _bytes(state_bytes, dev), _bytes(ws_bytes, dev)
-            check(lib.nif_head_forward(d, loss.data_ptr(), state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes,
-                                       _stream_of(hidden)), 'nif_head_forward')
-        ctx.save_for_backward(hidden, weight, bias, labels, indices, values, lse, state)
-        ctx.settings = settings
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        hidden, weight, bias, labels, indices, values, lse, state = ctx.saved_tensors
-        dev = hidden.device
-        d = _head_desc(hidden, weight, bias, labels, indices, values, lse, ctx.settings)
-        grad_out = grad_out.contiguous()
-        with _on(hidden):
-            dh, dw, db = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
-                          for t, need in zip((hidden, weight, bias), ctx.needs_input_grad))
-            ws_bytes = lib.nif_head_backward_workspace_bytes(d)
-            ws = _bytes(ws_bytes, dev)
-            check(lib.nif_head_backward(d, grad_out.data_ptr(), state.data_ptr(), state.numel(), _addr(dh), hidden.shape[1],
-                                        _addr(dw), weight.shape[1], _addr(db), ws.data_ptr(), ws_bytes, _stream_of(hidden)),
-                  'nif_head_backward')
-        return dh, dw, db, None, None, None, None, None
-
-
 def _check_head(what, hidden, weight, bias):
     _head_type(what, hidden, weight, bias)
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
@@ -1109,12 +1049,12 @@ def _check_head(what, hidden, weight, bias):
         raise ValueError(f'{what}: bias has shape {tuple(bias.shape)} for {weight.shape[0]} classes')
 
 
-def _linear_head(hidden, weight, bias, labels, targets, settings):
+def _linear_head(hidden, weight, bias, labels, indices, values, lse, temperature, ignore_index, reduction):
     lead = hidden.shape[:-1]
     hidden = _mat(hidden.reshape(-1, hidden.shape[-1]), 'hidden')
-    loss = _LinearHead.apply(hidden, _mat(weight, 'weight'), None if bias is None else bias.contiguous(), labels, *targets,
-                             settings)
-    return loss.reshape(lead) if settings[2] == _lib.NIF_REDUCE_NONE else loss
+    loss = _lib.nif_torch.linear_head(hidden, _mat(weight, 'weight'), None if bias is None else bias.contiguous(), labels, indices,
+                                      values, lse, temperature, ignore_index, reduction)
+    return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE else loss
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100, reduction='mean'):
@@ -1134,7 +1074,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     _check_head(what, hidden, weight, bias)
     _same_device(what, hidden, weight, target, bias)
     labels = target.detach().to(torch.int64).reshape(-1).contiguous()
-    return _linear_head(hidden, weight, bias, labels, (None, None, None), (1.0, int(ignore_index), reduction))
+    return _linear_head(hidden, weight, bias, labels, None, None, None, 1.0, int(ignore_index), reduction)
 
 
 def linear_topk_distillation(hidden, weight, top_values, top_indices, bias=None, *, temperature=1.0, top_lse=None,
@@ -1146,40 +1086,7 @@ def linear_topk_distillation(hidden, weight, top_values, top_indices, bias=None,
     _check_head(what, hidden, weight, bias)
     _check_top(what, hidden.shape[:-1], top_values, top_indices, top_lse)
     _same_device(what, hidden, weight, top_values, top_indices, bias, top_lse)
-    return _linear_head(hidden, weight, bias, None, _top_targets(top_values, top_indices, top_lse), (temperature, 0, reduction))
-
-
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, indices, values, lse, settings):
-        temperature, reduction = settings
-        n, classes = logits.shape
-        k, dev = indices.shape[1], logits.device
-        with _on(logits):
-            loss = torch.empty((n,) if reduction == _lib.NIF_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-            state_bytes, ws_bytes = lib.nif_distill_state_bytes(n, k), lib.nif_distill_workspace_bytes(n)
-            state, ws = _bytes(state_bytes, dev), _bytes(ws_bytes, dev)
-            check(lib.nif_distill_forward(logits.data_ptr(), _ld(logits), n, classes, _HEAD_DT[logits.dtype],
-                                          indices.data_ptr(), values.data_ptr(), _addr(lse), k, temperature, reduction,
-                                          loss.data_ptr(), state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes,
-                                          _stream_of(logits)), 'nif_distill_forward')
-        ctx.save_for_backward(logits, state)
-        ctx.settings = settings + (k,)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        logits, state = ctx.saved_tensors
-        temperature, reduction, k = ctx.settings
-        n, classes = logits.shape
-        grad_out = grad_out.contiguous()
-        with _on(logits):
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            check(lib.nif_distill_backward(logits.data_ptr(), _ld(logits), n, classes, _HEAD_DT[logits.dtype], k, temperature,
-                                           reduction, grad_out.data_ptr(), state.data_ptr(), state.numel(), grad.data_ptr(),
-                                           classes, _stream_of(logits)), 'nif_distill_backward')
-        return grad, None, None, None, None
+    return _linear_head(hidden, weight, bias, None, *_top_targets(top_values, top_indices, top_lse), temperature, 0, reduction)
 
 
 def topk_distillation(logits, top_values, top_indices, *, temperature=1.0, top_lse=None, reduction='mean'):
@@ -1200,8 +1107,8 @@ def topk_distillation(logits, top_values, top_indices, *, temperature=1.0, top_l
     lead = logits.shape[:-1]
     _check_top(what, lead, top_values, top_indices, top_lse)
     _same_device(what, logits, top_values, top_indices, top_lse)
-    loss = _Distill.apply(_mat(logits.reshape(-1, logits.shape[-1]), 'logits'), *_top_targets(top_values, top_indices, top_lse),
-                          (temperature, reduction))
+    loss = _lib.nif_torch.distill(_mat(logits.reshape(-1, logits.shape[-1]), 'logits'),
+                                  *_top_targets(top_values, top_indices, top_lse), temperature, reduction)
     return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE else loss
 
 
@@ -1217,13 +1124,7 @@ def top_logits(logits, k, *, temperature=1.0):
     _same_device(what, logits)
     lead = logits.shape[:-1]
     z = _mat(logits.detach().reshape(-1, logits.shape[-1]), 'logits')
-    n, dev = z.shape[0], z.device
-    with _on(z):
-        values = torch.empty((n, k), dtype=z.dtype, device=dev)
-        indices = torch.empty((n, k), dtype=torch.int32, device=dev)
-        lse = torch.empty((n,), dtype=torch.float32, device=dev)
-        check(lib.nif_top_logits(z.data_ptr(), _ld(z), n, z.shape[1], _HEAD_DT[z.dtype], k, temperature, values.data_ptr(),
-                                 indices.data_ptr(), lse.data_ptr(), _stream_of(z)), 'nif_top_logits')
+    values, indices, lse = _lib.nif_torch.top_logits(z, k, temperature)
     return values.reshape(*lead, k), indices.reshape(*lead, k), lse.reshape(lead)
 
 

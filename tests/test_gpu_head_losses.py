@@ -523,3 +523,13 @@ def test_a_teacher_and_a_student_head_together(ops):
         with torch.no_grad():
             for t, gr in ((w1, ga[0]), (b1, ga[1]), (w2, gb[0]), (b2, gb[1])):
                 t -= 0.1 * gr
+
+
+def test_errors_of_the_autograd_functions_are_the_librarys_own(ops):
+    from neuron_interpolation_model_fusion_amd import _lib
+    with pytest.raises(_lib.NifError, match='nif_top_logits failed with status -1'):
+        _lib.nif_torch.top_logits(torch.zeros(2, 3, device='cuda'), 4, 1.0)
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(torch.zeros(2, 3, device='cuda'), torch.zeros(4, 2, device='cuda'), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(_lib.NifError):  # one tensor on the host
+        ops.linear_cross_entropy(torch.zeros(2, 3, device='cuda'), torch.zeros(4, 3, device='cuda'), torch.zeros(2, dtype=torch.int64))
