@@ -17,25 +17,14 @@ namespace nif {
 
 // ---- targets ------------------------------------------------------------------------------------------------
 
-__global__ __launch_bounds__(256) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t n, int classes,
-                                                            Targets t) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) label_target(labels[i], ignore, classes, t.p[i], t.at[i], t.P[i]);
-}
-
 __global__ __launch_bounds__(256) void top_targets_kernel(const int32_t* __restrict__ indices, const float* __restrict__ values,
                                                           const float* __restrict__ lse, int64_t n, int classes, Targets t) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row < n) top_targets(indices, values, lse, row, classes, t, threadIdx.x & 63);
 }
 
-void launch_targets(const int64_t* labels, int64_t ignore, const int32_t* indices, const float* values, const float* lse, int64_t n, int k,
-                    int classes, const Targets& t, hipStream_t st) {
-  (void)k;
-  if (labels)
-    hipLaunchKernelGGL(label_targets_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, labels, ignore, n, classes, t);
-  else
-    hipLaunchKernelGGL(top_targets_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, indices, values, lse, n, classes, t);
+void launch_targets(const int32_t* indices, const float* values, const float* lse, int64_t n, int classes, const Targets& t, hipStream_t st) {
+  hipLaunchKernelGGL(top_targets_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, indices, values, lse, n, classes, t);
 }
 
 // ---- distillation of given logits ---------------------------------------------------------------------------

@@ -485,15 +485,27 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
 }
 
 // ---- the rows that count ------------------------------------------------------------------------------
-// One workgroup: rows[i] = i-th row with a target, inv[r] = its place or -1, count.
-__global__ __launch_bounds__(1024) void head_rows_kernel(const float* __restrict__ P, int64_t n, int* __restrict__ rows,
-                                                         int* __restrict__ inv, int* __restrict__ count) {
+// One workgroup: rows[i] = i-th row with a target, inv[r] = its place or -1, count; the targets themselves where they are
+// labels; loss 0 for rows without.
+__global__ __launch_bounds__(1024) void head_rows_kernel(Targets tg, const int64_t* __restrict__ labels, int64_t ignore, int classes,
+                                                         int64_t n, int* __restrict__ rows, int* __restrict__ inv,
+                                                         int* __restrict__ count, float* __restrict__ loss) {
   __shared__ int sh[17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
   for (int64_t r0 = 0; r0 < n; r0 += 1024) {
     const int64_t r = r0 + threadIdx.x;
-    const bool live = r < n && P[r] != NO_TARGET;
+    float P = NO_TARGET;
+    if (r < n) {
+      if (labels) {
+        label_target(labels[r], ignore, classes, tg.p[r], tg.at[r], P);
+        tg.P[r] = P;
+      } else {
+        P = tg.P[r];
+      }
+      if (P == NO_TARGET) loss[r] = 0.f;
+    }
+    const bool live = P != NO_TARGET;
     const unsigned long long m = __ballot(live);
     if (lane == 0) sh[wave] = __popcll(m);
     __syncthreads();
@@ -516,7 +528,7 @@ __global__ __launch_bounds__(1024) void head_rows_kernel(const float* __restrict
   if (threadIdx.x == 0) *count = base;
 }
 
-// x = h + m + l: three bf16 values, exact for 24 bits; infinities and NaN stay in the first one
+// x = h + m + l: three bf16 values, exact for 24 bits; an infinity becomes NaN
 __device__ __forceinline__ void split3(float x, short (&w)[3]) {
 #pragma unroll
   for (int pl = 0; pl < 3; ++pl) {
@@ -526,22 +538,16 @@ __device__ __forceinline__ void split3(float x, short (&w)[3]) {
   }
 }
 
-// dst[plane][i][0 .. ldd) = src[rows ? rows[i] : i][0 .. d), zeros behind d and in rows behind the last one.
-// One block per row, or per rows of a piece of the weight.
+// dst[plane][0 .. ldd) = src[0 .. d) by one block of 256, zeros behind d (everywhere: have = false)
 template <bool F32>
-__global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__ src, int64_t lds, int d, const int* __restrict__ rows,
-                                                        const int* __restrict__ count, int64_t nrows, short* __restrict__ dst,
-                                                        int64_t plane, int ldd) {
-  const int64_t i = blockIdx.x;
-  const bool have = i < (count ? (int64_t)*count : nrows);
-  const int64_t r = have ? (rows ? rows[i] : i) : 0;
+__device__ __forceinline__ void pack_row(const void* src, bool have, int d, short* dst, int64_t plane, int ldd) {
   for (int c = threadIdx.x * 8; c < ldd; c += 256 * 8) {
-    s16x8 w[3];
+    s16x8 w[F32 ? 3 : 1];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[0][e] = w[1][e] = w[2][e] = 0;
+    for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) w[pl] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
     if (have && c < d) {
-      if (F32) {
-        const float* p = (const float*)src + r * lds + c;
+      if constexpr (F32) {
+        const float* p = (const float*)src + c;
         float x[8];
         if (c + 8 <= d && !((uintptr_t)p & 15)) {
           *(f32x4*)x = ((const f32x4*)p)[0];
@@ -557,7 +563,7 @@ __global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__
           w[0][e] = t[0], w[1][e] = t[1], w[2][e] = t[2];
         }
       } else {
-        const short* p = (const short*)src + r * lds + c;
+        const short* p = (const short*)src + c;
         if (c + 8 <= d && !((uintptr_t)p & 15)) {
           w[0] = *(const s16x8*)p;
         } else {
@@ -567,29 +573,30 @@ __global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__
       }
     }
 #pragma unroll
-    for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) *(s16x8*)(dst + pl * plane + i * ldd + c) = w[pl];
+    for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) *(s16x8*)(dst + pl * plane + c) = w[pl];
   }
 }
 
-// ---- the loss of each row -------------------------------------------------------------------------------
+// the weight rows of a piece, a block each
+template <bool F32>
+__global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__ src, int64_t lds, int d, short* __restrict__ dst,
+                                                        int64_t plane, int ldd) {
+  const int64_t i = blockIdx.x;
+  pack_row<F32>((const char*)src + i * lds * (F32 ? 4 : 2), true, d, dst + i * ldd, plane, ldd);
+}
+
 // The targets' logits u = (hidden . weight[at] + bias) / tau as dot products of the inputs, in 32 bits: a wave for eight
-// targets of a packed row, their weight rows in flight together.  Bound by the gathered rows' bytes.
+// targets of a row, their weight rows in flight together.  Bound by the gathered rows' bytes.
 constexpr int DOTS = 8;
 template <int DT>
-__global__ __launch_bounds__(256) void head_dots_kernel(const void* __restrict__ hidden, int64_t ldh, const void* __restrict__ weight,
-                                                        int64_t ldw, const void* __restrict__ bias, int d, Targets tg, int groups,
-                                                        const int* __restrict__ rows, const int* __restrict__ count,
-                                                        float* __restrict__ uk) {
+__device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const void* weight, int64_t ldw, const void* bias, int d,
+                                            const Targets& tg, int64_t src, int k0, float* uk, int lane) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16;
-  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int i = unit / groups, k0 = unit % groups * DOTS;
-  if (i >= *count) return;
-  const int64_t src = rows[i];
-  const E* h = (const E*)hidden + src * ldh;
   const E* w[DOTS];
   float s[DOTS];
-  bool vec = (((uintptr_t)h | (uintptr_t)weight) & 15) == 0 && ldw % V == 0, any = false;
+  const bool vec = (((uintptr_t)h | (uintptr_t)weight) & 15) == 0 && ldw % V == 0;
+  bool any = false;
 #pragma unroll
   for (int q = 0; q < DOTS; ++q) {
     const int at = k0 + q < tg.k ? tg.at[src * tg.k + k0 + q] : -1;
@@ -619,10 +626,28 @@ __global__ __launch_bounds__(256) void head_dots_kernel(const void* __restrict__
     if (k0 + q >= tg.k) break;
     const float u = wave_sum_f32(s[q]);
     const int at = tg.at[src * tg.k + k0 + q];
-    if (lane == 0) uk[(int64_t)i * tg.k + k0 + q] = at < 0 ? 0.f : (u + (bias ? Elem<DT>::load(bias, at) : 0.f)) * tg.inv_tau;
+    if (lane == 0) uk[k0 + q] = at < 0 ? 0.f : (u + (bias ? Elem<DT>::load(bias, at) : 0.f)) * tg.inv_tau;
   }
 }
 
+// Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits.
+template <int DT>
+__global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int d,
+                                                             const int* __restrict__ rows, const int* __restrict__ count,
+                                                             short* __restrict__ dst, int64_t plane, int ldd,
+                                                             const void* __restrict__ weight, int64_t ldw, const void* __restrict__ bias,
+                                                             Targets tg, float* __restrict__ uk) {
+  const int64_t i = blockIdx.x;
+  const bool have = i < *count;
+  const int64_t src = have ? rows[i] : 0;
+  const typename Elem<DT>::t* h = (const typename Elem<DT>::t*)hidden + src * ldh;
+  pack_row<DT == NIF_F32>(h, have, d, dst + i * ldd, plane, ldd);
+  if (!have) return;
+  for (int k0 = (threadIdx.x >> 6) * DOTS; k0 < tg.k; k0 += 4 * DOTS)
+    target_dots<DT>(h, weight, ldw, bias, d, tg, src, k0, uk + i * tg.k, threadIdx.x & 63);
+}
+
+// ---- the loss of each row -------------------------------------------------------------------------------
 // 16 packed rows a block: joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.
 constexpr int FINISH_NT = 1024;
 __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
@@ -661,33 +686,30 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
   }
 }
 
-// rows without a target: loss 0 (before the finish kernel), gradient 0
-__global__ __launch_bounds__(256) void head_clear_loss_kernel(const int* __restrict__ inv, int64_t n, float* __restrict__ loss) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n && inv[i] < 0) loss[i] = 0.f;
-}
-
+// First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i], and what the products of dz are multiplied with.  Where
+// one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
+// near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
+// the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  The other blocks: gradient 0 for rows without a target.
 template <typename W>
-__global__ __launch_bounds__(256) void head_clear_rows_kernel(const int* __restrict__ inv, W* __restrict__ out, int64_t ld, int d) {
-  const int64_t r = blockIdx.x;
-  if (inv[r] >= 0) return;
-  for (int c = threadIdx.x; c < d; c += 256) out[r * ld + c] = 0;
-}
-
-// coef[i] = (gradient that arrives at row i) * tau * scale and cp[i] = coef[i] * P[i].  scale: f16 holds nothing below
-// 2^-24, so dz is scaled by the power of two that takes the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger);
-// the gradients' epilogues divide by it again.  bf16 and f32 need none.
 __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict__ grad, int per_row, int mean, Targets tg,
-                                                         const int* __restrict__ rows, const int* __restrict__ count, int f16,
-                                                         float* __restrict__ coef, float* __restrict__ cp, float* __restrict__ inv_scale) {
+                                                         const int* __restrict__ rows, const int* __restrict__ inv,
+                                                         const int* __restrict__ count, int64_t rows_all, int f16, float* __restrict__ coef,
+                                                         float* __restrict__ cp, float* __restrict__ inv_scale, W* __restrict__ out,
+                                                         int64_t ld, int d) {
+  if (blockIdx.x > 0) {
+    const int64_t r = (int64_t)(blockIdx.x - 1) * 4 + (threadIdx.x >> 8);
+    if (r < rows_all && inv[r] < 0)
+      for (int c = threadIdx.x & 255; c < d; c += 256) out[r * ld + c] = 0;
+    return;
+  }
   __shared__ float sh[16];
   const int n = *count;
-  const float w = tg.tau * (mean ? 1.f / max(1, n) : 1.f);
+  const float w = tg.tau * (mean ? 1.f / max(1, n) : 1.f), all = per_row ? 1.f : grad[0] * w;
   float scale = 1.f;
   if (f16) {
     float top = 0.f;
     for (int i = threadIdx.x; i < n; i += 1024) {
-      const float c = fabsf(grad[per_row ? rows[i] : 0] * w) * fmaxf(1.f, tg.P[rows[i]]);
+      const float c = (per_row ? fabsf(grad[rows[i]] * w) : 1.f) * fmaxf(1.f, tg.P[rows[i]]);
       top = c < INFINITY ? fmaxf(top, c) : top;
     }
     for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -700,9 +722,9 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
       scale = ldexpf(1.f, max(-100, min(100, 14 - e)));
     }
   }
-  if (threadIdx.x == 0) *inv_scale = 1.f / scale;
+  if (threadIdx.x == 0) *inv_scale = all / scale;
   for (int i = threadIdx.x; i < n; i += 1024) {
-    const float c = (per_row ? grad[rows[i]] : grad[0]) * w * scale;
+    const float c = (per_row ? grad[rows[i]] * w : 1.f) * scale;
     coef[i] = c;
     cp[i] = c * tg.P[rows[i]];
   }
@@ -1114,11 +1136,9 @@ static Side weight_side(const nif_head_desc* h, const Plan& p, int v0, int vc, s
     const char* src = (const char*)h->weight + (size_t)v0 * h->ldw * e;
     const int64_t plane = (int64_t)vc * p.ldd;
     if (h->dtype == NIF_F32)
-      hipLaunchKernelGGL(head_pack_kernel<true>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, nullptr, nullptr, (int64_t)vc, packed,
-                         plane, p.ldd);
+      hipLaunchKernelGGL(head_pack_kernel<true>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, packed, plane, p.ldd);
     else
-      hipLaunchKernelGGL(head_pack_kernel<false>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, nullptr, nullptr, (int64_t)vc, packed,
-                         plane, p.ldd);
+      hipLaunchKernelGGL(head_pack_kernel<false>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, packed, plane, p.ldd);
     s = Side{packed, plane, p.ldd, vc, p.ldd};
   } else {
     s = Side{(const short*)h->weight + (int64_t)v0 * h->ldw, 0, h->ldw, vc, p.d};
@@ -1154,16 +1174,10 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
 }
 
 template <int DT>
-static void finish(const nif_head_desc* h, const Plan& p, char* state, const float2* stats, int tiles, float* row_loss, hipStream_t st) {
-  const Targets tg = targets_of(h, p, state);
-  const int* rows = (const int*)(state + p.s_rows);
-  const int* count = (const int*)(state + p.s_count);
-  float* uk = (float*)(state + p.s_uk);
-  const int groups = (p.k + DOTS - 1) / DOTS;
-  hipLaunchKernelGGL(head_dots_kernel<DT>, dim3((unsigned)((p.n * groups + 3) / 4)), dim3(256), 0, st, h->hidden, h->ldh, h->weight, h->ldw,
-                     h->bias, p.d, tg, groups, rows, count, uk);
-  hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg, rows, count,
-                     (float*)(state + p.s_lse), uk, row_loss);
+static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStream_t st) {
+  hipLaunchKernelGGL(head_pack_rows_kernel<DT>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d,
+                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), (short*)(state + p.s_h), p.cap * p.ldd, p.ldd,
+                     h->weight, h->ldw, h->bias, targets_of(h, p, state), (float*)(state + p.s_uk));
 }
 
 struct BwdSpace {
@@ -1363,15 +1377,14 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
   float* row_loss = h->reduction == NIF_REDUCE_NONE ? loss : (float*)((char*)ws + f.bytes);
   if (p.n > 0) {
     const Targets tg = targets_of(h, p, s);
-    launch_targets(h->labels, h->ignore_index, h->top_indices, h->top_values, h->top_lse, p.n, p.k, p.v, tg, st);
-    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, tg.P, p.n, rows, inv, count);
-    hipLaunchKernelGGL(head_clear_loss_kernel, dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, st, inv, p.n, row_loss);
+    if (!h->labels) launch_targets(h->top_indices, h->top_values, h->top_lse, p.n, p.v, tg, st);
+    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, tg, h->labels, h->ignore_index, p.v, p.n, rows, inv, count, row_loss);
     if (h->dtype == NIF_F32)
-      hipLaunchKernelGGL(head_pack_kernel<true>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d, rows, count, p.n,
-                         (short*)(s + p.s_h), p.cap * p.ldd, p.ldd);
+      pack_rows<NIF_F32>(h, p, s, st);
+    else if (h->dtype == NIF_BF16)
+      pack_rows<NIF_BF16>(h, p, s, st);
     else
-      hipLaunchKernelGGL(head_pack_kernel<false>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d, rows, count, p.n,
-                         (short*)(s + p.s_h), p.cap * p.ldd, p.ldd);
+      pack_rows<NIF_F16>(h, p, s, st);
     int tiles = 0;
     if (h->dtype == NIF_F32)
       forward_products<F32>(h, p, s, (char*)ws, f, tiles, st);
@@ -1380,14 +1393,11 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
     else
       forward_products<F16>(h, p, s, (char*)ws, f, tiles, st);
     const float2* stats = (const float2*)((char*)ws + f.stats);
-    if (h->dtype == NIF_F32)
-      finish<NIF_F32>(h, p, s, stats, tiles, row_loss, st);
-    else if (h->dtype == NIF_BF16)
-      finish<NIF_BF16>(h, p, s, stats, tiles, row_loss, st);
-    else
-      finish<NIF_F16>(h, p, s, stats, tiles, row_loss, st);
+    hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg, rows, count,
+                       (float*)(s + p.s_lse), (const float*)(s + p.s_uk), row_loss);
   } else {
-    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, rows, inv, count);
+    hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, targets_of(h, p, s), nullptr, (int64_t)0, p.v, (int64_t)0, rows, inv,
+                       count, nullptr);
   }
   if (h->reduction != NIF_REDUCE_NONE)
     launch_reduce(row_loss, (const float*)(s + p.s_P), p.n, h->reduction == NIF_REDUCE_MEAN, (float*)(s + p.s_fcount), loss, st);
@@ -1428,17 +1438,17 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
     return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
   }
   const BwdSpace b = backward_space(p);
-  hipLaunchKernelGGL(head_coef_kernel, dim3(1), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
-                     h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_count),
-                     h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp), (float*)((char*)ws + b.scale));
-  if (dhidden && p.n > 0) {
-    if (h->dtype == NIF_F32)
-      hipLaunchKernelGGL(head_clear_rows_kernel<float>, dim3((unsigned)p.n), dim3(256), 0, st, (const int*)(s + p.s_inv), (float*)dhidden,
-                         lddh, p.d);
-    else
-      hipLaunchKernelGGL(head_clear_rows_kernel<short>, dim3((unsigned)p.n), dim3(256), 0, st, (const int*)(s + p.s_inv), (short*)dhidden,
-                         lddh, p.d);
-  }
+  const auto prepare = [&](auto* out) {
+    const unsigned clearing = out && p.n > 0 ? (unsigned)((p.n + 3) / 4) : 0;
+    hipLaunchKernelGGL(head_coef_kernel, dim3(1 + clearing), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
+                       h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_inv),
+                       (const int*)(s + p.s_count), p.n, h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp),
+                       (float*)((char*)ws + b.scale), out, lddh, p.d);
+  };
+  if (h->dtype == NIF_F32)
+    prepare((float*)dhidden);
+  else
+    prepare((short*)dhidden);
   if (h->dtype == NIF_F32)
     backward_products<F32>(h, p, s, (char*)ws, b, dhidden, lddh, dweight, lddw, dbias, st);
   else if (h->dtype == NIF_BF16)

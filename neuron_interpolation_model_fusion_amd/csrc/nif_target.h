@@ -128,9 +128,8 @@ __device__ __forceinline__ void label_target(int64_t y, int64_t ignore, int clas
   P = !live ? NO_TARGET : p;
 }
 
-// Fills p, at and P of n rows from labels or from top logits (nif_distill.hip).
-void launch_targets(const int64_t* labels, int64_t ignore, const int32_t* indices, const float* values, const float* lse, int64_t n, int k,
-                    int classes, const Targets& t, hipStream_t st);
+// Fills p, at and P of n rows from top logits (nif_distill.hip).
+void launch_targets(const int32_t* indices, const float* values, const float* lse, int64_t n, int classes, const Targets& t, hipStream_t st);
 
 // loss = sum or mean of the rows' losses over the rows that count; count = their number, at least 1 (nif_distill.hip).
 void launch_reduce(const float* row_loss, const float* P, int64_t n, bool mean, float* count, float* loss, hipStream_t st);
