@@ -490,42 +490,38 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
 __global__ __launch_bounds__(1024) void head_rows_kernel(Targets tg, const int64_t* __restrict__ labels, int64_t ignore, int classes,
                                                          int64_t n, int* __restrict__ rows, int* __restrict__ inv,
                                                          int* __restrict__ count, float* __restrict__ loss) {
-  __shared__ int sh[17];
+  // each thread a run of rows: counted, the counts scanned, then written
+  __shared__ int sh[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int base = 0;
-  for (int64_t r0 = 0; r0 < n; r0 += 1024) {
-    const int64_t r = r0 + threadIdx.x;
-    float P = NO_TARGET;
-    if (r < n) {
-      if (labels) {
-        label_target(labels[r], ignore, classes, tg.p[r], tg.at[r], P);
-        tg.P[r] = P;
-      } else {
-        P = tg.P[r];
-      }
-      if (P == NO_TARGET) loss[r] = 0.f;
+  const int64_t per = (n + 1023) / 1024, r0 = min(n, threadIdx.x * per), r1 = min(n, r0 + per);
+  int mine = 0;
+  for (int64_t r = r0; r < r1; ++r) {
+    float P;
+    if (labels) {
+      label_target(labels[r], ignore, classes, tg.p[r], tg.at[r], P);
+      tg.P[r] = P;
+    } else {
+      P = tg.P[r];
     }
-    const bool live = P != NO_TARGET;
-    const unsigned long long m = __ballot(live);
-    if (lane == 0) sh[wave] = __popcll(m);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int s = 0;
-      for (int w = 0; w < 16; ++w) {
-        const int c = sh[w];
-        sh[w] = s;
-        s += c;
-      }
-      sh[16] = s;
-    }
-    __syncthreads();
-    const int at = base + sh[wave] + __popcll(m & ((1ull << lane) - 1));
-    if (live) rows[at] = (int)r;
-    if (r < n) inv[r] = live ? at : -1;
-    base += sh[16];
-    __syncthreads();
+    mine += P != NO_TARGET;
+    inv[r] = P != NO_TARGET ? 0 : -1;
+    if (P == NO_TARGET) loss[r] = 0.f;
   }
-  if (threadIdx.x == 0) *count = base;
+  int upto = mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 63) sh[wave] = upto;
+  __syncthreads();
+  int at = upto - mine;
+  for (int w = 0; w < wave; ++w) at += sh[w];
+  if (threadIdx.x == 1023) *count = at + mine;
+  for (int64_t r = r0; r < r1; ++r)
+    if (inv[r] == 0) {  // written by this thread above
+      rows[at] = (int)r;
+      inv[r] = at++;
+    }
 }
 
 // x = h + m + l: three bf16 values, exact for 24 bits; an infinity becomes NaN
@@ -586,47 +582,43 @@ __global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__
 }
 
 // The targets' logits u = (hidden . weight[at] + bias) / tau as dot products of the inputs, in 32 bits: a wave for eight
-// targets of a row, their weight rows in flight together.  Bound by the gathered rows' bytes.
+// targets of a row, two for each 16 lanes (one or two targets: the whole wave), their weight rows in flight together.  Bound
+// by the gathered rows' bytes.
 constexpr int DOTS = 8;
 template <int DT>
 __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const void* weight, int64_t ldw, const void* bias, int d,
                                             const Targets& tg, int64_t src, int k0, float* uk, int lane) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16;
-  const E* w[DOTS];
-  float s[DOTS];
+  const int lanes = tg.k > 2 ? 16 : 64, l = lane & (lanes - 1), k = k0 + lane / lanes * 2;
   const bool vec = (((uintptr_t)h | (uintptr_t)weight) & 15) == 0 && ldw % V == 0;
-  bool any = false;
+  int at[2];
+  const E* w[2];
+  float s[2] = {0.f, 0.f};
 #pragma unroll
-  for (int q = 0; q < DOTS; ++q) {
-    const int at = k0 + q < tg.k ? tg.at[src * tg.k + k0 + q] : -1;
-    any |= at >= 0;
-    w[q] = (const E*)weight + (int64_t)max(at, 0) * ldw;
-    s[q] = 0.f;
+  for (int q = 0; q < 2; ++q) {
+    at[q] = k + q < tg.k ? tg.at[src * tg.k + k + q] : -1;
+    w[q] = (const E*)weight + (int64_t)max(at[q], 0) * ldw;
   }
-  if (any) {
-    int c = vec ? lane * V : d;
-    for (; c + V <= d; c += 64 * V) {
-      float x[V];
-      unpack16<DT>(*(const vec4f*)(h + c), x);
+  int c = vec ? l * V : d;
+#pragma unroll 4
+  for (; c + V <= d; c += lanes * V) {
+    float x[V], y[V], z[V];
+    unpack16<DT>(*(const vec4f*)(h + c), x);
+    unpack16<DT>(*(const vec4f*)(w[0] + c), y);
+    unpack16<DT>(*(const vec4f*)(w[1] + c), z);
 #pragma unroll
-      for (int q = 0; q < DOTS; ++q) {
-        if (k0 + q >= tg.k) break;
-        float y[V];
-        unpack16<DT>(*(const vec4f*)(w[q] + c), y);
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[q] = fmaf(x[e], y[e], s[q]);
-      }
-    }
-    for (c = (vec ? d / V * V : 0) + lane; c < d; c += 64)
-      for (int q = 0; q < DOTS && k0 + q < tg.k; ++q) s[q] = fmaf((float)h[c], (float)w[q][c], s[q]);
+    for (int e = 0; e < V; ++e) s[0] = fmaf(x[e], y[e], s[0]), s[1] = fmaf(x[e], z[e], s[1]);
   }
+  for (c = (vec ? d / V * V : 0) + l; c < d; c += lanes)
 #pragma unroll
-  for (int q = 0; q < DOTS; ++q) {
-    if (k0 + q >= tg.k) break;
-    const float u = wave_sum_f32(s[q]);
-    const int at = tg.at[src * tg.k + k0 + q];
-    if (lane == 0) uk[k0 + q] = at < 0 ? 0.f : (u + (bias ? Elem<DT>::load(bias, at) : 0.f)) * tg.inv_tau;
+    for (int q = 0; q < 2; ++q) s[q] = fmaf((float)h[c], (float)w[q][c], s[q]);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1)
+      if (o < lanes) s[q] += __shfl_xor(s[q], o, 64);
+    if (l == 0 && k + q < tg.k) uk[k + q] = at[q] < 0 ? 0.f : (s[q] + (bias ? Elem<DT>::load(bias, at[q]) : 0.f)) * tg.inv_tau;
   }
 }
 
@@ -736,27 +728,32 @@ template <class T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
                                                            const float* __restrict__ uk, const float* __restrict__ lse,
                                                            const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
-                                                           short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int planes) {
+                                                           short* __restrict__ dz, int64_t dz_plane, int64_t ldz) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (i >= *count) return;
   const int64_t src = rows[i];
   const int* at = tg.at + src * tg.k;
   const float* p = tg.p + src * tg.k;
-  for (int k = lane; k < tg.k; k += 64) {
-    const int v = at[k];
-    if (v < v0 || v >= v1) continue;
+  for (int k0 = 0; k0 < tg.k; k0 += 64) {
+    const int k = k0 + lane, v = k < tg.k ? at[k] : -1;
+    const bool mine = v >= v0 && v < v1;
+    if (!__any(mine)) continue;
     float sum = 0.f;
     bool first = true;
-    if (tg.k > 1)
-      for (int q = 0; q < tg.k; ++q)
-        if (at[q] == v) {
-          if (q < k) first = false;
-          sum += p[q];
-        }
-    if (tg.k == 1) sum = p[0];
-    if (!first) continue;
+    for (int q0 = 0; q0 < tg.k; q0 += 64) {
+      const int aq = q0 + lane < tg.k ? at[q0 + lane] : -1;
+      const float pq = q0 + lane < tg.k ? p[q0 + lane] : 0.f;
+      const int n = min(64, tg.k - q0);
+      for (int q = 0; q < n; ++q) {
+        const bool same = __builtin_amdgcn_readlane(aq, q) == v;
+        if (same && q0 + q < k) first = false;
+        sum += same ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pq), q)) : 0.f;
+      }
+    }
+    if (!mine || !first) continue;
     float x = cp[i] * expf(uk[(int64_t)i * tg.k + k] - lse[i]) - coef[i] * sum;
-    for (int pl = 0; pl < planes; ++pl) {
+#pragma unroll
+    for (int pl = 0; pl < T::PLANES; ++pl) {
       const short w = to16<T>(x);
       dz[pl * dz_plane + (int64_t)i * ldz + (v - v0)] = w;
       x -= (float)__builtin_bit_cast(typename T::t, w);
@@ -764,15 +761,14 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int
   }
 }
 
-// dbias of a piece: column sums of dz over stretches of BIAS_ROWS packed rows (256 columns a block, 8 a thread), joined in
-// order by head_bias_join_kernel.  Bound by the read of dz.
-constexpr int BIAS_ROWS = 256;
+// dbias of a piece: column sums of dz over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
+// head_bias_join_kernel.  Bound by the read of dz.
 template <class T>
 __global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int cols,
-                                                        const int* __restrict__ count, float* __restrict__ part) {
+                                                        const int* __restrict__ count, int stretch, float* __restrict__ part) {
   __shared__ float sh[8][256 + 8];
   const int c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8, group = threadIdx.x >> 5;
-  const int r0 = blockIdx.y * BIAS_ROWS, r1 = min(*count, r0 + BIAS_ROWS);
+  const int r0 = blockIdx.y * stretch, r1 = min(*count, r0 + stretch);
   if (r0 >= r1) return;
   float s[8] = {};
   if (c0 < ldz)
@@ -794,11 +790,11 @@ __global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict_
   if (c < cols) part[(int64_t)blockIdx.y * cols + c] = sum;
 }
 template <class T>
-__global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __restrict__ part, int cols, const int* __restrict__ count,
+__global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __restrict__ part, int cols, const int* __restrict__ count, int stretch,
                                                              const float* __restrict__ inv_scale, void* __restrict__ out) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
-  const int stretches = (*count + BIAS_ROWS - 1) / BIAS_ROWS;
+  const int stretches = (*count + stretch - 1) / stretch;
   float s = 0.f;
 #pragma unroll 8
   for (int q = 0; q < stretches; ++q) s += part[(int64_t)q * cols + c];
@@ -809,26 +805,33 @@ __global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __rest
     ((short*)out)[c] = to16<T>(s);
 }
 
-// out = (sum of the splits' partial sums, in order, + acc) * inv_scale, or acc = that sum
+// out = (sum of the splits' partial sums, in order, + acc) * inv_scale, or acc = that sum: 4 columns a thread, 1024 a block
 template <class T>
 __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict__ part, int splits, int64_t part_split, int64_t part_ld,
                                                         int n, const int* __restrict__ n_dev, int m, float* __restrict__ acc, int first,
-                                                        int last, void* __restrict__ out, int64_t out_ld, int out_f32,
-                                                        const int* __restrict__ rowmap, const float* __restrict__ inv_scale) {
+                                                        int last, void* __restrict__ out, int64_t out_ld, const int* __restrict__ rowmap,
+                                                        const float* __restrict__ inv_scale) {
   const int64_t i = blockIdx.x;
-  if (i >= (n_dev ? min(n, *n_dev) : n)) return;
-  const float inv = *inv_scale;
-  const int64_t o = (int64_t)(rowmap ? rowmap[i] : i) * out_ld;
-  for (int c = threadIdx.x; c < m; c += 256) {
-    float s = first ? 0.f : acc[i * part_ld + c];
-    for (int q = 0; q < splits; ++q) s += part[q * part_split + i * part_ld + c];
-    if (!last)
-      acc[i * part_ld + c] = s;
-    else if (out_f32)
-      ((float*)out)[o + c] = s * inv;
-    else
-      ((short*)out)[o + c] = to16<T>(s * inv);
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (i >= (n_dev ? min(n, *n_dev) : n) || c >= m) return;
+  const float* p = part + i * part_ld + c;  // rows are padded to a multiple of 4
+  f32x4 s = first ? f32x4{0.f, 0.f, 0.f, 0.f} : *(const f32x4*)(acc + i * part_ld + c);
+#pragma unroll 8
+  for (int q = 0; q < splits; ++q) s += *(const f32x4*)(p + q * part_split);
+  if (!last) {
+    *(f32x4*)(acc + i * part_ld + c) = s;
+    return;
   }
+  s *= *inv_scale;
+  const int64_t o = (int64_t)(rowmap ? rowmap[i] : i) * out_ld + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < m) {
+      if constexpr (T::PLANES == 3)
+        ((float*)out)[o + e] = s[e];
+      else
+        ((short*)out)[o + e] = to16<T>(s[e]);
+    }
 }
 
 // ---- small heads ----------------------------------------------------------------------------------------------
@@ -1065,31 +1068,42 @@ static Targets targets_of(const nif_head_desc* h, const Plan& p, char* state) {
   return t;
 }
 
-// Tile and split of a product, by what it would take: `rounds` of blocks that run at once, each its share of the k steps
-// (us a step, measured in the middle of long products with that many blocks on each CU) and a prologue and epilogue; a
-// split writes and reads its partial sums (f32, 4 TB/s).
+// Tile and split of a product, by what it would take: rounds of as many blocks as run at once, each its steps of 32 along
+// the contraction (`step` us and `share` more for each block on a CU) and a prologue and epilogue (`fixed` us), or its
+// bytes at the rate that the tile reaches (`rate`, 10^6 bytes a us), whichever is more; a split adds its partial sums and
+// the launch that joins them.  The constants are fitted to each tile's times on 32 products of 10^8 to 10^11 operations
+// (20 to 4000 rows, 256 to 2048 features, 1000 to 100000 classes; 10 % off at the median, and the tile chosen costs 2 %
+// over the best): 8192 x 4096 x 131072 takes 6.9 ms in tiles of 256 and 10.5 in tiles of 128; 1000 x 1024 x 4000 takes 27 and 15.5 us.
 struct Shape {
   int bm, bn, wm, splits;
 };
 struct Tile {
-  int bm, bn, wm, slots;
-  float step, fixed;
+  int bm, bn, wm, per_cu;
+  float step, share, fixed, rate;
 };
 static const Tile TILES[] = {
-    {256, 256, 2, 256, 0.85f, 8.f},
-    {128, 128, 2, 512, 0.52f, 5.f},
-    {128, 32, 4, 1024, 0.40f, 4.f},
+    {256, 256, 2, 1, 0.81f, 0.f, 11.f, 4.0f},
+    {128, 128, 2, 2, 0.06f, 0.295f, 5.9f, 3.5f},
+    {128, 64, 4, 3, 0.08f, 0.174f, 4.3f, 3.9f},
 };
-static Shape shape_of(int64_t m, int64_t n, int64_t ksteps, bool may_split) {
+// m x n results of a contraction over k, as `pairs` products of `planes` planes; `results`: they are written (else reduced)
+static Shape shape_of(int64_t m, int64_t n, int64_t k, int planes, bool results, bool may_split) {
+  const int64_t steps = (k + BK - 1) / BK * (planes == 3 ? 6 : 1);
   Shape best = {128, 128, 2, 1};
   float least = INFINITY;
   for (const Tile& t : TILES) {
     const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
     for (int splits = 1; splits <= (may_split ? 32 : 1); splits *= 2) {
-      if (splits > 1 && ksteps / splits < 8) break;
-      const float rounds = (float)((tiles * splits + t.slots - 1) / t.slots);
-      const float us = rounds * ((float)((ksteps + splits - 1) / splits) * t.step + t.fixed) +
-                       (splits > 1 ? 5.f + (float)splits * (float)m * (float)n * 8e-6f / 4.f : 0.f);
+      if (splits > 1 && steps / splits < 8) break;
+      const int64_t blocks = tiles * splits, slots = 256 * t.per_cu, rest = blocks % slots;
+      const float each = (float)((steps + splits - 1) / splits);
+      float us = (float)(blocks / slots) * (each * (t.step + t.share * (float)t.per_cu) + t.fixed);
+      if (rest) us += each * (t.step + t.share * (float)((rest + 255) / 256)) + t.fixed;
+      const float in = (float)(m + n) * (float)k * 2.f * (float)planes;
+      const float out = !results ? 0.f : (float)m * (float)n * (splits > 1 ? 4.f * (float)splits : planes == 3 ? 4.f : 2.f);
+      const float memory = (in + out) * 1e-6f / t.rate + 2.f;
+      us = us > memory ? us : memory;
+      if (splits > 1) us += 4.f + out * 1e-6f / 4.f;
       if (us < least) least = us, best = {t.bm, t.bn, t.wm, splits};
     }
   }
@@ -1102,17 +1116,16 @@ static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
   g.nt = (g.N + s.bn - 1) / s.bn;
   const dim3 grid((unsigned)((int64_t)g.mt * g.nt * g.splits));
   if (grid.x == 0) return;
-  if (s.bn == 32)
-    hipLaunchKernelGGL((head_gemm_kernel<T, 128, 32, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+  if (s.bn == 64)
+    hipLaunchKernelGGL((head_gemm_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
   else if (s.bn == 256)
     hipLaunchKernelGGL((head_gemm_kernel<T, 256, 256, 2, 4, TRA, TRB, EPI>), grid, dim3(512), 0, st, g);
   else
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
 }
 
-static int pairs_of(const Plan& p) { return p.planes == 3 ? 6 : 1; }
 // of the products that make logits of a piece of `classes`
-static Shape logit_shape(const Plan& p, int classes) { return shape_of(classes, p.n, (p.d + BK - 1) / BK * pairs_of(p), false); }
+static Shape logit_shape(const Plan& p, int classes) { return shape_of(classes, p.n, p.d, p.planes, false, false); }
 
 struct FwdSpace {
   size_t stats, w, bytes;
@@ -1183,14 +1196,15 @@ static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStr
 struct BwdSpace {
   size_t coef, cp, scale, dz, w, acc, part, bytes;
   int64_t ldz, dh_ld;
+  int stretch;
   Shape dh, dw;
 };
 static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
   b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
-  b.dh = shape_of(p.d, p.n, (p.piece + BK - 1) / BK * pairs_of(p), true);
-  b.dw = shape_of(p.d, p.piece, (p.n + BK - 1) / BK * pairs_of(p), true);
+  b.dh = shape_of(p.d, p.n, p.piece, p.planes, true, true);
+  b.dw = shape_of(p.d, p.piece, p.n, p.planes, true, true);
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
@@ -1200,7 +1214,9 @@ static BwdSpace backward_space(const Plan& p) {
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
   const size_t part_h = b.dh.splits > 1 ? (size_t)b.dh.splits * p.cap * b.dh_ld * 4 : 0;
   const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
-  const size_t part_b = (size_t)((p.n + BIAS_ROWS - 1) / BIAS_ROWS) * p.piece * 4;
+  b.stretch = 32;  // rows of a block of column sums: the fewest that leave at most 2048 blocks, up to 256
+  while (b.stretch < 256 && (p.n + b.stretch - 1) / b.stretch * ((p.piece + 255) / 256) > 2048) b.stretch *= 2;
+  const size_t part_b = (size_t)((p.n + b.stretch - 1) / b.stretch) * p.piece * 4;
   const size_t part = part_h > part_w ? part_h : part_w;
   b.part = take(at, part > part_b ? part : part_b);
   b.bytes = at;
@@ -1249,12 +1265,12 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     }
     if (p.n > 0)
       hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
-                       v0 + vc, dz, dz_plane, b.ldz, p.planes);
+                       v0 + vc, dz, dz_plane, b.ldz);
     if (dbias) {
       if (p.n > 0)
-        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, (unsigned)((p.n + BIAS_ROWS - 1) / BIAS_ROWS)), dim3(256), 0, st, dz,
-                           dz_plane, b.ldz, vc, count, part);
-      hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, inv_scale,
+        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, (unsigned)((p.n + b.stretch - 1) / b.stretch)), dim3(256), 0, st, dz,
+                           dz_plane, b.ldz, vc, count, b.stretch, part);
+      hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale,
                          (char*)dbias + (size_t)v0 * (f32 ? 4 : 2));
     }
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
@@ -1278,8 +1294,8 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       }
       run_gemm<T, true, true, EPI_OUT>(b.dw, g, st);
       if (g.splits > 1)
-        hipLaunchKernelGGL(head_join_kernel<T>, dim3(vc), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, vc, nullptr, p.d,
-                           nullptr, 1, 1, g.out, lddw, f32, nullptr, inv_scale);
+        hipLaunchKernelGGL(head_join_kernel<T>, dim3(vc, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, vc,
+                           nullptr, p.d, nullptr, 1, 1, g.out, lddw, nullptr, inv_scale);
     }
     if (dhidden) {  // [packed rows][features] += dz W, contraction over the classes of the piece
       GemmArgs g = {};
@@ -1307,8 +1323,8 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.acc_ld = b.dh_ld;
       run_gemm<T, true, false, EPI_OUT>(b.dh, g, st);
       if (g.splits > 1 && p.n > 0)
-        hipLaunchKernelGGL(head_join_kernel<T>, dim3((unsigned)p.n), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, (int)p.n, count,
-                           p.d, acc, first, last, dhidden, lddh, f32, rows, inv_scale);
+        hipLaunchKernelGGL(head_join_kernel<T>, dim3((unsigned)p.n, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split,
+                           b.dh_ld, (int)p.n, count, p.d, acc, first, last, dhidden, lddh, rows, inv_scale);
     }
   }
 }
