@@ -836,17 +836,17 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
 
 // ---- small heads ----------------------------------------------------------------------------------------------
 // A batch of a classifier's level fit (32 rows, 10 to 200 classes, 400 features) costs launches, not arithmetic: forward
-// one block per row, which keeps the row's dz (n x classes f32, at most 2 MiB) for the backward pass, a single launch of
+// one block per row, which keeps the row's dz (n x classes f32, at most 1 MiB) for the backward pass, a single launch of
 // dot products.  Sums in 32 bits, the row's loss in 64.
-constexpr int SMALL_V = 1024;
+constexpr int SMALL_V = 2048;
 
-template <int DT>
-__global__ __launch_bounds__(256) void head_small_forward_kernel(nif_head_desc h, Targets t, float* __restrict__ dz,
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void head_small_forward_kernel(nif_head_desc h, Targets t, float* __restrict__ dz,
                                                                  float* __restrict__ row_loss) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16, Q = 4;
-  __shared__ float u[SMALL_V], sh[8];
-  __shared__ double sh_loss[4];
+  __shared__ float u[SMALL_V], sh[2 * NT / 64];
+  __shared__ double sh_loss[NT / 64];
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int classes = h.classes, d = h.features;
@@ -868,7 +868,7 @@ __global__ __launch_bounds__(256) void head_small_forward_kernel(nif_head_desc h
   const E* x = (const E*)h.hidden + row * h.ldh;
   const E* w = (const E*)h.weight;
   const bool vec = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && h.ldw % V == 0;
-  for (int v0 = wave * Q; v0 < classes; v0 += 4 * Q) {
+  for (int v0 = wave * Q; v0 < classes; v0 += NT / 64 * Q) {
     float s[Q];
     const E* wr[Q];
 #pragma unroll
@@ -896,28 +896,32 @@ __global__ __launch_bounds__(256) void head_small_forward_kernel(nif_head_desc h
   }
   __syncthreads();
   float top = -INFINITY, sum = 0.f;
-  for (int v = threadIdx.x; v < classes; v += 256) top = fmaxf(top, u[v]);
+  for (int v = threadIdx.x; v < classes; v += NT) top = fmaxf(top, u[v]);
   top = wave_max_f32(top);
   const float ref = top == -INFINITY ? 0.f : top;
-  for (int v = threadIdx.x; v < classes; v += 256) sum += expf(u[v] - ref);
+  for (int v = threadIdx.x; v < classes; v += NT) sum += expf(u[v] - ref);
   sum = wave_sum_f32(sum);
   if (lane == 0) sh[2 * wave] = top, sh[2 * wave + 1] = sum;
   __syncthreads();
   top = sh[0], sum = sh[1];
-  for (int q = 1; q < 4; ++q) join(top, sum, sh[2 * q], sh[2 * q + 1]);
+  for (int q = 1; q < NT / 64; ++q) join(top, sum, sh[2 * q], sh[2 * q + 1]);
   const float lse = top + logf(sum);
   double loss = 0.0;
-  for (int k = threadIdx.x; k < t.k; k += 256) {
+  for (int k = threadIdx.x; k < t.k; k += NT) {
     const int at = t.at[row * t.k + k];
     if (at >= 0) loss += target_term(t, row, k, u[at], lse);
   }
   loss = wave_sum_f64(loss);
   if (lane == 0) sh_loss[wave] = loss;
   __syncthreads();
-  if (threadIdx.x == 0) row_loss[row] = (float)(((sh_loss[0] + sh_loss[1]) + (sh_loss[2] + sh_loss[3])) * t.tau2);
-  for (int v = threadIdx.x; v < classes; v += 256) u[v] = t.tau * P * expf(u[v] - lse);
+  if (threadIdx.x == 0) {
+    loss = 0.0;
+    for (int q = 0; q < NT / 64; ++q) loss += sh_loss[q];
+    row_loss[row] = (float)(loss * t.tau2);
+  }
+  for (int v = threadIdx.x; v < classes; v += NT) u[v] = t.tau * P * expf(u[v] - lse);
   __syncthreads();
-  for (int k = threadIdx.x; k < t.k; k += 256) {
+  for (int k = threadIdx.x; k < t.k; k += NT) {
     const int v = t.at[row * t.k + k];
     if (v < 0) continue;
     float p = 0.f;
@@ -930,23 +934,30 @@ __global__ __launch_bounds__(256) void head_small_forward_kernel(nif_head_desc h
     if (first) u[v] -= t.tau * p;
   }
   __syncthreads();
-  for (int v = threadIdx.x; v < classes; v += 256) dz[row * classes + v] = u[v];
+  for (int v = threadIdx.x; v < classes; v += NT) dz[row * classes + v] = u[v];
 }
 
-// Blocks of 64 columns x 4 parts of a sum: first those of dhidden (a row each), then those of dweight (4 classes each).
-template <int DT>
-__global__ __launch_bounds__(256) void head_small_backward_kernel(nif_head_desc h, const float* __restrict__ P, const float* __restrict__ dz,
-                                                                  const float* __restrict__ count, const float* __restrict__ grad,
-                                                                  void* __restrict__ dhidden, int64_t lddh, void* __restrict__ dweight,
-                                                                  int64_t lddw, void* __restrict__ dbias, int hidden_blocks, int stretches) {
+// Blocks of 64 columns x NT / 64 parts of a sum: first those of dhidden (a row each), then those of dweight (4 classes).
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void head_small_backward_kernel(nif_head_desc h, const float* __restrict__ P, const float* __restrict__ dz,
+                                                                 const float* __restrict__ count, const float* __restrict__ grad,
+                                                                 void* __restrict__ dhidden, int64_t lddh, void* __restrict__ dweight,
+                                                                 int64_t lddw, void* __restrict__ dbias, int hidden_blocks, int stretches) {
   typedef typename Elem<DT>::t E;
-  __shared__ float sh[4][4][64], shb[4][4];
+  constexpr int PARTS = NT / 64;
+  __shared__ float sh[4][PARTS][64], shb[4][PARTS];
   const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
   const int n = (int)h.rows, classes = h.classes, d = h.features;
   const bool per_row = h.reduction == NIF_REDUCE_NONE;
   const float share = h.reduction == NIF_REDUCE_MEAN ? 1.f / *count : 1.f;
   const int block = (int)blockIdx.x < hidden_blocks ? blockIdx.x : blockIdx.x - hidden_blocks;
   const int c = block % stretches * 64 + lane;
+  const auto total = [&](int q) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < PARTS; ++w) s += sh[q][w][lane];
+    return s;
+  };
   if ((int)blockIdx.x < hidden_blocks) {
     const int64_t row = block / stretches;
     E* out = (E*)dhidden + row * lddh;
@@ -958,11 +969,11 @@ __global__ __launch_bounds__(256) void head_small_backward_kernel(nif_head_desc 
     const E* w = (const E*)h.weight + min(c, d - 1);
     const float* z = dz + row * classes;
     float s = 0.f;
-#pragma unroll 8
-    for (int v = part; v < classes; v += 4) s = fmaf(z[v], (float)w[v * h.ldw], s);
+#pragma unroll 16
+    for (int v = part; v < classes; v += PARTS) s = fmaf(z[v], (float)w[v * h.ldw], s);
     sh[0][part][lane] = s;
     __syncthreads();
-    if (part == 0 && c < d) out[c] = (E)(coef * ((sh[0][0][lane] + sh[0][1][lane]) + (sh[0][2][lane] + sh[0][3][lane])));
+    if (part == 0 && c < d) out[c] = (E)(coef * total(0));
     return;
   }
   const int v0 = block / stretches * 4;
@@ -970,7 +981,7 @@ __global__ __launch_bounds__(256) void head_small_backward_kernel(nif_head_desc 
   const E* x = (const E*)h.hidden + min(c, d - 1);
   float s[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int r = part; r < n; r += 4) {
+  for (int r = part; r < n; r += PARTS) {
     if (P[r] == NO_TARGET) continue;  // whatever such a row holds
     const float coef = grad[per_row ? r : 0] * share, a = dweight ? (float)x[r * h.ldh] : 0.f;
 #pragma unroll
@@ -986,10 +997,14 @@ __global__ __launch_bounds__(256) void head_small_backward_kernel(nif_head_desc 
     if (lane == 0) shb[q][part] = sb[q];
   }
   __syncthreads();
-  const int v = v0 + part;  // each wave writes one of the four classes
-  if (v >= classes) return;
-  if (dweight && c < d) ((E*)dweight)[v * lddw + c] = (E)((sh[part][0][lane] + sh[part][1][lane]) + (sh[part][2][lane] + sh[part][3][lane]));
-  if (bias && lane == 0) ((E*)dbias)[v] = (E)((shb[part][0] + shb[part][1]) + (shb[part][2] + shb[part][3]));
+  const int v = v0 + part;  // each of the first four waves writes one of the classes
+  if (part >= 4 || v >= classes) return;
+  if (dweight && c < d) ((E*)dweight)[v * lddw + c] = (E)total(part);
+  if (bias && lane == 0) {
+    float b = 0.f;
+    for (int w = 0; w < PARTS; ++w) b += shb[part][w];
+    ((E*)dbias)[v] = (E)b;
+  }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
@@ -1032,9 +1047,9 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   if (c < 1024) c = 1024;
   if (c > p.v) c = p.v;
   p.piece = (int)c;
-  // Small: the weight fits a CU's reach many times over (each row's block reads it whole, from L2), and the whole product
-  // is too little for tiles of 128.
-  p.small = p.n <= 512 && p.v <= SMALL_V && (int64_t)p.v * p.d <= (1 << 19) && p.n * p.v * p.d <= (1 << 25);
+  // Small: the tiled path's launches cost 25 us more on the host than one block's read of the whole weight from L2 (32 x 1024 x
+  // 1000 bf16, a training step: 83 us against 110; 4 x 128 x 8000: 307 against 111, its sums over the classes are too long).
+  p.small = p.n <= 512 && p.v <= SMALL_V && (int64_t)p.v * p.d <= (1 << 20) && p.n * p.v <= (1 << 18) && p.n * p.v * p.d <= (1 << 25);
   size_t at = 0;
   p.s_p = take(at, (size_t)p.n * p.k * 4);
   p.s_at = take(at, (size_t)p.n * p.k * 4);
@@ -1329,6 +1344,14 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
   }
 }
 
+template <int DT>
+static void small_forward(const nif_head_desc* h, const Plan& p, const Targets& tg, float* dz, float* row_loss, hipStream_t st) {
+  if (p.v > 64)
+    hipLaunchKernelGGL((head_small_forward_kernel<DT, 1024>), dim3((unsigned)p.n), dim3(1024), 0, st, *h, tg, dz, row_loss);
+  else
+    hipLaunchKernelGGL((head_small_forward_kernel<DT, 256>), dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+}
+
 static int check_desc(const nif_head_desc* h, Plan& p) {
   if (!make_plan(h, p)) return NIF_ERR_INVALID_ARG;
   if (!h->weight || (h->rows > 0 && !h->hidden) || h->ldh < h->features || h->ldw < h->features) return NIF_ERR_INVALID_ARG;
@@ -1376,11 +1399,11 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
     float* dz = (float*)(s + p.s_dz);
     if (p.n > 0) {
       if (h->dtype == NIF_F32)
-        hipLaunchKernelGGL(head_small_forward_kernel<NIF_F32>, dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+        small_forward<NIF_F32>(h, p, tg, dz, row_loss, st);
       else if (h->dtype == NIF_BF16)
-        hipLaunchKernelGGL(head_small_forward_kernel<NIF_BF16>, dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+        small_forward<NIF_BF16>(h, p, tg, dz, row_loss, st);
       else
-        hipLaunchKernelGGL(head_small_forward_kernel<NIF_F16>, dim3((unsigned)p.n), dim3(256), 0, st, *h, tg, dz, row_loss);
+        small_forward<NIF_F16>(h, p, tg, dz, row_loss, st);
     }
     if (h->reduction != NIF_REDUCE_NONE)
       launch_reduce(row_loss, tg.P, p.n, h->reduction == NIF_REDUCE_MEAN, (float*)(s + p.s_count), loss, st);
@@ -1441,16 +1464,21 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
     const float* P = (const float*)(s + p.s_P);
     const float* dz = (const float*)(s + p.s_dz);
     const float* count = (const float*)(s + p.s_count);
-    const dim3 grid((unsigned)(hb + wb + bb));
+    const auto launch = [&](auto dt) {
+      const dim3 grid((unsigned)(hb + wb + bb));
+      if (p.v > 256)  // long sums over the classes
+        hipLaunchKernelGGL((head_small_backward_kernel<dt, 1024>), grid, dim3(1024), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh,
+                           dweight, lddw, dbias, hb, stretches);
+      else
+        hipLaunchKernelGGL((head_small_backward_kernel<dt, 256>), grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh,
+                           dweight, lddw, dbias, hb, stretches);
+    };
     if (h->dtype == NIF_F32)
-      hipLaunchKernelGGL(head_small_backward_kernel<NIF_F32>, grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh, dweight,
-                         lddw, dbias, hb, stretches);
+      launch(std::integral_constant<int, NIF_F32>());
     else if (h->dtype == NIF_BF16)
-      hipLaunchKernelGGL(head_small_backward_kernel<NIF_BF16>, grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh, dweight,
-                         lddw, dbias, hb, stretches);
+      launch(std::integral_constant<int, NIF_BF16>());
     else
-      hipLaunchKernelGGL(head_small_backward_kernel<NIF_F16>, grid, dim3(256), 0, st, *h, P, dz, count, grad_loss, dhidden, lddh, dweight,
-                         lddw, dbias, hb, stretches);
+      launch(std::integral_constant<int, NIF_F16>());
     return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
   }
   const BwdSpace b = backward_space(p);
