@@ -42,6 +42,11 @@ def parse_args():
                    help='Not a reference flag. The reference computes the classifier-head shares with '
                         'num_classes=args.num_models (run_alf.py:114), which only broadcasts against the logits when '
                         'the number of models equals the number of classes; this flag counts the dataset classes instead.')
+    p.add_argument('--head_loss', type=str, default='match', choices=ALFusion.head_losses,
+                   help="Not a reference flag. What the last level is fitted on: 'match' (the reference's), 'cross_entropy' "
+                        "(the labels) or 'top_logits' (the likeliest classes of the models, at --kd_temperature).")
+    p.add_argument('--kd_top_logits', type=int, default=32,
+                   help='Not a reference flag. Number of classes kept per sample under --head_loss top_logits.')
     c.add_data_args(p)
     return p.parse_args()
 
@@ -70,7 +75,8 @@ def build_fusion_config(args, models, dataset, device, num_classes):
         max_patience_epochs=args.max_patience_epochs, normalize_acts_for_kmeans=args.normalize_acts_for_kmeans,
         num_kmeans_runs=args.num_kmeans_runs, init_kmeans_with_2nd_acts=args.init_kmeans_with_2nd_acts,
         use_weighted_loss=args.use_weighted_loss, cls_head_weights=cls_head_weights, use_kd_on_head=False,
-        kd_temperature=-1, verbose=args.verbose)
+        kd_temperature=args.kd_temperature if args.head_loss == 'top_logits' else -1, verbose=args.verbose,
+        head_loss=args.head_loss, kd_top_logits=args.kd_top_logits)
 
 
 def main():

@@ -12,11 +12,13 @@ then Lloyd steps that only stream that N x N matrix (ops.KMeans); the targets T 
 gather-reduce pass over the activations; (3) is a cross-Gram + the device LAP kernel in scipy
 order.  (4) is autograd training and stays PyTorch, but its data path is on the device:
 batches are index gathers from resident tensors in the loader's exact sample order, and the
-(cluster-weighted) squared-error loss is one fused forward and one fused backward pass.
+(cluster-weighted) squared-error loss is one fused forward and one fused backward pass.  The last level
+may instead be fitted on the labels or on the models' top logits, with losses that take the head's input
+and weight (ops.linear_cross_entropy, ops.linear_topk_distillation).
 """
 import math
 import time
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 import torch.nn as nn
@@ -58,6 +60,11 @@ class ALFusionConfig:
     reset_level_parameters: list[int] = None
     weight_perturbation_per_level: list[float] | None = None
     verbose: bool = True
+    # Not in the reference: what the last level is fitted on.  'match' is the reference's (squared error or KLDivLoss
+    # on the mean logits, alf.py:398-454); 'cross_entropy' the labels y; 'top_logits' the kd_top_logits likeliest
+    # classes of the models' mean probabilities at kd_temperature.  The latter two never form the logits.
+    head_loss: str = 'match'
+    kd_top_logits: int = 32
 
 
 class ActivationDataset(Dataset):
@@ -132,6 +139,7 @@ class _GraphedBatch:
 
 class ALFusion:
     neuron_importance_methods = ['uniform', 'conductance', 'deeplift', 'featureablation']
+    head_losses = ['match', 'cross_entropy', 'top_logits']
     use_hip_graphs = True  # replay the per-batch forward/backward of the level fit as a HIP graph
 
     def __init__(self, models):
@@ -147,6 +155,30 @@ class ALFusion:
         method = fusion_config.neuron_importance_method
         if method not in self.neuron_importance_methods:
             raise ValueError(f'Invalid neuron importance method: {method}')
+        if fusion_config.head_loss not in self.head_losses:
+            raise ValueError(f'Invalid head loss: {fusion_config.head_loss}')
+        if fusion_config.head_loss != 'match':
+            self._head_loss_check(fusion_config)
+
+    def _head_loss_check(self, fusion_config):
+        """Before the first level is fitted: the last one is hours away on a large model."""
+        level = self.models[0].get_ordered_trainable_named_levels[-1]
+        self._body_and_head(level.network)
+        if level.output_width > 1 << 24:
+            raise ValueError(f'{level.output_width} classes: the targets of a loss on the head hold 2^24 at most')
+        if fusion_config.head_loss == 'top_logits':
+            if not 1 <= fusion_config.kd_top_logits <= ops.MAX_TOP_LOGITS:
+                raise ValueError(f'Invalid kd_top_logits: {fusion_config.kd_top_logits}')
+            if not 0 < fusion_config.kd_temperature < math.inf:
+                raise ValueError(f'Invalid kd_temperature: {fusion_config.kd_temperature}')
+            return
+        if fusion_config.y is None:
+            raise ValueError("head_loss='cross_entropy' needs the labels y")
+        y = torch.as_tensor(fusion_config.y).reshape(-1)
+        if y.shape[0] != fusion_config.X.shape[0]:
+            raise ValueError(f'{y.shape[0]} labels for {fusion_config.X.shape[0]} samples')
+        if bool(((y < 0) | (y >= level.output_width)).any()):
+            raise ValueError(f'labels must lie in [0, {level.output_width})')
 
     # -- layouts (alf.py:104-124) ------------------------------------------------------------------------
     def _flatten_acts(self, acts):
@@ -340,6 +372,41 @@ class ALFusion:
         T = self._calculate_centroids(num_classes, assignment, all_model_logits.T).T
         return T, assignment
 
+    # The two losses on the head (not in the reference) take the head's input and the head itself.  Their targets are
+    # float rows like every other level's, so that batching, sharding and graph replay treat them alike; class indices
+    # are exact in float32 up to 2^24.
+    @staticmethod
+    def _body_and_head(network):
+        """(the last level up to its nn.Linear, that nn.Linear)."""
+        if isinstance(network, nn.Linear):
+            return nn.Identity(), network
+        if isinstance(network, nn.Sequential) and len(network) and isinstance(network[-1], nn.Linear):
+            return network[:-1], network[-1]
+        raise ValueError(f'a loss on the head needs a last level that ends in nn.Linear, not {type(network).__name__}')
+
+    def _head_loss_targets(self, num_classes, fusion_config):
+        if fusion_config.head_loss == 'cross_entropy':
+            return torch.as_tensor(fusion_config.y, device=self.device).reshape(-1, 1).float()
+        tau, k = fusion_config.kd_temperature, min(fusion_config.kd_top_logits, num_classes)
+        probs, _ = self._last_level_grouping(num_classes, replace(fusion_config, use_kd_on_head=True))
+        values, indices, lse = ops.top_logits(tau * probs.float().log(), k, temperature=tau)
+        return torch.cat([values, indices.float(), lse[:, None]], dim=1)
+
+    @staticmethod
+    def _head_criterion(fusion_config):
+        tau = fusion_config.kd_temperature
+
+        def cross_entropy(hidden, head, y):
+            return ops.linear_cross_entropy(hidden, head.weight, y[:, 0].long(), head.bias)
+
+        def top_logits(hidden, head, y):
+            k = y.shape[1] // 2
+            return ops.linear_topk_distillation(hidden, head.weight, y[:, :k], y[:, k:2 * k].int(), head.bias,
+                                                temperature=tau, top_lse=y[:, 2 * k])
+        criterion = cross_entropy if fusion_config.head_loss == 'cross_entropy' else top_logits
+        criterion.on_head = True
+        return criterion
+
     def _criterion_vectorized(self, act_pred, act_true, cluster_weights):
         """mean(cluster_weights[c] * (pred - true)^2) (alf.py:414-422), one fused pass on the device."""
         return ops.weighted_mse(act_pred, act_true, cluster_weights)
@@ -421,6 +488,9 @@ class ALFusion:
         return torch.randperm(n, generator=g)
 
     def _batch_loss(self, network, criterion, x, y):
+        if getattr(criterion, 'on_head', False):
+            body, head = self._body_and_head(network)
+            return criterion(body(x), head, y)
         y_hat = network(x)
         if not getattr(criterion, 'native_layout', False):
             y_hat, y = self._flatten_acts(y_hat), self._flatten_acts(y)
@@ -460,7 +530,11 @@ class ALFusion:
 
         num_levels = get_num_levels(self.models)
         is_last_level = level_idx == num_levels - 1
-        if not is_last_level:
+        on_head = is_last_level and fusion_config.head_loss != 'match'
+        if on_head:
+            self._body_and_head(network)
+            T = self._head_loss_targets(target_width, fusion_config)
+        elif not is_last_level:
             T, assignment = self._k_means_v2(level_idx, target_width, fusion_config, level_X)
         else:
             T, assignment = self._last_level_grouping(target_width, fusion_config)
@@ -492,7 +566,8 @@ class ALFusion:
         disable_dropout(network)
         optimizer = self._get_optimizer(level_idx, network, fusion_config)
         scheduler = torch.optim.lr_scheduler.CosineAnnealingLR(optimizer, T_max=50)
-        criterion = self._get_criterion(level_idx, target_width, assignment, fusion_config, is_last_level)
+        criterion = self._head_criterion(fusion_config) if on_head else \
+            self._get_criterion(level_idx, target_width, assignment, fusion_config, is_last_level)
 
         # launch-bound inner loop -> one HIP graph per phase once a level has enough full batches to pay for it
         use_graphs = self.use_hip_graphs and level_X.is_cuda

@@ -1112,6 +1112,9 @@ def topk_distillation(logits, top_values, top_indices, *, temperature=1.0, top_l
     return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE else loss
 
 
+MAX_TOP_LOGITS = _lib.NIF_TOP_MAX_K  # the longest list of top logits a row
+
+
 def top_logits(logits, k, *, temperature=1.0):
     """The k largest logits of each row, what ``topk_distillation`` takes of a teacher: (values [..., k] of logits' type,
     indices [..., k] int32, lse [...] f32 = logsumexp(logits / temperature) over all classes).  Larger ones first, equal
