@@ -498,6 +498,7 @@ int nif_lsq_solve_f64(const double* G, int64_t ldg, const double* R, int64_t ldr
  * that is not a class makes its row NaN.  Rows that are left out have loss 0 and gradient 0, whatever they hold.
  * Reductions: NONE: loss[rows]; SUM; MEAN over the rows that count (0 when there are none).
  * hidden rows x features (ldh), weight classes x features (ldw), bias classes or NULL, all of `dtype`; any alignment.
+ * The logits are not kept, but for few rows: up to 64 MiB of them in 32 bits where that is faster than computing them again.
  * Products accumulate in 32 bits; f32 operands are split into three bf16 parts (f32-level accuracy).
  * `state` carries the forward pass's results to the backward pass, which needs the same inputs; the workspaces are
  * scratch of each call.  dhidden, dweight, dbias: of `dtype`, written in full; NULL where not wanted. */
@@ -520,6 +521,7 @@ typedef struct nif_head_desc {
   const float* top_lse;
   int32_t top; /* entries a row; 0 with labels */
   float temperature;
+  int32_t forward_only; /* not 0: no backward pass will follow */
 } nif_head_desc;
 size_t nif_head_state_bytes(const nif_head_desc* h);
 size_t nif_head_forward_workspace_bytes(const nif_head_desc* h);

@@ -46,7 +46,7 @@ class HeadDesc(_c.Structure):
     _fields_ = [('hidden', _vp), ('ldh', _i64), ('weight', _vp), ('ldw', _i64), ('bias', _vp), ('rows', _i64),
                 ('features', _c.c_int32), ('classes', _c.c_int32), ('dtype', _c.c_int32), ('reduction', _c.c_int32),
                 ('labels', _vp), ('ignore_index', _i64), ('top_indices', _vp), ('top_values', _vp), ('top_lse', _vp),
-                ('top', _c.c_int32), ('temperature', _c.c_float)]
+                ('top', _c.c_int32), ('temperature', _c.c_float), ('forward_only', _c.c_int32)]
 
 
 _desc = _c.POINTER(HeadDesc)

@@ -14,8 +14,12 @@
 // dz = coef * (P s) in 16 bits; the targets' entries are then rewritten with their -p; dW of the piece = dz^T hidden,
 // and dhidden += dz W.  Recomputing costs 8 n d v operations in place of 6 and saves n * v logits.
 //
-// 16-bit inputs run on v_mfma_f32_16x16x32 with 32-bit accumulation.  f32 inputs are split exactly into three bf16
-// planes (x = h + m + l, 24 bits) and a product runs as the six plane pairs above 2^-24: f32-level accuracy.
+// For few rows, where the product is bound by the weight's bytes or has too few tiles, up to 64 MiB of logits are kept in
+// 32 bits instead (head_kept_kernel).
+//
+// 16-bit inputs run on v_mfma_f32_16x16x32 with 32-bit accumulation (head_gemm_kernel).  f32 inputs are split exactly into
+// three bf16 planes (x = h + m + l, 24 bits) on their way into LDS and a product runs as the six plane pairs above 2^-24:
+// f32-level accuracy (head_gemm32_kernel).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -39,29 +43,38 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // that they keep their order against the loads between them; mfma_done() before the results are read.
 struct Bf16 {
   typedef __bf16 t;
-  static constexpr int PLANES = 1;
+  static constexpr bool WIDE = false;
   static __device__ __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
-struct F32 : Bf16 {  // as three bf16 planes
-  static constexpr int PLANES = 3;
+struct F32 {  // products as three bf16 planes; accumulators among the other registers, of which the tiles leave enough
+  typedef float t;
+  static constexpr bool WIDE = true;
+  static __device__ __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  }
 };
 struct F16 {
   typedef _Float16 t;
-  static constexpr int PLANES = 1;
+  static constexpr bool WIDE = false;
   static __device__ __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
 // the compiler does not know that the results take a few cycles more
-template <int FI, int FJ>
+template <class T, int FI, int FJ>
 __device__ __forceinline__ void mfma_done(f32x4 (&acc)[FI][FJ]) {
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
   for (int i = 0; i < FI; ++i)
 #pragma unroll
-    for (int j = 0; j < FJ; ++j) asm volatile("" : "+a"(acc[i][j]));
+    for (int j = 0; j < FJ; ++j) {
+      if constexpr (T::WIDE)
+        asm volatile("" : "+v"(acc[i][j]));
+      else
+        asm volatile("" : "+a"(acc[i][j]));
+    }
 }
 
 template <class T>
@@ -72,7 +85,7 @@ __device__ __forceinline__ short to16(float x) {
 // 16-bit types: 2^x by the hardware (2^-22 relative); f32: the library's e^x
 template <class T>
 __device__ __forceinline__ float head_exp(float x) {
-  return T::PLANES == 3 ? expf(x) : __builtin_amdgcn_exp2f(x);
+  return T::WIDE ? expf(x) : __builtin_amdgcn_exp2f(x);
 }
 
 constexpr int K_PAD = 64;      // packed operands hold zeros up to a multiple of this along the contraction
@@ -80,14 +93,13 @@ constexpr int DZ_PAD = 128;    // rows of dz
 constexpr int HEAD_PAD = 256;  // packed rows are padded to a multiple of the largest tile
 
 // One side of a product.  Plain side: element (r, k) at base[r * ld + k]; transposed side: base[k * ld + r].  Rows behind
-// rlim are read as the last one (their results are not stored), and so are k behind klim: there the other side, which
-// is always a packed one, holds zeros up to the next multiple of K_PAD.
+// rlim are read as the last one (their results are not stored).  16 bits: so are k behind klim, where the other side,
+// which is always a packed one, holds zeros up to the next multiple of K_PAD.
 struct Side {
-  const short* base;
-  int64_t plane;  // elements between the planes of a split f32 operand
+  const void* base;  // 16 bits or f32
   int64_t ld;
-  int rlim;       // transposed: a multiple of 8
-  int klim;       // plain: a multiple of 8
+  int rlim;          // 16 bits, transposed: a multiple of 8
+  int klim;          // 16 bits, plain: a multiple of 8
 };
 
 enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
@@ -107,8 +119,8 @@ struct GemmArgs {
   int64_t stat_ld;
   const float* lse;
   const float* cp;      // coef * P of each packed row
-  short* dz;            // [planes][rows][ldz]
-  int64_t dz_plane, ldz;
+  void* dz;             // [rows][ldz], 16 bits or f32
+  int64_t ldz;
   // EPI_OUT
   int out_kind;
   float* acc;           // OUT_F32 / OUT_ADD target, [split][n][acc_ld]; OUT_FINAL: added when not null
@@ -166,7 +178,7 @@ struct Stager {
   unsigned off[CW];    // bytes from there to this lane's 16, 32 bits (leading dimensions are at most HEAD_MAX_LD)
   int k_of[CW];        // the (first) k of those
   __device__ __forceinline__ void init(const Side& s, int r0, const void* lds, int wave, int lane) {
-    base = (const char*)(TR ? s.base : s.base + (int64_t)r0 * s.ld);
+    base = (const char*)s.base + (TR ? 0 : (int64_t)r0 * s.ld * 2);
 #pragma unroll
     for (int q = 0; q < CW; ++q) {
       const int c = (wave * CW + q) % PIECES;
@@ -232,6 +244,126 @@ struct Reader {
   }
 };
 
+// The last step of a product, a wave at a time.  acc[i][j][r]: n = n0 + 16 j + lane % 16, m = m0 + 16 i + 4 (lane / 16) + r
+// (EIGHT: m0 + 32 (i / 2) + 8 (lane / 16) + 4 (i % 2) + r) -- a lane holds four or eight neighbours along m.
+template <class T, int EPI, bool EIGHT, int FI, int FJ>
+__device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI][FJ], int m0, int n0, int lane, int N, int split,
+                                              int64_t stat_row) {
+  const int mw = m0 + (EIGHT ? 8 : 4) * (lane >> 4), nw = n0 + (lane & 15);
+  const auto m_of = [&](int i) { return mw + (EIGHT ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i); };
+  static_assert(DZ_PAD % (16 * FI) == 0);
+  if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
+    // in units of the exponential: natural for f32, of two for the 16-bit types
+    const float unit = T::WIDE ? 1.f : 1.4426950408889634f, scale = g.inv_tau * unit;
+    float bias[FI][4];  // times scale; -inf behind the last class
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bias[i][r] = m_of(i) + r < g.M ? 0.f : -INFINITY;
+    if (g.bias) {
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = min(m_of(i) + r, g.M - 1);
+          bias[i][r] += scale * (T::WIDE ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int n = nw + 16 * j;
+      if constexpr (EPI == EPI_STATS) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            acc[i][j][r] = fmaf(acc[i][j][r], scale, bias[i][r]);
+            top = fmaxf(top, acc[i][j][r]);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        float sum = 0.f;
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum += head_exp<T>(acc[i][j][r] - ref);  // a NaN stays in the sum
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lane < 16 && n < N) g.stats[stat_row * g.stat_ld + n] = make_float2(top / unit, sum);
+      } else if (m0 < g.ldz) {  // all or nothing of a wave's columns, of which DZ_PAD is a multiple
+        const bool live = n < N;
+        const float lse = live ? g.lse[n] * unit : 0.f, cp = live ? g.cp[n] : 0.f;
+        typedef typename std::conditional<T::WIDE, float, short>::type W;
+        W* out = (W*)g.dz + (int64_t)n * g.ldz;
+        constexpr int GROUP = EIGHT ? 2 : 1;
+#pragma unroll
+        for (int i0 = 0; i0 < FI; i0 += GROUP) {
+          W w[4 * GROUP];
+#pragma unroll
+          for (int e = 0; e < 4 * GROUP; ++e) {
+            const int i = i0 + e / 4, r = e % 4;
+            // Rounded to the 16-bit type (half a step, 2^-8 bf16 / 2^-11 f16, of each element; f16 after scaling by a
+            // power of two): the size of the rounding that the gradients themselves get.
+            float x = cp * head_exp<T>(fmaf(acc[i][j][r], scale, bias[i][r]) - lse);
+            x = live ? x : 0.f;
+            if constexpr (T::WIDE)
+              w[e] = x;
+            else
+              w[e] = to16<T>(x);
+          }
+          __builtin_memcpy(__builtin_assume_aligned(out + m_of(i0), sizeof(w)), w, sizeof(w));
+        }
+      }
+    }
+  } else {
+    const float inv = g.inv_scale ? *g.inv_scale : 1.f;
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int n = nw + 16 * j;
+      if (n >= N) continue;
+      float* arow = g.acc ? g.acc + split * g.acc_split + (int64_t)n * g.acc_ld : nullptr;
+      const int64_t orow = (int64_t)(g.rowmap ? g.rowmap[n] : n) * g.out_ld;
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+        const int m = m_of(i);
+        f32x4 x = acc[i][j];
+        if (m >= g.M) continue;
+        if (g.out_kind != OUT_FINAL) {  // acc rows are padded to a multiple of 4
+          f32x4* dst = (f32x4*)(arow + m);
+          *dst = g.out_kind == OUT_ADD ? *dst + x : x;
+          continue;
+        }
+        if (arow) x += *(const f32x4*)(arow + m);
+        x *= inv;
+        if constexpr (T::WIDE) {
+          float* o = (float*)g.out + orow + m;
+          if (m + 4 <= g.M && !(((uintptr_t)o) & 15)) {
+            *(f32x4*)o = x;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (m + r < g.M) o[r] = x[r];
+          }
+        } else {
+          s16x4 w;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[r] = to16<T>(x[r]);
+          short* o = (short*)g.out + orow + m;
+          if (m + 4 <= g.M && !(((uintptr_t)o) & 7)) {
+            *(s16x4*)o = w;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (m + r < g.M) o[r] = w[r];
+          }
+        }
+      }
+    }
+  }
+}
+
 template <class T, int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
@@ -245,9 +377,8 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   if (n0 >= (EPI == EPI_DZ ? (N + K_PAD - 1) / K_PAD * K_PAD : N)) return;
   const int K = g.k_dev ? min(g.K, *g.k_dev) : g.K;
   const int ktiles = (K + BK - 1) / BK;
-  const int total = ktiles * (T::PLANES == 3 ? 6 : 1);
-  const int per = (total + g.splits - 1) / g.splits;
-  const int t0 = min(split * per, total), t1 = min(t0 + per, total);
+  const int per = (ktiles + g.splits - 1) / g.splits;
+  const int t0 = min(split * per, ktiles), t1 = min(t0 + per, ktiles);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -266,20 +397,12 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   for (int i = 0; i < FI; ++i)
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  mfma_done(acc);  // written, before the first matrix instruction reads them
+  mfma_done<T>(acc);  // written, before the first matrix instruction reads them
 
-  // plane pairs, smallest products first: (l, h) (h, l) (m, m) (m, h) (h, m) (h, h)
-  // The tiles are issued in order: `at_a`, `at_b` walk along k, then to the next pair of planes.
+  // The tiles are issued in order: `at_a`, `at_b` walk along k.
   const int64_t step_a = BK * 2 * (TRA ? g.A.ld : 1), step_b = BK * 2 * (TRB ? g.B.ld : 1);
-  int pair = T::PLANES == 3 ? t0 / max(1, ktiles) : 0, kt = t0 - pair * ktiles;
-  const char *at_a = nullptr, *at_b = nullptr;
-  const auto aim = [&] {
-    const int pa = T::PLANES == 3 ? (0x001102 >> (4 * pair)) & 3 : 0;
-    const int pb = T::PLANES == 3 ? (0x010120 >> (4 * pair)) & 3 : 0;
-    at_a = sa.base + pa * g.A.plane * 2 + kt * step_a;
-    at_b = sb.base + pb * g.B.plane * 2 + kt * step_b;
-  };
-  aim();
+  int kt = t0;
+  const char *at_a = sa.base + kt * step_a, *at_b = sb.base + kt * step_b;
   int left = t1 - t0;  // tiles that are still to be issued; behind the last one it is issued again, for the count of loads
   const auto issue = [&](auto stage, int q) {
     if (q >= sa.CW)
@@ -291,11 +414,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
     if (q == sa.CW + sb.CW - 1 && --left > 0) {
       at_a += step_a;
       at_b += step_b;
-      if (++kt == ktiles && T::PLANES == 3) {
-        kt = 0;
-        ++pair;
-        aim();
-      }
+      ++kt;
     }
   };
   const auto issue_all = [&](auto stage) {
@@ -363,125 +482,192 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles issued again
   }
-  mfma_done(acc);
+  mfma_done<T>(acc);
 
-  // acc[i][j][r]: n = .. + 16 j + lane % 16, m = .. + 16 i + 4 (lane / 16) + r (EIGHT: .. + 32 (i / 2) + 8 (lane / 16) +
-  // 4 (i % 2) + r) -- a lane holds four or eight neighbours along m
-  const int mw = m0 + wm * WTM + (EIGHT ? 8 : 4) * (lane >> 4), nw = n0 + wn * WTN + (lane & 15);
-  const auto m_of = [&](int i) { return mw + (EIGHT ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i); };
-  static_assert(DZ_PAD % WTM == 0);
-  if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
-    // in units of the exponential: natural for f32, of two for the 16-bit types
-    const float unit = T::PLANES == 3 ? 1.f : 1.4426950408889634f, scale = g.inv_tau * unit;
-    float bias[FI][4];  // times scale; -inf behind the last class
+  head_epilogue<T, EPI, EIGHT>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, split, tm * WM + wm);
+}
+
+// ---- products of f32 operands -----------------------------------------------------------------------------
+// x = h + m + l: three bf16 values, exact for 24 bits; an infinity becomes NaN.  Two at a time.
+__device__ __forceinline__ void split3(float x, float y, unsigned (&w)[3]) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
+  for (int pl = 0; pl < 3; ++pl) {
+    w[pl] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{x, y}), bf16x2));
+    x -= __uint_as_float(w[pl] << 16);
+    y -= __uint_as_float(w[pl] & 0xffff0000u);
+  }
+}
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// A thread's share of a 32-deep tile of one side: a block of four rows and eight k, fetched into registers and stored as
+// three planes of bf16.  A unit u of 16 bytes in LDS holds the k 4 u .. 4 u + 3 and 16 + 4 u .. (both sides alike, so that
+// the order does not matter): four lanes fetch 64 neighbouring bytes of a row.  Row r has the slot r ^ (r / 16 & 3), which
+// spreads the stores of a transposed side (four neighbouring rows a lane) over all banks.
+template <int BT, bool TR>
+struct Splitter {
+  const float* base;
+  unsigned off[4];  // of the thread's rows
+  unsigned first;   // transposed: of the four at the first of its k
+  int u, row;       // transposed: the first of the four; plain: the rows are row + BT / 4 * j
+  bool whole;       // transposed: all four exist
+  __device__ __forceinline__ void init(const Side& s, int r0, int block) {
+    u = TR ? block / (BT / 4) : block & 3;
+    row = TR ? block % (BT / 4) * 4 : block >> 2;
+    base = (const float*)s.base + (TR ? (int64_t)r0 : (int64_t)r0 * s.ld);
+    whole = r0 + row + 4 <= s.rlim;
+    first = TR ? 4 * u * (unsigned)s.ld + row : 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) bias[i][r] = m_of(i) + r < g.M ? 0.f : -INFINITY;
-    if (g.bias) {
+    for (int j = 0; j < 4; ++j)
+      off[j] = TR ? (unsigned)min(row + j, s.rlim - 1 - r0) : (unsigned)min(row + BT / 4 * j, s.rlim - 1 - r0) * (unsigned)s.ld;
+  }
+  // keeps the rare path's addresses out of the loop's registers
+  static __device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  }
+  // plain: x[2 j], x[2 j + 1] are row j; transposed: x[i] are the four rows at its i-th k; zeros from klim on
+  __device__ __forceinline__ void load(const Side& s, int k0, int klim, f32x4 (&x)[8]) const {
+    if constexpr (!TR) {
+      const float* p = base + k0;
+      if (k0 + BK <= klim) {
 #pragma unroll
-      for (int i = 0; i < FI; ++i)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int m = min(m_of(i) + r, g.M - 1);
-          bias[i][r] += scale * (T::PLANES == 3 ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m]);
-        }
-    }
+          for (int q = 0; q < 2; ++q) x[2 * j + q] = *(const f32x4_any*)(p + off[j] + 16 * q + 4 * u);
+      } else {
+        const int have = klim - k0, k4 = opaque(4 * u);
 #pragma unroll
-    for (int j = 0; j < FJ; ++j) {
-      const int n = nw + 16 * j;
-      if constexpr (EPI == EPI_STATS) {
-        float top = -INFINITY;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < FI; ++i)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            acc[i][j][r] = fmaf(acc[i][j][r], scale, bias[i][r]);
-            top = fmaxf(top, acc[i][j][r]);
-          }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        float sum = 0.f;
-        const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int i = 0; i < FI; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sum += head_exp<T>(acc[i][j][r] - ref);  // a NaN stays in the sum
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (lane < 16 && n < N) g.stats[(int64_t)(tm * WM + wm) * g.stat_ld + n] = make_float2(top / unit, sum);
-      } else if (m0 + wm * WTM < g.ldz) {  // all or nothing of a wave's columns, of which DZ_PAD is a multiple
-        const bool live = n < N;
-        const float lse = live ? g.lse[n] * unit : 0.f, cp = live ? g.cp[n] : 0.f;
-        short* out = g.dz + (int64_t)n * g.ldz;
-        constexpr int GROUP = EIGHT ? 2 : 1;
-#pragma unroll
-        for (int i0 = 0; i0 < FI; i0 += GROUP) {
-          short w[T::PLANES][4 * GROUP];
-#pragma unroll
-          for (int e = 0; e < 4 * GROUP; ++e) {
-            const int i = i0 + e / 4, r = e % 4;
-            // Rounded to the 16-bit type (half a step, 2^-8 bf16 / 2^-11 f16, of each element; f16 after scaling by a
-            // power of two): the size of the rounding that the gradients themselves get.  f32: three exact planes.
-            float x = cp * head_exp<T>(fmaf(acc[i][j][r], scale, bias[i][r]) - lse);
-            x = live ? x : 0.f;
-#pragma unroll
-            for (int pl = 0; pl < T::PLANES; ++pl) {
-              const short h = to16<T>(x);
-              w[pl][e] = h;
-              x -= (float)__builtin_bit_cast(typename T::t, h);
+            for (int e = 0; e < 4; ++e) {
+              const int k = 16 * q + k4 + e;
+              const float y = p[off[j] + (unsigned)min(k, have - 1)];
+              x[2 * j + q][e] = k < have ? y : 0.f;
             }
-          }
-#pragma unroll
-          for (int pl = 0; pl < T::PLANES; ++pl) __builtin_memcpy(out + pl * g.dz_plane + m_of(i0), w[pl], 8 * GROUP);
-        }
       }
-    }
-  } else {
-    const float inv = g.inv_scale ? *g.inv_scale : 1.f;
+    } else {
+      const float* p = base + (int64_t)k0 * s.ld;
+      const unsigned ld = (unsigned)s.ld;
+      if (k0 + BK <= klim && whole) {
 #pragma unroll
-    for (int j = 0; j < FJ; ++j) {
-      const int n = nw + 16 * j;
-      if (n >= N) continue;
-      float* arow = g.acc ? g.acc + split * g.acc_split + (int64_t)n * g.acc_ld : nullptr;
-      const int64_t orow = (int64_t)(g.rowmap ? g.rowmap[n] : n) * g.out_ld;
+        for (int i = 0; i < 8; ++i) x[i] = *(const f32x4_any*)(p + (16 * (i >> 2) + (i & 3)) * s.ld + first);
+      } else {
+        const int have = klim - k0, k4 = opaque(4 * u);
 #pragma unroll
-      for (int i = 0; i < FI; ++i) {
-        const int m = m_of(i);
-        f32x4 x = acc[i][j];
-        if (m >= g.M) continue;
-        if (g.out_kind != OUT_FINAL) {  // acc rows are padded to a multiple of 4
-          f32x4* dst = (f32x4*)(arow + m);
-          *dst = g.out_kind == OUT_ADD ? *dst + x : x;
-          continue;
-        }
-        if (arow) x += *(const f32x4*)(arow + m);
-        x *= inv;
-        if constexpr (T::PLANES == 3) {
-          float* o = (float*)g.out + orow + m;
-          if (m + 4 <= g.M && !(((uintptr_t)o) & 15)) {
-            *(f32x4*)o = x;
-          } else {
+        for (int i = 0; i < 8; ++i) {
+          const int k = 16 * (i >> 2) + k4 + (i & 3);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (m + r < g.M) o[r] = x[r];
-          }
-        } else {
-          s16x4 w;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) w[r] = to16<T>(x[r]);
-          short* o = (short*)g.out + orow + m;
-          if (m + 4 <= g.M && !(((uintptr_t)o) & 7)) {
-            *(s16x4*)o = w;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (m + r < g.M) o[r] = w[r];
+          for (int j = 0; j < 4; ++j) {
+            const float y = p[(unsigned)min(k, have - 1) * ld + off[j]];
+            x[i][j] = k < have ? y : 0.f;
           }
         }
       }
     }
   }
+  __device__ __forceinline__ void store(char* lds, const f32x4 (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = TR ? row + j : row + BT / 4 * j;
+      u32x4 w[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        unsigned t[3];
+        split3(TR ? x[2 * e][j] : x[2 * j + e / 2][2 * e & 3], TR ? x[2 * e + 1][j] : x[2 * j + e / 2][2 * e + 1 & 3], t);
+        w[0][e] = t[0], w[1][e] = t[1], w[2][e] = t[2];
+      }
+      char* at = lds + (r ^ (r >> 4 & 3)) * 64 + (u ^ row_swizzle(r >> 2)) * 16;
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl) *(u32x4*)(at + pl * BT * 64) = w[pl];
+      __builtin_amdgcn_sched_barrier(0);  // a row at a time: registers
+    }
+  }
+};
+
+// The same products for f32: each workgroup splits the tiles that it reads (four bytes an element from memory, whatever the
+// planes), and the fragments of three planes serve six products.  One LDS stage of 32 k; the loads of the next two tiles are
+// in flight under the products, and the CU's other workgroup fills the waits.  4000 x 2048 x 50000: 196 TFLOP/s of the
+// operands' products (planes split beforehand, copied by the 16-bit kernel: 155; the library's f32: 153); 1 x 2048 x
+// 131072, forward and backward: 0.81 ms (planes split beforehand: 3.64, 10 bytes an element a pass).
+template <int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
+__global__ __launch_bounds__(256, 2) void head_gemm32_kernel(GemmArgs g) {
+  static_assert(WM * WN == 4 && BM + BN <= 256 && BM % 64 == 0 && BN % 64 == 0);
+  constexpr int WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
+  static_assert(WTM % 64 == 0 || (WTM == 32 && FI <= 2));
+  __shared__ __attribute__((aligned(1024))) char lds_a[3 * BM * 64];
+  __shared__ __attribute__((aligned(1024))) char lds_b[3 * BN * 64];
+  int split, tm, tn;
+  tile_of(blockIdx.x, gridDim.x, g.mt, g.nt, split, tm, tn);
+  const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
+  const int m0 = tm * BM, n0 = tn * BN;
+  if (n0 >= N) return;
+  const int K = g.k_dev ? min(g.K, *g.k_dev) : g.K;
+  const int ktiles = (K + BK - 1) / BK;
+  const int per = (ktiles + g.splits - 1) / g.splits;
+  const int t0 = min(split * per, ktiles), t1 = min(t0 + per, ktiles);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  // the first waves fetch A, the others B
+  Splitter<BM, TRA> sa;
+  Splitter<BN, TRB> sb;
+  const bool for_a = wave < BM / 64, for_b = !for_a && wave < (BM + BN) / 64;
+  sa.init(g.A, m0, for_a ? threadIdx.x : 0);
+  sb.init(g.B, n0, for_b ? threadIdx.x - BM : 0);
+  f32x4 x0[8], x1[8];
+  const auto load = [&](int t, f32x4(&x)[8]) {
+    if (for_a)
+      sa.load(g.A, t * BK, K, x);
+    else if (for_b)
+      sb.load(g.B, t * BK, K, x);
+  };
+  const auto fragment = [&](const char* lds, int rows, int w0, int pl, int i) {
+    const int r = lane & 15, at = w0 / 16 + i;
+    return *(const s16x8*)(lds + pl * rows * 64 + (w0 + 16 * i + (r ^ (at & 3))) * 64 + ((lane >> 4) ^ row_swizzle(r >> 2)) * 16);
+  };
+  f32x4 acc[FI][FJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  mfma_done<F32>(acc);  // written, before the first matrix instruction reads them
+  const auto step = [&](int t, f32x4(&x)[8]) {
+    if (for_a)
+      sa.store(lds_a, x);
+    else if (for_b)
+      sb.store(lds_b, x);
+    __syncthreads();
+    if (t + 2 < t1) load(t + 2, x);
+    s16x8 a[FI][3];
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl) a[i][pl] = fragment(lds_a, BM, wm * WTM, pl, i);
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      s16x8 b[3];
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl) b[pl] = fragment(lds_b, BN, wn * WTN, pl, j);
+      // smallest products first: (l, h) (h, l) (m, m) (m, h) (h, m) (h, h)
+#pragma unroll
+      for (int q = 0; q < 6; ++q)
+#pragma unroll
+        for (int i = 0; i < FI; ++i) F32::mfma(acc[i][j], a[i][(0x001102 >> (4 * q)) & 3], b[(0x010120 >> (4 * q)) & 3]);
+    }
+    __syncthreads();
+  };
+  if (t0 < t1) load(t0, x0);
+  if (t0 + 1 < t1) load(t0 + 1, x1);
+  for (int t = t0; t < t1; t += 2) {
+    step(t, x0);
+    if (t + 1 < t1) step(t + 1, x1);
+  }
+  mfma_done<F32>(acc);
+  head_epilogue<F32, EPI, false>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, split, tm * WM + wm);
 }
 
 // ---- the rows that count ------------------------------------------------------------------------------
@@ -524,61 +710,31 @@ __global__ __launch_bounds__(1024) void head_rows_kernel(Targets tg, const int64
     }
 }
 
-// x = h + m + l: three bf16 values, exact for 24 bits; an infinity becomes NaN
-__device__ __forceinline__ void split3(float x, short (&w)[3]) {
-#pragma unroll
-  for (int pl = 0; pl < 3; ++pl) {
-    const __bf16 h = (__bf16)x;
-    w[pl] = __builtin_bit_cast(short, h);
-    x -= (float)h;
-  }
-}
-
-// dst[plane][0 .. ldd) = src[0 .. d) by one block of 256, zeros behind d (everywhere: have = false)
-template <bool F32>
-__device__ __forceinline__ void pack_row(const void* src, bool have, int d, short* dst, int64_t plane, int ldd) {
-  for (int c = threadIdx.x * 8; c < ldd; c += 256 * 8) {
-    s16x8 w[F32 ? 3 : 1];
-#pragma unroll
-    for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) w[pl] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+// dst[0 .. ldd) = src[0 .. d) by one block of 256, zeros behind d (everywhere: have = false)
+template <typename W>
+__device__ __forceinline__ void pack_row(const W* src, bool have, int d, W* dst, int ldd) {
+  constexpr int V = 16 / sizeof(W);
+  for (int c = threadIdx.x * V; c < ldd; c += 256 * V) {
+    vec4f w = {0.f, 0.f, 0.f, 0.f};
     if (have && c < d) {
-      if constexpr (F32) {
-        const float* p = (const float*)src + c;
-        float x[8];
-        if (c + 8 <= d && !((uintptr_t)p & 15)) {
-          *(f32x4*)x = ((const f32x4*)p)[0];
-          *(f32x4*)(x + 4) = ((const f32x4*)p)[1];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = c + e < d ? p[e] : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          short t[3];
-          split3(x[e], t);
-          w[0][e] = t[0], w[1][e] = t[1], w[2][e] = t[2];
-        }
+      if (c + V <= d && !((uintptr_t)(src + c) & 15)) {
+        w = *(const vec4f*)(src + c);
       } else {
-        const short* p = (const short*)src + c;
-        if (c + 8 <= d && !((uintptr_t)p & 15)) {
-          w[0] = *(const s16x8*)p;
-        } else {
+        W x[V];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[0][e] = c + e < d ? p[e] : (short)0;
-        }
+        for (int e = 0; e < V; ++e) x[e] = c + e < d ? src[c + e] : (W)0;
+        __builtin_memcpy(&w, x, 16);
       }
     }
-#pragma unroll
-    for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) *(s16x8*)(dst + pl * plane + c) = w[pl];
+    *(vec4f*)(dst + c) = w;
   }
 }
 
 // the weight rows of a piece, a block each
-template <bool F32>
-__global__ __launch_bounds__(256) void head_pack_kernel(const void* __restrict__ src, int64_t lds, int d, short* __restrict__ dst,
-                                                        int64_t plane, int ldd) {
+template <typename W>
+__global__ __launch_bounds__(256) void head_pack_kernel(const W* __restrict__ src, int64_t lds, int d, W* __restrict__ dst, int ldd) {
   const int64_t i = blockIdx.x;
-  pack_row<F32>((const char*)src + i * lds * (F32 ? 4 : 2), true, d, dst + i * ldd, plane, ldd);
+  pack_row<W>(src + i * lds, true, d, dst + i * ldd, ldd);
 }
 
 // The targets' logits u = (hidden . weight[at] + bias) / tau as dot products of the inputs, in 32 bits: a wave for eight
@@ -626,14 +782,15 @@ __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const
 template <int DT>
 __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int d,
                                                              const int* __restrict__ rows, const int* __restrict__ count,
-                                                             short* __restrict__ dst, int64_t plane, int ldd,
-                                                             const void* __restrict__ weight, int64_t ldw, const void* __restrict__ bias,
-                                                             Targets tg, float* __restrict__ uk) {
+                                                             void* __restrict__ dst, int ldd, const void* __restrict__ weight,
+                                                             int64_t ldw, const void* __restrict__ bias, Targets tg,
+                                                             float* __restrict__ uk) {
+  typedef typename std::conditional<DT == NIF_F32, float, short>::type W;
   const int64_t i = blockIdx.x;
   const bool have = i < *count;
   const int64_t src = have ? rows[i] : 0;
   const typename Elem<DT>::t* h = (const typename Elem<DT>::t*)hidden + src * ldh;
-  pack_row<DT == NIF_F32>(h, have, d, dst + i * ldd, plane, ldd);
+  pack_row<W>((const W*)h, have, d, (W*)dst + i * ldd, ldd);
   if (!have) return;
   for (int k0 = (threadIdx.x >> 6) * DOTS; k0 < tg.k; k0 += 4 * DOTS)
     target_dots<DT>(h, weight, ldw, bias, d, tg, src, k0, uk + i * tg.k, threadIdx.x & 63);
@@ -728,7 +885,7 @@ template <class T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
                                                            const float* __restrict__ uk, const float* __restrict__ lse,
                                                            const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
-                                                           short* __restrict__ dz, int64_t dz_plane, int64_t ldz) {
+                                                           void* __restrict__ dz, int64_t ldz) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (i >= *count) return;
   const int64_t src = rows[i];
@@ -751,21 +908,17 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int
       }
     }
     if (!mine || !first) continue;
-    float x = cp[i] * expf(uk[(int64_t)i * tg.k + k] - lse[i]) - coef[i] * sum;
-#pragma unroll
-    for (int pl = 0; pl < T::PLANES; ++pl) {
-      const short w = to16<T>(x);
-      dz[pl * dz_plane + (int64_t)i * ldz + (v - v0)] = w;
-      x -= (float)__builtin_bit_cast(typename T::t, w);
-    }
+    const float x = cp[i] * expf(uk[(int64_t)i * tg.k + k] - lse[i]) - coef[i] * sum;
+    ((typename T::t*)dz)[(int64_t)i * ldz + (v - v0)] = (typename T::t)x;
   }
 }
 
 // dbias of a piece: column sums of dz over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
 // head_bias_join_kernel.  Bound by the read of dz.
 template <class T>
-__global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict__ dz, int64_t dz_plane, int64_t ldz, int cols,
+__global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __restrict__ dz, int64_t ldz, int cols,
                                                         const int* __restrict__ count, int stretch, float* __restrict__ part) {
+  typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   __shared__ float sh[8][256 + 8];
   const int c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8, group = threadIdx.x >> 5;
   const int r0 = blockIdx.y * stretch, r1 = min(*count, r0 + stretch);
@@ -773,13 +926,11 @@ __global__ __launch_bounds__(256) void head_bias_kernel(const short* __restrict_
   float s[8] = {};
   if (c0 < ldz)
 #pragma unroll 4
-    for (int r = r0 + group; r < r1; r += 8)
+    for (int r = r0 + group; r < r1; r += 8) {
+      const Eight x = *(const Eight*)(dz + (int64_t)r * ldz + c0);
 #pragma unroll
-      for (int pl = 0; pl < T::PLANES; ++pl) {
-        const s16x8 x = *(const s16x8*)(dz + pl * dz_plane + (int64_t)r * ldz + c0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += (float)__builtin_bit_cast(typename T::t, (short)x[e]);
-      }
+      for (int e = 0; e < 8; ++e) s[e] += (float)x[e];
+    }
 #pragma unroll
   for (int e = 0; e < 8; ++e) sh[group][(threadIdx.x & 31) * 8 + e] = s[e];
   __syncthreads();
@@ -799,10 +950,7 @@ __global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __rest
 #pragma unroll 8
   for (int q = 0; q < stretches; ++q) s += part[(int64_t)q * cols + c];
   s *= *inv_scale;
-  if (T::PLANES == 3)
-    ((float*)out)[c] = s;
-  else
-    ((short*)out)[c] = to16<T>(s);
+  ((typename T::t*)out)[c] = (typename T::t)s;
 }
 
 // out = (sum of the splits' partial sums, in order, + acc) * inv_scale, or acc = that sum: 4 columns a thread, 1024 a block
@@ -826,12 +974,72 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
   const int64_t o = (int64_t)(rowmap ? rowmap[i] : i) * out_ld + c;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (c + e < m) {
-      if constexpr (T::PLANES == 3)
-        ((float*)out)[o + e] = s[e];
-      else
-        ((short*)out)[o + e] = to16<T>(s[e]);
+    if (c + e < m) ((typename T::t*)out)[o + e] = (typename T::t)s[e];
+}
+
+// ---- kept logits ------------------------------------------------------------------------------------------------
+// u = (the splits' partial sums, in order, + bias) / tau, kept in 32 bits, and its (maximum, sum of exponentials) over
+// stretches of KEPT classes: a block a stretch of one packed row.
+constexpr int KEPT = 1024;
+template <class T>
+__global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict__ part, int splits, int64_t part_split, float* __restrict__ u,
+                                                        int64_t ldu, int v, const int* __restrict__ count, const void* __restrict__ bias,
+                                                        float inv_tau, float2* __restrict__ stats, int64_t stat_ld) {
+  __shared__ float sh_top[4], sh_sum[4];
+  const int64_t i = blockIdx.x;
+  if (i >= *count) return;
+  const int c = blockIdx.y * KEPT + threadIdx.x * 4;
+  f32x4 x = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (c < v) {  // rows are padded to a multiple of 4
+    f32x4* at = (f32x4*)(u + i * ldu + c);
+    f32x4 z;
+    if (splits > 1) {
+      z = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+      for (int q = 0; q < splits; ++q) z += *(const f32x4*)(part + q * part_split + i * ldu + c);
+    } else {
+      z = *at;
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < v) x[e] = (z[e] + (bias ? (float)((const typename T::t*)bias)[c + e] : 0.f)) * inv_tau;
+    *at = x;
+  }
+  float top = wave_max_f32(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+  const float ref = top == -INFINITY ? 0.f : top;
+  const float sum = wave_sum_f32(expf(x[0] - ref) + expf(x[1] - ref) + expf(x[2] - ref) + expf(x[3] - ref));  // a NaN stays in the sum
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) sh_top[wave] = top, sh_sum[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float s = sum;
+    for (int w = 1; w < 4; ++w) join(top, s, sh_top[w], sh_sum[w]);
+    stats[blockIdx.y * stat_ld + i] = make_float2(top, s);
+  }
+}
+
+// dz = cp exp(u - lse) of a piece of the classes, 8 a thread; zeros up to a multiple of K_PAD rows and in the padding of the
+// columns, where the products read them.  Rounded as head_gemm_kernel's.
+template <class T>
+__global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ u, int64_t ldu, int cols, const int* __restrict__ count,
+                                                           const float* __restrict__ lse, const float* __restrict__ cp,
+                                                           typename T::t* __restrict__ dz, int64_t ldz) {
+  typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
+  const int i = blockIdx.x, n = *count, c = blockIdx.y * 2048 + threadIdx.x * 8;
+  if (i >= (n + K_PAD - 1) / K_PAD * K_PAD || c >= ldz) return;
+  Eight w;
+  const bool live = i < n;
+  const float l = live ? lse[i] : 0.f, k = live ? cp[i] : 0.f;
+  const float* x = u + i * ldu + c;
+  if (live && c + 8 <= cols) {
+    const f32x4 lo = *(const f32x4*)x, hi = *(const f32x4*)(x + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(k * expf((e < 4 ? lo[e & 3] : hi[e & 3]) - l));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(live && c + e < cols ? k * expf(x[e] - l) : 0.f);
+  }
+  *(Eight*)(dz + (int64_t)i * ldz + c) = w;
 }
 
 // ---- small heads ----------------------------------------------------------------------------------------------
@@ -1013,12 +1221,15 @@ static inline int64_t round_up(int64_t x, int64_t q) { return (x + q - 1) / q * 
 
 struct Plan {
   int64_t n, cap;
-  int d, ldd, v, planes, k;
-  bool pack_w;       // the weight is copied by pieces: f32, or rows that 16-byte loads cannot take
+  int d, ldd, v, k;
+  int e;             // bytes of an operand's element
+  bool pack_w;       // the weight is copied by pieces: rows that the loads cannot take
   bool small;        // the small heads' kernels
+  bool keep;         // few rows: the logits are kept
   int piece;         // classes per piece (multiple of 256, or all)
   // state: what the backward pass reads
-  size_t s_p, s_at, s_P, s_dz, s_fcount, s_rows, s_inv, s_count, s_lse, s_uk, s_h, state;
+  size_t s_p, s_at, s_P, s_dz, s_fcount, s_rows, s_inv, s_count, s_lse, s_uk, s_h, s_u, state;
+  int64_t ldu;       // of the kept logits
 };
 
 static constexpr size_t PIECE_BYTES = (size_t)256 << 20;
@@ -1027,6 +1238,64 @@ static size_t take(size_t& at, size_t bytes) {
   const size_t r = at;
   at += (bytes + 255) / 256 * 256;
   return r;
+}
+
+struct Shape {
+  int bm, bn, wm, splits;
+  float us;  // what the model says
+};
+struct Tile {
+  int bm, bn, wm, per_cu;
+  float step, share, fixed, rate;
+};
+static const Tile TILES16[] = {
+    {256, 256, 2, 1, 0.81f, 0.f, 11.f, 4.0f},
+    {128, 128, 2, 2, 0.06f, 0.295f, 5.9f, 3.5f},
+    {128, 64, 4, 3, 0.08f, 0.174f, 4.3f, 3.9f},
+};
+static const Tile TILES32[] = {
+    {128, 128, 2, 2, 1.05f, 0.85f, 4.f, 3.7f},
+    {128, 64, 4, 2, 0.8f, 0.53f, 4.f, 3.7f},
+};
+// m x n results of a contraction over k, `e` bytes an element; `results`: bytes of one that is written (0: they are reduced)
+static Shape shape_of(int64_t m, int64_t n, int64_t k, int e, int results, bool may_split) {
+  const int64_t steps = (k + BK - 1) / BK;
+  Shape best = {128, 128, 2, 1, INFINITY};
+  const Tile* tiles = e == 4 ? TILES32 : TILES16;
+  for (int i = 0; i < (e == 4 ? 2 : 3); ++i) {
+    const Tile& t = tiles[i];
+    const int64_t count = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+    for (int splits = 1; splits <= (may_split ? 32 : 1); splits *= 2) {
+      if (splits > 1 && steps / splits < 8) break;
+      const int64_t blocks = count * splits, slots = 256 * t.per_cu, rest = blocks % slots;
+      const float each = (float)((steps + splits - 1) / splits);
+      float us = (float)(blocks / slots) * (each * (t.step + t.share * (float)t.per_cu) + t.fixed);
+      if (rest) us += each * (t.step + t.share * (float)((rest + 255) / 256)) + t.fixed;
+      const float in = (float)(m + n) * (float)k * (float)e;
+      const float out = !results ? 0.f : (float)m * (float)n * (splits > 1 ? 4.f * (float)splits : (float)results);
+      const float memory = (in + out) * 1e-6f / t.rate + 2.f;
+      us = us > memory ? us : memory;
+      if (splits > 1) us += 4.f + out * 1e-6f / 4.f;
+      if (us < best.us) best = {t.bm, t.bn, t.wm, splits, us};
+    }
+  }
+  return best;
+}
+
+static Shape logit_shape(const Plan& p, int classes) { return shape_of(classes, p.n, p.d, p.e, 0, false); }
+
+// Few rows: the product has few tiles, or is bound by the weight's bytes, which its repetition reads again.  Kept in 32 bits
+// the logits cost their bytes three times over (forward: written, read with the splits joined; backward: read for dz), and
+// the product may split its contraction.
+constexpr int64_t KEEP_BYTES = 64 << 20;
+static Shape kept_shape(const Plan& p, int classes) { return shape_of(classes, p.n, p.d, p.e, 4, true); }
+static bool kept_logits_are_faster(const Plan& p, bool forward_only) {
+  if (p.n == 0 || p.n * p.ldu * 4 > KEEP_BYTES) return false;
+  const int classes = p.pack_w ? p.piece : p.v;
+  const Shape s = kept_shape(p, classes);
+  const float mb = (float)p.n * (float)p.v * 1e-6f, twice = logit_shape(p, classes).us;
+  const float forward = s.us + (s.splits > 1 ? 0.f : 4.f + 8.f * mb / 4.f), backward = 4.f + (4.f + (float)p.e) * mb / 4.f;
+  return forward_only ? forward < twice : forward + backward < 2.f * twice;
 }
 
 static bool make_plan(const nif_head_desc* h, Plan& p) {
@@ -1039,10 +1308,9 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.ldd = (int)round_up(p.d, K_PAD);
   p.v = h->classes;
   p.k = h->top > 0 ? h->top : 1;
-  p.planes = h->dtype == NIF_F32 ? 3 : 1;
-  p.pack_w = h->dtype == NIF_F32 || p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0 ||
-             h->ldw > HEAD_MAX_LD;
-  const int64_t per = (p.pack_w && p.ldd > p.cap ? (int64_t)p.ldd : p.cap) * 2 * p.planes;  // bytes of one class of a piece
+  p.e = h->dtype == NIF_F32 ? 4 : 2;
+  p.pack_w = h->ldw > HEAD_MAX_LD || (p.e == 2 && (p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0));
+  const int64_t per = (p.pack_w && p.ldd > p.cap ? (int64_t)p.ldd : p.cap) * p.e;  // bytes of one class of a piece
   int64_t c = (int64_t)(PIECE_BYTES / per) / 256 * 256;
   if (c < 1024) c = 1024;
   if (c > p.v) c = p.v;
@@ -1066,7 +1334,10 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.s_inv = take(at, (size_t)p.cap * 4);
   p.s_lse = take(at, (size_t)p.cap * 4);
   p.s_uk = take(at, (size_t)p.cap * p.k * 4);
-  p.s_h = take(at, (size_t)p.cap * p.ldd * 2 * p.planes);
+  p.s_h = take(at, (size_t)p.cap * p.ldd * p.e);
+  p.ldu = round_up(p.v, 4);
+  p.keep = kept_logits_are_faster(p, h->forward_only != 0);
+  p.s_u = take(at, p.keep ? (size_t)p.n * p.ldu * 4 : 0);
   p.state = at;
   return true;
 }
@@ -1089,49 +1360,18 @@ static Targets targets_of(const nif_head_desc* h, const Plan& p, char* state) {
 // the launch that joins them.  The constants are fitted to each tile's times on 32 products of 10^8 to 10^11 operations
 // (20 to 4000 rows, 256 to 2048 features, 1000 to 100000 classes; 10 % off at the median, and the tile chosen costs 2 %
 // over the best): 8192 x 4096 x 131072 takes 6.9 ms in tiles of 256 and 10.5 in tiles of 128; 1000 x 1024 x 4000 takes 27 and 15.5 us.
-struct Shape {
-  int bm, bn, wm, splits;
-};
-struct Tile {
-  int bm, bn, wm, per_cu;
-  float step, share, fixed, rate;
-};
-static const Tile TILES[] = {
-    {256, 256, 2, 1, 0.81f, 0.f, 11.f, 4.0f},
-    {128, 128, 2, 2, 0.06f, 0.295f, 5.9f, 3.5f},
-    {128, 64, 4, 3, 0.08f, 0.174f, 4.3f, 3.9f},
-};
-// m x n results of a contraction over k, as `pairs` products of `planes` planes; `results`: they are written (else reduced)
-static Shape shape_of(int64_t m, int64_t n, int64_t k, int planes, bool results, bool may_split) {
-  const int64_t steps = (k + BK - 1) / BK * (planes == 3 ? 6 : 1);
-  Shape best = {128, 128, 2, 1};
-  float least = INFINITY;
-  for (const Tile& t : TILES) {
-    const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
-    for (int splits = 1; splits <= (may_split ? 32 : 1); splits *= 2) {
-      if (splits > 1 && steps / splits < 8) break;
-      const int64_t blocks = tiles * splits, slots = 256 * t.per_cu, rest = blocks % slots;
-      const float each = (float)((steps + splits - 1) / splits);
-      float us = (float)(blocks / slots) * (each * (t.step + t.share * (float)t.per_cu) + t.fixed);
-      if (rest) us += each * (t.step + t.share * (float)((rest + 255) / 256)) + t.fixed;
-      const float in = (float)(m + n) * (float)k * 2.f * (float)planes;
-      const float out = !results ? 0.f : (float)m * (float)n * (splits > 1 ? 4.f * (float)splits : planes == 3 ? 4.f : 2.f);
-      const float memory = (in + out) * 1e-6f / t.rate + 2.f;
-      us = us > memory ? us : memory;
-      if (splits > 1) us += 4.f + out * 1e-6f / 4.f;
-      if (us < least) least = us, best = {t.bm, t.bn, t.wm, splits};
-    }
-  }
-  return best;
-}
-
 template <class T, bool TRA, bool TRB, int EPI>
 static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
   g.mt = (g.M + s.bm - 1) / s.bm;
   g.nt = (g.N + s.bn - 1) / s.bn;
   const dim3 grid((unsigned)((int64_t)g.mt * g.nt * g.splits));
   if (grid.x == 0) return;
-  if (s.bn == 64)
+  if constexpr (T::WIDE) {
+    if (s.bn == 64)
+      hipLaunchKernelGGL((head_gemm32_kernel<128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+    else
+      hipLaunchKernelGGL((head_gemm32_kernel<128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+  } else if (s.bn == 64)
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
   else if (s.bn == 256)
     hipLaunchKernelGGL((head_gemm_kernel<T, 256, 256, 2, 4, TRA, TRB, EPI>), grid, dim3(512), 0, st, g);
@@ -1140,38 +1380,31 @@ static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
 }
 
 // of the products that make logits of a piece of `classes`
-static Shape logit_shape(const Plan& p, int classes) { return shape_of(classes, p.n, p.d, p.planes, false, false); }
-
 struct FwdSpace {
-  size_t stats, w, bytes;
+  size_t stats, w, part, bytes;
 };
 static FwdSpace forward_space(const Plan& p) {
   FwdSpace f;
   size_t at = 0;
   const Shape s = logit_shape(p, p.pack_w ? p.piece : p.v);
-  const int64_t tiles = (p.v / s.bm + p.v / p.piece + 2) * s.wm;
+  const int64_t tiles = p.keep ? (p.v + KEPT - 1) / KEPT : (p.v / s.bm + p.v / p.piece + 2) * s.wm;
   f.stats = take(at, (size_t)tiles * p.cap * 8);
-  f.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * 2 * p.planes : 0);
+  const int splits = p.keep ? kept_shape(p, p.pack_w ? p.piece : p.v).splits : 1;
+  f.part = take(at, splits > 1 ? (size_t)splits * p.n * p.ldu * 4 : 0);
+  f.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * p.e : 0);
   f.bytes = at;
   return f;
 }
 
 // the weight rows of a piece as a side with classes along its rows
-static Side weight_side(const nif_head_desc* h, const Plan& p, int v0, int vc, short* packed, hipStream_t st) {
-  Side s;
-  if (p.pack_w) {
-    const size_t e = h->dtype == NIF_F32 ? 4 : 2;
-    const char* src = (const char*)h->weight + (size_t)v0 * h->ldw * e;
-    const int64_t plane = (int64_t)vc * p.ldd;
-    if (h->dtype == NIF_F32)
-      hipLaunchKernelGGL(head_pack_kernel<true>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, packed, plane, p.ldd);
-    else
-      hipLaunchKernelGGL(head_pack_kernel<false>, dim3(vc), dim3(256), 0, st, src, h->ldw, p.d, packed, plane, p.ldd);
-    s = Side{packed, plane, p.ldd, vc, p.ldd};
-  } else {
-    s = Side{(const short*)h->weight + (int64_t)v0 * h->ldw, 0, h->ldw, vc, p.d};
-  }
-  return s;
+static Side weight_side(const nif_head_desc* h, const Plan& p, int v0, int vc, void* packed, hipStream_t st) {
+  const char* src = (const char*)h->weight + (size_t)v0 * h->ldw * p.e;
+  if (!p.pack_w) return Side{src, h->ldw, vc, p.d};
+  if (p.e == 4)
+    hipLaunchKernelGGL(head_pack_kernel<float>, dim3(vc), dim3(256), 0, st, (const float*)src, h->ldw, p.d, (float*)packed, p.ldd);
+  else
+    hipLaunchKernelGGL(head_pack_kernel<short>, dim3(vc), dim3(256), 0, st, (const short*)src, h->ldw, p.d, (short*)packed, p.ldd);
+  return Side{packed, p.ldd, vc, p.ldd};
 }
 
 static const void* bias_at(const nif_head_desc* h, int v0) {
@@ -1185,27 +1418,43 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
   for (int v0 = 0; v0 < p.v; v0 += p.pack_w ? p.piece : p.v) {
     const int vc = p.pack_w ? (p.v - v0 < p.piece ? p.v - v0 : p.piece) : p.v;
     GemmArgs g = {};
-    g.A = weight_side(h, p, v0, vc, (short*)(ws + f.w), st);
-    g.B = Side{(const short*)(state + p.s_h), p.cap * p.ldd, p.ldd, (int)p.cap, p.ldd};
+    g.A = weight_side(h, p, v0, vc, ws + f.w, st);
+    g.B = Side{state + p.s_h, p.ldd, (int)p.cap, p.ldd};
     g.M = vc;
     g.N = (int)p.n;
     g.n_dev = (const int*)(state + p.s_count);
-    g.K = p.ldd;
+    g.K = T::WIDE ? p.d : p.ldd;
     g.splits = 1;
     g.bias = bias_at(h, v0);
+    if (p.keep) {
+      const Shape ks = kept_shape(p, p.pack_w ? p.piece : p.v);
+      g.splits = ks.splits;
+      g.out_kind = OUT_F32;
+      g.acc = (float*)(ks.splits > 1 ? ws + f.part : state + p.s_u) + v0;
+      g.acc_ld = p.ldu;
+      g.acc_split = p.n * p.ldu;
+      run_gemm<T, false, false, EPI_OUT>(ks, g, st);
+      continue;
+    }
     g.inv_tau = h->labels ? 1.f : 1.f / h->temperature;
     g.stats = (float2*)(ws + f.stats) + (int64_t)tiles * p.cap;
     g.stat_ld = p.cap;
     run_gemm<T, false, false, EPI_STATS>(s, g, st);
     tiles += g.mt * s.wm;
   }
+  if (p.keep) {
+    const int splits = kept_shape(p, p.pack_w ? p.piece : p.v).splits;
+    tiles = (p.v + KEPT - 1) / KEPT;
+    hipLaunchKernelGGL(head_kept_kernel<T>, dim3((unsigned)p.n, tiles), dim3(256), 0, st, (const float*)(ws + f.part), splits,
+                       p.n * p.ldu, (float*)(state + p.s_u), p.ldu, p.v, (const int*)(state + p.s_count), h->bias,
+                       h->labels ? 1.f : 1.f / h->temperature, (float2*)(ws + f.stats), p.cap);
+  }
 }
 
 template <int DT>
 static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStream_t st) {
   hipLaunchKernelGGL(head_pack_rows_kernel<DT>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d,
-                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), (short*)(state + p.s_h), p.cap * p.ldd, p.ldd,
-                     h->weight, h->ldw, h->bias, targets_of(h, p, state), (float*)(state + p.s_uk));
+                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), (float*)(state + p.s_uk));
 }
 
 struct BwdSpace {
@@ -1218,14 +1467,14 @@ static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
   b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
-  b.dh = shape_of(p.d, p.n, p.piece, p.planes, true, true);
-  b.dw = shape_of(p.d, p.piece, p.n, p.planes, true, true);
+  b.dh = shape_of(p.d, p.n, p.piece, p.e, p.e, true);
+  b.dw = shape_of(p.d, p.piece, p.n, p.e, p.e, true);
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
   b.scale = take(at, 4);
-  b.dz = take(at, (size_t)p.cap * b.ldz * 2 * p.planes);
-  b.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * 2 * p.planes : 0);
+  b.dz = take(at, (size_t)p.cap * b.ldz * p.e);
+  b.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * p.e : 0);
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
   const size_t part_h = b.dh.splits > 1 ? (size_t)b.dh.splits * p.cap * b.dh_ld * 4 : 0;
   const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
@@ -1243,55 +1492,57 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
                               int64_t lddh, void* dweight, int64_t lddw, void* dbias, hipStream_t st) {
   const int* count = (const int*)(state + p.s_count);
   const int* rows = (const int*)(state + p.s_rows);
-  const short* hp = (const short*)(state + p.s_h);
+  const void* hp = state + p.s_h;
   const Targets tg = targets_of(h, p, (char*)state);
   const float* lse = (const float*)(state + p.s_lse);
   const float* uk = (const float*)(state + p.s_uk);
   const float* coef = (const float*)(ws + b.coef);
   const float* cp = (const float*)(ws + b.cp);
   const float* inv_scale = (const float*)(ws + b.scale);
-  short* dz = (short*)(ws + b.dz);
+  typedef typename T::t W;
+  W* dz = (W*)(ws + b.dz);
   float* acc = (float*)(ws + b.acc);
   float* part = (float*)(ws + b.part);
   const int f32 = h->dtype == NIF_F32;
-  const int64_t dz_plane = p.cap * b.ldz;
   for (int v0 = 0; v0 < p.v; v0 += p.piece) {
     const int vc = p.v - v0 < p.piece ? p.v - v0 : p.piece;
     const bool first = v0 == 0, last = v0 + vc == p.v;
-    const Side w = weight_side(h, p, v0, vc, (short*)(ws + b.w), st);
-    const int kz = (int)round_up(vc, K_PAD);  // columns of dz that are written
-    {
+    const Side w = weight_side(h, p, v0, vc, ws + b.w, st);
+    const int kz = T::WIDE ? vc : (int)round_up(vc, K_PAD);  // the contraction over the piece's columns of dz
+    if (p.keep) {
+      hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + 2047) / 2048)), dim3(256), 0, st,
+                         (const float*)(state + p.s_u) + v0, p.ldu, vc, count, lse, cp, dz, b.ldz);
+    } else {
       GemmArgs g = {};
       g.A = w;
-      g.B = Side{hp, p.cap * p.ldd, p.ldd, (int)p.cap, p.ldd};
+      g.B = Side{hp, p.ldd, (int)p.cap, p.ldd};
       g.M = vc;
       g.N = (int)round_up(p.n, K_PAD);
       g.n_dev = count;
-      g.K = p.ldd;
+      g.K = T::WIDE ? p.d : p.ldd;
       g.splits = 1;
       g.bias = bias_at(h, v0);
       g.inv_tau = tg.inv_tau;
       g.lse = lse;
       g.cp = cp;
       g.dz = dz;
-      g.dz_plane = dz_plane;
       g.ldz = b.ldz;
       run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc), g, st);
     }
     if (p.n > 0)
       hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
-                       v0 + vc, dz, dz_plane, b.ldz);
+                       v0 + vc, dz, b.ldz);
     if (dbias) {
       if (p.n > 0)
         hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, (unsigned)((p.n + b.stretch - 1) / b.stretch)), dim3(256), 0, st, dz,
-                           dz_plane, b.ldz, vc, count, b.stretch, part);
+                           b.ldz, vc, count, b.stretch, part);
       hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale,
                          (char*)dbias + (size_t)v0 * (f32 ? 4 : 2));
     }
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
       GemmArgs g = {};
-      g.A = Side{hp, p.cap * p.ldd, p.ldd, p.ldd, (int)p.cap};
-      g.B = Side{dz, dz_plane, b.ldz, kz, (int)p.cap};
+      g.A = Side{hp, p.ldd, p.ldd, (int)p.cap};
+      g.B = Side{dz, b.ldz, kz, (int)p.cap};
       g.M = p.d;
       g.N = vc;
       g.K = (int)p.cap;
@@ -1317,7 +1568,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.A = w;
       g.A.klim = w.rlim;
       g.A.rlim = p.pack_w ? p.ldd : p.d;
-      g.B = Side{dz, dz_plane, b.ldz, (int)p.cap, kz};
+      g.B = Side{dz, b.ldz, (int)p.cap, kz};
       g.M = p.d;
       g.N = (int)p.n;
       g.n_dev = count;
@@ -1450,7 +1701,7 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
   Plan p;
   const int rc = check_desc(h, p);
   if (rc != NIF_OK) return rc;
-  if ((p.n > 0 && !grad_loss) || (dhidden && lddh < h->features) || (dweight && lddw < h->features)) return NIF_ERR_INVALID_ARG;
+  if (h->forward_only || (p.n > 0 && !grad_loss) || (dhidden && lddh < h->features) || (dweight && lddw < h->features)) return NIF_ERR_INVALID_ARG;
   if (!state || state_bytes < nif_head_state_bytes(h) || !ws || ws_bytes < nif_head_backward_workspace_bytes(h)) return NIF_ERR_WORKSPACE;
   if (!dhidden && !dweight && !dbias) return NIF_OK;
   hipStream_t st = (hipStream_t)stream;

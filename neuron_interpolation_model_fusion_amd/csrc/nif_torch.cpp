@@ -64,7 +64,8 @@ variable_list once(variable_list grads, const Tensor& grad_loss) {
 }
 
 nif_head_desc describe(const Tensor& hidden, const Tensor& weight, const Tensor& bias, const Tensor& labels, const Tensor& indices,
-                       const Tensor& values, const Tensor& lse, double temperature, int64_t ignore_index, int64_t reduction) {
+                       const Tensor& values, const Tensor& lse, double temperature, int64_t ignore_index, int64_t reduction,
+                       bool forward_only) {
   nif_head_desc d;
   d.hidden = data<void>(hidden);
   d.ldh = ld_of(hidden);
@@ -83,17 +84,18 @@ nif_head_desc describe(const Tensor& hidden, const Tensor& weight, const Tensor&
   d.top_lse = data<float>(lse);
   d.top = indices.defined() ? (int32_t)indices.size(1) : 0;
   d.temperature = (float)temperature;
+  d.forward_only = forward_only;
   return d;
 }
 
 struct LinearHead : torch::autograd::Function<LinearHead> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Optional& bias_, const Optional& labels_,
                         const Optional& indices_, const Optional& values_, const Optional& lse_, double temperature,
-                        int64_t ignore_index, int64_t reduction) {
+                        int64_t ignore_index, int64_t reduction, bool forward_only) {
     const c10::DeviceGuard guard(hidden.device());
     const Tensor bias = or_none(bias_), labels = or_none(labels_), indices = or_none(indices_), values = or_none(values_),
                  lse = or_none(lse_);
-    const nif_head_desc d = describe(hidden, weight, bias, labels, indices, values, lse, temperature, ignore_index, reduction);
+    const nif_head_desc d = describe(hidden, weight, bias, labels, indices, values, lse, temperature, ignore_index, reduction, forward_only);
     Tensor loss = loss_of(d.rows, d.reduction, hidden);
     const size_t state_bytes = nif_head_state_bytes(&d), ws_bytes = nif_head_forward_workspace_bytes(&d);
     Tensor state = bytes(state_bytes, hidden), ws = bytes(ws_bytes, hidden);
@@ -110,11 +112,11 @@ struct LinearHead : torch::autograd::Function<LinearHead> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const Tensor &hidden = s[0], &weight = s[1], &bias = s[2], &state = s[7];
-    variable_list r(10);
+    variable_list r(11);
     if (!grads[0].defined()) return r;
     const c10::DeviceGuard guard(hidden.device());
     const nif_head_desc d = describe(hidden, weight, bias, s[3], s[4], s[5], s[6], ctx->saved_data["temperature"].toDouble(),
-                                     ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt());
+                                     ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt(), false);
     const Tensor grad = grads[0].contiguous();
     const auto like = [](const Tensor& t) { return at::empty(t.sizes(), t.options()); };
     // counted over the tensors that were given: the bias is the third where there is one
@@ -170,7 +172,8 @@ struct Distill : torch::autograd::Function<Distill> {
 
 Tensor linear_head(const Tensor& hidden, const Tensor& weight, const Optional& bias, const Optional& labels, const Optional& indices,
                    const Optional& values, const Optional& lse, double temperature, int64_t ignore_index, int64_t reduction) {
-  return LinearHead::apply(hidden, weight, bias, labels, indices, values, lse, temperature, ignore_index, reduction);
+  const bool grads = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
+  return LinearHead::apply(hidden, weight, bias, labels, indices, values, lse, temperature, ignore_index, reduction, !grads);
 }
 
 Tensor distill(const Tensor& logits, const Tensor& indices, const Tensor& values, const Optional& lse, double temperature,
