@@ -346,20 +346,48 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
             for (int r = 0; r < 4; ++r)
               if (m + r < g.M) o[r] = x[r];
           }
-        } else {
-          s16x4 w;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) w[r] = to16<T>(x[r]);
-          short* o = (short*)g.out + orow + m;
-          if (m + 4 <= g.M && !(((uintptr_t)o) & 7)) {
-            *(s16x4*)o = w;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (m + r < g.M) o[r] = w[r];
-          }
         }
       }
+    }
+  }
+}
+
+// Results in 16 bits, out[rowmap[n]][m] = (acc + what the pieces before left) * inv_scale, a wave at a time through its own
+// part of LDS: a lane's four neighbours are 8 bytes of a row, whole rows of 2 * 16 FI bytes leave in 16-byte stores.  Units
+// of 16 bytes are xor-ed with the row, which keeps both sides free of bank conflicts.
+typedef __attribute__((ext_vector_type(8), aligned(2))) short s16x8_any;
+template <class T, int FI, int FJ>
+__device__ __forceinline__ void head_store(const GemmArgs& g, f32x4 (&acc)[FI][FJ], int m0, int n0, int lane, int N, char* lds) {
+  constexpr int U = 2 * FI;  // units of a row
+  const float inv = g.inv_scale ? *g.inv_scale : 1.f;
+#pragma unroll
+  for (int j = 0; j < FJ; ++j) {
+    const int r = 16 * j + (lane & 15);
+    const float* before = g.acc && n0 + r < N ? g.acc + (int64_t)(n0 + r) * g.acc_ld : nullptr;
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+      const int m = m0 + 16 * i + 4 * (lane >> 4);
+      f32x4 x = acc[i][j];
+      if (before && m < g.M) x += *(const f32x4*)(before + m);  // rows are padded to a multiple of 4
+      s16x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = to16<T>(x[e] * inv);
+      *(s16x4*)(lds + r * U * 16 + ((2 * i + (lane >> 5)) ^ (r & (U - 1))) * 16 + (lane >> 4 & 1) * 8) = w;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+  for (int e = lane; e < 16 * FJ * U; e += 64) {
+    const int r = e / U, u = e % U, n = n0 + r, m = m0 + 8 * u;
+    if (n >= N || m >= g.M) continue;
+    const s16x8 w = *(const s16x8*)(lds + r * U * 16 + (u ^ (r & (U - 1))) * 16);
+    short* o = (short*)g.out + (int64_t)(g.rowmap ? g.rowmap[n] : n) * g.out_ld + m;
+    if (m + 8 <= g.M) {
+      *(s16x8_any*)o = w;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (m + q < g.M) o[q] = w[q];
     }
   }
 }
@@ -367,8 +395,8 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
 template <class T, int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
-  __shared__ __attribute__((aligned(1024))) char lds_a[4][BM * 64];
-  __shared__ __attribute__((aligned(1024))) char lds_b[4][BN * 64];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * (BM + BN) * 64];
+  char *const lds_a = lds, *const lds_b = lds + 4 * BM * 64;
   int split, tm, tn;
   tile_of(blockIdx.x, gridDim.x, g.mt, g.nt, split, tm, tn);
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
@@ -484,6 +512,13 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   }
   mfma_done<T>(acc);
 
+  if constexpr (EPI == EPI_OUT && TRA)
+    if (g.out_kind == OUT_FINAL) {
+      __syncthreads();  // no wave's loads still write the stages
+      static_assert(2 * BM * BN <= sizeof(lds));
+      head_store<T>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, lds + wave * 2 * WTM * WTN);
+      return;
+    }
   head_epilogue<T, EPI, EIGHT>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, split, tm * WM + wm);
 }
 
@@ -1265,7 +1300,7 @@ static Shape shape_of(int64_t m, int64_t n, int64_t k, int e, int results, bool 
   for (int i = 0; i < (e == 4 ? 2 : 3); ++i) {
     const Tile& t = tiles[i];
     const int64_t count = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
-    for (int splits = 1; splits <= (may_split ? 32 : 1); splits *= 2) {
+    for (int splits = 1; splits <= (may_split ? 128 : 1); splits *= 2) {
       if (splits > 1 && steps / splits < 8) break;
       const int64_t blocks = count * splits, slots = 256 * t.per_cu, rest = blocks % slots;
       const float each = (float)((steps + splits - 1) / splits);
