@@ -1281,19 +1281,20 @@ struct Shape {
 };
 struct Tile {
   int bm, bn, wm, per_cu;
-  float step, share, fixed, rate;
+  float step, share, fixed, rate[3];
 };
 static const Tile TILES16[] = {
-    {256, 256, 2, 1, 0.81f, 0.f, 11.f, 4.0f},
-    {128, 128, 2, 2, 0.06f, 0.295f, 5.9f, 3.5f},
-    {128, 64, 4, 3, 0.08f, 0.174f, 4.3f, 3.9f},
+    {256, 256, 2, 1, 0.81f, 0.f, 11.f, {4.2f, 3.3f, 3.3f}},
+    {128, 128, 2, 2, 0.06f, 0.295f, 5.9f, {4.5f, 3.6f, 3.1f}},
+    {128, 64, 4, 3, 0.08f, 0.174f, 4.3f, {4.8f, 3.2f, 3.0f}},
 };
 static const Tile TILES32[] = {
-    {128, 128, 2, 2, 1.05f, 0.85f, 4.f, 3.7f},
-    {128, 64, 4, 2, 0.8f, 0.53f, 4.f, 3.7f},
+    {128, 128, 2, 2, 1.05f, 0.85f, 4.f, {3.0f, 2.9f, 3.8f}},
+    {128, 64, 4, 2, 0.8f, 0.53f, 4.f, {4.0f, 3.7f, 3.2f}},
 };
+enum { LOGITS = 0, DHIDDEN = 1, DWEIGHT = 2 };  // the products
 // m x n results of a contraction over k, `e` bytes an element; `results`: bytes of one that is written (0: they are reduced)
-static Shape shape_of(int64_t m, int64_t n, int64_t k, int e, int results, bool may_split) {
+static Shape shape_of(int product, int64_t m, int64_t n, int64_t k, int e, int results, bool may_split) {
   const int64_t steps = (k + BK - 1) / BK;
   Shape best = {128, 128, 2, 1, INFINITY};
   const Tile* tiles = e == 4 ? TILES32 : TILES16;
@@ -1308,7 +1309,7 @@ static Shape shape_of(int64_t m, int64_t n, int64_t k, int e, int results, bool 
       if (rest) us += each * (t.step + t.share * (float)((rest + 255) / 256)) + t.fixed;
       const float in = (float)(m + n) * (float)k * (float)e;
       const float out = !results ? 0.f : (float)m * (float)n * (splits > 1 ? 4.f * (float)splits : (float)results);
-      const float memory = (in + out) * 1e-6f / t.rate + 2.f;
+      const float memory = (in + out) * 1e-6f / t.rate[product] + 2.f;
       us = us > memory ? us : memory;
       if (splits > 1) us += 4.f + out * 1e-6f / 4.f;
       if (us < best.us) best = {t.bm, t.bn, t.wm, splits, us};
@@ -1317,13 +1318,13 @@ static Shape shape_of(int64_t m, int64_t n, int64_t k, int e, int results, bool 
   return best;
 }
 
-static Shape logit_shape(const Plan& p, int classes) { return shape_of(classes, p.n, p.d, p.e, 0, false); }
+static Shape logit_shape(const Plan& p, int classes) { return shape_of(LOGITS, classes, p.n, p.d, p.e, 0, false); }
 
 // Few rows: the product has few tiles, or is bound by the weight's bytes, which its repetition reads again.  Kept in 32 bits
 // the logits cost their bytes three times over (forward: written, read with the splits joined; backward: read for dz), and
 // the product may split its contraction.
 constexpr int64_t KEEP_BYTES = 64 << 20;
-static Shape kept_shape(const Plan& p, int classes) { return shape_of(classes, p.n, p.d, p.e, 4, true); }
+static Shape kept_shape(const Plan& p, int classes) { return shape_of(LOGITS, classes, p.n, p.d, p.e, 4, true); }
 static bool kept_logits_are_faster(const Plan& p, bool forward_only) {
   if (p.n == 0 || p.n * p.ldu * 4 > KEEP_BYTES) return false;
   const int classes = p.pack_w ? p.piece : p.v;
@@ -1502,8 +1503,8 @@ static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
   b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
-  b.dh = shape_of(p.d, p.n, p.piece, p.e, p.e, true);
-  b.dw = shape_of(p.d, p.piece, p.n, p.e, p.e, true);
+  b.dh = shape_of(DHIDDEN, p.d, p.n, p.piece, p.e, p.e, true);
+  b.dw = shape_of(DWEIGHT, p.d, p.piece, p.n, p.e, p.e, true);
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
