@@ -189,7 +189,7 @@ __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restri
   if (threadIdx.x == 0) {
     s = 0.0, c = 0;
     for (int w = 0; w < (int)blockDim.x / 64; ++w) s += sh[w], c += sc[w];
-    *count = (float)(c > 0 ? c : 1);
+    if (count) *count = (float)(c > 0 ? c : 1);
     loss[0] = (float)(mean ? s / (c > 0 ? c : 1) : s);
   }
 }

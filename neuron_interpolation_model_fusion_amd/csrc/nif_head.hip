@@ -737,7 +737,7 @@ __global__ __launch_bounds__(1024) void head_rows_kernel(Targets tg, const int64
   __syncthreads();
   int at = upto - mine;
   for (int w = 0; w < wave; ++w) at += sh[w];
-  if (threadIdx.x == 1023) *count = at + mine;
+  if (threadIdx.x == 1023) count[0] = at + mine, count[1] = 0;
   for (int64_t r = r0; r < r1; ++r)
     if (inv[r] == 0) {  // written by this thread above
       rows[at] = (int)r;
@@ -832,41 +832,66 @@ __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restr
 }
 
 // ---- the loss of each row -------------------------------------------------------------------------------
-// 16 packed rows a block: joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.
+// 16 packed rows a block: joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.  The
+// block that is done last (`done`, cleared by head_rows_kernel) reduces the losses: sum or mean over the rows that count,
+// in a fixed order and 64 bits.
 constexpr int FINISH_NT = 1024;
 __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
                                                                 const int* __restrict__ rows, const int* __restrict__ count,
-                                                                float* __restrict__ lse, const float* __restrict__ uk,
-                                                                float* __restrict__ loss) {
+                                                                float* __restrict__ lse, const float* __restrict__ uk, float* loss,
+                                                                int64_t all_rows, int reduction, int* done, float* __restrict__ reduced) {
   constexpr int PARTS = FINISH_NT / 16;
   __shared__ float sh_top[16][PARTS + 1], sh_sum[16][PARTS + 1];
-  const int i0 = blockIdx.x * 16, n = *count;
-  if (i0 >= n) return;
-  const int r = threadIdx.x & 15, part = threadIdx.x >> 4;
-  float top = -INFINITY, sum = 0.f;
-  if (i0 + r < n)
+  __shared__ double sh[16];
+  __shared__ int last;
+  const int i0 = blockIdx.x * 16, n = *count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (i0 < n) {
+    const int r = threadIdx.x & 15, part = threadIdx.x >> 4;
+    float top = -INFINITY, sum = 0.f;
+    if (i0 + r < n)
 #pragma unroll 4
-    for (int t = part; t < tiles; t += PARTS) {
-      const float2 x = stats[(int64_t)t * stat_ld + i0 + r];
-      join(top, sum, x.x, x.y);
+      for (int t = part; t < tiles; t += PARTS) {
+        const float2 x = stats[(int64_t)t * stat_ld + i0 + r];
+        join(top, sum, x.x, x.y);
+      }
+    sh_top[r][part] = top;
+    sh_sum[r][part] = sum;
+    __syncthreads();
+    const int i = i0 + wave;  // a wave a row
+    if (i < n) {
+      top = sh_top[wave][lane], sum = sh_sum[wave][lane];
+      const float all = wave_max_f32(top), ref = all == -INFINITY ? 0.f : all;
+      sum = wave_sum_f32(sum * expf(top - ref));
+      const float l = all + logf(sum);
+      const int64_t src = rows[i];
+      double s = 0.0;
+      for (int k = lane; k < tg.k; k += 64) s += target_term(tg, src, k, uk[(int64_t)i * tg.k + k], l);
+      s = wave_sum_f64(s);
+      if (lane == 0) {
+        lse[i] = l;
+        loss[src] = (float)(s * tg.tau2);
+      }
     }
-  sh_top[r][part] = top;
-  sh_sum[r][part] = sum;
+  }
+  if (reduction == NIF_REDUCE_NONE) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the losses have left, before the block counts as done
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;  // a wave a row
-  const int i = i0 + wave;
-  if (i >= n) return;
-  top = sh_top[wave][lane], sum = sh_sum[wave][lane];
-  const float all = wave_max_f32(top), ref = all == -INFINITY ? 0.f : all;
-  sum = wave_sum_f32(sum * expf(top - ref));
-  const float l = all + logf(sum);
-  const int64_t src = rows[i];
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+    if (last) __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
   double s = 0.0;
-  for (int k = lane; k < tg.k; k += 64) s += target_term(tg, src, k, uk[(int64_t)i * tg.k + k], l);
+  for (int64_t r = threadIdx.x; r < all_rows; r += FINISH_NT) s += (double)loss[r];
   s = wave_sum_f64(s);
-  if (lane == 0) {
-    lse[i] = l;
-    loss[src] = (float)(s * tg.tau2);
+  if (lane == 0) sh[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < 16; ++w) s += sh[w];
+    *reduced = (float)(reduction == NIF_REDUCE_MEAN ? s / max(1, n) : s);
   }
 }
 
@@ -916,14 +941,9 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
 
 // The targets' entries of a piece of dz: coef (P s - sum of the row's p with that class).  The first of equal classes
 // writes, with the sum over all of them in order.  One wave per packed row.
-template <class T>
-__global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
-                                                           const float* __restrict__ uk, const float* __restrict__ lse,
-                                                           const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
-                                                           void* __restrict__ dz, int64_t ldz) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (i >= *count) return;
-  const int64_t src = rows[i];
+template <class W>
+__device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, const float* uk, float lse, float coef, float cp, int v0,
+                                               int v1, W* dz, int lane) {
   const int* at = tg.at + src * tg.k;
   const float* p = tg.p + src * tg.k;
   for (int k0 = 0; k0 < tg.k; k0 += 64) {
@@ -942,22 +962,30 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int
         sum += same ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pq), q)) : 0.f;
       }
     }
-    if (!mine || !first) continue;
-    const float x = cp[i] * expf(uk[(int64_t)i * tg.k + k] - lse[i]) - coef[i] * sum;
-    ((typename T::t*)dz)[(int64_t)i * ldz + (v - v0)] = (typename T::t)x;
+    if (mine && first) dz[v - v0] = (W)(cp * expf(uk[k] - lse) - coef * sum);
   }
+}
+template <class T>
+__global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
+                                                           const float* __restrict__ uk, const float* __restrict__ lse,
+                                                           const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
+                                                           typename T::t* __restrict__ dz, int64_t ldz) {
+  const int64_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= *count) return;
+  target_entries(tg, rows[i], uk + i * tg.k, lse[i], coef[i], cp[i], v0, v1, dz + i * ldz, threadIdx.x & 63);
 }
 
 // dbias of a piece: column sums of dz over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
-// head_bias_join_kernel.  Bound by the read of dz.
+// head_bias_join_kernel where there are several.  Bound by the read of dz.
 template <class T>
 __global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __restrict__ dz, int64_t ldz, int cols,
-                                                        const int* __restrict__ count, int stretch, float* __restrict__ part) {
+                                                        const int* __restrict__ count, int stretch, float* __restrict__ part,
+                                                        const float* __restrict__ inv_scale, typename T::t* __restrict__ out) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   __shared__ float sh[8][256 + 8];
   const int c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8, group = threadIdx.x >> 5;
   const int r0 = blockIdx.y * stretch, r1 = min(*count, r0 + stretch);
-  if (r0 >= r1) return;
+  if (r0 >= r1 && gridDim.y > 1) return;
   float s[8] = {};
   if (c0 < ldz)
 #pragma unroll 4
@@ -973,7 +1001,11 @@ __global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __r
 #pragma unroll
   for (int q = 0; q < 8; ++q) sum += sh[q][threadIdx.x];
   const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c < cols) part[(int64_t)blockIdx.y * cols + c] = sum;
+  if (c >= cols) return;
+  if (gridDim.y > 1)
+    part[(int64_t)blockIdx.y * cols + c] = sum;
+  else
+    out[c] = (typename T::t)(sum * *inv_scale);
 }
 template <class T>
 __global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __restrict__ part, int cols, const int* __restrict__ count, int stretch,
@@ -1053,28 +1085,38 @@ __global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict_
   }
 }
 
-// dz = cp exp(u - lse) of a piece of the classes, 8 a thread; zeros up to a multiple of K_PAD rows and in the padding of the
-// columns, where the products read them.  Rounded as head_gemm_kernel's.
+// dz = cp exp(u - lse) of a piece of the classes, 8 a thread, and the targets' entries; zeros up to a multiple of K_PAD rows
+// and in the padding of the columns, where the products read them.  Rounded as head_gemm_kernel's.
+constexpr int KEPT_DZ = 2048;
 template <class T>
-__global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ u, int64_t ldu, int cols, const int* __restrict__ count,
-                                                           const float* __restrict__ lse, const float* __restrict__ cp,
-                                                           typename T::t* __restrict__ dz, int64_t ldz) {
+__global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ u, int64_t ldu, int v0, int cols, Targets tg,
+                                                           const int* __restrict__ rows, const int* __restrict__ count,
+                                                           const float* __restrict__ uk, const float* __restrict__ lse,
+                                                           const float* __restrict__ coef, const float* __restrict__ cp, typename T::t* dz,
+                                                           int64_t ldz) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
-  const int i = blockIdx.x, n = *count, c = blockIdx.y * 2048 + threadIdx.x * 8;
-  if (i >= (n + K_PAD - 1) / K_PAD * K_PAD || c >= ldz) return;
-  Eight w;
+  const int n = *count, c0 = blockIdx.y * KEPT_DZ, c = c0 + threadIdx.x * 8;
+  const int64_t i = blockIdx.x;
+  if (i >= (n + K_PAD - 1) / K_PAD * K_PAD) return;
   const bool live = i < n;
   const float l = live ? lse[i] : 0.f, k = live ? cp[i] : 0.f;
-  const float* x = u + i * ldu + c;
-  if (live && c + 8 <= cols) {
-    const f32x4 lo = *(const f32x4*)x, hi = *(const f32x4*)(x + 4);
+  if (c < ldz) {
+    Eight w;
+    const float* x = u + i * ldu + v0 + c;
+    if (live && c + 8 <= cols) {
+      const f32x4 lo = *(const f32x4*)x, hi = *(const f32x4*)(x + 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(k * expf((e < 4 ? lo[e & 3] : hi[e & 3]) - l));
-  } else {
+      for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(k * expf((e < 4 ? lo[e & 3] : hi[e & 3]) - l));
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(live && c + e < cols ? k * expf(x[e] - l) : 0.f);
+      for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(live && c + e < cols ? k * expf(x[e] - l) : 0.f);
+    }
+    *(Eight*)(dz + i * ldz + c) = w;
   }
-  *(Eight*)(dz + (int64_t)i * ldz + c) = w;
+  if (!live) return;
+  __syncthreads();  // the entries are stored again behind the others
+  if (threadIdx.x < 64)
+    target_entries(tg, rows[i], uk + i * tg.k, l, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ), dz + i * ldz + c0, threadIdx.x);
 }
 
 // ---- small heads ----------------------------------------------------------------------------------------------
@@ -1263,7 +1305,7 @@ struct Plan {
   bool keep;         // few rows: the logits are kept
   int piece;         // classes per piece (multiple of 256, or all)
   // state: what the backward pass reads
-  size_t s_p, s_at, s_P, s_dz, s_fcount, s_rows, s_inv, s_count, s_lse, s_uk, s_h, s_u, state;
+  size_t s_p, s_at, s_P, s_dz, s_rows, s_inv, s_count, s_lse, s_uk, s_h, s_u, state;
   int64_t ldu;       // of the kept logits
 };
 
@@ -1358,14 +1400,13 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.s_p = take(at, (size_t)p.n * p.k * 4);
   p.s_at = take(at, (size_t)p.n * p.k * 4);
   p.s_P = take(at, (size_t)p.n * 4);
-  p.s_count = take(at, 4);
+  p.s_count = take(at, 8);  // the rows that count; the blocks that are done
   p.s_dz = 0;
   if (p.small) {
     p.s_dz = take(at, (size_t)p.n * p.v * 4);
     p.state = at;
     return true;
   }
-  p.s_fcount = take(at, 4);
   p.s_rows = take(at, (size_t)p.cap * 4);
   p.s_inv = take(at, (size_t)p.cap * 4);
   p.s_lse = take(at, (size_t)p.cap * 4);
@@ -1514,7 +1555,7 @@ static BwdSpace backward_space(const Plan& p) {
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
   const size_t part_h = b.dh.splits > 1 ? (size_t)b.dh.splits * p.cap * b.dh_ld * 4 : 0;
   const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
-  b.stretch = 32;  // rows of a block of column sums: the fewest that leave at most 2048 blocks, up to 256
+  b.stretch = p.n <= 64 ? 64 : 32;  // rows of a block of column sums: the fewest that leave at most 2048 blocks, up to 256
   while (b.stretch < 256 && (p.n + b.stretch - 1) / b.stretch * ((p.piece + 255) / 256) > 2048) b.stretch *= 2;
   const size_t part_b = (size_t)((p.n + b.stretch - 1) / b.stretch) * p.piece * 4;
   const size_t part = part_h > part_w ? part_h : part_w;
@@ -1546,8 +1587,8 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     const Side w = weight_side(h, p, v0, vc, ws + b.w, st);
     const int kz = T::WIDE ? vc : (int)round_up(vc, K_PAD);  // the contraction over the piece's columns of dz
     if (p.keep) {
-      hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + 2047) / 2048)), dim3(256), 0, st,
-                         (const float*)(state + p.s_u) + v0, p.ldu, vc, count, lse, cp, dz, b.ldz);
+      hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + KEPT_DZ - 1) / KEPT_DZ)), dim3(256),
+                         0, st, (const float*)(state + p.s_u), p.ldu, v0, vc, tg, rows, count, uk, lse, coef, cp, dz, b.ldz);
     } else {
       GemmArgs g = {};
       g.A = w;
@@ -1565,15 +1606,17 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.ldz = b.ldz;
       run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc), g, st);
     }
-    if (p.n > 0)
+    if (p.n > 0 && !p.keep)
       hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
                        v0 + vc, dz, b.ldz);
     if (dbias) {
+      W* out = (W*)dbias + v0;
+      const unsigned stretches = (unsigned)((p.n + b.stretch - 1) / b.stretch);
       if (p.n > 0)
-        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, (unsigned)((p.n + b.stretch - 1) / b.stretch)), dim3(256), 0, st, dz,
-                           b.ldz, vc, count, b.stretch, part);
-      hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale,
-                         (char*)dbias + (size_t)v0 * (f32 ? 4 : 2));
+        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, stretches), dim3(256), 0, st, dz, b.ldz, vc, count, b.stretch, part,
+                           inv_scale, out);
+      if (stretches != 1)
+        hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale, out);
     }
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
       GemmArgs g = {};
@@ -1720,13 +1763,12 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
       forward_products<F16>(h, p, s, (char*)ws, f, tiles, st);
     const float2* stats = (const float2*)((char*)ws + f.stats);
     hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg, rows, count,
-                       (float*)(s + p.s_lse), (const float*)(s + p.s_uk), row_loss);
+                       (float*)(s + p.s_lse), (const float*)(s + p.s_uk), row_loss, p.n, h->reduction, count + 1, loss);
   } else {
     hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, targets_of(h, p, s), nullptr, (int64_t)0, p.v, (int64_t)0, rows, inv,
                        count, nullptr);
+    if (h->reduction != NIF_REDUCE_NONE) launch_reduce(row_loss, nullptr, 0, false, nullptr, loss, st);
   }
-  if (h->reduction != NIF_REDUCE_NONE)
-    launch_reduce(row_loss, (const float*)(s + p.s_P), p.n, h->reduction == NIF_REDUCE_MEAN, (float*)(s + p.s_fcount), loss, st);
   return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
 }
 
