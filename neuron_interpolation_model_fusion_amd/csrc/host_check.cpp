@@ -78,6 +78,40 @@ int main() {
   EXPECT(nif_refit_pairs(NULL, 4, NULL, NULL, NULL, 4, 4, NULL, NULL) == NIF_ERR_INVALID_ARG);
   EXPECT(nif_lsq_refit_f32(NULL, 4, 4, 4, NULL, 4, 4, 0, NULL, 4, NULL, 4, NULL, &i32, NULL, 0, NULL) ==
          NIF_ERR_INVALID_ARG);
+  {
+    // head losses: sizes of the three variants (small, kept logits, recomputed), refusals before any launch
+    float f4[64];
+    int64_t y4[16];
+    nif_head_desc h;
+    memset(&h, 0, sizeof(h));
+    h.hidden = f4, h.weight = f4, h.labels = y4;
+    h.ldh = 64, h.ldw = 64, h.features = 64, h.rows = 4, h.classes = 10, h.dtype = NIF_F32, h.temperature = 1.f;
+    EXPECT(nif_head_state_bytes(&h) >= 4 * 10 * 4);
+    EXPECT(nif_head_state_bytes(NULL) == 0);
+    h.classes = 200000;
+    const size_t kept = nif_head_state_bytes(&h);
+    EXPECT(kept > (size_t)4 * 200000 * 4);
+    h.rows = 100000;
+    EXPECT(nif_head_state_bytes(&h) < (size_t)100000 * 200000);
+    EXPECT(nif_head_forward_workspace_bytes(&h) > 0);
+    EXPECT(nif_head_backward_workspace_bytes(&h) < (size_t)1 << 32);
+    EXPECT(nif_head_forward(&h, f4, f4, 16, f4, 16, NULL) == NIF_ERR_WORKSPACE);
+    EXPECT(nif_head_backward(&h, f4, f4, 16, NULL, 0, f4, 64, NULL, f4, 16, NULL) == NIF_ERR_WORKSPACE);
+    h.forward_only = 1;
+    EXPECT(nif_head_backward(&h, f4, f4, 16, NULL, 0, f4, 64, NULL, f4, 16, NULL) == NIF_ERR_INVALID_ARG);
+    h.forward_only = 0, h.rows = -1;
+    EXPECT(nif_head_forward(&h, f4, f4, (size_t)-1, f4, (size_t)-1, NULL) == NIF_ERR_INVALID_ARG);
+    EXPECT(nif_head_state_bytes(&h) == 0);
+    h.rows = 0;
+    EXPECT(nif_head_state_bytes(&h) > 0 && nif_head_backward_workspace_bytes(&h) > 0);
+    h.rows = 4, h.dtype = 99;
+    EXPECT(nif_head_forward(&h, f4, f4, (size_t)-1, f4, (size_t)-1, NULL) == NIF_ERR_INVALID_ARG);
+    EXPECT(nif_distill_state_bytes(4, 8) > 0);
+    EXPECT(nif_distill_forward(NULL, 8, 4, 8, NIF_F32, NULL, NULL, NULL, 2, 1.f, NIF_REDUCE_MEAN, f4, f4, 1 << 20, f4, 1 << 20, NULL) ==
+           NIF_ERR_INVALID_ARG);
+    EXPECT(nif_top_logits(NULL, 8, 4, 8, NIF_F32, 2, 1.f, f4, &i32, f4, NULL) == NIF_ERR_INVALID_ARG);
+    EXPECT(nif_top_logits(f4, 8, 4, 8, NIF_F32, 9, 1.f, f4, &i32, f4, NULL) == NIF_ERR_INVALID_ARG);
+  }
   // profile slots: out-of-range slots are refused, an empty slot collects nothing
   EXPECT(nif_profile_collect(-1, &f64, &i64) == NIF_ERR_INVALID_ARG);
   EXPECT(nif_profile_collect(NIF_PROFILE_SLOTS, &f64, &i64) == NIF_ERR_INVALID_ARG);
