@@ -1065,7 +1065,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     zero gradients whatever they hold, and 'mean' runs over the others (0 when there are none).  A target that is no class
     makes its row NaN.  Differentiable once w.r.t. hidden, weight and bias; the loss is f32, f32 inputs compute at f32
     accuracy and 16-bit ones accumulate in 32 bits.  Memory beyond the gradients: the packed hidden rows and pieces of
-    the classes of about 256 MiB."""
+    the classes of about 256 MiB; for few rows, where that is faster, up to 64 MiB of logits are kept in f32."""
     what = 'linear_cross_entropy'
     reduction = _reduction(what, reduction)
     if target.is_floating_point() or target.dtype == torch.bool or tuple(target.shape) != tuple(hidden.shape[:-1]):
