@@ -3,10 +3,14 @@
 // own thread.  Arguments are checked in ops.py; here are buffers, streams, devices and gradients only.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
+
+#include <unordered_set>
 
 #include "../../include/nif.h"
 
@@ -47,6 +51,34 @@ const T* data(const Tensor& t) {
   return t.defined() ? (const T*)t.const_data_ptr() : nullptr;
 }
 void* out(Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+// A leaf's gradient accumulator lives as long as a graph that ends in it and stays on the stream of the pass that made it.
+// Captured together with a later pass, that stream would have to wait for the capturing one, which ends the process: a
+// captured backward pass that would get there is refused.
+void refuse_capture_of_live_leaves(const Tensor& like) {
+  hipStreamCaptureStatus status;
+  if (hipStreamIsCapturing((hipStream_t)stream_of(like), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const c10::Stream here = c10::impl::VirtualGuardImpl(like.device().type()).getStream(like.device());
+  std::vector<torch::autograd::Node*> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  const auto current = torch::autograd::get_current_node();
+  if (current) todo.push_back(current.get());
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+      if (!node->task_should_compute_output(i)) continue;
+      torch::autograd::Node* next = node->next_edge(i).function.get();
+      if (!next || !seen.insert(next).second) continue;
+      todo.push_back(next);
+      if (!dynamic_cast<torch::autograd::AccumulateGrad*>(next)) continue;
+      const auto stream = next->stream();
+      if (stream && *stream != here)
+        throw NifError("an autograd graph of an earlier pass over the same leaves is alive on another stream: a backward pass cannot be "
+                       "captured with it; drop that pass's loss and outputs first");
+    }
+  }
+}
 
 // Gradients that are differentiated again fail, instead of counting as constants.
 variable_list once(variable_list grads, const Tensor& grad_loss) {
@@ -115,6 +147,7 @@ struct LinearHead : torch::autograd::Function<LinearHead> {
     variable_list r(11);
     if (!grads[0].defined()) return r;
     const c10::DeviceGuard guard(hidden.device());
+    refuse_capture_of_live_leaves(hidden);
     const nif_head_desc d = describe(hidden, weight, bias, s[3], s[4], s[5], s[6], ctx->saved_data["temperature"].toDouble(),
                                      ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt(), false);
     const Tensor grad = grads[0].contiguous();
@@ -159,6 +192,7 @@ struct Distill : torch::autograd::Function<Distill> {
     variable_list r(6);
     if (!grads[0].defined()) return r;
     const c10::DeviceGuard guard(logits.device());
+    refuse_capture_of_live_leaves(logits);
     const Tensor grad = grads[0].contiguous();
     r[0] = at::empty(logits.sizes(), logits.options());
     check(nif_distill_backward(data<void>(logits), ld_of(logits), logits.size(0), (int)logits.size(1), type_of(logits),

@@ -1049,12 +1049,17 @@ def _check_head(what, hidden, weight, bias):
         raise ValueError(f'{what}: bias has shape {tuple(bias.shape)} for {weight.shape[0]} classes')
 
 
+def _rows(t):
+    """[..., c] as [rows, c]; a view of the same shape would be a node of the autograd graph."""
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
 def _linear_head(hidden, weight, bias, labels, indices, values, lse, temperature, ignore_index, reduction):
     lead = hidden.shape[:-1]
-    hidden = _mat(hidden.reshape(-1, hidden.shape[-1]), 'hidden')
+    hidden = _mat(_rows(hidden), 'hidden')
     loss = _lib.nif_torch.linear_head(hidden, _mat(weight, 'weight'), None if bias is None else bias.contiguous(), labels, indices,
                                       values, lse, temperature, ignore_index, reduction)
-    return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE else loss
+    return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE and len(lead) != 1 else loss
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100, reduction='mean'):
@@ -1107,9 +1112,8 @@ def topk_distillation(logits, top_values, top_indices, *, temperature=1.0, top_l
     lead = logits.shape[:-1]
     _check_top(what, lead, top_values, top_indices, top_lse)
     _same_device(what, logits, top_values, top_indices, top_lse)
-    loss = _lib.nif_torch.distill(_mat(logits.reshape(-1, logits.shape[-1]), 'logits'),
-                                  *_top_targets(top_values, top_indices, top_lse), temperature, reduction)
-    return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE else loss
+    loss = _lib.nif_torch.distill(_mat(_rows(logits), 'logits'), *_top_targets(top_values, top_indices, top_lse), temperature, reduction)
+    return loss.reshape(lead) if reduction == _lib.NIF_REDUCE_NONE and len(lead) != 1 else loss
 
 
 MAX_TOP_LOGITS = _lib.NIF_TOP_MAX_K  # the longest list of top logits a row
@@ -1126,7 +1130,7 @@ def top_logits(logits, k, *, temperature=1.0):
         raise ValueError(f'{what}: 1 to min(classes, {_lib.NIF_TOP_MAX_K}) top logits, got {k} of {tuple(logits.shape)}')
     _same_device(what, logits)
     lead = logits.shape[:-1]
-    z = _mat(logits.detach().reshape(-1, logits.shape[-1]), 'logits')
+    z = _mat(_rows(logits.detach()), 'logits')
     values, indices, lse = _lib.nif_torch.top_logits(z, k, temperature)
     return values.reshape(*lead, k), indices.reshape(*lead, k), lse.reshape(lead)
 

@@ -546,6 +546,49 @@ def test_captured_training_steps_replay(ops):
         torch.cuda.synchronize()
 
 
+def test_capture_is_refused_while_an_eager_graph_of_the_same_leaves_lives(ops):
+    """A leaf's accumulator stays on the stream of the pass that made it; captured, that stream would wait for the capture,
+    which ends the process."""
+    h, w = (torch.randn(n, 64, device='cuda').requires_grad_() for n in (40, 6000))
+    z = torch.randn(20, 50, device='cuda').requires_grad_()
+    y = torch.randint(0, 6000, (40,), device='cuda')
+    top = torch.zeros(20, 3, device='cuda'), torch.arange(60, device='cuda').view(20, 3) % 50
+
+    def head():
+        return ops.linear_cross_entropy(h, w, y)
+
+    def logits():
+        return ops.topk_distillation(z, *top)
+
+    def grads(loss, leaves):
+        return [loss.detach().clone()] + [g.clone() for g in torch.autograd.grad(loss, leaves)]
+    for call, leaves in ((head, (h, w)), (logits, (z,))):
+        kept = call()  # its graph holds the leaves' accumulators
+        want = grads(call(), leaves)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match='earlier pass'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                grads(call(), leaves)
+        for grad_mode in (False, True):  # nothing to capture backwards
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph), torch.set_grad_enabled(grad_mode):
+                alone = call().detach()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(alone, want[0])
+        del kept
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = grads(call(), leaves)
+        for _ in range(3):
+            for t in got:
+                t.fill_(7)
+            graph.replay()
+            grads(call(), leaves)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_teacher_and_a_student_head_together(ops):
     """As they are used: the teacher's top logits once, the student's steps from them -- through logits that are kept and
     through the head, which agree."""
