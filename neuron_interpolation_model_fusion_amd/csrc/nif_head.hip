@@ -19,7 +19,7 @@
 //
 // 16-bit inputs run on v_mfma_f32_16x16x32 with 32-bit accumulation (head_gemm_kernel).  f32 inputs are split exactly into
 // three bf16 planes (x = h + m + l, 24 bits) on their way into LDS and a product runs as the six plane pairs above 2^-24:
-// f32-level accuracy (head_gemm32_kernel).
+// f32-level accuracy (head_gemm_any_kernel, which also takes 16-bit weights whose rows are off 16-byte borders).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   head_epilogue<T, EPI, EIGHT>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, split, tm * WM + wm);
 }
 
-// ---- products of f32 operands -----------------------------------------------------------------------------
+// ---- products through registers -----------------------------------------------------------------------------
 // x = h + m + l: three bf16 values, exact for 24 bits; an infinity becomes NaN.  Two at a time.
 __device__ __forceinline__ void split3(float x, float y, unsigned (&w)[3]) {
   typedef __attribute__((ext_vector_type(2))) float f32x2;
@@ -548,8 +548,9 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 // three planes of bf16.  A unit u of 16 bytes in LDS holds the k 4 u .. 4 u + 3 and 16 + 4 u .. (both sides alike, so that
 // the order does not matter): four lanes fetch 64 neighbouring bytes of a row.  Row r has the slot r ^ (r / 16 & 3), which
 // spreads the stores of a transposed side (four neighbouring rows a lane) over all banks.
-template <int BT, bool TR>
+template <class T, int BT, bool TR>
 struct Splitter {
+  typedef f32x4 Regs[8];
   const float* base;
   unsigned off[4];  // of the thread's rows
   unsigned first;   // transposed: of the four at the first of its k
@@ -631,18 +632,93 @@ struct Splitter {
   }
 };
 
-// The same products for f32: each workgroup splits the tiles that it reads (four bytes an element from memory, whatever the
+// The same for 16-bit operands of any alignment, one plane: a unit u holds the k 8 u .. 8 u + 7.
+template <class T, int BT, bool TR>
+struct Mover {
+  typedef s16x8 Regs[4];  // plain: a row each; transposed: halves are the four rows at one k
+  typedef __attribute__((ext_vector_type(4), aligned(2))) short s16x4_any;
+  const short* base;
+  unsigned off[4], first;
+  int u, row;
+  bool whole;
+  __device__ __forceinline__ void init(const Side& s, int r0, int block) {
+    u = TR ? block / (BT / 4) : block & 3;
+    row = TR ? block % (BT / 4) * 4 : block >> 2;
+    base = (const short*)s.base + (TR ? (int64_t)r0 : (int64_t)r0 * s.ld);
+    whole = r0 + row + 4 <= s.rlim;
+    first = TR ? 8 * u * (unsigned)s.ld + row : 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      off[j] = TR ? (unsigned)min(row + j, s.rlim - 1 - r0) : (unsigned)min(row + BT / 4 * j, s.rlim - 1 - r0) * (unsigned)s.ld;
+  }
+  static __device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  }
+  __device__ __forceinline__ void load(const Side& s, int k0, int klim, Regs& x) const {
+    const int have = klim - k0;
+    if constexpr (!TR) {
+      const short* p = base + k0;
+      if (have >= BK) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = *(const s16x8_any*)(p + off[j] + 8 * u);
+      } else {
+        const int k8 = opaque(8 * u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const short y = p[off[j] + (unsigned)min(k8 + e, have - 1)];
+            x[j][e] = k8 + e < have ? y : (short)0;
+          }
+      }
+    } else {
+      const short* p = base + (int64_t)k0 * s.ld;
+      if (have >= BK && whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const s16x4 y = *(const s16x4_any*)(p + i * s.ld + first);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i >> 1][4 * (i & 1) + j] = y[j];
+        }
+      } else {
+        const int k8 = opaque(8 * u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const short y = p[(unsigned)min(k8 + i, have - 1) * (unsigned)s.ld + off[j]];
+            x[i >> 1][4 * (i & 1) + j] = k8 + i < have ? y : (short)0;
+          }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, const Regs& x) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = TR ? row + j : row + BT / 4 * j;
+      s16x8 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = TR ? x[e >> 1][4 * (e & 1) + j] : x[j][e];
+      *(s16x8*)(lds + (r ^ (r >> 4 & 3)) * 64 + (u ^ row_swizzle(r >> 2)) * 16) = w;
+    }
+  }
+};
+
+// The same products for f32 and for 16-bit operands of any alignment, through registers.  f32: each workgroup splits the tiles that it reads (four bytes an element from memory, whatever the
 // planes), and the fragments of three planes serve six products.  One LDS stage of 32 k; the loads of the next two tiles are
 // in flight under the products, and the CU's other workgroup fills the waits.  4000 x 2048 x 50000: 196 TFLOP/s of the
 // operands' products (planes split beforehand, copied by the 16-bit kernel: 155; the library's f32: 153); 1 x 2048 x
 // 131072, forward and backward: 0.81 ms (planes split beforehand: 3.64, 10 bytes an element a pass).
-template <int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
-__global__ __launch_bounds__(256, 2) void head_gemm32_kernel(GemmArgs g) {
+template <class T, int BM, int BN, int WM, int WN, bool TRA, bool TRB, int EPI>
+__global__ __launch_bounds__(256, 2) void head_gemm_any_kernel(GemmArgs g) {
   static_assert(WM * WN == 4 && BM + BN <= 256 && BM % 64 == 0 && BN % 64 == 0);
+  constexpr int PLANES = T::WIDE ? 3 : 1, PAIRS = T::WIDE ? 6 : 1;
   constexpr int WTM = BM / WM, WTN = BN / WN, FI = WTM / 16, FJ = WTN / 16;
   static_assert(WTM % 64 == 0 || (WTM == 32 && FI <= 2));
-  __shared__ __attribute__((aligned(1024))) char lds_a[3 * BM * 64];
-  __shared__ __attribute__((aligned(1024))) char lds_b[3 * BN * 64];
+  __shared__ __attribute__((aligned(1024))) char lds_a[PLANES * BM * 64];
+  __shared__ __attribute__((aligned(1024))) char lds_b[PLANES * BN * 64];
+  __shared__ __attribute__((aligned(1024))) char lds_out[EPI == EPI_OUT && !T::WIDE ? 2 * BM * BN : 16];
   int split, tm, tn;
   tile_of(blockIdx.x, gridDim.x, g.mt, g.nt, split, tm, tn);
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
@@ -655,13 +731,14 @@ __global__ __launch_bounds__(256, 2) void head_gemm32_kernel(GemmArgs g) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   // the first waves fetch A, the others B
-  Splitter<BM, TRA> sa;
-  Splitter<BN, TRB> sb;
+  typename std::conditional<T::WIDE, Splitter<T, BM, TRA>, Mover<T, BM, TRA>>::type sa;
+  typename std::conditional<T::WIDE, Splitter<T, BN, TRB>, Mover<T, BN, TRB>>::type sb;
+  typedef typename decltype(sa)::Regs Regs;
   const bool for_a = wave < BM / 64, for_b = !for_a && wave < (BM + BN) / 64;
   sa.init(g.A, m0, for_a ? threadIdx.x : 0);
   sb.init(g.B, n0, for_b ? threadIdx.x - BM : 0);
-  f32x4 x0[8], x1[8];
-  const auto load = [&](int t, f32x4(&x)[8]) {
+  Regs x0, x1;
+  const auto load = [&](int t, Regs& x) {
     if (for_a)
       sa.load(g.A, t * BK, K, x);
     else if (for_b)
@@ -676,29 +753,29 @@ __global__ __launch_bounds__(256, 2) void head_gemm32_kernel(GemmArgs g) {
   for (int i = 0; i < FI; ++i)
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  mfma_done<F32>(acc);  // written, before the first matrix instruction reads them
-  const auto step = [&](int t, f32x4(&x)[8]) {
+  mfma_done<T>(acc);  // written, before the first matrix instruction reads them
+  const auto step = [&](int t, Regs& x) {
     if (for_a)
       sa.store(lds_a, x);
     else if (for_b)
       sb.store(lds_b, x);
     __syncthreads();
     if (t + 2 < t1) load(t + 2, x);
-    s16x8 a[FI][3];
+    s16x8 a[FI][PLANES];
 #pragma unroll
     for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int pl = 0; pl < 3; ++pl) a[i][pl] = fragment(lds_a, BM, wm * WTM, pl, i);
+      for (int pl = 0; pl < PLANES; ++pl) a[i][pl] = fragment(lds_a, BM, wm * WTM, pl, i);
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
-      s16x8 b[3];
+      s16x8 b[PLANES];
 #pragma unroll
-      for (int pl = 0; pl < 3; ++pl) b[pl] = fragment(lds_b, BN, wn * WTN, pl, j);
+      for (int pl = 0; pl < PLANES; ++pl) b[pl] = fragment(lds_b, BN, wn * WTN, pl, j);
       // smallest products first: (l, h) (h, l) (m, m) (m, h) (h, m) (h, h)
 #pragma unroll
-      for (int q = 0; q < 6; ++q)
+      for (int q = 6 - PAIRS; q < 6; ++q)
 #pragma unroll
-        for (int i = 0; i < FI; ++i) F32::mfma(acc[i][j], a[i][(0x001102 >> (4 * q)) & 3], b[(0x010120 >> (4 * q)) & 3]);
+        for (int i = 0; i < FI; ++i) T::mfma(acc[i][j], a[i][(0x001102 >> (4 * q)) & 3], b[(0x010120 >> (4 * q)) & 3]);
     }
     __syncthreads();
   };
@@ -708,8 +785,14 @@ __global__ __launch_bounds__(256, 2) void head_gemm32_kernel(GemmArgs g) {
     step(t, x0);
     if (t + 1 < t1) step(t + 1, x1);
   }
-  mfma_done<F32>(acc);
-  head_epilogue<F32, EPI, false>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, split, tm * WM + wm);
+  mfma_done<T>(acc);
+  if constexpr (EPI == EPI_OUT && !T::WIDE)
+    if (g.out_kind == OUT_FINAL) {
+      static_assert(2 * BM * BN <= sizeof(lds_out));
+      head_store<T>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, lds_out + wave * 2 * WTM * WTN);
+      return;
+    }
+  head_epilogue<T, EPI, false>(g, acc, m0 + wm * WTM, n0 + wn * WTN, lane, N, split, tm * WM + wm);
 }
 
 // ---- the rows that count ------------------------------------------------------------------------------
@@ -820,7 +903,8 @@ __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const
   }
 }
 
-// Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits.
+// Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits (uk; not
+// where the logits are kept).
 template <int DT>
 __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int d,
                                                              const int* __restrict__ rows, const int* __restrict__ count,
@@ -833,7 +917,7 @@ __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restr
   const int64_t src = have ? rows[i] : 0;
   const typename Elem<DT>::t* h = (const typename Elem<DT>::t*)hidden + src * ldh;
   pack_row<W>((const W*)h, have, d, (W*)dst + i * ldd, ldd);
-  if (!have) return;
+  if (!have || !uk) return;
   for (int k0 = (threadIdx.x >> 6) * DOTS; k0 < tg.k; k0 += 4 * DOTS)
     target_dots<DT>(h, weight, ldw, bias, d, tg, src, k0, uk + i * tg.k, threadIdx.x & 63);
 }
@@ -845,7 +929,8 @@ __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restr
 constexpr int FINISH_NT = 1024;
 __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
                                                                 const int* __restrict__ rows, const int* __restrict__ count,
-                                                                float* __restrict__ lse, const float* __restrict__ uk, float* loss,
+                                                                float* __restrict__ lse, const float* __restrict__ uk,
+                                                                const float* __restrict__ u, int64_t ldu, float* loss,
                                                                 int64_t all_rows, int reduction, int* done, float* __restrict__ reduced) {
   constexpr int PARTS = FINISH_NT / 16;
   __shared__ float sh_top[16][PARTS + 1], sh_sum[16][PARTS + 1];
@@ -872,7 +957,8 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
       const float l = all + logf(sum);
       const int64_t src = rows[i];
       double s = 0.0;
-      for (int k = lane; k < tg.k; k += 64) s += target_term(tg, src, k, uk[(int64_t)i * tg.k + k], l);
+      for (int k = lane; k < tg.k; k += 64)
+        s += target_term(tg, src, k, u ? u[i * ldu + max(0, tg.at[src * tg.k + k])] : uk[(int64_t)i * tg.k + k], l);
       s = wave_sum_f64(s);
       if (lane == 0) {
         lse[i] = l;
@@ -948,8 +1034,8 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
 
 // The targets' entries of a piece of dz: coef (P s - sum of the row's p with that class).  The first of equal classes
 // writes, with the sum over all of them in order.  One wave per packed row.
-template <class W>
-__device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, const float* uk, float lse, float coef, float cp, int v0,
+template <class W, class U>
+__device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U&& u_of, float lse, float coef, float cp, int v0,
                                                int v1, W* dz, int lane) {
   const int* at = tg.at + src * tg.k;
   const float* p = tg.p + src * tg.k;
@@ -969,7 +1055,7 @@ __device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, c
         sum += same ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pq), q)) : 0.f;
       }
     }
-    if (mine && first) dz[v - v0] = (W)(cp * expf(uk[k] - lse) - coef * sum);
+    if (mine && first) dz[v - v0] = (W)(cp * expf(u_of(k, v) - lse) - coef * sum);
   }
 }
 template <class T>
@@ -979,7 +1065,8 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int
                                                            typename T::t* __restrict__ dz, int64_t ldz) {
   const int64_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= *count) return;
-  target_entries(tg, rows[i], uk + i * tg.k, lse[i], coef[i], cp[i], v0, v1, dz + i * ldz, threadIdx.x & 63);
+  target_entries(tg, rows[i], [&](int k, int) { return uk[i * tg.k + k]; }, lse[i], coef[i], cp[i], v0, v1, dz + i * ldz,
+                 threadIdx.x & 63);
 }
 
 // dbias of a piece: column sums of dz over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
@@ -1098,9 +1185,8 @@ constexpr int KEPT_DZ = 2048;
 template <class T>
 __global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ u, int64_t ldu, int v0, int cols, Targets tg,
                                                            const int* __restrict__ rows, const int* __restrict__ count,
-                                                           const float* __restrict__ uk, const float* __restrict__ lse,
-                                                           const float* __restrict__ coef, const float* __restrict__ cp, typename T::t* dz,
-                                                           int64_t ldz) {
+                                                           const float* __restrict__ lse, const float* __restrict__ coef,
+                                                           const float* __restrict__ cp, typename T::t* dz, int64_t ldz) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   const int n = *count, c0 = blockIdx.y * KEPT_DZ, c = c0 + threadIdx.x * 8;
   const int64_t i = blockIdx.x;
@@ -1123,7 +1209,8 @@ __global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restri
   if (!live) return;
   __syncthreads();  // the entries are stored again behind the others
   if (threadIdx.x < 64)
-    target_entries(tg, rows[i], uk + i * tg.k, l, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ), dz + i * ldz + c0, threadIdx.x);
+    target_entries(tg, rows[i], [&](int, int v) { return u[i * ldu + v]; }, l, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ),
+                   dz + i * ldz + c0, threadIdx.x);
 }
 
 // ---- small heads ----------------------------------------------------------------------------------------------
@@ -1307,7 +1394,9 @@ struct Plan {
   int64_t n, cap;
   int d, ldd, v, k;
   int e;             // bytes of an operand's element
-  bool pack_w;       // the weight is copied by pieces: rows that the loads cannot take
+  // How the passes read the weight: head_gemm_any_kernel (f32; 16 bits with rows that direct loads cannot take, few rows of
+  // hidden), or head_gemm_kernel, from a copy by pieces where the rows are such.
+  bool any_f, any_b, pack_f, pack_b;
   bool small;        // the small heads' kernels
   bool keep;         // few rows: the logits are kept
   int piece;         // classes per piece (multiple of 256, or all)
@@ -1325,6 +1414,7 @@ static size_t take(size_t& at, size_t bytes) {
 }
 
 struct Shape {
+  bool any;  // of head_gemm_any_kernel
   int bm, bn, wm, splits;
   float us;  // what the model says
 };
@@ -1337,17 +1427,22 @@ static const Tile TILES16[] = {
     {128, 128, 2, 2, 0.06f, 0.295f, 5.9f, {4.5f, 3.6f, 3.1f}},
     {128, 64, 4, 3, 0.08f, 0.174f, 4.3f, {4.8f, 3.2f, 3.0f}},
 };
+static const Tile TILES_ANY16[] = {
+    {128, 128, 2, 2, 0.4f, 0.35f, 4.f, {4.0f, 3.5f, 3.0f}},
+    {128, 64, 4, 2, 0.35f, 0.25f, 4.f, {4.0f, 3.5f, 3.0f}},
+};
 static const Tile TILES32[] = {
     {128, 128, 2, 2, 1.05f, 0.85f, 4.f, {3.0f, 2.9f, 3.8f}},
     {128, 64, 4, 2, 0.8f, 0.53f, 4.f, {4.0f, 3.7f, 3.2f}},
 };
 enum { LOGITS = 0, DHIDDEN = 1, DWEIGHT = 2 };  // the products
 // m x n results of a contraction over k, `e` bytes an element; `results`: bytes of one that is written (0: they are reduced)
-static Shape shape_of(int product, int64_t m, int64_t n, int64_t k, int e, int results, bool may_split) {
+static Shape shape_of(int product, int64_t m, int64_t n, int64_t k, int e, int results, bool may_split, bool any) {
   const int64_t steps = (k + BK - 1) / BK;
-  Shape best = {128, 128, 2, 1, INFINITY};
-  const Tile* tiles = e == 4 ? TILES32 : TILES16;
-  for (int i = 0; i < (e == 4 ? 2 : 3); ++i) {
+  Shape best = {true, 128, 128, 2, 1, INFINITY};
+  const Tile* tiles = e == 4 ? TILES32 : any ? TILES_ANY16 : TILES16;
+  any |= e == 4;
+  for (int i = 0; i < (any ? 2 : 3); ++i) {
     const Tile& t = tiles[i];
     const int64_t count = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
     for (int splits = 1; splits <= (may_split ? 128 : 1); splits *= 2) {
@@ -1361,29 +1456,34 @@ static Shape shape_of(int product, int64_t m, int64_t n, int64_t k, int e, int r
       const float memory = (in + out) * 1e-6f / t.rate[product] + 2.f;
       us = us > memory ? us : memory;
       if (splits > 1) us += 4.f + out * 1e-6f / 4.f;
-      if (us < best.us) best = {t.bm, t.bn, t.wm, splits, us};
+      if (us < best.us) best = {any, t.bm, t.bn, t.wm, splits, us};
     }
   }
   return best;
 }
 
-static Shape logit_shape(const Plan& p, int classes) { return shape_of(LOGITS, classes, p.n, p.d, p.e, 0, false); }
+static Shape logit_shape(const Plan& p, int classes, bool any) { return shape_of(LOGITS, classes, p.n, p.d, p.e, 0, false, any); }
 
 // Few rows: the product has few tiles, or is bound by the weight's bytes, which its repetition reads again.  Kept in 32 bits
 // the logits cost their bytes three times over (forward: written, read with the splits joined; backward: read for dz), and
 // the product may split its contraction.  bf16, forward and backward: 1 x 2048 x 131072 0.66 -> 0.50 ms, 300 x 2048 x 50000
 // 0.50 -> 0.42 ms; f32: 32 x 2048 x 131072 1.9 -> 0.86 ms (with the 128 x 64 tiles' deeper prefetch).
 constexpr int64_t KEEP_BYTES = 64 << 20;
-static Shape kept_shape(const Plan& p, int classes) { return shape_of(LOGITS, classes, p.n, p.d, p.e, 4, true); }
+static Shape kept_shape(const Plan& p, int classes) { return shape_of(LOGITS, classes, p.n, p.d, p.e, 4, true, p.any_f); }
 static bool kept_logits_are_faster(const Plan& p, bool forward_only) {
   if (p.n == 0 || p.n * p.ldu * 4 > KEEP_BYTES) return false;
-  const int classes = p.pack_w ? p.piece : p.v;
-  const Shape s = kept_shape(p, classes);
-  const float mb = (float)p.n * (float)p.v * 1e-6f, twice = logit_shape(p, classes).us;
+  // the same for both passes, whatever the weight's address and strides in each
+  const Shape s = shape_of(LOGITS, p.v, p.n, p.d, p.e, 4, true, false);
+  const float mb = (float)p.n * (float)p.v * 1e-6f, once = logit_shape(p, p.v, false).us;
   const float forward = s.us + (s.splits > 1 ? 0.f : 4.f + 8.f * mb / 4.f), backward = 4.f + (4.f + (float)p.e) * mb / 4.f;
-  return forward_only ? forward < twice : forward + backward < 2.f * twice;
+  const float dots = (float)p.n * (float)p.k * (float)p.d * (float)p.e * 1e-6f / 6.f;  // the targets' logits, otherwise
+  return forward_only ? forward < once + dots : forward + backward < 2.f * once + dots;
 }
 
+// Weights in 16 bits whose rows are off 16-byte borders: up to so many rows of hidden they go through registers, from there
+// on a copy pays.  bf16, losses only: 300 x 1001 x 60000 106 us to 135, 1000 x 1001 x 60000 240 to 205; backward: 30 x 2050
+// x 100001 313 us to 558, 100 x 1001 x 60000 298 to 220.
+constexpr int64_t ANY_ROWS_F = 512, ANY_ROWS_B = 64;
 static bool make_plan(const nif_head_desc* h, Plan& p) {
   if (!h || h->rows < 0 || h->features <= 0 || h->classes <= 0 || h->top < 0) return false;
   if (h->dtype != NIF_F32 && h->dtype != NIF_BF16 && h->dtype != NIF_F16) return false;
@@ -1395,8 +1495,13 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.v = h->classes;
   p.k = h->top > 0 ? h->top : 1;
   p.e = h->dtype == NIF_F32 ? 4 : 2;
-  p.pack_w = h->ldw > HEAD_MAX_LD || (p.e == 2 && (p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0));
-  const int64_t per = (p.pack_w && p.ldd > p.cap ? (int64_t)p.ldd : p.cap) * p.e;  // bytes of one class of a piece
+  const bool odd = p.e == 2 && (p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0);
+  const bool far = h->ldw > HEAD_MAX_LD;
+  p.any_f = p.e == 4 || (odd && !far && p.n <= ANY_ROWS_F);
+  p.any_b = p.e == 4 || (odd && !far && p.n <= ANY_ROWS_B);
+  p.pack_f = far || (odd && !p.any_f);
+  p.pack_b = far || (odd && !p.any_b);
+  const int64_t per = (p.pack_b && p.ldd > p.cap ? (int64_t)p.ldd : p.cap) * p.e;  // bytes of one class of a piece
   int64_t c = (int64_t)(PIECE_BYTES / per) / 256 * 256;
   if (c < 1024) c = 1024;
   if (c > p.v) c = p.v;
@@ -1418,11 +1523,11 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   p.s_rows = take(at, (size_t)p.cap * 4);
   p.s_inv = take(at, (size_t)p.cap * 4);
   p.s_lse = take(at, (size_t)p.cap * 4);
-  p.s_uk = take(at, (size_t)p.cap * p.k * 4);
   p.s_h = take(at, (size_t)p.cap * p.ldd * p.e);
   p.ldu = round_up(p.v, 4);
   p.keep = kept_logits_are_faster(p, h->forward_only != 0);
   p.s_u = take(at, p.keep ? (size_t)p.n * p.ldu * 4 : 0);
+  p.s_uk = take(at, p.keep ? 0 : (size_t)p.cap * p.k * 4);
   p.state = at;
   return true;
 }
@@ -1451,17 +1556,23 @@ static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
   g.nt = (g.N + s.bn - 1) / s.bn;
   const dim3 grid((unsigned)((int64_t)g.mt * g.nt * g.splits));
   if (grid.x == 0) return;
-  if constexpr (T::WIDE) {
+  if (s.any && (T::WIDE || !TRB)) {
+    if constexpr (T::WIDE || !TRB) {  // 16 bits: dweight does not read the weight
+      if (s.bn == 64)
+        hipLaunchKernelGGL((head_gemm_any_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+      else
+        hipLaunchKernelGGL((head_gemm_any_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+    }
+    return;
+  }
+  if constexpr (!T::WIDE) {
     if (s.bn == 64)
-      hipLaunchKernelGGL((head_gemm32_kernel<128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
-    else
-      hipLaunchKernelGGL((head_gemm32_kernel<128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
-  } else if (s.bn == 64)
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
   else if (s.bn == 256)
     hipLaunchKernelGGL((head_gemm_kernel<T, 256, 256, 2, 4, TRA, TRB, EPI>), grid, dim3(512), 0, st, g);
   else
     hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+  }
 }
 
 // of the products that make logits of a piece of `classes`
@@ -1471,20 +1582,20 @@ struct FwdSpace {
 static FwdSpace forward_space(const Plan& p) {
   FwdSpace f;
   size_t at = 0;
-  const Shape s = logit_shape(p, p.pack_w ? p.piece : p.v);
+  const Shape s = logit_shape(p, p.pack_f ? p.piece : p.v, p.any_f);
   const int64_t tiles = p.keep ? (p.v + KEPT - 1) / KEPT : (p.v / s.bm + p.v / p.piece + 2) * s.wm;
   f.stats = take(at, (size_t)tiles * p.cap * 8);
-  const int splits = p.keep ? kept_shape(p, p.pack_w ? p.piece : p.v).splits : 1;
+  const int splits = p.keep ? kept_shape(p, p.pack_f ? p.piece : p.v).splits : 1;
   f.part = take(at, splits > 1 ? (size_t)splits * p.n * p.ldu * 4 : 0);
-  f.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * p.e : 0);
+  f.w = take(at, p.pack_f ? (size_t)p.piece * p.ldd * p.e : 0);
   f.bytes = at;
   return f;
 }
 
 // the weight rows of a piece as a side with classes along its rows
-static Side weight_side(const nif_head_desc* h, const Plan& p, int v0, int vc, void* packed, hipStream_t st) {
+static Side weight_side(const nif_head_desc* h, const Plan& p, int v0, int vc, bool pack, void* packed, hipStream_t st) {
   const char* src = (const char*)h->weight + (size_t)v0 * h->ldw * p.e;
-  if (!p.pack_w) return Side{src, h->ldw, vc, p.d};
+  if (!pack) return Side{src, h->ldw, vc, p.d};
   if (p.e == 4)
     hipLaunchKernelGGL(head_pack_kernel<float>, dim3(vc), dim3(256), 0, st, (const float*)src, h->ldw, p.d, (float*)packed, p.ldd);
   else
@@ -1498,21 +1609,21 @@ static const void* bias_at(const nif_head_desc* h, int v0) {
 
 template <class T>
 static void forward_products(const nif_head_desc* h, const Plan& p, char* state, char* ws, const FwdSpace& f, int& tiles, hipStream_t st) {
-  const Shape s = logit_shape(p, p.pack_w ? p.piece : p.v);
+  const Shape s = logit_shape(p, p.pack_f ? p.piece : p.v, p.any_f);
   tiles = 0;
-  for (int v0 = 0; v0 < p.v; v0 += p.pack_w ? p.piece : p.v) {
-    const int vc = p.pack_w ? (p.v - v0 < p.piece ? p.v - v0 : p.piece) : p.v;
+  for (int v0 = 0; v0 < p.v; v0 += p.pack_f ? p.piece : p.v) {
+    const int vc = p.pack_f ? (p.v - v0 < p.piece ? p.v - v0 : p.piece) : p.v;
     GemmArgs g = {};
-    g.A = weight_side(h, p, v0, vc, ws + f.w, st);
+    g.A = weight_side(h, p, v0, vc, p.pack_f, ws + f.w, st);
     g.B = Side{state + p.s_h, p.ldd, (int)p.cap, p.ldd};
     g.M = vc;
     g.N = (int)p.n;
     g.n_dev = (const int*)(state + p.s_count);
-    g.K = T::WIDE ? p.d : p.ldd;
+    g.K = p.any_f ? p.d : p.ldd;
     g.splits = 1;
     g.bias = bias_at(h, v0);
     if (p.keep) {
-      const Shape ks = kept_shape(p, p.pack_w ? p.piece : p.v);
+      const Shape ks = kept_shape(p, p.pack_f ? p.piece : p.v);
       g.splits = ks.splits;
       g.out_kind = OUT_F32;
       g.acc = (float*)(ks.splits > 1 ? ws + f.part : state + p.s_u) + v0;
@@ -1528,7 +1639,7 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
     tiles += g.mt * s.wm;
   }
   if (p.keep) {
-    const int splits = kept_shape(p, p.pack_w ? p.piece : p.v).splits;
+    const int splits = kept_shape(p, p.pack_f ? p.piece : p.v).splits;
     tiles = (p.v + KEPT - 1) / KEPT;
     hipLaunchKernelGGL(head_kept_kernel<T>, dim3((unsigned)p.n, tiles), dim3(256), 0, st, (const float*)(ws + f.part), splits,
                        p.n * p.ldu, (float*)(state + p.s_u), p.ldu, p.v, (const int*)(state + p.s_count), h->bias,
@@ -1539,7 +1650,7 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
 template <int DT>
 static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStream_t st) {
   hipLaunchKernelGGL(head_pack_rows_kernel<DT>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d,
-                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), (float*)(state + p.s_uk));
+                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), p.keep ? nullptr : (float*)(state + p.s_uk));
 }
 
 struct BwdSpace {
@@ -1552,14 +1663,14 @@ static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
   b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
-  b.dh = shape_of(DHIDDEN, p.d, p.n, p.piece, p.e, p.e, true);
-  b.dw = shape_of(DWEIGHT, p.d, p.piece, p.n, p.e, p.e, true);
+  b.dh = shape_of(DHIDDEN, p.d, p.n, p.piece, p.e, p.e, true, p.any_b);
+  b.dw = shape_of(DWEIGHT, p.d, p.piece, p.n, p.e, p.e, true, false);
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
   b.scale = take(at, 4);
   b.dz = take(at, (size_t)p.cap * b.ldz * p.e);
-  b.w = take(at, p.pack_w ? (size_t)p.piece * p.ldd * p.e : 0);
+  b.w = take(at, p.pack_b ? (size_t)p.piece * p.ldd * p.e : 0);
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
   const size_t part_h = b.dh.splits > 1 ? (size_t)b.dh.splits * p.cap * b.dh_ld * 4 : 0;
   const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
@@ -1592,11 +1703,11 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
   for (int v0 = 0; v0 < p.v; v0 += p.piece) {
     const int vc = p.v - v0 < p.piece ? p.v - v0 : p.piece;
     const bool first = v0 == 0, last = v0 + vc == p.v;
-    const Side w = weight_side(h, p, v0, vc, ws + b.w, st);
-    const int kz = T::WIDE ? vc : (int)round_up(vc, K_PAD);  // the contraction over the piece's columns of dz
+    const Side w = weight_side(h, p, v0, vc, p.pack_b, ws + b.w, st);
+    const int kz = p.any_b ? vc : (int)round_up(vc, K_PAD);  // the contraction over the piece's columns of dz
     if (p.keep) {
       hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + KEPT_DZ - 1) / KEPT_DZ)), dim3(256),
-                         0, st, (const float*)(state + p.s_u), p.ldu, v0, vc, tg, rows, count, uk, lse, coef, cp, dz, b.ldz);
+                         0, st, (const float*)(state + p.s_u), p.ldu, v0, vc, tg, rows, count, lse, coef, cp, dz, b.ldz);
     } else {
       GemmArgs g = {};
       g.A = w;
@@ -1604,7 +1715,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.M = vc;
       g.N = (int)round_up(p.n, K_PAD);
       g.n_dev = count;
-      g.K = T::WIDE ? p.d : p.ldd;
+      g.K = p.any_b ? p.d : p.ldd;
       g.splits = 1;
       g.bias = bias_at(h, v0);
       g.inv_tau = tg.inv_tau;
@@ -1612,7 +1723,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.cp = cp;
       g.dz = dz;
       g.ldz = b.ldz;
-      run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc), g, st);
+      run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc, p.any_b), g, st);
     }
     if (p.n > 0 && !p.keep)
       hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
@@ -1629,7 +1740,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
       GemmArgs g = {};
       g.A = Side{hp, p.ldd, p.ldd, (int)p.cap};
-      g.B = Side{dz, b.ldz, kz, (int)p.cap};
+      g.B = Side{dz, b.ldz, (int)round_up(vc, K_PAD), (int)p.cap};
       g.M = p.d;
       g.N = vc;
       g.K = (int)p.cap;
@@ -1654,7 +1765,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       GemmArgs g = {};
       g.A = w;
       g.A.klim = w.rlim;
-      g.A.rlim = p.pack_w ? p.ldd : p.d;
+      g.A.rlim = p.pack_b ? p.ldd : p.d;
       g.B = Side{dz, b.ldz, (int)p.cap, kz};
       g.M = p.d;
       g.N = (int)p.n;
@@ -1771,7 +1882,7 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
       forward_products<F16>(h, p, s, (char*)ws, f, tiles, st);
     const float2* stats = (const float2*)((char*)ws + f.stats);
     hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg, rows, count,
-                       (float*)(s + p.s_lse), (const float*)(s + p.s_uk), row_loss, p.n, h->reduction, count + 1, loss);
+                       (float*)(s + p.s_lse), (const float*)(s + p.s_uk), p.keep ? (const float*)(s + p.s_u) : nullptr, p.ldu, row_loss, p.n, h->reduction, count + 1, loss);
   } else {
     hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, targets_of(h, p, s), nullptr, (int64_t)0, p.v, (int64_t)0, rows, inv,
                        count, nullptr);

@@ -245,6 +245,48 @@ def test_rows_far_apart(ops, dt, k):
     _check_head(ops, dt, 300, 100, 500, k=k, layout=apart, seed=7)
 
 
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n', [5, 63, 65, 300, 600])
+def test_rows_off_16_byte_borders(ops, dt, n):
+    """Few and many rows against a weight that direct loads cannot take, with and without kept logits."""
+    for d, v, k in ((131, 1543, None), (77, 9001, 6)):
+        _check_head(ops, dt, n, d, v, k=k, tau=2.0 if k else 1.0, empty=0.2, seed=n + d)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_many_targets_of_few_classes(ops, dt):
+    _check_head(ops, dt, 1100, 962, 251, k=93, tau=4.0, empty=0.1, seed=9)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n', [5, 700])
+def test_saved_tensors_that_come_back_elsewhere(ops, dt, n):
+    """Saved tensors may return at another address, with other strides, than the forward pass saw."""
+    g = torch.Generator(device='cuda').manual_seed(21)
+    h = torch.randn(n, 776, generator=g, device='cuda').to(dt)
+    w = torch.randn(5003, 776, generator=g, device='cuda').to(dt)
+    y = torch.randint(0, 5003, (n,), generator=g, device='cuda')
+
+    def grads(hook, weight):
+        x, weight = h.clone().requires_grad_(), weight.detach().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(hook, lambda t: t):
+            loss = ops.linear_cross_entropy(x, weight, y)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, weight)))
+
+    def moved(t):
+        if t.dim() != 2:
+            return t
+        out = torch.empty(t.shape[0], t.shape[1] + 3, dtype=t.dtype, device=t.device)[:, 1:-2]
+        return out.copy_(t)
+    far = moved(w)
+    for hook, weight in ((moved, w), (lambda t: t.clone(), far)):
+        want, got = grads(lambda t: t, weight), grads(hook, weight)
+        assert torch.equal(got[0], want[0])
+        # the same products by another kernel: each is off by its bound of the formula's, here in the large
+        for a, b in zip(got[1:], want[1:]):
+            assert float((a - b).float().norm()) <= 4 * max(U16[dt], 64 * U) * float(b.float().norm())
+
+
 def test_kept_logits_of_a_weight_that_is_packed_in_pieces(ops):
     """Rows that 16-byte loads cannot take, more bytes of them than a piece holds."""
     _check_head(ops, torch.bfloat16, 4, 50001, 2700, seed=8)
