@@ -923,22 +923,25 @@ __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restr
 }
 
 // ---- the loss of each row -------------------------------------------------------------------------------
-// 16 packed rows a block: joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.  The
+// ROWS packed rows a block (16, a line of the statistics; two where there are at most FINISH_FEW rows, for more blocks: 41 rows
+// of 2180 tiles 17 us to 8): joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.  The
 // block that is done last (`done`, cleared by head_rows_kernel) reduces the losses: sum or mean over the rows that count,
 // in a fixed order and 64 bits.
 constexpr int FINISH_NT = 1024;
+constexpr int64_t FINISH_FEW = 512;
+template <int ROWS>
 __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
                                                                 const int* __restrict__ rows, const int* __restrict__ count,
                                                                 float* __restrict__ lse, const float* __restrict__ uk,
                                                                 const float* __restrict__ u, int64_t ldu, float* loss,
                                                                 int64_t all_rows, int reduction, int* done, float* __restrict__ reduced) {
-  constexpr int PARTS = FINISH_NT / 16;
-  __shared__ float sh_top[16][PARTS + 1], sh_sum[16][PARTS + 1];
+  constexpr int PARTS = FINISH_NT / ROWS;
+  __shared__ float sh_top[ROWS][PARTS + 1], sh_sum[ROWS][PARTS + 1];
   __shared__ double sh[16];
   __shared__ int last;
-  const int i0 = blockIdx.x * 16, n = *count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i0 = blockIdx.x * ROWS, n = *count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (i0 < n) {
-    const int r = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int r = threadIdx.x % ROWS, part = threadIdx.x / ROWS;
     float top = -INFINITY, sum = 0.f;
     if (i0 + r < n)
 #pragma unroll 4
@@ -950,8 +953,10 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
     sh_sum[r][part] = sum;
     __syncthreads();
     const int i = i0 + wave;  // a wave a row
-    if (i < n) {
+    if (wave < ROWS && i < n) {
       top = sh_top[wave][lane], sum = sh_sum[wave][lane];
+#pragma unroll
+      for (int p = 64 + lane; p < PARTS; p += 64) join(top, sum, sh_top[wave][p], sh_sum[wave][p]);
       const float all = wave_max_f32(top), ref = all == -INFINITY ? 0.f : all;
       sum = wave_sum_f32(sum * expf(top - ref));
       const float l = all + logf(sum);
@@ -1881,8 +1886,15 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
     else
       forward_products<F16>(h, p, s, (char*)ws, f, tiles, st);
     const float2* stats = (const float2*)((char*)ws + f.stats);
-    hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg, rows, count,
-                       (float*)(s + p.s_lse), (const float*)(s + p.s_uk), p.keep ? (const float*)(s + p.s_u) : nullptr, p.ldu, row_loss, p.n, h->reduction, count + 1, loss);
+    const auto finish = [&](auto each) {
+      hipLaunchKernelGGL(head_finish_kernel<each>, dim3((unsigned)((p.n + each - 1) / each)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg,
+                         rows, count, (float*)(s + p.s_lse), (const float*)(s + p.s_uk), p.keep ? (const float*)(s + p.s_u) : nullptr,
+                         p.ldu, row_loss, p.n, h->reduction, count + 1, loss);
+    };
+    if (p.n <= FINISH_FEW)
+      finish(std::integral_constant<int, 2>());
+    else
+      finish(std::integral_constant<int, 16>());
   } else {
     hipLaunchKernelGGL(head_rows_kernel, dim3(1), dim3(1024), 0, st, targets_of(h, p, s), nullptr, (int64_t)0, p.v, (int64_t)0, rows, inv,
                        count, nullptr);
