@@ -343,6 +343,40 @@ def test_masked_classes_and_extreme_logits(ops, dt):
     assert abs(float(loss) - float(ref)) < 1e-4 * float(ref)
 
 
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, d, v', [(5, 776, 20011), (40, 131, 9001), (700, 72, 3001), (1100, 264, 1543)])
+def test_masked_classes_of_large_heads(ops, dt, n, d, v):
+    """Masked classes, a masked label, a row of +inf logits and one of NaN, with and without kept logits."""
+    g = torch.Generator().manual_seed(n)
+    live = v // 3
+    h, w = torch.randn(n, d, generator=g).to(dt), (torch.randn(v, d, generator=g) / math.sqrt(d)).to(dt)
+    y = torch.randint(0, live, (n,), generator=g)
+    for low in (-math.inf, torch.finfo(dt).min):
+        b = torch.zeros(v, dtype=dt)
+        b[live:] = low
+        y[0], y[1] = live + 1 if low == -math.inf else 0, -100
+        x = h.clone()
+        x[1], x[2, 0] = math.nan, math.nan
+        hg, wg, bg = (t.cuda().requires_grad_() for t in (x, w, b))
+        loss = ops.linear_cross_entropy(hg, wg, y.cuda(), bg, reduction='none')
+        up = torch.ones(n, device='cuda')
+        up[2] = 0.0
+        z = h.double() @ w.double()[:live].t()
+        want = torch.nn.functional.cross_entropy(z, y.clamp(0, live - 1), reduction='none')
+        du = (d + 12) * U * float((h.double().abs() @ w.double().abs().t()).max())
+        got = loss.detach().cpu().double()
+        assert got[1] == 0 and torch.isnan(got[2]) and (got[0] == math.inf or low != -math.inf)
+        assert torch.all((got - want)[3:].abs() <= 2 * du + 2.0 ** -18 + 2 * U * want[3:].abs())
+        keep = torch.arange(n) != 2
+        hg, wg, bg = (t.cuda().requires_grad_() for t in (x[keep], w, b))
+        loss = ops.linear_cross_entropy(hg, wg, y[keep].cuda(), bg, reduction='sum')
+        dh, dw, db = torch.autograd.grad(loss, (hg, wg, bg))
+        assert all(torch.isfinite(t).all() for t in (dh, dw, db)) and torch.all(dh[1] == 0)
+        masked = torch.arange(v) >= live
+        masked[int(y[0])] = False
+        assert torch.all(dw.cpu()[masked] == 0) and torch.all(db.cpu()[masked] == 0)
+
+
 def test_targets_that_do_not_exist_make_their_row_nan(ops):
     h, w = torch.randn(6, 16).cuda().requires_grad_(), torch.randn(9, 16).cuda().requires_grad_()
     y = torch.tensor([0, 9, -1, 2 ** 40, 8, -100]).cuda()
