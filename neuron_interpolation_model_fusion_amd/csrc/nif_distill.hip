@@ -325,7 +325,7 @@ __device__ __forceinline__ float kth_largest(float x, int k, float* sh) {
   return x;
 }
 
-constexpr int TOP_LIST = 2048;
+constexpr int TOP_LIST = 8;  // keys a thread in the list
 
 // Any row: the k-th largest order by four passes of eight bits each, then everything above it and the first of its
 // equals by class.  `key` ends with the k entries, unordered beyond that.
@@ -382,7 +382,8 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
                                                         void* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16, U = DT == NIF_F32 ? 4 : 2;
-  __shared__ unsigned long long key[TOP_LIST];
+  constexpr int LIST = TOP_LIST * NT;
+  __shared__ unsigned long long key[LIST];
   __shared__ float sh[NT];
   __shared__ int sh_n;
   const int64_t row = blockIdx.x;
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
   run.init();
   const auto put = [&](float x, int c) {
     const int at = atomicAdd(&sh_n, 1);
-    if (at < TOP_LIST) key[at] = key_of(x, c);
+    if (at < LIST) key[at] = key_of(x, c);
   };
   if ((int)threadIdx.x < r.loose()) {
     const float x[1] = {(float)r.z[r.loose_at(threadIdx.x)]};
@@ -427,15 +428,15 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
   if (k <= NT && stretch > 0) bar = kth_largest<NT>(mine, k, sh);
   __syncthreads();
   int n = sh_n;
-  if (k > NT || n > TOP_LIST || l != l || n < k) {  // l is NaN where the row holds NaN or +inf, which floats do not order
+  if (k > NT || n > LIST || l != l || n < k) {  // l is NaN where the row holds NaN or +inf, which floats do not order
     __syncthreads();
     select_by_digits<DT, NT>(r.z, classes, k, key, (unsigned*)sh, &sh_n);
     n = k;
   } else if (n > 2 * k) {
-    unsigned long long mykeys[TOP_LIST / NT];
+    unsigned long long mykeys[TOP_LIST];
     const unsigned long long least = (unsigned long long)order_of(bar) << 32;
 #pragma unroll
-    for (int q = 0; q < TOP_LIST / NT; ++q) {
+    for (int q = 0; q < TOP_LIST; ++q) {
       const int at = q * NT + threadIdx.x;
       mykeys[q] = at < n ? key[at] : 0;
     }
@@ -443,7 +444,7 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
     if (threadIdx.x == 0) sh_n = 0;
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < TOP_LIST / NT; ++q)
+    for (int q = 0; q < TOP_LIST; ++q)
       if (q * NT < n && mykeys[q] > least) key[atomicAdd(&sh_n, 1)] = mykeys[q];  // no key is `least` itself: classes end below
     __syncthreads();
     n = sh_n;
@@ -537,9 +538,9 @@ extern "C" int nif_distill_forward(const void* logits, int64_t ld, int64_t rows,
   float* row_loss = reduction == NIF_REDUCE_NONE ? loss : (float*)ws;
   clear_err();
   if (rows > 0) {
-    // a block of 1024 where rows alone do not fill the machine and are long
-    if (rows < 1024 && classes >= 8192)
-      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, logits, ld, classes,
+    // blocks of 512 where rows are few and long (256 x 131072 f32: 27 us to 36; 777 x 50001 f16: 25 to 20, with 1024 threads 36)
+    if (rows <= 256 && (int64_t)classes * (dtype == NIF_F32 ? 4 : 2) >= 96 << 10)
+      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 512>), dim3((unsigned)rows), dim3(512), 0, st, logits, ld, classes,
                                             t, top_indices, top_values, top_lse, (float*)((char*)state + s.lse), row_loss));
     else
       NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, t,
@@ -581,8 +582,19 @@ extern "C" int nif_top_logits(const void* logits, int64_t ld, int64_t rows, int 
   if (rows == 0) return NIF_OK;
   hipStream_t st = (hipStream_t)stream;
   clear_err();
-  if (rows < 1024 && classes >= 8192)
+  // Threads a row.  The bar is of use for k up to three quarters of them (2048 x 50001 bf16, k = 500: 307 us with 1024 threads,
+  // 672 with 512; k = 300: 150 with 512, 606 by digits with 256), and the list holds enough for long rows of many
+  // (2048 x 131072, k = 200: 255 us with 512, 880 with 256).  Else wider blocks where rows are few or long (2048 x 131072 f32,
+  // k = 20: 280 us with 512, 323 with 256; but 2048 x 50001 bf16: 113, 78).  Many of short rows are selected by digits at once
+  // (2048 x 3000, k = 700: 112 us with 256 threads, 313 with 1024), and so are over three quarters of 1024 (2048 x 50001, k = 1024: 618 us with 256
+  // threads, 956 with 1024; 400 rows: 468 and 256).
+  const int64_t bytes = (int64_t)classes * (dtype == NIF_F32 ? 4 : 2);
+  const bool wide = top > 192 || (top > 128 && bytes >= 256 << 10) || (rows <= 512 && bytes >= 96 << 10) || bytes >= 512 << 10;
+  if (top > 384 && classes >= 8192 && (top <= 768 || rows < 1024))
     NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, logits, ld, classes, top,
+                                          1.f / temperature, values, indices, lse));
+  else if (wide && top <= 384)
+    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 512>), dim3((unsigned)rows), dim3(512), 0, st, logits, ld, classes, top,
                                           1.f / temperature, values, indices, lse));
   else
     NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, top,

@@ -492,6 +492,20 @@ def test_top_logits(ops, dt, n, v, k):
 
 
 @pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, v, k', [(3, 131072, 200), (5, 140001, 129), (2, 50001, 384), (2, 50001, 385), (3, 20011, 768), (2, 9000, 1000),
+                                     (1100, 8200, 1000), (1030, 8200, 700), (600, 49153, 16)])
+def test_top_logits_of_every_block_width(ops, dt, n, v, k):
+    """Equal 16-bit logits abound: ties go to the lower class."""
+    g = torch.Generator(device='cuda').manual_seed(v + k)
+    z = (3 * torch.randn(n, v, generator=g, device='cuda')).to(dt)
+    values, indices, lse = ops.top_logits(z, k, temperature=2.0)
+    order = torch.sort(z.float(), dim=1, descending=True, stable=True)
+    assert torch.equal(values.float(), order.values[:, :k]) and torch.equal(indices.long(), order.indices[:, :k])
+    want = torch.logsumexp(z.double() / 2, 1)
+    assert torch.all((lse.double() - want).abs() <= 2.0 ** -18 + 2 * U * want.abs())
+
+
+@pytest.mark.parametrize('dt', TYPES)
 def test_top_logits_of_ties_masks_and_nan(ops, dt):
     n, v, k = 8, 3000, 30
     g = torch.Generator().manual_seed(9)
