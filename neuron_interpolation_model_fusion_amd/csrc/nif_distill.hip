@@ -50,16 +50,17 @@ struct RowView {
 
 // 2^x. 16-bit inputs: the hardware's (2^-22 relative); f32: the library's exponential of the natural argument.
 template <int DT>
-__device__ __forceinline__ float exp_of(float x, float scale, float shift) {
-  return DT == NIF_F32 ? expf(fmaf(x, scale, -shift)) : __builtin_amdgcn_exp2f(fmaf(x, scale, -shift));
+__device__ __forceinline__ float exp_of(float x) {
+  return DT == NIF_F32 ? expf(x) : __builtin_amdgcn_exp2f(x);
 }
-// what logits are multiplied with before exp_of: 1 / tau, and log2(e) where the hardware's exponential is used
+// what differences of logits are multiplied with before exp_of: 1 / tau, and log2(e) where the hardware's exponential is used
 template <int DT>
 __device__ __forceinline__ float exp_scale(float inv_tau) {
   return DT == NIF_F32 ? inv_tau : inv_tau * 1.4426950408889634f;
 }
 
-// Running (maximum, sum of exponentials) of scaled logits: one rescaling per batch of elements.
+// Running (maximum, sum of exponentials): one rescaling per batch of elements.  The maximum is subtracted before anything is
+// scaled: a type's lowest value, the mask of a class, is finite, its product with log2(e) or 1 / tau need not be.
 template <int DT>
 struct Running {
   float top, sum;  // top in the logits' own units
@@ -69,26 +70,26 @@ struct Running {
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) m = fmaxf(m, x[e]);
-    const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.f : now * scale;
+    const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.f : now;
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += exp_of<DT>(x[e], scale, ref);
-    sum = sum * exp_of<DT>(top, scale, ref) + s;
+    for (int e = 0; e < N; ++e) s += exp_of<DT>((x[e] - ref) * scale);
+    sum = sum * exp_of<DT>((top - ref) * scale) + s;
     top = now;
     return m;
   }
   // the block's lse in natural units; every thread gets it.  sh: 2 * waves floats
   template <int NT>
   __device__ __forceinline__ float lse(float scale, float inv_tau, float* sh) {
-    const float wtop = wave_max_f32(top), ref = wtop == -INFINITY ? 0.f : wtop * scale;
-    const float wsum = wave_sum_f32(sum * exp_of<DT>(top, scale, ref));
+    const float wtop = wave_max_f32(top), ref = wtop == -INFINITY ? 0.f : wtop;
+    const float wsum = wave_sum_f32(sum * exp_of<DT>((top - ref) * scale));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (lane == 0) sh[2 * wave] = wtop, sh[2 * wave + 1] = wsum;
     __syncthreads();
-    float t = sh[0] * inv_tau, s = sh[1];
+    float t = sh[0], s = sh[1];
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) join(t, s, sh[2 * w] * inv_tau, sh[2 * w + 1]);
-    return t + logf(s);
+    for (int w = 1; w < NT / 64; ++w) join(t, s, sh[2 * w], sh[2 * w + 1], inv_tau);
+    return t * inv_tau + logf(s);
   }
 };
 
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restric
   const float coef = live ? (per_row ? grad[row] : count ? grad[0] / *count : grad[0]) * t.tau : 0.f;
   const float cp = live ? coef * P : 0.f, l = lse[row];
   const float scale = exp_scale<DT>(t.inv_tau), shift = DT == NIF_F32 ? l : l * 1.4426950408889634f;
-  const auto dz = [&](float x) { return live ? cp * exp_of<DT>(x, scale, shift) : 0.f; };
+  const auto dz = [&](float x) { return live ? cp * exp_of<DT>(fmaf(x, scale, -shift)) : 0.f; };
   int c0, c1;  // this block's columns
   if (((uintptr_t)r.z & 15) == ((uintptr_t)o & 15)) {
     const int v0 = min(r.vecs, (int)blockIdx.y * (stretch / V)), v1 = min(r.vecs, v0 + stretch / V);
@@ -375,7 +376,7 @@ __device__ __forceinline__ void select_by_digits(const typename Elem<DT>::t* z, 
 // whatever comes later must exceed it; it is taken anew after 1, 2, 4, 8, .. stretches, which leaves about 6 k elements
 // of a row of 131072 (k log2 of the stretches) in a list in LDS.  The last bar cuts the list to little more than k, which are sorted.  Rows that
 // this does not fit (more than the list holds: ties at the bar, rising rows; NaN) are selected by digits instead.  The
-// log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 260 us,
+// log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 263 us,
 // 4.1 TB/s; 400 x 1000 f32 in 13 us, a launch's latency.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,

@@ -57,10 +57,10 @@ __device__ __forceinline__ void unpack16(vec4f raw, float (&x)[Elem<DT>::PER16])
   for (int e = 0; e < Elem<DT>::PER16; ++e) x[e] = (float)v[e];
 }
 
-// (max, sum of exp(. - max)) pairs: the empty one is (-inf, 0); NaN stays in the sum
-__device__ __forceinline__ void join(float& top, float& sum, float t2, float s2) {
+// (max, sum of exp((. - max) / tau)) pairs: the empty one is (-inf, 0); NaN stays in the sum
+__device__ __forceinline__ void join(float& top, float& sum, float t2, float s2, float inv_tau = 1.f) {
   const float m = fmaxf(top, t2), ref = m == -INFINITY ? 0.f : m;
-  sum = sum * expf(top - ref) + s2 * expf(t2 - ref);
+  sum = sum * expf((top - ref) * inv_tau) + s2 * expf((t2 - ref) * inv_tau);
   top = m;
 }
 

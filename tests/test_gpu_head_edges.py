@@ -1,0 +1,84 @@
+"""-m gpu: the head losses and top_logits where sizes and values are at their ends, against their formulas in 64 bits.
+
+Tolerances, from the unit roundoff of each step (u16: half a step of the type, u = 2^-24), where the logits z themselves are
+exact (given, or sums of few small integers): exponents are differences of logits, R = max (z - z') / tau over the unmasked
+ones, so du = 4 u R (difference, 1 / tau, product, the exponential's argument); a sum of exponentials 2^-20 (fast
+exponentials 2^-21 relative, the sum itself), a logarithm 2^-22, together under 2^-18:
+  row loss    tau^2 P (2 du + 2^-18) + 2 u |loss|
+  gradients   of logits: u16 |dz| + (2 du + 2^-18) c q, q = P s + p
+              of a head: dz rounded to u16 as well, c sum (u16 + 2 du + 2^-18 + K u) q |x| over a contraction of K, u16 |out|
+  f16         2^-25 for subnormals of an output
+"""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_head_losses import TYPES, U, U16, _formula, _targets
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def ops():
+    from neuron_interpolation_model_fusion_amd import ops
+    return ops
+
+
+def _check_logits(ops, z, values, indices, tau, reach, reduction='none'):
+    """topk_distillation and its gradient; reach: the largest difference of two unmasked logits of a row."""
+    n = z.shape[0]
+    p, at, live = _targets(values=values, indices=indices, tau=tau)
+    zg = z.cuda().requires_grad_()
+    loss = ops.topk_distillation(zg, values.cuda(), indices.cuda(), temperature=tau, reduction=reduction)
+    got, = torch.autograd.grad(loss.sum(), zg)
+    want, rows, dz, q, coef = _formula(z.double(), p, at, live, tau, reduction, torch.ones(n))
+    du = 4 * U * reach / tau
+    tol = tau * tau * p.sum(1) * (2 * du + 2.0 ** -18) + 2 * U * rows.abs() + 1e-30
+    tol = tol if reduction == 'none' else tol.sum() / (max(1, int(live.sum())) if reduction == 'mean' else 1) + U * want.abs()
+    off = (loss.detach().cpu().double() - want).abs()
+    assert torch.all(off <= tol), float((off / tol).max())
+    bound = U16[z.dtype] * dz.abs() + (2 * du + 2.0 ** -18) * coef * q + (2.0 ** -25 if z.dtype == torch.float16 else 1e-37)
+    off = (got.cpu().double() - dz).abs()
+    assert torch.all(off <= bound), float((off / bound).max())
+
+
+def _top(n, k, classes, g):
+    return torch.randn(n, k, generator=g), torch.stack([torch.randperm(classes, generator=g)[:k] for _ in range(n)])
+
+
+@pytest.mark.parametrize('tau', [1.0, 0.5, 2.0])
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, v', [(3, 40), (5, 1001), (3, 30001), (300, 3001), (3, 262147)])
+def test_classes_masked_by_the_lowest_value(ops, dt, tau, n, v):
+    """finfo.min in a stretch of classes as wide as many threads' first loads, in the odd elements at a row's ends, in every
+    class but one."""
+    g = torch.Generator().manual_seed(v)
+    low = torch.finfo(dt).min
+    z = (3 * torch.randn(n, v, generator=g)).to(dt)
+    z[0, : v - v // 8 - 1] = low
+    z[1, 0], z[1, v - 2:] = low, low
+    z[2, : v - 2], z[2, v - 1] = low, low
+    values, _ = _top(n, 4, v, g)
+    indices = torch.stack([torch.tensor([v - 3, v - 4, v - 2, -1]) for _ in range(n)])
+    indices[1], indices[2] = torch.tensor([1, 2, 3, 4]), torch.tensor([v - 2, -1, -1, -1])
+    _check_logits(ops, z, values, indices, tau, 40.0)
+    _check_logits(ops, z, values, indices, tau, 40.0, 'mean')
+    k = min(30, v)
+    got, at, lse = ops.top_logits(z.cuda(), k, temperature=tau)
+    want = torch.logsumexp(z.double() / tau, 1)
+    assert torch.all((lse.cpu().double() - want).abs() <= 2.0 ** -18 + 2 * U * want.abs() + 4 * U * 40 / tau)
+    order = torch.sort(z.float(), dim=1, descending=True, stable=True)
+    assert torch.equal(got.cpu().float(), order.values[:, :k]) and torch.equal(at.cpu().long(), order.indices[:, :k])
+
+
+@pytest.mark.parametrize('tau', [1.0, 0.5, 2.0])
+@pytest.mark.parametrize('dt', TYPES)
+def test_the_log_sum_exp_of_a_row_of_lowest_values(ops, dt, tau):
+    """low / tau + log V, which low absorbs; beyond float32's range it is -inf."""
+    for v in (1, 7, 1000, 140001):
+        z = torch.full((2, v), torch.finfo(dt).min, dtype=dt)
+        values, at, lse = ops.top_logits(z.cuda(), 1, temperature=tau)
+        want = torch.logsumexp(z.double() / tau, 1).float()
+        assert torch.equal(at.cpu(), torch.zeros(2, 1, dtype=torch.int32)) and torch.equal(values.cpu(), z[:, :1])
+        assert torch.allclose(lse.cpu(), want, rtol=2.0 ** -22, atol=2.0 ** -18)
