@@ -70,7 +70,7 @@ struct Running {
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) m = fmaxf(m, x[e]);
-    const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.f : now;
+    const float now = fmaxf(top, m), ref = reference_of(now);
     float s = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) s += exp_of<DT>((x[e] - ref) * scale);
@@ -81,7 +81,7 @@ struct Running {
   // the block's lse in natural units; every thread gets it.  sh: 2 * waves floats
   template <int NT>
   __device__ __forceinline__ float lse(float scale, float inv_tau, float* sh) {
-    const float wtop = wave_max_f32(top), ref = wtop == -INFINITY ? 0.f : wtop;
+    const float wtop = wave_max_f32(top), ref = reference_of(wtop);
     const float wsum = wave_sum_f32(sum * exp_of<DT>((top - ref) * scale));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (lane == 0) sh[2 * wave] = wtop, sh[2 * wave + 1] = wsum;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict
   }
   constexpr int U = DT == NIF_F32 ? 4 : 2;
   stream_row<DT, NT, U>(r, [&](const float (&x)[U * Elem<DT>::PER16], int) { run.add(x, scale); });
-  const float lse = run.template lse<NT>(scale, t.inv_tau, sh);
+  const float l = run.template lse<NT>(scale, t.inv_tau, sh), lse = l == INFINITY ? NAN : l;  // no softmax of infinite logits
   double s = 0.0;
   for (int k = threadIdx.x; k < t.k; k += NT) {
     const int at = t.at[row * t.k + k];
@@ -376,7 +376,7 @@ __device__ __forceinline__ void select_by_digits(const typename Elem<DT>::t* z, 
 // whatever comes later must exceed it; it is taken anew after 1, 2, 4, 8, .. stretches, which leaves about 6 k elements
 // of a row of 131072 (k log2 of the stretches) in a list in LDS.  The last bar cuts the list to little more than k, which are sorted.  Rows that
 // this does not fit (more than the list holds: ties at the bar, rising rows; NaN) are selected by digits instead.  The
-// log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 263 us,
+// log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 258 us,
 // 4.1 TB/s; 400 x 1000 f32 in 13 us, a launch's latency.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,
@@ -429,7 +429,7 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
   if (k <= NT && stretch > 0) bar = kth_largest<NT>(mine, k, sh);
   __syncthreads();
   int n = sh_n;
-  if (k > NT || n > LIST || l != l || n < k) {  // l is NaN where the row holds NaN or +inf, which floats do not order
+  if (k > NT || n > LIST || !(l < INFINITY) || n < k) {  // l is NaN where the row holds NaN, which floats do not order
     __syncthreads();
     select_by_digits<DT, NT>(r.z, classes, k, key, (unsigned*)sh, &sh_n);
     n = k;

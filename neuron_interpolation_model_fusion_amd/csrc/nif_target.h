@@ -57,9 +57,13 @@ __device__ __forceinline__ void unpack16(vec4f raw, float (&x)[Elem<DT>::PER16])
   for (int e = 0; e < Elem<DT>::PER16; ++e) x[e] = (float)v[e];
 }
 
-// (max, sum of exp((. - max) / tau)) pairs: the empty one is (-inf, 0); NaN stays in the sum
+// What is subtracted before an exponential where `top` is the largest: nothing where it is infinite.
+__device__ __forceinline__ float reference_of(float top) { return fabsf(top) == INFINITY ? 0.f : top; }
+
+// (max, sum of exp((. - reference) / tau)) pairs: the empty one is (-inf, 0), one that holds +inf (+inf, +inf); NaN stays in
+// the sum
 __device__ __forceinline__ void join(float& top, float& sum, float t2, float s2, float inv_tau = 1.f) {
-  const float m = fmaxf(top, t2), ref = m == -INFINITY ? 0.f : m;
+  const float m = fmaxf(top, t2), ref = reference_of(m);
   sum = sum * expf((top - ref) * inv_tau) + s2 * expf((t2 - ref) * inv_tau);
   top = m;
 }

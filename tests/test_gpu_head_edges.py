@@ -82,3 +82,27 @@ def test_the_log_sum_exp_of_a_row_of_lowest_values(ops, dt, tau):
         want = torch.logsumexp(z.double() / tau, 1).float()
         assert torch.equal(at.cpu(), torch.zeros(2, 1, dtype=torch.int32)) and torch.equal(values.cpu(), z[:, :1])
         assert torch.allclose(lse.cpu(), want, rtol=2.0 ** -22, atol=2.0 ** -18)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('v', [1, 9, 1001, 140001])
+def test_top_logits_of_rows_that_hold_infinity(ops, dt, v):
+    """The log-sum-exp of a row that holds +inf is +inf, wherever it stands and whatever else is there but NaN."""
+    g = torch.Generator().manual_seed(v)
+    z = (3 * torch.randn(9, v, generator=g)).to(dt)
+    z[1:5], z[5] = (z[1:5].float() * 300).to(dt), -math.inf
+    for row, c in enumerate((0, v - 1, v // 2, v // 3)):
+        z[row, c] = math.inf
+    z[4, v // 4:] = math.inf
+    z[5, v // 2] = math.inf
+    z[6, v // 2] = math.nan
+    z[7, 0], z[7, v - 1] = math.inf, math.nan
+    k = min(v, 5)
+    values, at, lse = ops.top_logits(z.cuda(), k, temperature=2.0)
+    lse = lse.cpu()
+    assert torch.all(lse[:6] == math.inf) and lse[6].isnan() and lse[7].isnan() and torch.isfinite(lse[8])
+    order = torch.sort(z[:6].float(), dim=1, descending=True, stable=True)
+    assert torch.equal(values.cpu()[:6].float(), order.values[:, :k]) and torch.equal(at.cpu()[:6].long(), order.indices[:, :k])
+    # nothing finite is left of a loss on such a row
+    loss = ops.topk_distillation(z.cuda(), torch.zeros(9, 1).cuda(), torch.zeros(9, 1, dtype=torch.int64).cuda(), reduction='none')
+    assert not torch.isfinite(loss[:8]).any() and torch.isfinite(loss[8])
