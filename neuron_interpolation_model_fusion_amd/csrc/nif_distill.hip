@@ -4,6 +4,8 @@
 //   u = z / tau, s[v] = exp(u[v] - lse), loss = tau^2 ( sum_k p_k (log p_k - u[at_k]) + P lse ),
 //   dloss / dz[v] = tau ( P s[v] - sum_{k : at_k = v} p_k ).
 //
+// A row's log-sum-exp stays in two parts, its largest logit and the sum of the exponentials from there: s[v] is exp((z[v] -
+// top) / tau) / sum, as exact for logits of a thousand as for small ones.
 // All of it is bound by memory: the loss reads the logits once, the gradient reads them again and writes as much.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -78,18 +80,17 @@ struct Running {
     top = now;
     return m;
   }
-  // the block's lse in natural units; every thread gets it.  sh: 2 * waves floats
+  // the block's; every thread gets them.  sh: 2 * waves floats
   template <int NT>
-  __device__ __forceinline__ float lse(float scale, float inv_tau, float* sh) {
+  __device__ __forceinline__ void join_block(float scale, float inv_tau, float* sh) {
     const float wtop = wave_max_f32(top), ref = reference_of(wtop);
     const float wsum = wave_sum_f32(sum * exp_of<DT>((top - ref) * scale));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (lane == 0) sh[2 * wave] = wtop, sh[2 * wave + 1] = wsum;
     __syncthreads();
-    float t = sh[0], s = sh[1];
+    top = sh[0], sum = sh[1];
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) join(t, s, sh[2 * w], sh[2 * w + 1], inv_tau);
-    return t * inv_tau + logf(s);
+    for (int w = 1; w < NT / 64; ++w) join(top, sum, sh[2 * w], sh[2 * w + 1], inv_tau);
   }
 };
 
@@ -130,8 +131,8 @@ __device__ __forceinline__ void stream_row(const RowView<DT>& r, F&& f) {
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
                                                           const int32_t* __restrict__ indices, const float* __restrict__ values,
-                                                          const float* __restrict__ top_lse, float* __restrict__ lse_out,
-                                                          float* __restrict__ loss) {
+                                                          const float* __restrict__ top_lse, float* __restrict__ top_out,
+                                                          float* __restrict__ sum_out, float* __restrict__ loss) {
   __shared__ float sh[2 * NT / 64], sh_P;
   __shared__ double sh_loss[NT / 64];
   const int64_t row = blockIdx.x;
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict
   }
   __syncthreads();
   if (sh_P == NO_TARGET) {
-    if (threadIdx.x == 0) loss[row] = 0.f, lse_out[row] = 0.f;
+    if (threadIdx.x == 0) loss[row] = 0.f, top_out[row] = 0.f, sum_out[row] = 1.f;
     return;
   }
   const RowView<DT> r(logits, row * ld, classes);
@@ -155,11 +156,12 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict
   }
   constexpr int U = DT == NIF_F32 ? 4 : 2;
   stream_row<DT, NT, U>(r, [&](const float (&x)[U * Elem<DT>::PER16], int) { run.add(x, scale); });
-  const float l = run.template lse<NT>(scale, t.inv_tau, sh), lse = l == INFINITY ? NAN : l;  // no softmax of infinite logits
+  run.template join_block<NT>(scale, t.inv_tau, sh);
+  const float top = run.top, sum = top == INFINITY ? NAN : run.sum, log_sum = logf(sum);  // no softmax of infinite logits
   double s = 0.0;
   for (int k = threadIdx.x; k < t.k; k += NT) {
     const int at = t.at[row * t.k + k];
-    if (at >= 0) s += target_term(t, row, k, (float)r.z[at] * t.inv_tau, lse);
+    if (at >= 0) s += target_term(t, row, k, ((double)(float)r.z[at] - (double)top) * (double)t.inv_tau, log_sum);
   }
   s = wave_sum_f64(s);
   if (lane == 0) sh_loss[wave] = s;
@@ -167,7 +169,8 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict
   if (threadIdx.x == 0) {
     s = 0.0;
     for (int w = 0; w < NT / 64; ++w) s += sh_loss[w];
-    lse_out[row] = lse;
+    top_out[row] = top;
+    sum_out[row] = sum;
     loss[row] = (float)(s * t.tau2);
   }
 }
@@ -205,7 +208,8 @@ void launch_reduce(const float* row_loss, const float* P, int64_t n, bool mean, 
 // 4096 x 131072 bf16 in 418 us, 5.1 TB/s of both; 777 x 50001 f16 in 29 us.
 template <int DT>
 __global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
-                                                           const float* __restrict__ lse, const float* __restrict__ grad, int per_row,
+                                                           const float* __restrict__ tops, const float* __restrict__ sums,
+                                                           const float* __restrict__ grad, int per_row,
                                                            const float* __restrict__ count, void* __restrict__ out, int64_t ldo,
                                                            int stretch) {
   typedef typename Elem<DT>::t E;
@@ -216,9 +220,8 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restric
   const float P = t.P[row];
   const bool live = P != NO_TARGET;
   const float coef = live ? (per_row ? grad[row] : count ? grad[0] / *count : grad[0]) * t.tau : 0.f;
-  const float cp = live ? coef * P : 0.f, l = lse[row];
-  const float scale = exp_scale<DT>(t.inv_tau), shift = DT == NIF_F32 ? l : l * 1.4426950408889634f;
-  const auto dz = [&](float x) { return live ? cp * exp_of<DT>(fmaf(x, scale, -shift)) : 0.f; };
+  const float cp = live ? coef * P / sums[row] : 0.f, top = tops[row], scale = exp_scale<DT>(t.inv_tau);
+  const auto dz = [&](float x) { return live ? cp * exp_of<DT>((x - top) * scale) : 0.f; };
   int c0, c1;  // this block's columns
   if (((uintptr_t)r.z & 15) == ((uintptr_t)o & 15)) {
     const int v0 = min(r.vecs, (int)blockIdx.y * (stretch / V)), v1 = min(r.vecs, v0 + stretch / V);
@@ -421,7 +424,8 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
     }
     ++stretch;
   });
-  const float l = run.template lse<NT>(scale, inv_tau, sh);
+  run.template join_block<NT>(scale, inv_tau, sh);
+  const float l = run.top * inv_tau + logf(run.sum);
   __syncthreads();
   if (threadIdx.x == 0) lse[row] = l;
   // the row's loose ends (fewer than 16), whatever they are
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
 static bool good_type(int dt) { return dt == NIF_F32 || dt == NIF_BF16 || dt == NIF_F16; }
 
 struct DistillState {
-  size_t p, at, P, lse, count, bytes;
+  size_t p, at, P, top, sum, count, bytes;
 };
 static DistillState distill_state(int64_t n, int k) {
   DistillState s;
@@ -477,7 +481,8 @@ static DistillState distill_state(int64_t n, int k) {
   s.p = take((size_t)n * k * 4);
   s.at = take((size_t)n * k * 4);
   s.P = take((size_t)n * 4);
-  s.lse = take((size_t)n * 4);
+  s.top = take((size_t)n * 4);
+  s.sum = take((size_t)n * 4);
   s.count = take(4);
   s.bytes = at;
   return s;
@@ -542,10 +547,10 @@ extern "C" int nif_distill_forward(const void* logits, int64_t ld, int64_t rows,
     // blocks of 512 where rows are few and long (256 x 131072 f32: 27 us to 36; 777 x 50001 f16: 25 to 20, with 1024 threads 36)
     if (rows <= 256 && (int64_t)classes * (dtype == NIF_F32 ? 4 : 2) >= 96 << 10)
       NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 512>), dim3((unsigned)rows), dim3(512), 0, st, logits, ld, classes,
-                                            t, top_indices, top_values, top_lse, (float*)((char*)state + s.lse), row_loss));
+                                            t, top_indices, top_values, top_lse, (float*)((char*)state + s.top), (float*)((char*)state + s.sum), row_loss));
     else
       NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, t,
-                                            top_indices, top_values, top_lse, (float*)((char*)state + s.lse), row_loss));
+                                            top_indices, top_values, top_lse, (float*)((char*)state + s.top), (float*)((char*)state + s.sum), row_loss));
   }
   if (reduction != NIF_REDUCE_NONE)
     launch_reduce(row_loss, t.P, rows, reduction == NIF_REDUCE_MEAN, (float*)((char*)state + s.count), loss, st);
@@ -568,7 +573,7 @@ extern "C" int nif_distill_backward(const void* logits, int64_t ld, int64_t rows
   const dim3 grid((unsigned)rows, (unsigned)((classes + stretch - 1) / stretch));
   clear_err();
   NIF_BY_TYPE(dtype, hipLaunchKernelGGL(distill_grad_kernel<D>, grid, dim3(256), 0, st, logits, ld, classes, t,
-                                        (const float*)((const char*)state + s.lse), grad_loss, reduction == NIF_REDUCE_NONE,
+                                        (const float*)((const char*)state + s.top), (const float*)((const char*)state + s.sum), grad_loss, reduction == NIF_REDUCE_NONE,
                                         reduction == NIF_REDUCE_MEAN ? (const float*)((const char*)state + s.count) : nullptr, dlogits,
                                         ldd, stretch));
   return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;

@@ -963,7 +963,7 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
       const int64_t src = rows[i];
       double s = 0.0;
       for (int k = lane; k < tg.k; k += 64)
-        s += target_term(tg, src, k, u ? u[i * ldu + max(0, tg.at[src * tg.k + k])] : uk[(int64_t)i * tg.k + k], l);
+        s += target_term(tg, src, k, (double)(u ? u[i * ldu + max(0, tg.at[src * tg.k + k])] : uk[(int64_t)i * tg.k + k]) - (double)l, 0.f);
       s = wave_sum_f64(s);
       if (lane == 0) {
         lse[i] = l;
@@ -1293,7 +1293,7 @@ __global__ __launch_bounds__(NT) void head_small_forward_kernel(nif_head_desc h,
   double loss = 0.0;
   for (int k = threadIdx.x; k < t.k; k += NT) {
     const int at = t.at[row * t.k + k];
-    if (at >= 0) loss += target_term(t, row, k, u[at], lse);
+    if (at >= 0) loss += target_term(t, row, k, (double)u[at] - (double)lse, 0.f);
   }
   loss = wave_sum_f64(loss);
   if (lane == 0) sh_loss[wave] = loss;

@@ -79,11 +79,13 @@ __device__ __forceinline__ float wave_sum_f32(float x) {
   return x;
 }
 
-// one target's term of a row's loss / tau^2; an entry of no weight adds nothing, whatever its logit is
-__device__ __forceinline__ double target_term(const Targets& t, int64_t row, int k, float u, float lse) {
+// One target's term of a row's loss / tau^2; an entry of no weight adds nothing, whatever its logit is.  `u` is its logit's
+// distance from the row's largest, over tau, `log_sum` the logarithm of the row's exponentials from there: the log-sum-exp of
+// large logits in 32 bits would be off by half a step of theirs.
+__device__ __forceinline__ double target_term(const Targets& t, int64_t row, int k, double u, float log_sum) {
   const float p = t.p[row * t.k + k];
   if (t.at[row * t.k + k] < 0 || p == 0.f) return 0.0;
-  return (double)p * ((double)logf(p) - (double)u + (double)lse);
+  return (double)p * ((double)logf(p) - u + (double)log_sum);
 }
 
 // p_k = exp(t_k / tau - L), L = lse of the teacher's row where given, else over the row's entries.  Entries of a

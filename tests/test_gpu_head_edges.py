@@ -106,3 +106,26 @@ def test_top_logits_of_rows_that_hold_infinity(ops, dt, v):
     # nothing finite is left of a loss on such a row
     loss = ops.topk_distillation(z.cuda(), torch.zeros(9, 1).cuda(), torch.zeros(9, 1, dtype=torch.int64).cuda(), reduction='none')
     assert not torch.isfinite(loss[:8]).any() and torch.isfinite(loss[8])
+
+
+@pytest.mark.parametrize('tau', [1.0, 0.7])
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, v', [(3, 5), (9, 1001), (200, 30001), (300, 3001)])
+def test_distillation_of_large_logits(ops, dt, tau, n, v):
+    """Logits near a thousand, either sign: what is computed from them depends on their differences alone."""
+    g = torch.Generator().manual_seed(n + v)
+    z = (3 * torch.randn(n, v, generator=g) + torch.where(torch.arange(n) % 2 == 0, 1000.0, -1000.0)[:, None]).to(dt)
+    values, indices = _top(n, min(v, 6), v, g)
+    reach = float((z.double().amax(1) - z.double().amin(1)).max())
+    _check_logits(ops, z, values, indices, tau, reach)
+
+
+@pytest.mark.parametrize('tau', [1.0, 0.5])
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('low', ['lowest', 'a thousand'])
+def test_distillation_of_rows_of_one_value(ops, dt, tau, low):
+    """Every class alike, at the type's lowest value (a row whose mask leaves nothing) too: the softmax is 1 / V."""
+    for n, v in ((2, 3), (3, 1001), (2, 140001)):
+        z = torch.full((n, v), torch.finfo(dt).min if low == 'lowest' else 1000.0, dtype=dt)
+        values, indices = _top(n, 3, v, torch.Generator().manual_seed(v))
+        _check_logits(ops, z, values, indices, tau, 0.0)
