@@ -9,6 +9,9 @@
 // target (ignored label, padding) is left out: the rows that count are packed to the front (`rows`, `count` on the
 // device), and tiles behind them end at once -- such rows cost nothing and nothing in them reaches a result.
 //
+// A row's log-sum-exp stays in two parts, its largest logit and the sum of the exponentials from there: s is
+// exp((z - top) / tau) / sum, with differences of logits only.
+//
 // Forward: one matrix product whose epilogue reduces each tile of u to (maximum, sum of exponentials) per row; the
 // logits never leave registers.  Backward, in pieces of the classes: the product again, its epilogue writing
 // dz = coef * (P s) in 16 bits; the targets' entries are then rewritten with their -p; dW of the piece = dz^T hidden,
@@ -82,7 +85,8 @@ __device__ __forceinline__ short to16(float x) {
   return __builtin_bit_cast(short, (typename T::t)x);  // round to nearest even
 }
 
-// 16-bit types: 2^x by the hardware (2^-22 relative); f32: the library's e^x
+// 16-bit types: 2^x by the hardware (2^-22 relative); f32: the library's e^x.  x: a difference of logits times 1 / tau in that
+// unit -- the difference first, since a type's lowest value times log2(e) or 1 / tau is infinite.
 template <class T>
 __device__ __forceinline__ float head_exp(float x) {
   return T::WIDE ? expf(x) : __builtin_amdgcn_exp2f(x);
@@ -117,8 +121,8 @@ struct GemmArgs {
   float inv_tau;
   float2* stats;        // [m tile * waves in m][stat_ld]
   int64_t stat_ld;
-  const float* lse;
-  const float* cp;      // coef * P of each packed row
+  const float* top;     // the largest logit of each packed row
+  const float* cp;      // coef * P / (the row's sum of exponentials from there)
   void* dz;             // [rows][ldz], 16 bits or f32
   int64_t ldz;
   // EPI_OUT
@@ -253,9 +257,8 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
   const auto m_of = [&](int i) { return mw + (EIGHT ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i); };
   static_assert(DZ_PAD % (16 * FI) == 0);
   if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
-    // in units of the exponential: natural for f32, of two for the 16-bit types
-    const float unit = T::WIDE ? 1.f : 1.4426950408889634f, scale = g.inv_tau * unit;
-    float bias[FI][4];  // times scale; -inf behind the last class
+    const float scale = g.inv_tau * (T::WIDE ? 1.f : 1.4426950408889634f);
+    float bias[FI][4];  // -inf behind the last class
 #pragma unroll
     for (int i = 0; i < FI; ++i)
 #pragma unroll
@@ -266,7 +269,7 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int m = min(m_of(i) + r, g.M - 1);
-          bias[i][r] += scale * (T::WIDE ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m]);
+          bias[i][r] += T::WIDE ? ((const float*)g.bias)[m] : (float)((const typename T::t*)g.bias)[m];
         }
     }
 #pragma unroll
@@ -278,7 +281,7 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
         for (int i = 0; i < FI; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            acc[i][j][r] = fmaf(acc[i][j][r], scale, bias[i][r]);
+            acc[i][j][r] += bias[i][r];
             top = fmaxf(top, acc[i][j][r]);
           }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
@@ -288,13 +291,13 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum += head_exp<T>(acc[i][j][r] - ref);  // a NaN stays in the sum
+          for (int r = 0; r < 4; ++r) sum += head_exp<T>((acc[i][j][r] - ref) * scale);  // a NaN stays in the sum
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        if (lane < 16 && n < N) g.stats[stat_row * g.stat_ld + n] = make_float2(top / unit, sum);
+        if (lane < 16 && n < N) g.stats[stat_row * g.stat_ld + n] = make_float2(top, sum);
       } else if (m0 < g.ldz) {  // all or nothing of a wave's columns, of which DZ_PAD is a multiple
         const bool live = n < N;
-        const float lse = live ? g.lse[n] * unit : 0.f, cp = live ? g.cp[n] : 0.f;
+        const float top = live ? g.top[n] : 0.f, cp = live ? g.cp[n] : 0.f;
         typedef typename std::conditional<T::WIDE, float, short>::type W;
         W* out = (W*)g.dz + (int64_t)n * g.ldz;
         constexpr int GROUP = EIGHT ? 2 : 1;
@@ -306,7 +309,7 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
             const int i = i0 + e / 4, r = e % 4;
             // Rounded to the 16-bit type (half a step, 2^-8 bf16 / 2^-11 f16, of each element; f16 after scaling by a
             // power of two): the size of the rounding that the gradients themselves get.
-            float x = cp * head_exp<T>(fmaf(acc[i][j][r], scale, bias[i][r]) - lse);
+            float x = cp * head_exp<T>((acc[i][j][r] + bias[i][r] - top) * scale);
             x = live ? x : 0.f;
             if constexpr (T::WIDE)
               w[e] = x;
@@ -862,13 +865,13 @@ __global__ __launch_bounds__(256) void head_pack_kernel(const W* __restrict__ sr
   pack_row<W>(src + i * lds, true, d, dst + i * ldd, ldd);
 }
 
-// The targets' logits u = (hidden . weight[at] + bias) / tau as dot products of the inputs, in 32 bits: a wave for eight
+// The targets' logits z = hidden . weight[at] + bias as dot products of the inputs, in 32 bits: a wave for eight
 // targets of a row, two for each 16 lanes (one or two targets: the whole wave), their weight rows in flight together.  Bound
 // by the gathered rows' bytes (3686 rows of 64 targets, 2048 features, bf16, 0.93 GB: 150 us, 6.2 TB/s, caches included).
 constexpr int DOTS = 8;
 template <int DT>
 __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const void* weight, int64_t ldw, const void* bias, int d,
-                                            const Targets& tg, int64_t src, int k0, float* uk, int lane) {
+                                            const Targets& tg, int64_t src, int k0, float* zk, int lane) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16;
   const int lanes = tg.k > 2 ? 16 : 64, l = lane & (lanes - 1), k = k0 + lane / lanes * 2;
@@ -899,32 +902,32 @@ __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const
 #pragma unroll
     for (int o = 32; o; o >>= 1)
       if (o < lanes) s[q] += __shfl_xor(s[q], o, 64);
-    if (l == 0 && k + q < tg.k) uk[k + q] = at[q] < 0 ? 0.f : (s[q] + (bias ? Elem<DT>::load(bias, at[q]) : 0.f)) * tg.inv_tau;
+    if (l == 0 && k + q < tg.k) zk[k + q] = at[q] < 0 ? 0.f : s[q] + (bias ? Elem<DT>::load(bias, at[q]) : 0.f);
   }
 }
 
-// Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits (uk; not
+// Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits (zk; not
 // where the logits are kept).
 template <int DT>
 __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int d,
                                                              const int* __restrict__ rows, const int* __restrict__ count,
                                                              void* __restrict__ dst, int ldd, const void* __restrict__ weight,
                                                              int64_t ldw, const void* __restrict__ bias, Targets tg,
-                                                             float* __restrict__ uk) {
+                                                             float* __restrict__ zk) {
   typedef typename std::conditional<DT == NIF_F32, float, short>::type W;
   const int64_t i = blockIdx.x;
   const bool have = i < *count;
   const int64_t src = have ? rows[i] : 0;
   const typename Elem<DT>::t* h = (const typename Elem<DT>::t*)hidden + src * ldh;
   pack_row<W>((const W*)h, have, d, (W*)dst + i * ldd, ldd);
-  if (!have || !uk) return;
+  if (!have || !zk) return;
   for (int k0 = (threadIdx.x >> 6) * DOTS; k0 < tg.k; k0 += 4 * DOTS)
-    target_dots<DT>(h, weight, ldw, bias, d, tg, src, k0, uk + i * tg.k, threadIdx.x & 63);
+    target_dots<DT>(h, weight, ldw, bias, d, tg, src, k0, zk + i * tg.k, threadIdx.x & 63);
 }
 
 // ---- the loss of each row -------------------------------------------------------------------------------
 // ROWS packed rows a block (16, a line of the statistics; two where there are at most FINISH_FEW rows, for more blocks: 41 rows
-// of 2180 tiles 17 us to 8): joins the tiles' (maximum, sum) pairs into lse, and writes each row's loss to its own place.  The
+// of 2180 tiles 17 us to 8): joins the tiles' (maximum, sum) pairs, and writes each row's loss to its own place.  The
 // block that is done last (`done`, cleared by head_rows_kernel) reduces the losses: sum or mean over the rows that count,
 // in a fixed order and 64 bits.
 constexpr int FINISH_NT = 1024;
@@ -932,8 +935,8 @@ constexpr int64_t FINISH_FEW = 512;
 template <int ROWS>
 __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
                                                                 const int* __restrict__ rows, const int* __restrict__ count,
-                                                                float* __restrict__ lse, const float* __restrict__ uk,
-                                                                const float* __restrict__ u, int64_t ldu, float* loss,
+                                                                float* __restrict__ tops, float* __restrict__ sums,
+                                                                const float* __restrict__ zk, const float* __restrict__ z, int64_t ldz, float* loss,
                                                                 int64_t all_rows, int reduction, int* done, float* __restrict__ reduced) {
   constexpr int PARTS = FINISH_NT / ROWS;
   __shared__ float sh_top[ROWS][PARTS + 1], sh_sum[ROWS][PARTS + 1];
@@ -947,7 +950,7 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
 #pragma unroll 4
       for (int t = part; t < tiles; t += PARTS) {
         const float2 x = stats[(int64_t)t * stat_ld + i0 + r];
-        join(top, sum, x.x, x.y);
+        join(top, sum, x.x, x.y, tg.inv_tau);
       }
     sh_top[r][part] = top;
     sh_sum[r][part] = sum;
@@ -956,17 +959,20 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
     if (wave < ROWS && i < n) {
       top = sh_top[wave][lane], sum = sh_sum[wave][lane];
 #pragma unroll
-      for (int p = 64 + lane; p < PARTS; p += 64) join(top, sum, sh_top[wave][p], sh_sum[wave][p]);
-      const float all = wave_max_f32(top), ref = all == -INFINITY ? 0.f : all;
-      sum = wave_sum_f32(sum * expf(top - ref));
-      const float l = all + logf(sum);
+      for (int p = 64 + lane; p < PARTS; p += 64) join(top, sum, sh_top[wave][p], sh_sum[wave][p], tg.inv_tau);
+      const float all = wave_max_f32(top);
+      sum = wave_sum_f32(sum * expf((top - reference_of(all)) * tg.inv_tau));
+      const float log_sum = logf(sum);
       const int64_t src = rows[i];
       double s = 0.0;
       for (int k = lane; k < tg.k; k += 64)
-        s += target_term(tg, src, k, (double)(u ? u[i * ldu + max(0, tg.at[src * tg.k + k])] : uk[(int64_t)i * tg.k + k]) - (double)l, 0.f);
+        s += target_term(tg, src, k,
+                         ((double)(z ? z[i * ldz + max(0, tg.at[src * tg.k + k])] : zk[(int64_t)i * tg.k + k]) - (double)all) * (double)tg.inv_tau,
+                         log_sum);
       s = wave_sum_f64(s);
       if (lane == 0) {
-        lse[i] = l;
+        tops[i] = all;
+        sums[i] = sum;
         loss[src] = (float)(s * tg.tau2);
       }
     }
@@ -993,14 +999,15 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
   }
 }
 
-// First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i], and what the products of dz are multiplied with.  Where
+// First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i] / (the row's sum of exponentials), and what the products of dz are multiplied with.  Where
 // one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
 // near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
 // the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  The other blocks: gradient 0 for rows without a target.
 template <typename W>
 __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict__ grad, int per_row, int mean, Targets tg,
                                                          const int* __restrict__ rows, const int* __restrict__ inv,
-                                                         const int* __restrict__ count, int64_t rows_all, int f16, float* __restrict__ coef,
+                                                         const int* __restrict__ count, const float* __restrict__ sums, int64_t rows_all,
+                                                         int f16, float* __restrict__ coef,
                                                          float* __restrict__ cp, float* __restrict__ inv_scale, W* __restrict__ out,
                                                          int64_t ld, int d) {
   if (blockIdx.x > 0) {
@@ -1033,14 +1040,14 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
   for (int i = threadIdx.x; i < n; i += 1024) {
     const float c = (per_row ? grad[rows[i]] * w : 1.f) * scale;
     coef[i] = c;
-    cp[i] = c * tg.P[rows[i]];
+    cp[i] = c * tg.P[rows[i]] / sums[i];
   }
 }
 
 // The targets' entries of a piece of dz: coef (P s - sum of the row's p with that class).  The first of equal classes
 // writes, with the sum over all of them in order.  One wave per packed row.
 template <class W, class U>
-__device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U&& u_of, float lse, float coef, float cp, int v0,
+__device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U&& z_of, float top, float coef, float cp, int v0,
                                                int v1, W* dz, int lane) {
   const int* at = tg.at + src * tg.k;
   const float* p = tg.p + src * tg.k;
@@ -1060,17 +1067,17 @@ __device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U
         sum += same ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pq), q)) : 0.f;
       }
     }
-    if (mine && first) dz[v - v0] = (W)(cp * expf(u_of(k, v) - lse) - coef * sum);
+    if (mine && first) dz[v - v0] = (W)(cp * expf((z_of(k, v) - top) * tg.inv_tau) - coef * sum);
   }
 }
 template <class T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
-                                                           const float* __restrict__ uk, const float* __restrict__ lse,
+                                                           const float* __restrict__ zk, const float* __restrict__ tops,
                                                            const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
                                                            typename T::t* __restrict__ dz, int64_t ldz) {
   const int64_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= *count) return;
-  target_entries(tg, rows[i], [&](int k, int) { return uk[i * tg.k + k]; }, lse[i], coef[i], cp[i], v0, v1, dz + i * ldz,
+  target_entries(tg, rows[i], [&](int k, int) { return zk[i * tg.k + k]; }, tops[i], coef[i], cp[i], v0, v1, dz + i * ldz,
                  threadIdx.x & 63);
 }
 
@@ -1144,11 +1151,11 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
 }
 
 // ---- kept logits ------------------------------------------------------------------------------------------------
-// u = (the splits' partial sums, in order, + bias) / tau, kept in 32 bits, and its (maximum, sum of exponentials) over
+// z = the splits' partial sums, in order, + bias, kept in 32 bits, and its (maximum, sum of exponentials) over
 // stretches of KEPT classes: a block a stretch of one packed row.
 constexpr int KEPT = 1024;
 template <class T>
-__global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict__ part, int splits, int64_t part_split, float* __restrict__ u,
+__global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict__ part, int splits, int64_t part_split, float* __restrict__ kept,
                                                         int64_t ldu, int v, const int* __restrict__ count, const void* __restrict__ bias,
                                                         float inv_tau, float2* __restrict__ stats, int64_t stat_ld) {
   __shared__ float sh_top[4], sh_sum[4];
@@ -1157,7 +1164,7 @@ __global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict_
   const int c = blockIdx.y * KEPT + threadIdx.x * 4;
   f32x4 x = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   if (c < v) {  // rows are padded to a multiple of 4
-    f32x4* at = (f32x4*)(u + i * ldu + c);
+    f32x4* at = (f32x4*)(kept + i * ldu + c);
     f32x4 z;
     if (splits > 1) {
       z = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1168,53 +1175,57 @@ __global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict_
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (c + e < v) x[e] = (z[e] + (bias ? (float)((const typename T::t*)bias)[c + e] : 0.f)) * inv_tau;
+      if (c + e < v) x[e] = z[e] + (bias ? (float)((const typename T::t*)bias)[c + e] : 0.f);
     *at = x;
   }
   float top = wave_max_f32(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
   const float ref = top == -INFINITY ? 0.f : top;
-  const float sum = wave_sum_f32(expf(x[0] - ref) + expf(x[1] - ref) + expf(x[2] - ref) + expf(x[3] - ref));  // a NaN stays in the sum
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += expf((x[e] - ref) * inv_tau);  // a NaN stays in the sum
+  sum = wave_sum_f32(sum);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (lane == 0) sh_top[wave] = top, sh_sum[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     float s = sum;
-    for (int w = 1; w < 4; ++w) join(top, s, sh_top[w], sh_sum[w]);
+    for (int w = 1; w < 4; ++w) join(top, s, sh_top[w], sh_sum[w], inv_tau);
     stats[blockIdx.y * stat_ld + i] = make_float2(top, s);
   }
 }
 
-// dz = cp exp(u - lse) of a piece of the classes, 8 a thread, and the targets' entries; zeros up to a multiple of K_PAD rows
+// dz = cp exp((z - top) / tau) of a piece of the classes, 8 a thread, and the targets' entries; zeros up to a multiple of K_PAD rows
 // and in the padding of the columns, where the products read them.  Rounded as head_gemm_kernel's.
 constexpr int KEPT_DZ = 2048;
 template <class T>
-__global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ u, int64_t ldu, int v0, int cols, Targets tg,
+__global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ z, int64_t ldu, int v0, int cols, Targets tg,
                                                            const int* __restrict__ rows, const int* __restrict__ count,
-                                                           const float* __restrict__ lse, const float* __restrict__ coef,
+                                                           const float* __restrict__ tops, const float* __restrict__ coef,
                                                            const float* __restrict__ cp, typename T::t* dz, int64_t ldz) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   const int n = *count, c0 = blockIdx.y * KEPT_DZ, c = c0 + threadIdx.x * 8;
   const int64_t i = blockIdx.x;
   if (i >= (n + K_PAD - 1) / K_PAD * K_PAD) return;
   const bool live = i < n;
-  const float l = live ? lse[i] : 0.f, k = live ? cp[i] : 0.f;
+  const float top = live ? tops[i] : 0.f, k = live ? cp[i] : 0.f;
+  const auto one = [&](float x) { return (typename T::t)(k * expf((x - top) * tg.inv_tau)); };
   if (c < ldz) {
     Eight w;
-    const float* x = u + i * ldu + v0 + c;
+    const float* x = z + i * ldu + v0 + c;
     if (live && c + 8 <= cols) {
       const f32x4 lo = *(const f32x4*)x, hi = *(const f32x4*)(x + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(k * expf((e < 4 ? lo[e & 3] : hi[e & 3]) - l));
+      for (int e = 0; e < 8; ++e) w[e] = one(e < 4 ? lo[e & 3] : hi[e & 3]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = (typename T::t)(live && c + e < cols ? k * expf(x[e] - l) : 0.f);
+      for (int e = 0; e < 8; ++e) w[e] = live && c + e < cols ? one(x[e]) : (typename T::t)0.f;
     }
     *(Eight*)(dz + i * ldz + c) = w;
   }
   if (!live) return;
   __syncthreads();  // the entries are stored again behind the others
   if (threadIdx.x < 64)
-    target_entries(tg, rows[i], [&](int, int v) { return u[i * ldu + v]; }, l, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ),
+    target_entries(tg, rows[i], [&](int, int v) { return z[i * ldu + v]; }, top, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ),
                    dz + i * ldz + c0, threadIdx.x);
 }
 
@@ -1275,7 +1286,7 @@ __global__ __launch_bounds__(NT) void head_small_forward_kernel(nif_head_desc h,
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       s[q] = wave_sum_f32(s[q]);
-      if (lane == 0 && v0 + q < classes) u[v0 + q] = (s[q] + (h.bias ? Elem<DT>::load(h.bias, v0 + q) : 0.f)) * t.inv_tau;
+      if (lane == 0 && v0 + q < classes) u[v0 + q] = s[q] + (h.bias ? Elem<DT>::load(h.bias, v0 + q) : 0.f);
     }
   }
   __syncthreads();
@@ -1283,17 +1294,17 @@ __global__ __launch_bounds__(NT) void head_small_forward_kernel(nif_head_desc h,
   for (int v = threadIdx.x; v < classes; v += NT) top = fmaxf(top, u[v]);
   top = wave_max_f32(top);
   const float ref = top == -INFINITY ? 0.f : top;
-  for (int v = threadIdx.x; v < classes; v += NT) sum += expf(u[v] - ref);
+  for (int v = threadIdx.x; v < classes; v += NT) sum += expf((u[v] - ref) * t.inv_tau);
   sum = wave_sum_f32(sum);
   if (lane == 0) sh[2 * wave] = top, sh[2 * wave + 1] = sum;
   __syncthreads();
   top = sh[0], sum = sh[1];
-  for (int q = 1; q < NT / 64; ++q) join(top, sum, sh[2 * q], sh[2 * q + 1]);
-  const float lse = top + logf(sum);
+  for (int q = 1; q < NT / 64; ++q) join(top, sum, sh[2 * q], sh[2 * q + 1], t.inv_tau);
+  const float log_sum = logf(sum);
   double loss = 0.0;
   for (int k = threadIdx.x; k < t.k; k += NT) {
     const int at = t.at[row * t.k + k];
-    if (at >= 0) loss += target_term(t, row, k, (double)u[at] - (double)lse, 0.f);
+    if (at >= 0) loss += target_term(t, row, k, ((double)u[at] - (double)top) * (double)t.inv_tau, log_sum);
   }
   loss = wave_sum_f64(loss);
   if (lane == 0) sh_loss[wave] = loss;
@@ -1303,7 +1314,8 @@ __global__ __launch_bounds__(NT) void head_small_forward_kernel(nif_head_desc h,
     for (int q = 0; q < NT / 64; ++q) loss += sh_loss[q];
     row_loss[row] = (float)(loss * t.tau2);
   }
-  for (int v = threadIdx.x; v < classes; v += NT) u[v] = t.tau * P * expf(u[v] - lse);
+  const float cp = t.tau * P / sum;
+  for (int v = threadIdx.x; v < classes; v += NT) u[v] = cp * expf((u[v] - top) * t.inv_tau);
   __syncthreads();
   for (int k = threadIdx.x; k < t.k; k += NT) {
     const int v = t.at[row * t.k + k];
@@ -1406,7 +1418,7 @@ struct Plan {
   bool keep;         // few rows: the logits are kept
   int piece;         // classes per piece (multiple of 256, or all)
   // state: what the backward pass reads
-  size_t s_p, s_at, s_P, s_dz, s_rows, s_inv, s_count, s_lse, s_uk, s_h, s_u, state;
+  size_t s_p, s_at, s_P, s_dz, s_rows, s_inv, s_count, s_top, s_sum, s_zk, s_h, s_z, state;
   int64_t ldu;       // of the kept logits
 };
 
@@ -1527,12 +1539,13 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   }
   p.s_rows = take(at, (size_t)p.cap * 4);
   p.s_inv = take(at, (size_t)p.cap * 4);
-  p.s_lse = take(at, (size_t)p.cap * 4);
+  p.s_top = take(at, (size_t)p.cap * 4);
+  p.s_sum = take(at, (size_t)p.cap * 4);
   p.s_h = take(at, (size_t)p.cap * p.ldd * p.e);
   p.ldu = round_up(p.v, 4);
   p.keep = kept_logits_are_faster(p, h->forward_only != 0);
-  p.s_u = take(at, p.keep ? (size_t)p.n * p.ldu * 4 : 0);
-  p.s_uk = take(at, p.keep ? 0 : (size_t)p.cap * p.k * 4);
+  p.s_z = take(at, p.keep ? (size_t)p.n * p.ldu * 4 : 0);
+  p.s_zk = take(at, p.keep ? 0 : (size_t)p.cap * p.k * 4);
   p.state = at;
   return true;
 }
@@ -1631,7 +1644,7 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
       const Shape ks = kept_shape(p, p.pack_f ? p.piece : p.v);
       g.splits = ks.splits;
       g.out_kind = OUT_F32;
-      g.acc = (float*)(ks.splits > 1 ? ws + f.part : state + p.s_u) + v0;
+      g.acc = (float*)(ks.splits > 1 ? ws + f.part : state + p.s_z) + v0;
       g.acc_ld = p.ldu;
       g.acc_split = p.n * p.ldu;
       run_gemm<T, false, false, EPI_OUT>(ks, g, st);
@@ -1647,7 +1660,7 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
     const int splits = kept_shape(p, p.pack_f ? p.piece : p.v).splits;
     tiles = (p.v + KEPT - 1) / KEPT;
     hipLaunchKernelGGL(head_kept_kernel<T>, dim3((unsigned)p.n, tiles), dim3(256), 0, st, (const float*)(ws + f.part), splits,
-                       p.n * p.ldu, (float*)(state + p.s_u), p.ldu, p.v, (const int*)(state + p.s_count), h->bias,
+                       p.n * p.ldu, (float*)(state + p.s_z), p.ldu, p.v, (const int*)(state + p.s_count), h->bias,
                        h->labels ? 1.f : 1.f / h->temperature, (float2*)(ws + f.stats), p.cap);
   }
 }
@@ -1655,7 +1668,7 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
 template <int DT>
 static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStream_t st) {
   hipLaunchKernelGGL(head_pack_rows_kernel<DT>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d,
-                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), p.keep ? nullptr : (float*)(state + p.s_uk));
+                     (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), p.keep ? nullptr : (float*)(state + p.s_zk));
 }
 
 struct BwdSpace {
@@ -1695,8 +1708,8 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
   const int* rows = (const int*)(state + p.s_rows);
   const void* hp = state + p.s_h;
   const Targets tg = targets_of(h, p, (char*)state);
-  const float* lse = (const float*)(state + p.s_lse);
-  const float* uk = (const float*)(state + p.s_uk);
+  const float* tops = (const float*)(state + p.s_top);
+  const float* zk = (const float*)(state + p.s_zk);
   const float* coef = (const float*)(ws + b.coef);
   const float* cp = (const float*)(ws + b.cp);
   const float* inv_scale = (const float*)(ws + b.scale);
@@ -1712,7 +1725,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     const int kz = p.any_b ? vc : (int)round_up(vc, K_PAD);  // the contraction over the piece's columns of dz
     if (p.keep) {
       hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + KEPT_DZ - 1) / KEPT_DZ)), dim3(256),
-                         0, st, (const float*)(state + p.s_u), p.ldu, v0, vc, tg, rows, count, lse, coef, cp, dz, b.ldz);
+                         0, st, (const float*)(state + p.s_z), p.ldu, v0, vc, tg, rows, count, tops, coef, cp, dz, b.ldz);
     } else {
       GemmArgs g = {};
       g.A = w;
@@ -1724,14 +1737,14 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.splits = 1;
       g.bias = bias_at(h, v0);
       g.inv_tau = tg.inv_tau;
-      g.lse = lse;
+      g.top = tops;
       g.cp = cp;
       g.dz = dz;
       g.ldz = b.ldz;
       run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc, p.any_b), g, st);
     }
     if (p.n > 0 && !p.keep)
-      hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, uk, lse, coef, cp, v0,
+      hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, zk, tops, coef, cp, v0,
                        v0 + vc, dz, b.ldz);
     if (dbias) {
       W* out = (W*)dbias + v0;
@@ -1888,7 +1901,7 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
     const float2* stats = (const float2*)((char*)ws + f.stats);
     const auto finish = [&](auto each) {
       hipLaunchKernelGGL(head_finish_kernel<each>, dim3((unsigned)((p.n + each - 1) / each)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg,
-                         rows, count, (float*)(s + p.s_lse), (const float*)(s + p.s_uk), p.keep ? (const float*)(s + p.s_u) : nullptr,
+                         rows, count, (float*)(s + p.s_top), (float*)(s + p.s_sum), (const float*)(s + p.s_zk), p.keep ? (const float*)(s + p.s_z) : nullptr,
                          p.ldu, row_loss, p.n, h->reduction, count + 1, loss);
     };
     if (p.n <= FINISH_FEW)
@@ -1946,7 +1959,7 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
     const unsigned clearing = out && p.n > 0 ? (unsigned)((p.n + 3) / 4) : 0;
     hipLaunchKernelGGL(head_coef_kernel, dim3(1 + clearing), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
                        h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_inv),
-                       (const int*)(s + p.s_count), p.n, h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp),
+                       (const int*)(s + p.s_count), (const float*)(s + p.s_sum), p.n, h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp),
                        (float*)((char*)ws + b.scale), out, lddh, p.d);
   };
   if (h->dtype == NIF_F32)

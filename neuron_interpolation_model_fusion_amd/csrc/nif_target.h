@@ -62,7 +62,7 @@ __device__ __forceinline__ float reference_of(float top) { return fabsf(top) == 
 
 // (max, sum of exp((. - reference) / tau)) pairs: the empty one is (-inf, 0), one that holds +inf (+inf, +inf); NaN stays in
 // the sum
-__device__ __forceinline__ void join(float& top, float& sum, float t2, float s2, float inv_tau = 1.f) {
+__device__ __forceinline__ void join(float& top, float& sum, float t2, float s2, float inv_tau) {
   const float m = fmaxf(top, t2), ref = reference_of(m);
   sum = sum * expf((top - ref) * inv_tau) + s2 * expf((t2 - ref) * inv_tau);
   top = m;

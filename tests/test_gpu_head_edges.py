@@ -129,3 +129,57 @@ def test_distillation_of_rows_of_one_value(ops, dt, tau, low):
         z = torch.full((n, v), torch.finfo(dt).min if low == 'lowest' else 1000.0, dtype=dt)
         values, indices = _top(n, 3, v, torch.Generator().manual_seed(v))
         _check_logits(ops, z, values, indices, tau, 0.0)
+
+
+HEADS = [(5, 64, 40), (300, 64, 600), (600, 64, 700), (5, 64, 20011), (40, 72, 9001), (40, 67, 9001), (1100, 72, 3001), (600, 67, 3001)]
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('k, tau', [(None, 1.0), (5, 2.0)])
+@pytest.mark.parametrize('n, d, v', HEADS)
+def test_heads_of_large_logits(ops, dt, k, tau, n, d, v):
+    """Logits near a thousand that are exact in 32 bits -- sums of -1, 0 and 1 and a bias of 1024 -- in the small form, with
+    and without kept logits, with odd rows: the row's sum, not its rounded log-sum-exp, is what the softmax is divided by."""
+    g = torch.Generator().manual_seed(n + v)
+    h, w = (torch.randint(-1, 2, (rows, d), generator=g).to(dt) for rows in (n, v))
+    b = torch.full((v,), 1024.0).to(dt)
+    if k is None:
+        y = torch.randint(0, v, (n,), generator=g)
+        p, at, live = _targets(labels=y)
+    else:
+        values, indices = _top(n, k, v, g)
+        p, at, live = _targets(values=values, indices=indices, tau=tau)
+    hg, wg, bg = (t.cuda().requires_grad_() for t in (h, w, b))
+    if k is None:
+        loss = ops.linear_cross_entropy(hg, wg, y.cuda(), bg, reduction='none')
+    else:
+        loss = ops.linear_topk_distillation(hg, wg, values.cuda(), indices.cuda(), bg, temperature=tau, reduction='none')
+    got = torch.autograd.grad(loss.sum(), (hg, wg, bg))
+    h, w = h.double(), w.double()
+    z = h @ w.t() + 1024.0
+    want, rows, dz, q, coef = _formula(z, p, at, live, tau, 'none', torch.ones(n))
+    du = 4 * U * float((z.amax(1) - z.amin(1)).max()) / tau
+    tol = tau * tau * p.sum(1) * (2 * du + 2.0 ** -18) + 2 * U * rows.abs()
+    off = (loss.detach().cpu().double() - want).abs()
+    assert torch.all(off <= tol), float((off / tol).max())
+    cq, rel = coef * q, (U16[dt] if dt != torch.float32 else 2 * U) + 2 * du + 2.0 ** -18
+    for x, ref, size, length in ((got[0], dz @ w, cq @ w.abs(), v), (got[1], dz.t() @ h, cq.t() @ h.abs(), n), (got[2], dz.sum(0), cq.sum(0), n)):
+        bound = U16[dt] * ref.abs() + (rel + (length + 64) * U) * size + (2.0 ** -24 if dt == torch.float16 else 1e-37)
+        off = (x.cpu().double() - ref).abs()
+        assert torch.all(off <= bound), float((off / bound).max())
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, d, v', HEADS)
+def test_heads_whose_classes_are_all_masked_by_the_lowest_value(ops, dt, n, d, v):
+    """z = low for every class: the softmax is 1 / V, the loss log V."""
+    h, w = torch.ones(n, d, dtype=dt), torch.zeros(v, d, dtype=dt)
+    b = torch.full((v,), torch.finfo(dt).min, dtype=dt)
+    y = torch.arange(n) * 7 % v
+    hg, wg, bg = (t.cuda().requires_grad_() for t in (h, w, b))
+    loss = ops.linear_cross_entropy(hg, wg, y.cuda(), bg, reduction='none')
+    db, = torch.autograd.grad(loss.sum(), bg)
+    assert torch.all((loss.detach().cpu().double() - math.log(v)).abs() <= 2.0 ** -18 + 2 * U * math.log(v))
+    want = n / v - torch.bincount(y, minlength=v).double()
+    q = n / v + torch.bincount(y, minlength=v).double()
+    assert torch.all((db.cpu().double() - want).abs() <= U16[dt] * want.abs() + (U16[dt] + 2.0 ** -18 + (n + 64) * U) * q)
