@@ -527,7 +527,8 @@ size_t nif_head_state_bytes(const nif_head_desc* h);
 size_t nif_head_forward_workspace_bytes(const nif_head_desc* h);
 size_t nif_head_backward_workspace_bytes(const nif_head_desc* h);
 int nif_head_forward(const nif_head_desc* h, float* loss, void* state, size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
-/* grad_loss: one f32 (MEAN, SUM) or rows of them (NONE), on the device */
+/* grad_loss: one f32 (MEAN, SUM) or rows of them (NONE), on the device; may be NULL for no rows.  Where no row counts it is
+ * not read, and the gradients are zeros. */
 int nif_head_backward(const nif_head_desc* h, const float* grad_loss, const void* state, size_t state_bytes, void* dhidden,
                       int64_t lddh, void* dweight, int64_t lddw, void* dbias, void* ws, size_t ws_bytes, void* stream);
 

@@ -1002,7 +1002,8 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
 // First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i] / (the row's sum of exponentials), and what the products of dz are multiplied with.  Where
 // one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
 // near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
-// the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  The other blocks: gradient 0 for rows without a target.
+// the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  Where no row counts the arriving gradient is not read
+// (there may be none, and zeros stay zeros whatever it holds).  The other blocks: gradient 0 for rows without a target.
 template <typename W>
 __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict__ grad, int per_row, int mean, Targets tg,
                                                          const int* __restrict__ rows, const int* __restrict__ inv,
@@ -1018,7 +1019,7 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
   }
   __shared__ float sh[16];
   const int n = *count;
-  const float w = tg.tau * (mean ? 1.f / max(1, n) : 1.f), all = per_row ? 1.f : grad[0] * w;
+  const float w = tg.tau * (mean ? 1.f / max(1, n) : 1.f), all = per_row || n == 0 ? 1.f : grad[0] * w;
   float scale = 1.f;
   if (f16) {
     float top = 0.f;

@@ -183,3 +183,38 @@ def test_heads_whose_classes_are_all_masked_by_the_lowest_value(ops, dt, n, d, v
     want = n / v - torch.bincount(y, minlength=v).double()
     q = n / v + torch.bincount(y, minlength=v).double()
     assert torch.all((db.cpu().double() - want).abs() <= U16[dt] * want.abs() + (U16[dt] + 2.0 ** -18 + (n + 64) * U) * q)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n', [0, 5, 700])
+@pytest.mark.parametrize('d, v', [(24, 40), (264, 9001)])
+def test_no_row_that_counts_has_no_gradient_whatever_arrives(ops, dt, n, d, v):
+    h, w, b = (torch.ones(*s, dtype=dt, device='cuda').requires_grad_() for s in ((n, d), (v, d), (v,)))
+    y = torch.full((n,), -100, device='cuda')
+    for reduction in ('mean', 'sum', 'none'):
+        for up in (math.nan, math.inf):
+            loss = ops.linear_cross_entropy(h, w, y, b, reduction=reduction)
+            for x in torch.autograd.grad(loss, (h, w, b), grad_outputs=torch.full_like(loss, up)):
+                assert torch.all(x == 0)
+
+
+@pytest.mark.parametrize('reduction', [0, 1, 2])
+@pytest.mark.parametrize('d, v', [(24, 40), (264, 9001)])
+def test_no_rows_need_no_arriving_gradient(d, v, reduction):
+    """Through the C ABI: zero rows, no gradient given, zeros in dweight and dbias."""
+    import ctypes
+
+    from neuron_interpolation_model_fusion_amd import _lib
+    lib, st = _lib.lib, torch.cuda.current_stream().cuda_stream
+    w, dw, db = torch.ones(v, d, device='cuda'), torch.full((v, d), 7.0, device='cuda'), torch.full((v,), 7.0, device='cuda')
+    desc = _lib.HeadDesc(ldh=d, weight=w.data_ptr(), ldw=d, rows=0, features=d, classes=v, dtype=_lib.NIF_F32, reduction=reduction,
+                         ignore_index=-100, temperature=1.0)
+    at = ctypes.byref(desc)
+    state, ws, ws_b = (torch.empty(f(at), dtype=torch.uint8, device='cuda') for f in (
+        lib.nif_head_state_bytes, lib.nif_head_forward_workspace_bytes, lib.nif_head_backward_workspace_bytes))
+    loss = torch.full((1,), 7.0, device='cuda')
+    assert lib.nif_head_forward(at, loss.data_ptr(), state.data_ptr(), state.numel(), ws.data_ptr(), ws.numel(), st) == 0
+    assert lib.nif_head_backward(at, None, state.data_ptr(), state.numel(), None, d, dw.data_ptr(), d, db.data_ptr(), ws_b.data_ptr(),
+                                 ws_b.numel(), st) == 0
+    torch.cuda.synchronize()
+    assert torch.all(dw == 0) and torch.all(db == 0) and (reduction == 0 or float(loss) == 0)
