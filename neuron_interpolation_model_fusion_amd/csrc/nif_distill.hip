@@ -21,12 +21,12 @@ namespace nif {
 
 __global__ __launch_bounds__(256) void top_targets_kernel(const int32_t* __restrict__ indices, const float* __restrict__ values,
                                                           const float* __restrict__ lse, int64_t n, int classes, Targets t) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = row_block() * 4 + (threadIdx.x >> 6);
   if (row < n) top_targets(indices, values, lse, row, classes, t, threadIdx.x & 63);
 }
 
 void launch_targets(const int32_t* indices, const float* values, const float* lse, int64_t n, int classes, const Targets& t, hipStream_t st) {
-  hipLaunchKernelGGL(top_targets_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, indices, values, lse, n, classes, t);
+  hipLaunchKernelGGL(top_targets_kernel, row_grid((n + 3) / 4), dim3(256), 0, st, indices, values, lse, n, classes, t);
 }
 
 // ---- distillation of given logits ---------------------------------------------------------------------------
@@ -129,13 +129,14 @@ __device__ __forceinline__ void stream_row(const RowView<DT>& r, F&& f) {
 // One block per row: the targets' probabilities, (max, sum of exponentials) in one pass over the logits, the targets'
 // terms and the row's loss.  Bound by the read of the logits: 4096 x 131072 bf16 in 206 us, 5.2 TB/s.
 template <int DT, int NT>
-__global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
+__global__ __launch_bounds__(NT) void distill_rows_kernel(const void* __restrict__ logits, int64_t ld, int64_t n, int classes, Targets t,
                                                           const int32_t* __restrict__ indices, const float* __restrict__ values,
                                                           const float* __restrict__ top_lse, float* __restrict__ top_out,
                                                           float* __restrict__ sum_out, float* __restrict__ loss) {
   __shared__ float sh[2 * NT / 64], sh_P;
   __shared__ double sh_loss[NT / 64];
-  const int64_t row = blockIdx.x;
+  const int64_t row = row_block();
+  if (row >= n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (wave == 0) {
     const float P = top_targets(indices, values, top_lse, row, classes, t, lane);
@@ -207,14 +208,15 @@ void launch_reduce(const float* row_loss, const float* P, int64_t n, bool mean, 
 // loads and stores, also where the row starts off a 16-byte border (the output's rows then start alike, or go by element);
 // 4096 x 131072 bf16 in 418 us, 5.1 TB/s of both; 777 x 50001 f16 in 29 us.
 template <int DT>
-__global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restrict__ logits, int64_t ld, int classes, Targets t,
+__global__ __launch_bounds__(256) void distill_grad_kernel(const void* __restrict__ logits, int64_t ld, int64_t n, int classes, Targets t,
                                                            const float* __restrict__ tops, const float* __restrict__ sums,
                                                            const float* __restrict__ grad, int per_row,
                                                            const float* __restrict__ count, void* __restrict__ out, int64_t ldo,
                                                            int stretch) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16, U = 4;
-  const int64_t row = (int64_t)gridDim.x - 1 - blockIdx.x;
+  const int64_t row = n - 1 - row_block();
+  if (row < 0) return;
   const RowView<DT> r(logits, row * ld, classes);
   E* o = (E*)out + row * ldo;
   const float P = t.P[row];
@@ -382,7 +384,7 @@ __device__ __forceinline__ void select_by_digits(const typename Elem<DT>::t* z, 
 // log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 258 us,
 // 4.1 TB/s; 400 x 1000 f32 in 13 us, a launch's latency.
 template <int DT, int NT>
-__global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int classes, int k, float inv_tau,
+__global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int64_t rows, int classes, int k, float inv_tau,
                                                         void* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse) {
   typedef typename Elem<DT>::t E;
   constexpr int V = Elem<DT>::PER16, U = DT == NIF_F32 ? 4 : 2;
@@ -390,7 +392,8 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
   __shared__ unsigned long long key[LIST];
   __shared__ float sh[NT];
   __shared__ int sh_n;
-  const int64_t row = blockIdx.x;
+  const int64_t row = row_block();
+  if (row >= rows) return;
   const RowView<DT> r(logits, row * ld, classes);
   const float scale = exp_scale<DT>(inv_tau);
   if (threadIdx.x == 0) sh_n = 0;
@@ -546,10 +549,10 @@ extern "C" int nif_distill_forward(const void* logits, int64_t ld, int64_t rows,
   if (rows > 0) {
     // blocks of 512 where rows are few and long (256 x 131072 f32: 27 us to 36; 777 x 50001 f16: 25 to 20, with 1024 threads 36)
     if (rows <= 256 && (int64_t)classes * (dtype == NIF_F32 ? 4 : 2) >= 96 << 10)
-      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 512>), dim3((unsigned)rows), dim3(512), 0, st, logits, ld, classes,
+      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 512>), row_grid(rows), dim3(512), 0, st, logits, ld, rows, classes,
                                             t, top_indices, top_values, top_lse, (float*)((char*)state + s.top), (float*)((char*)state + s.sum), row_loss));
     else
-      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, t,
+      NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 256>), row_grid(rows), dim3(256), 0, st, logits, ld, rows, classes, t,
                                             top_indices, top_values, top_lse, (float*)((char*)state + s.top), (float*)((char*)state + s.sum), row_loss));
   }
   if (reduction != NIF_REDUCE_NONE)
@@ -570,9 +573,9 @@ extern "C" int nif_distill_backward(const void* logits, int64_t ld, int64_t rows
   const DistillState s = distill_state(rows, top);
   const Targets t = distill_targets((char*)state, s, top, temperature);
   const int stretch = 16384;
-  const dim3 grid((unsigned)rows, (unsigned)((classes + stretch - 1) / stretch));
+  const dim3 grid = row_grid(rows, (unsigned)((classes + stretch - 1) / stretch));
   clear_err();
-  NIF_BY_TYPE(dtype, hipLaunchKernelGGL(distill_grad_kernel<D>, grid, dim3(256), 0, st, logits, ld, classes, t,
+  NIF_BY_TYPE(dtype, hipLaunchKernelGGL(distill_grad_kernel<D>, grid, dim3(256), 0, st, logits, ld, rows, classes, t,
                                         (const float*)((const char*)state + s.top), (const float*)((const char*)state + s.sum), grad_loss, reduction == NIF_REDUCE_NONE,
                                         reduction == NIF_REDUCE_MEAN ? (const float*)((const char*)state + s.count) : nullptr, dlogits,
                                         ldd, stretch));
@@ -597,13 +600,13 @@ extern "C" int nif_top_logits(const void* logits, int64_t ld, int64_t rows, int 
   const int64_t bytes = (int64_t)classes * (dtype == NIF_F32 ? 4 : 2);
   const bool wide = top > 192 || (top > 128 && bytes >= 256 << 10) || (rows <= 512 && bytes >= 96 << 10) || bytes >= 512 << 10;
   if (top > 384 && classes >= 8192 && (top <= 768 || rows < 1024))
-    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, logits, ld, classes, top,
+    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 1024>), row_grid(rows), dim3(1024), 0, st, logits, ld, rows, classes, top,
                                           1.f / temperature, values, indices, lse));
   else if (wide && top <= 384)
-    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 512>), dim3((unsigned)rows), dim3(512), 0, st, logits, ld, classes, top,
+    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 512>), row_grid(rows), dim3(512), 0, st, logits, ld, rows, classes, top,
                                           1.f / temperature, values, indices, lse));
   else
-    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, classes, top,
+    NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 256>), row_grid(rows), dim3(256), 0, st, logits, ld, rows, classes, top,
                                           1.f / temperature, values, indices, lse));
   return launch_ok() ? NIF_OK : NIF_ERR_LAUNCH;
 }

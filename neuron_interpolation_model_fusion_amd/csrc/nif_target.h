@@ -22,6 +22,14 @@ struct Targets {
   double tau2;
 };
 
+// Blocks of rows: along x up to 2^21 of them (a dimension takes fewer than 2^32 threads, of which blocks have up to 1024), the
+// rest along z.  The last ones may lie behind the rows.
+inline dim3 row_grid(int64_t blocks, unsigned y = 1) {
+  const int64_t x = blocks < (1 << 21) ? blocks : 1 << 21;
+  return dim3((unsigned)x, y, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t row_block() { return (int64_t)blockIdx.z * gridDim.x + blockIdx.x; }
+
 typedef __attribute__((ext_vector_type(4))) float vec4f;
 typedef __attribute__((ext_vector_type(8))) short vec8s;
 

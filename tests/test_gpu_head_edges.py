@@ -218,3 +218,30 @@ def test_no_rows_need_no_arriving_gradient(d, v, reduction):
                                  ws_b.numel(), st) == 0
     torch.cuda.synchronize()
     assert torch.all(dw == 0) and torch.all(db == 0) and (reduction == 0 or float(loss) == 0)
+
+
+MANY = (1 << 24) + 5  # 256 threads a row are more than 2^32 in one grid dimension
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_more_rows_than_a_grid_dimension_holds(ops, dt):
+    """Logits, top logits and their distillation of 2^24 + 5 rows: the same numbers as the rows' last and first alone."""
+    n, v, k = MANY, 4, 2
+    g = torch.Generator(device='cuda').manual_seed(3)
+    z = torch.randn(n, v, generator=g, device='cuda').to(dt)
+    z[12345:12400] = z[0]
+    z.requires_grad_()
+    values, indices, lse = ops.top_logits(z, k, temperature=2.0)
+    assert torch.equal(values.float(), z.detach().float().topk(k, dim=1).values)
+    assert torch.equal(z.detach().gather(1, indices.long()), values)
+    loss = ops.topk_distillation(z, values, indices, temperature=2.0, top_lse=lse, reduction='none')
+    dz, = torch.autograd.grad(loss, z, grad_outputs=torch.ones_like(loss))
+    for part in (slice(0, 70), slice(n // 2, n // 2 + 70), slice(n - 70, n)):
+        few = z.detach()[part].requires_grad_()
+        top = ops.top_logits(few, k, temperature=2.0)
+        assert torch.equal(top[0], values[part]) and torch.equal(top[1], indices[part]) and torch.equal(top[2], lse[part])
+        alone = ops.topk_distillation(few, *top[:2], temperature=2.0, top_lse=top[2], reduction='none')
+        assert torch.equal(alone, loss[part])
+        assert torch.equal(torch.autograd.grad(alone, few, grad_outputs=torch.ones_like(alone))[0], dz[part])
+    mean = ops.topk_distillation(z, values, indices, temperature=2.0, top_lse=lse)
+    assert abs(float(mean.detach()) - float(loss.double().mean())) <= 2 * U * abs(float(mean.detach()))
