@@ -116,6 +116,7 @@ struct GemmArgs {
   int K;                // contraction length (at most *k_dev when given)
   const int* k_dev;
   int mt, nt, splits;
+  int first, tiles;     // of this launch's, and all of them (tiles x splits)
   // EPI_STATS / EPI_DZ: the logit's last steps
   const void* bias;     // of the first class of the piece; f32 or the 16-bit type
   float inv_tau;
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * (BM + BN) * 64];
   char *const lds_a = lds, *const lds_b = lds + 4 * BM * 64;
   int split, tm, tn;
-  tile_of(blockIdx.x, gridDim.x, g.mt, g.nt, split, tm, tn);
+  tile_of(g.first + blockIdx.x, g.tiles, g.mt, g.nt, split, tm, tn);
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
   const int m0 = tm * BM, n0 = tn * BN;
   // dz is an operand of the next products: rows up to a multiple of K_PAD are written, as zeros
@@ -723,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_any_kernel(GemmArgs g) {
   __shared__ __attribute__((aligned(1024))) char lds_b[PLANES * BN * 64];
   __shared__ __attribute__((aligned(1024))) char lds_out[EPI == EPI_OUT && !T::WIDE ? 2 * BM * BN : 16];
   int split, tm, tn;
-  tile_of(blockIdx.x, gridDim.x, g.mt, g.nt, split, tm, tn);
+  tile_of(g.first + blockIdx.x, g.tiles, g.mt, g.nt, split, tm, tn);
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
   const int m0 = tm * BM, n0 = tn * BN;
   if (n0 >= N) return;
@@ -909,13 +910,14 @@ __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const
 // Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits (zk; not
 // where the logits are kept).
 template <int DT>
-__global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int d,
+__global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int64_t all, int d,
                                                              const int* __restrict__ rows, const int* __restrict__ count,
                                                              void* __restrict__ dst, int ldd, const void* __restrict__ weight,
                                                              int64_t ldw, const void* __restrict__ bias, Targets tg,
                                                              float* __restrict__ zk) {
   typedef typename std::conditional<DT == NIF_F32, float, short>::type W;
-  const int64_t i = blockIdx.x;
+  const int64_t i = row_block();
+  if (i >= all) return;
   const bool have = i < *count;
   const int64_t src = have ? rows[i] : 0;
   const typename Elem<DT>::t* h = (const typename Elem<DT>::t*)hidden + src * ldh;
@@ -942,7 +944,8 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
   __shared__ float sh_top[ROWS][PARTS + 1], sh_sum[ROWS][PARTS + 1];
   __shared__ double sh[16];
   __shared__ int last;
-  const int i0 = blockIdx.x * ROWS, n = *count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i0 = row_block() * ROWS;
+  const int n = *count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (i0 < n) {
     const int r = threadIdx.x % ROWS, part = threadIdx.x / ROWS;
     float top = -INFINITY, sum = 0.f;
@@ -955,7 +958,7 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
     sh_top[r][part] = top;
     sh_sum[r][part] = sum;
     __syncthreads();
-    const int i = i0 + wave;  // a wave a row
+    const int64_t i = i0 + wave;  // a wave a row
     if (wave < ROWS && i < n) {
       top = sh_top[wave][lane], sum = sh_sum[wave][lane];
 #pragma unroll
@@ -967,7 +970,7 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
       double s = 0.0;
       for (int k = lane; k < tg.k; k += 64)
         s += target_term(tg, src, k,
-                         ((double)(z ? z[i * ldz + max(0, tg.at[src * tg.k + k])] : zk[(int64_t)i * tg.k + k]) - (double)all) * (double)tg.inv_tau,
+                         ((double)(z ? z[i * ldz + max(0, tg.at[src * tg.k + k])] : zk[i * tg.k + k]) - (double)all) * (double)tg.inv_tau,
                          log_sum);
       s = wave_sum_f64(s);
       if (lane == 0) {
@@ -982,7 +985,7 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+    last = atomicAdd(done, 1) == (int)(gridDim.x * gridDim.z) - 1;
     if (last) __threadfence();
   }
   __syncthreads();
@@ -1011,8 +1014,8 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
                                                          int f16, float* __restrict__ coef,
                                                          float* __restrict__ cp, float* __restrict__ inv_scale, W* __restrict__ out,
                                                          int64_t ld, int d) {
-  if (blockIdx.x > 0) {
-    const int64_t r = (int64_t)(blockIdx.x - 1) * 4 + (threadIdx.x >> 8);
+  if (row_block() > 0) {
+    const int64_t r = (row_block() - 1) * 4 + (threadIdx.x >> 8);
     if (r < rows_all && inv[r] < 0)
       for (int c = threadIdx.x & 255; c < d; c += 256) out[r * ld + c] = 0;
     return;
@@ -1076,7 +1079,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int
                                                            const float* __restrict__ zk, const float* __restrict__ tops,
                                                            const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
                                                            typename T::t* __restrict__ dz, int64_t ldz) {
-  const int64_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t i = row_block() * 4 + (threadIdx.x >> 6);
   if (i >= *count) return;
   target_entries(tg, rows[i], [&](int k, int) { return zk[i * tg.k + k]; }, tops[i], coef[i], cp[i], v0, v1, dz + i * ldz,
                  threadIdx.x & 63);
@@ -1133,7 +1136,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* __restrict_
                                                         int n, const int* __restrict__ n_dev, int m, float* __restrict__ acc, int first,
                                                         int last, void* __restrict__ out, int64_t out_ld, const int* __restrict__ rowmap,
                                                         const float* __restrict__ inv_scale) {
-  const int64_t i = blockIdx.x;
+  const int64_t i = row_block();
   const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (i >= (n_dev ? min(n, *n_dev) : n) || c >= m) return;
   const float* p = part + i * part_ld + c;  // rows are padded to a multiple of 4
@@ -1506,6 +1509,7 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   if (!h || h->rows < 0 || h->features <= 0 || h->classes <= 0 || h->top < 0) return false;
   if (h->dtype != NIF_F32 && h->dtype != NIF_BF16 && h->dtype != NIF_F16) return false;
   if (h->rows > (1 << 30) || h->features > (1 << 20) || h->classes > (1 << 28) || h->top > NIF_TOP_MAX_K) return false;
+  if (h->rows * h->classes > (int64_t)1 << 43) return false;  // tiles of a product are counted in 31 bits
   p.n = h->rows;
   p.cap = round_up(p.n > 0 ? p.n : 1, HEAD_PAD);
   p.d = h->features;
@@ -1573,24 +1577,28 @@ template <class T, bool TRA, bool TRB, int EPI>
 static void run_gemm(const Shape& s, GemmArgs& g, hipStream_t st) {
   g.mt = (g.M + s.bm - 1) / s.bm;
   g.nt = (g.N + s.bn - 1) / s.bn;
-  const dim3 grid((unsigned)((int64_t)g.mt * g.nt * g.splits));
-  if (grid.x == 0) return;
-  if (s.any && (T::WIDE || !TRB)) {
-    if constexpr (T::WIDE || !TRB) {  // 16 bits: dweight does not read the weight
-      if (s.bn == 64)
-        hipLaunchKernelGGL((head_gemm_any_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
-      else
-        hipLaunchKernelGGL((head_gemm_any_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+  g.tiles = g.mt * g.nt * g.splits;
+  // a launch takes fewer than 2^32 threads; multiples of eight blocks, so that a tile's XCD does not change
+  constexpr int MOST = 1 << 20;
+  for (g.first = 0; g.first < g.tiles; g.first += MOST) {
+    const dim3 grid(g.tiles - g.first < MOST ? g.tiles - g.first : MOST);
+    if (s.any && (T::WIDE || !TRB)) {
+      if constexpr (T::WIDE || !TRB) {  // 16 bits: dweight does not read the weight
+        if (s.bn == 64)
+          hipLaunchKernelGGL((head_gemm_any_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+        else
+          hipLaunchKernelGGL((head_gemm_any_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+      }
+      continue;
     }
-    return;
-  }
-  if constexpr (!T::WIDE) {
-    if (s.bn == 64)
-    hipLaunchKernelGGL((head_gemm_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
-  else if (s.bn == 256)
-    hipLaunchKernelGGL((head_gemm_kernel<T, 256, 256, 2, 4, TRA, TRB, EPI>), grid, dim3(512), 0, st, g);
-  else
-    hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+    if constexpr (!T::WIDE) {
+      if (s.bn == 64)
+        hipLaunchKernelGGL((head_gemm_kernel<T, 128, 64, 4, 1, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+      else if (s.bn == 256)
+        hipLaunchKernelGGL((head_gemm_kernel<T, 256, 256, 2, 4, TRA, TRB, EPI>), grid, dim3(512), 0, st, g);
+      else
+        hipLaunchKernelGGL((head_gemm_kernel<T, 128, 128, 2, 2, TRA, TRB, EPI>), grid, dim3(256), 0, st, g);
+    }
   }
 }
 
@@ -1668,7 +1676,7 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
 
 template <int DT>
 static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStream_t st) {
-  hipLaunchKernelGGL(head_pack_rows_kernel<DT>, dim3((unsigned)p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.d,
+  hipLaunchKernelGGL(head_pack_rows_kernel<DT>, row_grid(p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.cap, p.d,
                      (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), p.keep ? nullptr : (float*)(state + p.s_zk));
 }
 
@@ -1695,6 +1703,7 @@ static BwdSpace backward_space(const Plan& p) {
   const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
   b.stretch = p.n <= 64 ? 64 : 32;  // rows of a block of column sums: the fewest that leave at most 2048 blocks, up to 256
   while (b.stretch < 256 && (p.n + b.stretch - 1) / b.stretch * ((p.piece + 255) / 256) > 2048) b.stretch *= 2;
+  while ((p.n + b.stretch - 1) / b.stretch > 65535) b.stretch *= 2;  // a grid takes no more along y
   const size_t part_b = (size_t)((p.n + b.stretch - 1) / b.stretch) * p.piece * 4;
   const size_t part = part_h > part_w ? part_h : part_w;
   b.part = take(at, part > part_b ? part : part_b);
@@ -1745,7 +1754,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc, p.any_b), g, st);
     }
     if (p.n > 0 && !p.keep)
-      hipLaunchKernelGGL(head_targets_kernel<T>, dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, tg, rows, count, zk, tops, coef, cp, v0,
+      hipLaunchKernelGGL(head_targets_kernel<T>, row_grid((p.n + 3) / 4), dim3(256), 0, st, tg, rows, count, zk, tops, coef, cp, v0,
                        v0 + vc, dz, b.ldz);
     if (dbias) {
       W* out = (W*)dbias + v0;
@@ -1777,7 +1786,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       }
       run_gemm<T, true, true, EPI_OUT>(b.dw, g, st);
       if (g.splits > 1)
-        hipLaunchKernelGGL(head_join_kernel<T>, dim3(vc, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, vc,
+        hipLaunchKernelGGL(head_join_kernel<T>, row_grid(vc, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split, b.dh_ld, vc,
                            nullptr, p.d, nullptr, 1, 1, g.out, lddw, nullptr, inv_scale);
     }
     if (dhidden) {  // [packed rows][features] += dz W, contraction over the classes of the piece
@@ -1806,7 +1815,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.acc_ld = b.dh_ld;
       run_gemm<T, true, false, EPI_OUT>(b.dh, g, st);
       if (g.splits > 1 && p.n > 0)
-        hipLaunchKernelGGL(head_join_kernel<T>, dim3((unsigned)p.n, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split,
+        hipLaunchKernelGGL(head_join_kernel<T>, row_grid(p.n, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split,
                            b.dh_ld, (int)p.n, count, p.d, acc, first, last, dhidden, lddh, rows, inv_scale);
     }
   }
@@ -1901,7 +1910,7 @@ extern "C" int nif_head_forward(const nif_head_desc* h, float* loss, void* state
       forward_products<F16>(h, p, s, (char*)ws, f, tiles, st);
     const float2* stats = (const float2*)((char*)ws + f.stats);
     const auto finish = [&](auto each) {
-      hipLaunchKernelGGL(head_finish_kernel<each>, dim3((unsigned)((p.n + each - 1) / each)), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg,
+      hipLaunchKernelGGL(head_finish_kernel<each>, row_grid((p.n + each - 1) / each), dim3(FINISH_NT), 0, st, stats, p.cap, tiles, tg,
                          rows, count, (float*)(s + p.s_top), (float*)(s + p.s_sum), (const float*)(s + p.s_zk), p.keep ? (const float*)(s + p.s_z) : nullptr,
                          p.ldu, row_loss, p.n, h->reduction, count + 1, loss);
     };
@@ -1957,8 +1966,8 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
   }
   const BwdSpace b = backward_space(p);
   const auto prepare = [&](auto* out) {
-    const unsigned clearing = out && p.n > 0 ? (unsigned)((p.n + 3) / 4) : 0;
-    hipLaunchKernelGGL(head_coef_kernel, dim3(1 + clearing), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
+    const int64_t clearing = out && p.n > 0 ? (p.n + 3) / 4 : 0;
+    hipLaunchKernelGGL(head_coef_kernel, row_grid(1 + clearing), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
                        h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_inv),
                        (const int*)(s + p.s_count), (const float*)(s + p.s_sum), p.n, h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp),
                        (float*)((char*)ws + b.scale), out, lddh, p.d);

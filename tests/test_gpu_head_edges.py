@@ -245,3 +245,50 @@ def test_more_rows_than_a_grid_dimension_holds(ops, dt):
         assert torch.equal(torch.autograd.grad(alone, few, grad_outputs=torch.ones_like(alone))[0], dz[part])
     mean = ops.topk_distillation(z, values, indices, temperature=2.0, top_lse=lse)
     assert abs(float(mean.detach()) - float(loss.double().mean())) <= 2 * U * abs(float(mean.detach()))
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_a_head_of_more_rows_than_a_grid_dimension_holds(ops, dt):
+    n, d, v = MANY, 8, 5
+    g = torch.Generator(device='cuda').manual_seed(4)
+    h = torch.randint(-2, 3, (n, d), generator=g, device='cuda').to(dt).requires_grad_()
+    w = torch.randint(-2, 3, (v, d), generator=g, device='cuda').to(dt).requires_grad_()
+    b = torch.zeros(v, dtype=dt, device='cuda').requires_grad_()
+    y = torch.randint(-1, v, (n,), generator=g, device='cuda')
+    loss = ops.linear_cross_entropy(h, w, y, b, ignore_index=-1, reduction='sum')
+    dh, dw, db = torch.autograd.grad(loss, (h, w, b), grad_outputs=torch.tensor(2.0 ** -12, device='cuda'))
+    want, dz_all, size = 0.0, [], 0.0
+    for lo in range(0, n, 1 << 22):  # the formula, a part of the rows at a time
+        part = slice(lo, min(n, lo + (1 << 22)))
+        x, live = h.detach()[part].double(), y[part] >= 0
+        logs = torch.log_softmax(x @ w.detach().double().t(), 1)
+        at = y[part].clamp(min=0)[:, None]
+        want += float(-(logs.gather(1, at)[:, 0] * live).sum())
+        dz = logs.exp().scatter_add_(1, at, torch.full_like(at, -1.0, dtype=torch.float64)) * live[:, None] * 2.0 ** -12
+        got = dh[part].double()
+        ref = dz @ w.detach().double()
+        # a row's |dz| sums to at most 2 . 2^-12, weights are at most 2: each rounding of dz, the sum's and the result's
+        assert float((got - ref).abs().max()) <= 2.0 ** -12 * 4 * (2 * U16[dt] + 2.0 ** -17) + 2.0 ** -24
+        dz_all.append((dz.t() @ x, dz.sum(0)))
+        size = size + dz.abs().sum(0)
+    assert abs(float(loss.detach()) - want) <= 2.0 ** -18 * n + 2 * U * want
+    dw_ref, db_ref = sum(p[0] for p in dz_all), sum(p[1] for p in dz_all)
+    # n additions of 32 bits in chains of at most 2^24 / 128, dz's rounding once
+    slack = U16[dt] + 2.0 ** -17 + 2.0 ** 17 * U
+    assert torch.all((dw.double() - dw_ref).abs() <= U16[dt] * dw_ref.abs() + 2 * slack * size[:, None])
+    assert torch.all((db.double() - db_ref).abs() <= U16[dt] * db_ref.abs() + slack * size)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_more_tiles_of_a_product_than_one_launch_takes(ops, dt):
+    """2^21 rows against 2^15 + 1 classes: over 2^20 tiles of the logits' product."""
+    n, d, v = 1 << 21, 16, (1 << 15) + 1
+    g = torch.Generator(device='cuda').manual_seed(5)
+    h = torch.randint(-1, 2, (n, d), generator=g, device='cuda').to(dt)
+    w = torch.randint(-1, 2, (v, d), generator=g, device='cuda').to(dt)
+    y = torch.randint(0, v, (n,), generator=g, device='cuda')
+    loss = ops.linear_cross_entropy(h, w, y, reduction='none')
+    for part in (slice(0, 100), slice(n // 2 - 50, n // 2 + 50), slice(n - 100, n)):
+        z = h[part].double() @ w.double().t()
+        want = torch.logsumexp(z, 1) - z.gather(1, y[part][:, None])[:, 0]
+        assert torch.all((loss[part].double() - want).abs() <= 2.0 ** -18 + 2 * U * want + 8 * U * 32)
