@@ -419,7 +419,8 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
     if (anew ? m >= bar : m > bar) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = base + u * NT + (int)threadIdx.x;
+        int i = base + u * NT + (int)threadIdx.x;
+        asm volatile("" : "+v"(i));  // of this rare path alone: shared with the loads it costs registers that they spill
 #pragma unroll
         for (int e = 0; e < V; ++e)
           if ((anew ? x[u * V + e] >= bar : x[u * V + e] > bar) && i < r.vecs) put(x[u * V + e], r.head + i * V + e);
