@@ -381,8 +381,8 @@ __device__ __forceinline__ void select_by_digits(const typename Elem<DT>::t* z, 
 // whatever comes later must exceed it; it is taken anew after 1, 2, 4, 8, .. stretches, which leaves about 6 k elements
 // of a row of 131072 (k log2 of the stretches) in a list in LDS.  The last bar cuts the list to little more than k, which are sorted.  Rows that
 // this does not fit (more than the list holds: ties at the bar, rising rows; NaN) are selected by digits instead.  The
-// log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 258 us,
-// 4.1 TB/s; 400 x 1000 f32 in 13 us, a launch's latency.
+// log-sum-exp goes along.  Bound by the read of the logits and the exponentials: 4096 x 131072 bf16, k = 64, in 237 us,
+// 4.5 TB/s; 400 x 1000 f32 in 12 us, a launch's latency.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restrict__ logits, int64_t ld, int64_t rows, int classes, int k, float inv_tau,
                                                         void* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse) {
@@ -408,7 +408,8 @@ __global__ __launch_bounds__(NT, 8) void top_logits_kernel(const void* __restric
     const float x[1] = {(float)r.z[r.loose_at(threadIdx.x)]};
     run.add(x, scale);
   }
-  float bar = -INFINITY, mine = -INFINITY;
+  // more entries than threads: no bar, such rows are selected by digits and this pass makes the log-sum-exp only
+  float bar = k <= NT ? -INFINITY : INFINITY, mine = -INFINITY;
   int stretch = 0;
   stream_row<DT, NT, U>(r, [&](const float (&x)[U * V], int base) {
     const float m = run.add(x, scale);
@@ -592,14 +593,16 @@ extern "C" int nif_top_logits(const void* logits, int64_t ld, int64_t rows, int 
   if (rows == 0) return NIF_OK;
   hipStream_t st = (hipStream_t)stream;
   clear_err();
-  // Threads a row.  The bar is of use for k up to three quarters of them (2048 x 50001 bf16, k = 500: 307 us with 1024 threads,
-  // 672 with 512; k = 300: 150 with 512, 606 by digits with 256), and the list holds enough for long rows of many
-  // (2048 x 131072, k = 200: 255 us with 512, 880 with 256).  Else wider blocks where rows are few or long (2048 x 131072 f32,
-  // k = 20: 280 us with 512, 323 with 256; but 2048 x 50001 bf16: 113, 78).  Many of short rows are selected by digits at once
-  // (2048 x 3000, k = 700: 112 us with 256 threads, 313 with 1024), and so are over three quarters of 1024 (2048 x 50001, k = 1024: 618 us with 256
-  // threads, 956 with 1024; 400 rows: 468 and 256).
+  // Threads a row.  The bar is of use for k up to three quarters of them (2048 x 50001 bf16, k = 500: 328 us with 1024 threads,
+  // 685 with 512; k = 300: 152 with 512, 565 by digits with 256), and the list of 512 holds enough for more entries of long rows
+  // (2048 x 131072, k = 200: 233 us, 837 with 256; but 4096 rows, k = 160: 406, 315).  Wider blocks also where rows are few and entries are not
+  // (64 x 131072 bf16, k = 128: 67 us with 512, 78 with 256; k = 10: 52, 47), else not (2048 x 131072 f32, k = 20: 284 us with
+  // 512, 233 with 256; 2048 x 50001 bf16: 117, 72); rows over 1 MiB are as wide as the longest measured ones need.  Many of
+  // short rows are selected by digits at once (2048 x 3000, k = 700: 108 us with 256 threads, 309 with 1024), and so are over
+  // three quarters of 1024 (2048 x 50001, k = 1024: 584 us with 256 threads, 951 with 1024; 400 rows: 437 and 257).
   const int64_t bytes = (int64_t)classes * (dtype == NIF_F32 ? 4 : 2);
-  const bool wide = top > 192 || (top > 128 && bytes >= 256 << 10) || (rows <= 512 && bytes >= 96 << 10) || bytes >= 512 << 10;
+  const bool few = bytes >= 192 << 10 && (rows <= 256 ? top >= 64 : rows <= 512 && top > 128);
+  const bool wide = top > 192 || (top > 160 && bytes >= 512 << 10) || few || bytes > 1 << 20;
   if (top > 384 && classes >= 8192 && (top <= 768 || rows < 1024))
     NIF_BY_TYPE(dtype, hipLaunchKernelGGL((top_logits_kernel<D, 1024>), row_grid(rows), dim3(1024), 0, st, logits, ld, rows, classes, top,
                                           1.f / temperature, values, indices, lse));
