@@ -2,11 +2,13 @@
 
 The library is built in-tree (``csrc/libnif.so``, see ``__graft_entry__.build``).
 There is no fallback: if the shared object is missing or a symbol is absent the
-import fails loudly, and every op raises on a non-zero status.
+import fails loudly (nif_torch.so: the first call that needs it), and every op
+raises on a non-zero status.
 """
 import ctypes
 import importlib.util
 import os
+import threading
 
 # torch first: libnif.so must bind to the HIP runtime torch has already loaded.  Loading the
 # system libamdhip64 before torch's own copy puts two runtimes in one process and the second
@@ -141,12 +143,15 @@ class NifError(RuntimeError):
     pass
 
 
+def _need(path):
+    if not os.path.exists(path):
+        raise ImportError(
+            f'{path} is missing: build it with `python -c "import __graft_entry__ as g; g.build()"` '
+            f'or `make -C {os.path.dirname(path)}`. There is no CPU fallback.')
+
+
 def _load():
-    for path in (LIB_PATH, TORCH_PATH):
-        if not os.path.exists(path):
-            raise ImportError(
-                f'{path} is missing: build it with `python -c "import __graft_entry__ as g; g.build()"` '
-                f'or `make -C {os.path.dirname(path)}`. There is no CPU fallback.')
+    _need(LIB_PATH)
     lib = ctypes.CDLL(LIB_PATH)
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is absent
@@ -156,6 +161,7 @@ def _load():
 
 
 def _load_torch():
+    _need(TORCH_PATH)
     spec = importlib.util.spec_from_file_location('nif_torch', TORCH_PATH)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)  # finds libnif.so, loaded above, beside itself
@@ -164,7 +170,17 @@ def _load_torch():
 
 
 lib = _load()
-nif_torch = _load_torch()
+_torch_lock = threading.Lock()
+
+
+def __getattr__(name):
+    """`nif_torch` is loaded by its first use: it is built for one torch and one Python, libnif.so serves without it."""
+    if name != 'nif_torch':
+        raise AttributeError(f'module {__name__!r} has no attribute {name!r}')
+    with _torch_lock:
+        if name not in globals():
+            globals()[name] = _load_torch()
+    return globals()[name]
 
 
 def check(status, what):
