@@ -44,11 +44,15 @@ def parse_args():
                         'the number of models equals the number of classes; this flag counts the dataset classes instead.')
     p.add_argument('--head_loss', type=str, default='match', choices=ALFusion.head_losses,
                    help="Not a reference flag. What the last level is fitted on: 'match' (the reference's), 'cross_entropy' "
-                        "(the labels) or 'top_logits' (the likeliest classes of the models, at --kd_temperature).")
+                        "(the labels) or 'top_logits' (the likeliest classes of the models, at --kd_temperature). "
+                        "--run_last_layer_kd distils from the models in any case: after 'cross_entropy' as after 'match'.")
     p.add_argument('--kd_top_logits', type=int, default=32,
                    help='Not a reference flag. Number of classes kept per sample under --head_loss top_logits.')
     c.add_data_args(p)
-    return p.parse_args()
+    args = p.parse_args()
+    if args.head_loss == 'top_logits' and args.run_last_layer_kd and args.use_kl_kd_on_head:
+        p.error('--use_kl_kd_on_head and --head_loss top_logits are two losses of the same phase')
+    return args
 
 
 def build_fusion_config(args, models, dataset, device, num_classes):
@@ -105,6 +109,8 @@ def main():
 
     if args.run_last_layer_kd:
         print('Running ALFusion with last layer knowledge distillation')
+        if cfg.head_loss == 'cross_entropy':  # labels are no teacher
+            cfg.head_loss = 'match'
         cfg.use_kd_on_head = args.use_kl_kd_on_head
         cfg.kd_temperature = args.kd_temperature
         cfg.skip_levels = list(range(get_num_levels(models) - 1))

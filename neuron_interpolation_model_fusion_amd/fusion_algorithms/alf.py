@@ -162,6 +162,8 @@ class ALFusion:
 
     def _head_loss_check(self, fusion_config):
         """Before the first level is fitted: the last one is hours away on a large model."""
+        if fusion_config.use_kd_on_head:
+            raise ValueError(f'use_kd_on_head and head_loss={fusion_config.head_loss!r} are two losses for the last level')
         level = self.models[0].get_ordered_trainable_named_levels[-1]
         self._body_and_head(level.network)
         if level.output_width > 1 << 24:

@@ -1,0 +1,68 @@
+"""not-gpu: which loss each phase of run_alf.py fits the last level with, and the choices that contradict each other."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from neuron_interpolation_model_fusion_amd.fusion_algorithms import ALFusion
+from tests.test_alf_head_loss import _config, _models
+
+SCRIPTS = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'main_scripts', 'run_individual_algorithms')
+
+
+@pytest.fixture
+def run_alf(monkeypatch, tmp_path):
+    """run(*flags) -> [(head_loss, use_kd_on_head, kd_temperature, skipped levels)] of its fits, which are not made."""
+    monkeypatch.syspath_prepend(SCRIPTS)
+    import _common as c
+    import run_alf as script
+    models = _models()
+    fits = []
+    monkeypatch.setattr(c, 'load_models', lambda *a: models)
+    monkeypatch.setattr(c, 'fusion_dataset', lambda *a: None)
+    monkeypatch.setattr(c, 'fusion_samples', lambda *a, **k: (torch.zeros(4, 64), torch.zeros(4, dtype=torch.long)))
+    monkeypatch.setattr(c, 'num_classes_of', lambda *a: 10)
+    monkeypatch.setattr(c, 'report', lambda *a: None)
+    monkeypatch.setattr(script, 'get_classifier_head_weights', lambda *a, **k: np.ones((2, 10)))
+    monkeypatch.setattr(torch, 'save', lambda *a, **k: None)
+
+    def fuse(self, cfg):
+        self._config_check(cfg)
+        fits.append((cfg.head_loss, cfg.use_kd_on_head, cfg.kd_temperature, cfg.skip_levels))
+    monkeypatch.setattr(ALFusion, 'fuse', fuse)
+
+    def run(*flags):
+        monkeypatch.setattr(sys, 'argv', ['run_alf.py', '--model_savedir', str(tmp_path), '--num_fusion_samples', '4', '--num_models', '2',
+                                          '--device', 'cpu', *flags])
+        fits.clear()
+        script.main()
+        return list(fits)
+    return run
+
+
+@pytest.mark.parametrize('kl', [False, True])
+@pytest.mark.parametrize('loss', ['match', 'cross_entropy'])
+def test_the_distillation_phase_distils(run_alf, loss, kl):
+    flags = ['--use_kl_kd_on_head'] if kl else []
+    fits = run_alf('--head_loss', loss, '--run_last_layer_kd', '--kd_temperature', '3', *flags)
+    assert [f[:2] for f in fits[:3]] == [(loss, False)] * 3 and len(fits) == 4
+    assert fits[3] == ('match', kl, 3.0, [0])
+
+
+def test_the_distillation_phase_keeps_top_logits(run_alf):
+    fits = run_alf('--head_loss', 'top_logits', '--run_last_layer_kd', '--kd_temperature', '3')
+    assert [f[:3] for f in fits] == [('top_logits', False, 3.0)] * 4 and fits[3][3] == [0]
+
+
+def test_two_distillations_at_once_are_refused(run_alf, capsys):
+    with pytest.raises(SystemExit):
+        run_alf('--head_loss', 'top_logits', '--run_last_layer_kd', '--use_kl_kd_on_head')
+    assert '--use_kl_kd_on_head' in capsys.readouterr().err
+
+
+@pytest.mark.parametrize('loss', ['cross_entropy', 'top_logits'])
+def test_a_loss_on_the_head_and_kd_on_head_contradict(loss):
+    with pytest.raises(ValueError, match='use_kd_on_head'):
+        ALFusion(_models()).fuse(_config(torch.zeros(4, 64), head_loss=loss, kd_temperature=2.0, use_kd_on_head=True))
