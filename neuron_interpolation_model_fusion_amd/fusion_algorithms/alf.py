@@ -379,12 +379,20 @@ class ALFusion:
     # are exact in float32 up to 2^24.
     @staticmethod
     def _body_and_head(network):
-        """(the last level up to its nn.Linear, that nn.Linear)."""
+        """(the last level up to its nn.Linear, that nn.Linear), neither of which is called as a whole: what hangs on their
+        calls is refused."""
         if isinstance(network, nn.Linear):
-            return nn.Identity(), network
-        if isinstance(network, nn.Sequential) and len(network) and isinstance(network[-1], nn.Linear):
-            return network[:-1], network[-1]
-        raise ValueError(f'a loss on the head needs a last level that ends in nn.Linear, not {type(network).__name__}')
+            body, head = nn.Identity(), network
+        elif isinstance(network, nn.Sequential) and len(network) and isinstance(network[-1], nn.Linear):
+            body, head = network[:-1], network[-1]
+        else:
+            raise ValueError(f'a loss on the head needs a last level that ends in nn.Linear, not {type(network).__name__}')
+        for module in (network, head):
+            if getattr(module.forward, '__func__', None) not in (nn.Linear.forward, nn.Sequential.forward):
+                raise ValueError(f'a loss on the head does not call {type(module).__name__}, which has a forward of its own')
+            if module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
+                raise ValueError(f'a loss on the head does not call {type(module).__name__}, which has hooks: remove them first')
+        return body, head
 
     def _head_loss_targets(self, num_classes, fusion_config):
         if fusion_config.head_loss == 'cross_entropy':
@@ -622,6 +630,8 @@ class ALFusion:
     def fuse(self, fusion_config, fused_hat=None):
         """alf.py:596-638; fuses IN PLACE into fused_hat (a copy of models[0] when None)."""
         self._config_check(fusion_config)
+        if fused_hat is not None and fusion_config.head_loss != 'match':
+            self._body_and_head(fused_hat.get_ordered_trainable_named_levels[-1].network)
         num_levels = get_num_levels(self.models)
         start_time = time.time()
         self.ni_scores = [{} for _ in range(len(self.models))]

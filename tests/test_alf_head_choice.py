@@ -66,3 +66,46 @@ def test_two_distillations_at_once_are_refused(run_alf, capsys):
 def test_a_loss_on_the_head_and_kd_on_head_contradict(loss):
     with pytest.raises(ValueError, match='use_kd_on_head'):
         ALFusion(_models()).fuse(_config(torch.zeros(4, 64), head_loss=loss, kd_temperature=2.0, use_kd_on_head=True))
+
+
+def _hook(*args):
+    return None
+
+
+@pytest.mark.parametrize('watch', [
+    lambda net, head: head.register_forward_hook(_hook), lambda net, head: head.register_forward_pre_hook(_hook),
+    lambda net, head: head.register_full_backward_hook(_hook), lambda net, head: head.register_full_backward_pre_hook(_hook),
+    lambda net, head: net.register_forward_hook(_hook), lambda net, head: net.register_forward_pre_hook(_hook),
+    lambda net, head: net.register_full_backward_hook(_hook)])
+@pytest.mark.parametrize('loss', ['cross_entropy', 'top_logits'])
+def test_hooks_that_the_loss_would_pass_by_are_refused(loss, watch):
+    """The loss takes the head's input and weight: the head and the level's Sequential are not called."""
+    models = _models()
+    network = models[0].get_ordered_trainable_named_levels[-1].network
+    handle = watch(network, network[-1])
+    cfg = _config(torch.zeros(4, 64), head_loss=loss, kd_temperature=2.0)
+    with pytest.raises(ValueError, match='hooks'):
+        ALFusion(models).fuse(cfg)
+    with pytest.raises(ValueError, match='hooks'):  # on the model that is fused into
+        ALFusion(_models()).fuse(cfg, models[0])
+    handle.remove()
+    ALFusion(models)._config_check(cfg)
+
+
+def test_a_head_with_a_forward_of_its_own_is_refused():
+    class Scaled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Twice(torch.nn.Sequential):
+        def forward(self, x):
+            return 2 * super().forward(x)
+    for network in (Scaled(4, 3), torch.nn.Sequential(torch.nn.Flatten(), Scaled(4, 3)), Twice(torch.nn.Flatten(), torch.nn.Linear(4, 3))):
+        with pytest.raises(ValueError, match='forward of its own'):
+            ALFusion._body_and_head(network)
+    wrapped = torch.nn.Linear(4, 3)
+    wrapped.forward = lambda x: 2 * torch.nn.Linear.forward(wrapped, x)
+    with pytest.raises(ValueError, match='forward of its own'):
+        ALFusion._body_and_head(wrapped)
+    body, head = ALFusion._body_and_head(torch.nn.Sequential(torch.nn.Flatten(), torch.nn.Linear(4, 3)))
+    assert len(body) == 1 and head.out_features == 3
