@@ -179,8 +179,8 @@ class ALFusion:
         y = torch.as_tensor(fusion_config.y).reshape(-1)
         if y.shape[0] != fusion_config.X.shape[0]:
             raise ValueError(f'{y.shape[0]} labels for {fusion_config.X.shape[0]} samples')
-        if bool(((y < 0) | (y >= level.output_width)).any()):
-            raise ValueError(f'labels must lie in [0, {level.output_width})')
+        if bool(((y < 0) | (y >= level.output_width) | (y != y.long())).any()):
+            raise ValueError(f'labels must lie in [0, {level.output_width}) and be whole')
 
     # -- layouts (alf.py:104-124) ------------------------------------------------------------------------
     def _flatten_acts(self, acts):

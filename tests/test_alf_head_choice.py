@@ -109,3 +109,12 @@ def test_a_head_with_a_forward_of_its_own_is_refused():
         ALFusion._body_and_head(wrapped)
     body, head = ALFusion._body_and_head(torch.nn.Sequential(torch.nn.Flatten(), torch.nn.Linear(4, 3)))
     assert len(body) == 1 and head.out_features == 3
+
+
+@pytest.mark.parametrize('y', [torch.tensor([0.0, 1.5, 2.0, 3.0]), torch.tensor([0.0, float('nan'), 1.0, 2.0]),
+                               torch.tensor([0.0, float('inf'), 1.0, 2.0])])
+def test_labels_that_are_no_whole_numbers_are_refused(y):
+    """They travel as float rows and are cut to whole numbers on the way into the loss."""
+    with pytest.raises(ValueError, match='labels must'):
+        ALFusion(_models()).fuse(_config(torch.zeros(4, 64), head_loss='cross_entropy', y=y))
+    ALFusion(_models())._config_check(_config(torch.zeros(4, 64), head_loss='cross_entropy', y=torch.tensor([0.0, 9.0, 1.0, 2.0])))
