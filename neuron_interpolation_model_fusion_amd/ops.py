@@ -1017,6 +1017,10 @@ def _temperature(what, temperature):
     return temperature
 
 
+def _are_integers(t):
+    return not (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool)
+
+
 def _check_top(what, lead, values, indices, lse):
     if values.shape != indices.shape or values.dim() < 1 or tuple(values.shape[:-1]) != tuple(lead):
         raise ValueError(f'{what}: top_values / top_indices must be {tuple(lead)} + (k,), got {tuple(values.shape)} / '
@@ -1024,7 +1028,7 @@ def _check_top(what, lead, values, indices, lse):
     k = values.shape[-1]
     if not 1 <= k <= _lib.NIF_TOP_MAX_K:
         raise ValueError(f'{what}: 1 to {_lib.NIF_TOP_MAX_K} top logits a row, got {k}')
-    if not values.is_floating_point() or indices.is_floating_point() or indices.dtype == torch.bool:
+    if not values.is_floating_point() or not _are_integers(indices):
         raise TypeError(f'{what}: top_values must be floating and top_indices integers, got {values.dtype} / {indices.dtype}')
     if lse is not None and (tuple(lse.shape) != tuple(lead) or not lse.is_floating_point()):
         raise ValueError(f'{what}: top_lse must be floating of shape {tuple(lead)}, got {lse.dtype} {tuple(lse.shape)}')
@@ -1033,8 +1037,11 @@ def _check_top(what, lead, values, indices, lse):
 def _top_targets(values, indices, lse):
     """Contiguous (indices int32, values f32, lse f32 or None) of a teacher's top logits, a row each."""
     k = values.shape[-1]
-    if indices.dtype == torch.int64:
-        indices = indices.clamp(-1, 2 ** 31 - 1)
+    if indices.dtype == torch.uint64:  # the upper half would come back negative
+        indices = indices.view(torch.int64)
+        indices = torch.where(indices < 0, 2 ** 31 - 1, indices)
+    if indices.dtype != torch.int32:
+        indices = indices.to(torch.int64).clamp(-1, 2 ** 31 - 1)
     indices = indices.detach().to(torch.int32).reshape(-1, k).contiguous()
     values = values.detach().float().reshape(-1, k).contiguous()
     return indices, values, None if lse is None else lse.detach().float().reshape(-1).contiguous()
@@ -1073,7 +1080,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     the classes of about 256 MiB; for few rows, where that is faster, up to 64 MiB of logits are kept in f32."""
     what = 'linear_cross_entropy'
     reduction = _reduction(what, reduction)
-    if target.is_floating_point() or target.dtype == torch.bool or tuple(target.shape) != tuple(hidden.shape[:-1]):
+    if not _are_integers(target) or tuple(target.shape) != tuple(hidden.shape[:-1]):
         raise ValueError(f'{what}: target must be integers of shape {tuple(hidden.shape[:-1])}, got {target.dtype} '
                          f'{tuple(target.shape)}')
     _check_head(what, hidden, weight, bias)
