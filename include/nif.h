@@ -499,6 +499,8 @@ int nif_lsq_solve_f64(const double* G, int64_t ldg, const double* R, int64_t ldr
  * Reductions: NONE: loss[rows]; SUM; MEAN over the rows that count (0 when there are none).
  * hidden rows x features (ldh), weight classes x features (ldw), bias classes or NULL, all of `dtype`; any alignment.
  * The logits are not kept, but for few rows: up to 64 MiB of them in 32 bits where that is faster than computing them again.
+ * Up to 2^30 rows, 2^20 features, 2^28 classes and 2^43 logits.  Sizes of state and workspaces: the packed hidden rows; forward
+ * 8 bytes a row for every 32 to 128 classes; backward pieces of 256 MiB, or of 1024 classes, of the logits' gradient.
  * Products accumulate in 32 bits; f32 operands are split into three bf16 parts (f32-level accuracy).
  * `state` carries the forward pass's results to the backward pass, which needs the same inputs; the workspaces are
  * scratch of each call.  dhidden, dweight, dbias: of `dtype`, written in full; NULL where not wanted. */

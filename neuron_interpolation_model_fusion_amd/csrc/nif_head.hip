@@ -1610,7 +1610,7 @@ static FwdSpace forward_space(const Plan& p) {
   FwdSpace f;
   size_t at = 0;
   const Shape s = logit_shape(p, p.pack_f ? p.piece : p.v, p.any_f);
-  const int64_t tiles = p.keep ? (p.v + KEPT - 1) / KEPT : (p.v / s.bm + p.v / p.piece + 2) * s.wm;
+  const int64_t tiles = p.keep ? (p.v + KEPT - 1) / KEPT : (p.v / s.bm + (p.pack_f ? p.v / p.piece : 0) + 2) * s.wm;
   f.stats = take(at, (size_t)tiles * p.cap * 8);
   const int splits = p.keep ? kept_shape(p, p.pack_f ? p.piece : p.v).splits : 1;
   f.part = take(at, splits > 1 ? (size_t)splits * p.n * p.ldu * 4 : 0);

@@ -1076,8 +1076,13 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     alike; target: integers of hidden's leading shape.  Rows with ``ignore_index`` are left out: they cost nothing, get
     zero gradients whatever they hold, and 'mean' runs over the others (0 when there are none).  A target that is no class
     makes its row NaN.  Differentiable once w.r.t. hidden, weight and bias; the loss is f32, f32 inputs compute at f32
-    accuracy and 16-bit ones accumulate in 32 bits.  Memory beyond the gradients: the packed hidden rows and pieces of
-    the classes of about 256 MiB; for few rows, where that is faster, up to 64 MiB of logits are kept in f32."""
+    accuracy and 16-bit ones accumulate in 32 bits.
+
+    Memory beyond the gradients: the packed hidden rows; forward 8 bytes a row for every 32 (few rows) to 128 classes;
+    backward pieces of the classes of 256 MiB, or of 1024 classes where a row of them is more, for the gradient of the
+    logits, 4 bytes a feature of each row where there are several pieces, and partial sums of products that are split.  A
+    16-bit weight whose rows are off 16-byte borders may be copied by such pieces.  For few rows, where that is faster, up to
+    64 MiB of logits are kept in f32."""
     what = 'linear_cross_entropy'
     reduction = _reduction(what, reduction)
     if not _are_integers(target) or tuple(target.shape) != tuple(hidden.shape[:-1]):
