@@ -501,7 +501,9 @@ int nif_lsq_solve_f64(const double* G, int64_t ldg, const double* R, int64_t ldr
  * The logits are not kept, but for few rows: up to 64 MiB of them in 32 bits where that is faster than computing them again.
  * Up to 2^30 rows, 2^20 features, 2^28 classes and 2^43 logits.  Sizes of state and workspaces: the packed hidden rows; forward
  * 8 bytes a row for every 32 to 128 classes; backward pieces of 256 MiB, or of 1024 classes, of the logits' gradient.
- * Products accumulate in 32 bits; f32 operands are split into three bf16 parts (f32-level accuracy).
+ * Products accumulate in 32 bits; f32 operands are split into three bf16 parts (f32-level accuracy; an infinite one becomes
+ * NaN, but for small heads: mask classes by the bias).  Of 16-bit operands the logits' gradient is rounded to their type
+ * before its products.
  * `state` carries the forward pass's results to the backward pass, which needs the same inputs; the workspaces are
  * scratch of each call.  dhidden, dweight, dbias: of `dtype`, written in full; NULL where not wanted. */
 #define NIF_REDUCE_NONE 0
@@ -545,7 +547,8 @@ int nif_distill_backward(const void* logits, int64_t ld, int64_t rows, int class
                          void* stream);
 
 /* ---- a teacher's top logits: the `top` largest of each row, larger first and equal ones by the lower class (NaN before
- * everything), their classes, and logsumexp(row / temperature).  values: rows x top of `dtype`; contiguous outputs. */
+ * everything), their classes, and logsumexp(row / temperature): +inf for a row that holds +inf, NaN for one that holds NaN.
+ * values: rows x top of `dtype`; contiguous outputs. */
 int nif_top_logits(const void* logits, int64_t ld, int64_t rows, int classes, int dtype, int top, float temperature, void* values,
                    int32_t* indices, float* lse, void* stream);
 

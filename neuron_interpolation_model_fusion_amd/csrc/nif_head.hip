@@ -309,7 +309,9 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
           for (int e = 0; e < 4 * GROUP; ++e) {
             const int i = i0 + e / 4, r = e % 4;
             // Rounded to the 16-bit type (half a step, 2^-8 bf16 / 2^-11 f16, of each element; f16 after scaling by a
-            // power of two): the size of the rounding that the gradients themselves get.
+            // power of two): the size of the rounding that the gradients themselves get.  Their error grows by it -- not
+            // seen for labels (1537 x 776 x 50001 bf16: 1.66e-3 -> 1.67e-3 relative), 1.4 times for distillation (2048 x 1000
+            // x 32000 f16: 2.1e-4 -> 2.9e-4); two 16-bit parts would double the products of the backward pass.
             float x = cp * head_exp<T>((acc[i][j][r] + bias[i][r] - top) * scale);
             x = live ? x : 0.f;
             if constexpr (T::WIDE)
