@@ -96,7 +96,8 @@ __device__ __forceinline__ double target_term(const Targets& t, int64_t row, int
   return (double)p * ((double)logf(p) - u + (double)log_sum);
 }
 
-// p_k = exp(t_k / tau - L), L = lse of the teacher's row where given, else over the row's entries.  Entries of a
+// p_k = exp(t_k / tau - L), L = lse of the teacher's row where given, else over the row's entries, whose largest is subtracted
+// before anything is scaled.  Entries of a
 // negative class or of value -inf carry nothing; a class that does not exist makes the row NaN.  One wave per row.
 __device__ __forceinline__ float top_targets(const int32_t* __restrict__ indices, const float* __restrict__ values,
                                             const float* __restrict__ lse, int64_t row, int classes, const Targets& t, int lane) {
@@ -107,22 +108,21 @@ __device__ __forceinline__ float top_targets(const int32_t* __restrict__ indices
   for (int k = lane; k < t.k; k += 64) {
     const bool have = at[k] >= 0 && val[k] != -INFINITY;
     any |= have;
-    if (have) top = fmaxf(top, val[k] * t.inv_tau);
+    if (have) top = fmaxf(top, val[k]);
   }
   const bool live = __any(any);
   top = wave_max_f32(top);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
   for (int k = lane; k < t.k; k += 64)
-    if (at[k] >= 0 && val[k] != -INFINITY) sum += expf(val[k] * t.inv_tau - ref);
+    if (at[k] >= 0 && val[k] != -INFINITY) sum += expf((val[k] - ref) * t.inv_tau);
   sum = wave_sum_f32(sum);
-  const float L = lse ? lse[row] : ref + logf(sum);
   float P = 0.f;
   for (int k = lane; k < t.k; k += 64) {
     const bool have = at[k] >= 0 && val[k] != -INFINITY;
     const bool good = at[k] < classes;
-    // without lse: exp(. - ref) / sum, which adds up to one to rounding
-    const float e = lse ? expf(val[k] * t.inv_tau - L) : expf(val[k] * t.inv_tau - ref) / sum;
+    // without lse: exp((. - ref) / tau) / sum, which adds up to one to rounding
+    const float e = lse ? expf(fmaf(val[k], t.inv_tau, -lse[row])) : expf((val[k] - ref) * t.inv_tau) / sum;
     const float p = !have ? 0.f : good ? e : NAN;
     t.at[row * t.k + k] = !have ? -1 : good ? at[k] : 0;
     t.p[row * t.k + k] = p;

@@ -29,6 +29,8 @@ def _check_logits(ops, z, values, indices, tau, reach, reduction='none'):
     """topk_distillation and its gradient; reach: the largest difference of two unmasked logits of a row."""
     n = z.shape[0]
     p, at, live = _targets(values=values, indices=indices, tau=tau)
+    t = (values.double() / tau).masked_fill((indices < 0) | (values == -math.inf), -math.inf)
+    p = torch.where(live[:, None], torch.softmax(t, 1), torch.zeros_like(p))  # log V is lost in a log-sum-exp of lowest values
     zg = z.cuda().requires_grad_()
     loss = ops.topk_distillation(zg, values.cuda(), indices.cuda(), temperature=tau, reduction=reduction)
     got, = torch.autograd.grad(loss.sum(), zg)
@@ -292,3 +294,24 @@ def test_more_tiles_of_a_product_than_one_launch_takes(ops, dt):
         z = h[part].double() @ w.double().t()
         want = torch.logsumexp(z, 1) - z.gather(1, y[part][:, None])[:, 0]
         assert torch.all((loss[part].double() - want).abs() <= 2.0 ** -18 + 2 * U * want + 8 * U * 32)
+
+
+@pytest.mark.parametrize('tau', [1.0, 0.5, 0.7])
+@pytest.mark.parametrize('shift', [1000.0, -1000.0, 'lowest'])
+def test_teachers_of_large_logits(ops, tau, shift):
+    """A teacher's distribution over its entries is one of their differences; entries all at the lowest value are alike."""
+    n, v, k = 40, 300, 70
+    g = torch.Generator().manual_seed(17)
+    values, indices = _top(n, k, v, g)
+    values = torch.full((n, k), torch.finfo(torch.float32).min) if shift == 'lowest' else 3 * values + shift
+    indices[3, 1:], indices[4, 60:] = -1, -1
+    reach = 0.0 if shift == 'lowest' else float((values.amax(1) - values.amin(1)).max())
+    for dt in TYPES:
+        z = torch.randn(n, v, generator=g).to(dt)
+        _check_logits(ops, z, values, indices, tau, max(10.0, reach))
+    # through a head: the same targets, logits that are exact
+    h, w = torch.randint(-1, 2, (n, 64), generator=g).float(), torch.randint(-1, 2, (v, 64), generator=g).float()
+    z = h @ w.t()
+    a = ops.linear_topk_distillation(h.cuda(), w.cuda(), values.cuda(), indices.cuda(), temperature=tau, reduction='none')
+    b = ops.topk_distillation(z.cuda(), values.cuda(), indices.cuda(), temperature=tau, reduction='none')
+    assert torch.isfinite(a).all() and torch.allclose(a, b, rtol=4 * U, atol=tau * tau * (2.0 ** -18 + 16 * U * 64 / tau))
