@@ -4,8 +4,9 @@ Tensors supply device memory and the current HIP stream; every computation below
 runs in libnif.so.  Inputs must live on a HIP device: there is no CPU path.
 """
 import ctypes
-
+import math
 import os
+
 import torch
 
 from . import _lib
@@ -998,6 +999,13 @@ def _same_device(what, first, *ts):
             raise ValueError(f'{what}: tensors are on different devices: {first.device} and {t.device}')
 
 
+def _check_sizes(what, rows, classes, features=1):
+    """The kernels' limits, before a size is handed on in 32 bits."""
+    if rows > 2 ** 30 or classes > 2 ** 28 or features > 2 ** 20 or rows * classes > 2 ** 43:
+        raise ValueError(f'{what}: at most 2^30 rows, 2^20 features, 2^28 classes and 2^43 logits, got {rows} rows'
+                         + (f' of {features} features' if features > 1 else '') + f' and {classes} classes')
+
+
 def _reduction(what, reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{what}: reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
@@ -1054,6 +1062,7 @@ def _check_head(what, hidden, weight, bias):
                          f'{tuple(hidden.shape)} and {tuple(weight.shape)}')
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f'{what}: bias has shape {tuple(bias.shape)} for {weight.shape[0]} classes')
+    _check_sizes(what, math.prod(hidden.shape[:-1]), *weight.shape)
 
 
 def _rows(t):
@@ -1126,6 +1135,7 @@ def topk_distillation(logits, top_values, top_indices, *, temperature=1.0, top_l
     if logits.dim() < 1 or logits.shape[-1] == 0:
         raise ValueError(f'{what}: logits must be [..., classes], got {tuple(logits.shape)}')
     lead = logits.shape[:-1]
+    _check_sizes(what, math.prod(lead), logits.shape[-1])
     _check_top(what, lead, top_values, top_indices, top_lse)
     _same_device(what, logits, top_values, top_indices, top_lse)
     loss = _lib.nif_torch.distill(_mat(_rows(logits), 'logits'), *_top_targets(top_values, top_indices, top_lse), temperature, reduction)
@@ -1145,8 +1155,9 @@ def top_logits(logits, k, *, temperature=1.0):
     temperature, k = _temperature(what, temperature), int(k)
     if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], _lib.NIF_TOP_MAX_K):
         raise ValueError(f'{what}: 1 to min(classes, {_lib.NIF_TOP_MAX_K}) top logits, got {k} of {tuple(logits.shape)}')
-    _same_device(what, logits)
     lead = logits.shape[:-1]
+    _check_sizes(what, math.prod(lead), logits.shape[-1])
+    _same_device(what, logits)
     z = _mat(_rows(logits.detach()), 'logits')
     values, indices, lse = _lib.nif_torch.top_logits(z, k, temperature)
     return values.reshape(*lead, k), indices.reshape(*lead, k), lse.reshape(lead)

@@ -27,3 +27,23 @@ def test_indices_of_every_integer_type_keep_their_classes(dt):
 def test_other_types_are_refused(call, dt):
     with pytest.raises((TypeError, ValueError), match='integers'):
         call(torch.zeros(2, 3, dtype=dt))
+
+
+def _wide(*shape):
+    return torch.zeros(1).expand(*shape)  # no memory behind it
+
+
+@pytest.mark.parametrize('call', [
+    lambda: ops.linear_cross_entropy(_wide(2, 1), _wide(2 ** 32 + 5, 1), torch.zeros(2, dtype=torch.int64)),
+    lambda: ops.linear_cross_entropy(_wide(2, 2 ** 32 + 8), _wide(5, 2 ** 32 + 8), torch.zeros(2, dtype=torch.int64)),
+    lambda: ops.linear_cross_entropy(_wide(2 ** 31, 8), W, torch.zeros(1, dtype=torch.int64).expand(2 ** 31)),
+    lambda: ops.linear_cross_entropy(_wide(2 ** 29, 8), _wide(2 ** 15, 8), torch.zeros(1, dtype=torch.int64).expand(2 ** 29)),
+    lambda: ops.linear_topk_distillation(_wide(2, 1), _wide(2 ** 28 + 1, 1), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.int32)),
+    lambda: ops.topk_distillation(_wide(2, 2 ** 32 + 5), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.int32)),
+    lambda: ops.topk_distillation(_wide(2 ** 31, 5), _wide(2 ** 31, 3), torch.zeros(1, dtype=torch.int32).expand(2 ** 31, 3)),
+    lambda: ops.top_logits(_wide(2, 2 ** 32 + 5), 3),
+    lambda: ops.top_logits(_wide(3, 2 ** 31, 5), 3)])
+def test_sizes_beyond_the_limits_are_refused(call):
+    """Not cut to 32 bits: 2^32 + 5 classes are not 5."""
+    with pytest.raises(ValueError, match='at most'):
+        call()
