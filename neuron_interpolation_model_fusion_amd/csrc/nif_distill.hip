@@ -549,7 +549,7 @@ extern "C" int nif_distill_forward(const void* logits, int64_t ld, int64_t rows,
   float* row_loss = reduction == NIF_REDUCE_NONE ? loss : (float*)ws;
   clear_err();
   if (rows > 0) {
-    // blocks of 512 where rows are few and long (256 x 131072 f32: 27 us to 36; 777 x 50001 f16: 25 to 20, with 1024 threads 36)
+    // blocks of 512 where rows are few and long (256 x 131072 f32: 28 us to 34; 777 x 50001 f16: 26 to 21, with 1024 threads 38)
     if (rows <= 256 && (int64_t)classes * (dtype == NIF_F32 ? 4 : 2) >= 96 << 10)
       NIF_BY_TYPE(dtype, hipLaunchKernelGGL((distill_rows_kernel<D, 512>), row_grid(rows), dim3(512), 0, st, logits, ld, rows, classes,
                                             t, top_indices, top_values, top_lse, (float*)((char*)state + s.top), (float*)((char*)state + s.sum), row_loss));

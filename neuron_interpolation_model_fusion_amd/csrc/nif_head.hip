@@ -1004,8 +1004,8 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
   }
 }
 
-// First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i] / (the row's sum of exponentials), and what the products of dz are multiplied with.  Where
-// one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
+// First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i] / (the row's sum of exponentials), and what the products of
+// dz are multiplied with.  Where one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
 // near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
 // the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  Where no row counts the arriving gradient is not read
 // (there may be none, and zeros stay zeros whatever it holds).  The other blocks: gradient 0 for rows without a target.
