@@ -503,7 +503,7 @@ int nif_lsq_solve_f64(const double* G, int64_t ldg, const double* R, int64_t ldr
  * 8 bytes a row for every 32 to 128 classes; backward pieces of 256 MiB, or of 1024 classes, of the logits' gradient.
  * Products accumulate in 32 bits; f32 operands are split into three bf16 parts (f32-level accuracy; an infinite one becomes
  * NaN, but for small heads: mask classes by the bias).  Of 16-bit operands the logits' gradient is rounded to their type
- * before its products.
+ * before its products, of up to 64 rows to two parts of that type.
  * `state` carries the forward pass's results to the backward pass, which needs the same inputs; the workspaces are
  * scratch of each call.  dhidden, dweight, dbias: of `dtype`, written in full; NULL where not wanted. */
 #define NIF_REDUCE_NONE 0

@@ -17,6 +17,9 @@
 // dz = coef * (P s) in 16 bits; the targets' entries are then rewritten with their -p; dW of the piece = dz^T hidden,
 // and dhidden += dz W.  Recomputing costs 8 n d v operations in place of 6 and saves n * v logits.
 //
+// Up to 64 rows of 16 bits dz is written in two 16-bit parts, the second behind the first's rows (`Plan::two`): what the
+// rounding of a few rows takes off does not average out.
+//
 // For few rows, where the product is bound by the weight's bytes or has too few tiles, up to 64 MiB of logits are kept in
 // 32 bits instead (head_kept_kernel).
 //
@@ -115,6 +118,7 @@ struct GemmArgs {
   const int* n_dev;
   int K;                // contraction length (at most *k_dev when given)
   const int* k_dev;
+  int two;              // not 0: the second part of dz lies so many rows behind the first, and K (if *k_dev is not 0) covers both
   int mt, nt, splits;
   int first, tiles;     // of this launch's, and all of them (tiles x splits)
   // EPI_STATS / EPI_DZ: the logit's last steps
@@ -257,6 +261,7 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
   const int mw = m0 + (EIGHT ? 8 : 4) * (lane >> 4), nw = n0 + (lane & 15);
   const auto m_of = [&](int i) { return mw + (EIGHT ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i); };
   static_assert(DZ_PAD % (16 * FI) == 0);
+  constexpr bool TWO_PARTS = EPI == EPI_DZ && !T::WIDE && FI == 2;  // tiles of 128 x 64, which such few rows take
   if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
     const float scale = g.inv_tau * (T::WIDE ? 1.f : 1.4426950408889634f);
     float bias[FI][4];  // -inf behind the last class
@@ -302,6 +307,24 @@ __device__ __forceinline__ void head_epilogue(const GemmArgs& g, f32x4 (&acc)[FI
         typedef typename std::conditional<T::WIDE, float, short>::type W;
         W* out = (W*)g.dz + (int64_t)n * g.ldz;
         constexpr int GROUP = EIGHT ? 2 : 1;
+        if constexpr (TWO_PARTS) {
+          if (g.two) {
+            if (n >= g.two) continue;
+#pragma unroll
+            for (int i = 0; i < FI; ++i) {
+              W hi[4], lo[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float x = live ? cp * head_exp<T>((acc[i][j][r] + bias[i][r] - top) * scale) : 0.f;
+                hi[r] = to16<T>(x);
+                lo[r] = to16<T>(x - (float)__builtin_bit_cast(typename T::t, hi[r]));
+              }
+              __builtin_memcpy(__builtin_assume_aligned(out + m_of(i), sizeof(hi)), hi, sizeof(hi));
+              __builtin_memcpy(__builtin_assume_aligned(out + (int64_t)g.two * g.ldz + m_of(i), sizeof(lo)), lo, sizeof(lo));
+            }
+            continue;
+          }
+        }
 #pragma unroll
         for (int i0 = 0; i0 < FI; i0 += GROUP) {
           W w[4 * GROUP];
@@ -416,7 +439,7 @@ __global__ __launch_bounds__(64 * WM * WN) void head_gemm_kernel(GemmArgs g) {
   const int m0 = tm * BM, n0 = tn * BN;
   // dz is an operand of the next products: rows up to a multiple of K_PAD are written, as zeros
   if (n0 >= (EPI == EPI_DZ ? (N + K_PAD - 1) / K_PAD * K_PAD : N)) return;
-  const int K = g.k_dev ? min(g.K, *g.k_dev) : g.K;
+  const int K = !g.k_dev ? g.K : g.two && *g.k_dev > 0 ? g.K : min(g.K, *g.k_dev);
   const int ktiles = (K + BK - 1) / BK;
   const int per = (ktiles + g.splits - 1) / g.splits;
   const int t0 = min(split * per, ktiles), t1 = min(t0 + per, ktiles);
@@ -730,7 +753,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_any_kernel(GemmArgs g) {
   const int N = g.n_dev ? min(g.N, *g.n_dev) : g.N;
   const int m0 = tm * BM, n0 = tn * BN;
   if (n0 >= N) return;
-  const int K = g.k_dev ? min(g.K, *g.k_dev) : g.K;
+  const int K = !g.k_dev ? g.K : g.two && *g.k_dev > 0 ? g.K : min(g.K, *g.k_dev);
   const int ktiles = (K + BK - 1) / BK;
   const int per = (ktiles + g.splits - 1) / g.splits;
   const int t0 = min(split * per, ktiles), t1 = min(t0 + per, ktiles);
@@ -912,7 +935,7 @@ __device__ __forceinline__ void target_dots(const typename Elem<DT>::t* h, const
 // Packs the hidden rows that count, a block each (rows behind the last one: zeros), and takes their targets' logits (zk; not
 // where the logits are kept).
 template <int DT>
-__global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int64_t all, int d,
+__global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restrict__ hidden, int64_t ldh, int64_t all, int two, int d,
                                                              const int* __restrict__ rows, const int* __restrict__ count,
                                                              void* __restrict__ dst, int ldd, const void* __restrict__ weight,
                                                              int64_t ldw, const void* __restrict__ bias, Targets tg,
@@ -920,11 +943,12 @@ __global__ __launch_bounds__(256) void head_pack_rows_kernel(const void* __restr
   typedef typename std::conditional<DT == NIF_F32, float, short>::type W;
   const int64_t i = row_block();
   if (i >= all) return;
-  const bool have = i < *count;
-  const int64_t src = have ? rows[i] : 0;
+  const int64_t row = two && i >= two && i < 2 * two ? i - two : i;  // once more for the second part of dz
+  const bool have = row < *count;
+  const int64_t src = have ? rows[row] : 0;
   const typename Elem<DT>::t* h = (const typename Elem<DT>::t*)hidden + src * ldh;
   pack_row<W>((const W*)h, have, d, (W*)dst + i * ldd, ldd);
-  if (!have || !zk) return;
+  if (!have || !zk || row != i) return;
   for (int k0 = (threadIdx.x >> 6) * DOTS; k0 < tg.k; k0 += 4 * DOTS)
     target_dots<DT>(h, weight, ldw, bias, d, tg, src, k0, zk + i * tg.k, threadIdx.x & 63);
 }
@@ -1051,10 +1075,10 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
 }
 
 // The targets' entries of a piece of dz: coef (P s - sum of the row's p with that class).  The first of equal classes
-// writes, with the sum over all of them in order.  One wave per packed row.
+// writes, with the sum over all of them in order; dz2: the second part, or null.  One wave per packed row.
 template <class W, class U>
 __device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U&& z_of, float top, float coef, float cp, int v0,
-                                               int v1, W* dz, int lane) {
+                                               int v1, W* dz, W* dz2, int lane) {
   const int* at = tg.at + src * tg.k;
   const float* p = tg.p + src * tg.k;
   for (int k0 = 0; k0 < tg.k; k0 += 64) {
@@ -1073,25 +1097,29 @@ __device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U
         sum += same ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pq), q)) : 0.f;
       }
     }
-    if (mine && first) dz[v - v0] = (W)(cp * expf((z_of(k, v) - top) * tg.inv_tau) - coef * sum);
+    if (mine && first) {
+      const float x = cp * expf((z_of(k, v) - top) * tg.inv_tau) - coef * sum;
+      dz[v - v0] = (W)x;
+      if (dz2) dz2[v - v0] = (W)(x - (float)(W)x);
+    }
   }
 }
 template <class T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
                                                            const float* __restrict__ zk, const float* __restrict__ tops,
                                                            const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
-                                                           typename T::t* __restrict__ dz, int64_t ldz) {
+                                                           typename T::t* __restrict__ dz, int64_t ldz, int two) {
   const int64_t i = row_block() * 4 + (threadIdx.x >> 6);
   if (i >= *count) return;
   target_entries(tg, rows[i], [&](int k, int) { return zk[i * tg.k + k]; }, tops[i], coef[i], cp[i], v0, v1, dz + i * ldz,
-                 threadIdx.x & 63);
+                 two ? dz + (i + two) * ldz : nullptr, threadIdx.x & 63);
 }
 
-// dbias of a piece: column sums of dz over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
+// dbias of a piece: column sums of dz (of both parts) over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
 // head_bias_join_kernel where there are several.  Bound by the read of dz (2048 x 32000 f16, 125 MB: 20 us).
 template <class T>
 __global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __restrict__ dz, int64_t ldz, int cols,
-                                                        const int* __restrict__ count, int stretch, float* __restrict__ part,
+                                                        const int* __restrict__ count, int two, int stretch, float* __restrict__ part,
                                                         const float* __restrict__ inv_scale, typename T::t* __restrict__ out) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   __shared__ float sh[8][256 + 8];
@@ -1103,6 +1131,12 @@ __global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __r
 #pragma unroll 4
     for (int r = r0 + group; r < r1; r += 8) {
       const Eight x = *(const Eight*)(dz + (int64_t)r * ldz + c0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += (float)x[e];
+    }
+  if (two && c0 < ldz)
+    for (int r = r0 + group; r < r1; r += 8) {
+      const Eight x = *(const Eight*)(dz + (int64_t)(r + two) * ldz + c0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] += (float)x[e];
     }
@@ -1201,38 +1235,47 @@ __global__ __launch_bounds__(256) void head_kept_kernel(const float* __restrict_
 }
 
 // dz = cp exp((z - top) / tau) of a piece of the classes, 8 a thread, and the targets' entries; zeros up to a multiple of K_PAD rows
-// and in the padding of the columns, where the products read them.  Rounded as head_gemm_kernel's.
+// and in the padding of the columns, where the products read them.  Rounded as head_gemm_kernel's, or in two parts.
 constexpr int KEPT_DZ = 2048;
 template <class T>
 __global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ z, int64_t ldu, int v0, int cols, Targets tg,
                                                            const int* __restrict__ rows, const int* __restrict__ count,
                                                            const float* __restrict__ tops, const float* __restrict__ coef,
-                                                           const float* __restrict__ cp, typename T::t* dz, int64_t ldz) {
+                                                           const float* __restrict__ cp, typename T::t* dz, int64_t ldz, int two) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   const int n = *count, c0 = blockIdx.y * KEPT_DZ, c = c0 + threadIdx.x * 8;
   const int64_t i = blockIdx.x;
-  if (i >= (n + K_PAD - 1) / K_PAD * K_PAD) return;
+  if (i >= (two ? two : (n + K_PAD - 1) / K_PAD * K_PAD)) return;
   const bool live = i < n;
   const float top = live ? tops[i] : 0.f, k = live ? cp[i] : 0.f;
-  const auto one = [&](float x) { return (typename T::t)(k * expf((x - top) * tg.inv_tau)); };
+  const auto one = [&](float x) { return k * expf((x - top) * tg.inv_tau); };
   if (c < ldz) {
-    Eight w;
+    float y[8];
     const float* x = z + i * ldu + v0 + c;
     if (live && c + 8 <= cols) {
       const f32x4 lo = *(const f32x4*)x, hi = *(const f32x4*)(x + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = one(e < 4 ? lo[e & 3] : hi[e & 3]);
+      for (int e = 0; e < 8; ++e) y[e] = one(e < 4 ? lo[e & 3] : hi[e & 3]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = live && c + e < cols ? one(x[e]) : (typename T::t)0.f;
+      for (int e = 0; e < 8; ++e) y[e] = live && c + e < cols ? one(x[e]) : 0.f;
     }
+    Eight w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = (typename T::t)y[e];
     *(Eight*)(dz + i * ldz + c) = w;
+    if (two) {
+      Eight w2;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w2[e] = (typename T::t)(y[e] - (float)w[e]);
+      *(Eight*)(dz + (i + two) * ldz + c) = w2;
+    }
   }
   if (!live) return;
   __syncthreads();  // the entries are stored again behind the others
   if (threadIdx.x < 64)
     target_entries(tg, rows[i], [&](int, int v) { return z[i * ldu + v]; }, top, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ),
-                   dz + i * ldz + c0, threadIdx.x);
+                   dz + i * ldz + c0, two ? dz + (i + two) * ldz + c0 : nullptr, threadIdx.x);
 }
 
 // ---- small heads ----------------------------------------------------------------------------------------------
@@ -1422,11 +1465,18 @@ struct Plan {
   bool any_f, any_b, pack_f, pack_b;
   bool small;        // the small heads' kernels
   bool keep;         // few rows: the logits are kept
+  int two;           // very few rows of 16 bits: dz in two parts, so many rows apart; else 0
   int piece;         // classes per piece (multiple of 256, or all)
   // state: what the backward pass reads
   size_t s_p, s_at, s_P, s_dz, s_rows, s_inv, s_count, s_top, s_sum, s_zk, s_h, s_z, state;
   int64_t ldu;       // of the kept logits
 };
+
+// Rows up to which dz has two parts.  One rounding more of each element is 1.4 times the error where many count alike, but up
+// to 2.3 times where few do (1 x 64 x 110210 bf16, 13 targets: dweight 1.7e-3 -> 3.0e-3 of its norm; in two parts 1.7e-3).
+// For so few rows the products are bound by the weight's bytes and pad their rows to 32 or 64 anyway: a step of 2048 x 131072
+// bf16 takes 475 -> 477 us with 1 row, 492 -> 509 with 32, 521 -> 559 with 64; 2050 x 100001 485 -> 508, 520 -> 535, 548 -> 620.
+static constexpr int TWO_ROWS = 64;
 
 static constexpr size_t PIECE_BYTES = (size_t)256 << 20;
 
@@ -1522,6 +1572,7 @@ static bool make_plan(const nif_head_desc* h, Plan& p) {
   const bool odd = p.e == 2 && (p.d % 8 != 0 || h->ldw % 8 != 0 || ((uintptr_t)h->weight & 15) != 0);
   const bool far = h->ldw > HEAD_MAX_LD;
   p.any_f = p.e == 4 || (odd && !far && p.n <= ANY_ROWS_F);
+  p.two = p.e == 4 || p.n == 0 || p.n > TWO_ROWS ? 0 : p.n <= 16 ? 16 : p.n <= 32 ? 32 : TWO_ROWS;
   p.any_b = p.e == 4 || (odd && !far && p.n <= ANY_ROWS_B);
   p.pack_f = far || (odd && !p.any_f);
   p.pack_b = far || (odd && !p.any_b);
@@ -1678,13 +1729,13 @@ static void forward_products(const nif_head_desc* h, const Plan& p, char* state,
 
 template <int DT>
 static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStream_t st) {
-  hipLaunchKernelGGL(head_pack_rows_kernel<DT>, row_grid(p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.cap, p.d,
+  hipLaunchKernelGGL(head_pack_rows_kernel<DT>, row_grid(p.cap), dim3(256), 0, st, h->hidden, h->ldh, p.cap, p.two, p.d,
                      (const int*)(state + p.s_rows), (const int*)(state + p.s_count), state + p.s_h, p.ldd, h->weight, h->ldw, h->bias, targets_of(h, p, state), p.keep ? nullptr : (float*)(state + p.s_zk));
 }
 
 struct BwdSpace {
   size_t coef, cp, scale, dz, w, acc, part, bytes;
-  int64_t ldz, dh_ld;
+  int64_t ldz, dh_ld, part_rows;  // part_rows: of a split's partial sums of dhidden
   int stretch;
   Shape dh, dw;
 };
@@ -1692,8 +1743,11 @@ static BwdSpace backward_space(const Plan& p) {
   BwdSpace b;
   b.ldz = round_up(p.piece, DZ_PAD);
   b.dh_ld = round_up(p.d, 4);
-  b.dh = shape_of(DHIDDEN, p.d, p.n, p.piece, p.e, p.e, true, p.any_b);
-  b.dw = shape_of(DWEIGHT, p.d, p.piece, p.n, p.e, p.e, true, false);
+  // Two parts: each in tiles of its own where the weight goes through registers (a step of 48 x 2050 x 100001 bf16: 600 us, in
+  // 128 x 128 tiles over both 711).
+  const int64_t rows = p.two ? 2 * p.two : p.n;
+  b.dh = shape_of(DHIDDEN, p.d, p.two && p.any_b ? p.two : rows, p.piece, p.e, p.e, true, p.any_b);
+  b.dw = shape_of(DWEIGHT, p.d, p.piece, rows, p.e, p.e, true, false);
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
@@ -1701,7 +1755,8 @@ static BwdSpace backward_space(const Plan& p) {
   b.dz = take(at, (size_t)p.cap * b.ldz * p.e);
   b.w = take(at, p.pack_b ? (size_t)p.piece * p.ldd * p.e : 0);
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
-  const size_t part_h = b.dh.splits > 1 ? (size_t)b.dh.splits * p.cap * b.dh_ld * 4 : 0;
+  b.part_rows = p.two ? 2 * p.two : p.cap;
+  const size_t part_h = b.dh.splits > 1 || p.two ? (size_t)b.dh.splits * b.part_rows * b.dh_ld * 4 : 0;
   const size_t part_w = b.dw.splits > 1 ? (size_t)b.dw.splits * p.piece * b.dh_ld * 4 : 0;
   b.stretch = p.n <= 64 ? 64 : 32;  // rows of a block of column sums: the fewest that leave at most 2048 blocks, up to 256
   while (b.stretch < 256 && (p.n + b.stretch - 1) / b.stretch * ((p.piece + 255) / 256) > 2048) b.stretch *= 2;
@@ -1737,7 +1792,8 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     const int kz = p.any_b ? vc : (int)round_up(vc, K_PAD);  // the contraction over the piece's columns of dz
     if (p.keep) {
       hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + KEPT_DZ - 1) / KEPT_DZ)), dim3(256),
-                         0, st, (const float*)(state + p.s_z), p.ldu, v0, vc, tg, rows, count, tops, coef, cp, dz, b.ldz);
+                         0, st, (const float*)(state + p.s_z), p.ldu, v0, vc, tg, rows, count, tops, coef, cp, dz, b.ldz,
+                         p.two);
     } else {
       GemmArgs g = {};
       g.A = w;
@@ -1753,16 +1809,17 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.cp = cp;
       g.dz = dz;
       g.ldz = b.ldz;
-      run_gemm<T, false, false, EPI_DZ>(logit_shape(p, vc, p.any_b), g, st);
+      g.two = p.two;
+      run_gemm<T, false, false, EPI_DZ>(p.two ? Shape{p.any_b, 128, 64, 4, 1, 0.f} : logit_shape(p, vc, p.any_b), g, st);
     }
     if (p.n > 0 && !p.keep)
       hipLaunchKernelGGL(head_targets_kernel<T>, row_grid((p.n + 3) / 4), dim3(256), 0, st, tg, rows, count, zk, tops, coef, cp, v0,
-                       v0 + vc, dz, b.ldz);
+                       v0 + vc, dz, b.ldz, p.two);
     if (dbias) {
       W* out = (W*)dbias + v0;
       const unsigned stretches = (unsigned)((p.n + b.stretch - 1) / b.stretch);
       if (p.n > 0)
-        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, stretches), dim3(256), 0, st, dz, b.ldz, vc, count, b.stretch, part,
+        hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, stretches), dim3(256), 0, st, dz, b.ldz, vc, count, p.two, b.stretch, part,
                            inv_scale, out);
       if (stretches != 1)
         hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale, out);
@@ -1773,8 +1830,9 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.B = Side{dz, b.ldz, (int)round_up(vc, K_PAD), (int)p.cap};
       g.M = p.d;
       g.N = vc;
-      g.K = (int)p.cap;
+      g.K = p.two ? 2 * p.two : (int)p.cap;
       g.k_dev = count;
+      g.two = p.two;
       g.splits = b.dw.splits;
       g.out = (char*)dweight + (size_t)v0 * lddw * (f32 ? 4 : 2);
       g.out_ld = lddw;
@@ -1798,27 +1856,28 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
       g.A.rlim = p.pack_b ? p.ldd : p.d;
       g.B = Side{dz, b.ldz, (int)p.cap, kz};
       g.M = p.d;
-      g.N = (int)p.n;
-      g.n_dev = count;
+      g.N = p.two ? 2 * p.two : (int)p.n;
+      g.n_dev = p.two ? nullptr : count;
       g.K = kz;
       g.splits = b.dh.splits;
       g.out = dhidden;
       g.out_ld = lddh;
       g.rowmap = rows;
       g.inv_scale = inv_scale;
-      if (g.splits > 1) {
+      const bool join = g.splits > 1 || p.two;  // the two parts' results are joined like splits, of which they are two each
+      if (join) {
         g.out_kind = OUT_F32;
         g.acc = part;
-        g.acc_split = p.cap * b.dh_ld;
+        g.acc_split = b.part_rows * b.dh_ld;
       } else {
         g.out_kind = last ? OUT_FINAL : first ? OUT_F32 : OUT_ADD;
         g.acc = first && last ? nullptr : acc;
       }
       g.acc_ld = b.dh_ld;
       run_gemm<T, true, false, EPI_OUT>(b.dh, g, st);
-      if (g.splits > 1 && p.n > 0)
-        hipLaunchKernelGGL(head_join_kernel<T>, row_grid(p.n, (p.d + 1023) / 1024), dim3(256), 0, st, part, g.splits, g.acc_split,
-                           b.dh_ld, (int)p.n, count, p.d, acc, first, last, dhidden, lddh, rows, inv_scale);
+      if (join && p.n > 0)
+        hipLaunchKernelGGL(head_join_kernel<T>, row_grid(p.n, (p.d + 1023) / 1024), dim3(256), 0, st, part,
+                           p.two ? 2 * g.splits : g.splits, p.two ? p.two * b.dh_ld : g.acc_split, b.dh_ld, (int)p.n, count, p.d, acc, first, last, dhidden, lddh, rows, inv_scale);
     }
   }
 }

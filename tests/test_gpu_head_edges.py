@@ -315,3 +315,46 @@ def test_teachers_of_large_logits(ops, tau, shift):
     a = ops.linear_topk_distillation(h.cuda(), w.cuda(), values.cuda(), indices.cuda(), temperature=tau, reduction='none')
     b = ops.topk_distillation(z.cuda(), values.cuda(), indices.cuda(), temperature=tau, reduction='none')
     assert torch.isfinite(a).all() and torch.allclose(a, b, rtol=4 * U, atol=tau * tau * (2.0 ** -18 + 16 * U * 64 / tau))
+
+
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('k', [None, 1, 13])
+@pytest.mark.parametrize('n, d, v', [(1, 64, 11021), (2, 72, 30011), (5, 67, 9001), (31, 264, 9001), (32, 64, 5003), (33, 40, 9001),
+                                     (64, 520, 4099), (60, 131, 3001), (16, 8, 300011), (64, 16, 300001)])
+@pytest.mark.parametrize('reduction', ['mean', 'none'])
+def test_gradients_of_few_rows_are_rounded_once(ops, dt, k, n, d, v, reduction):
+    """The roundings of a few rows' logit gradients would not average out: they are held in two 16-bit parts, together at
+    least 2^-16 (2^-21) of them, with and without kept logits, in one piece and in several."""
+    g = torch.Generator().manual_seed(n + d + v)
+    h, w = torch.randn(n, d, generator=g).to(dt), (torch.randn(v, d, generator=g) * 2 / math.sqrt(d)).to(dt)
+    b = torch.randn(v, generator=g).to(dt)
+    if k is None:
+        y = torch.randint(0, v, (n,), generator=g)
+        if n > 3:
+            y[1] = -100
+        p, at, live = _targets(labels=y)
+    else:
+        values, indices = _top(n, k, v, g)
+        if n > 3:
+            indices[1] = -1
+        p, at, live = _targets(values=values, indices=indices, tau=2.0)
+    tau = 1.0 if k is None else 2.0
+    up = torch.rand(n, generator=g) + 0.5 if reduction == 'none' else torch.ones(n)
+    hg, wg, bg = (t.cuda().requires_grad_() for t in (h, w, b))
+    if k is None:
+        loss = ops.linear_cross_entropy(hg, wg, y.cuda(), bg, reduction=reduction)
+    else:
+        loss = ops.linear_topk_distillation(hg, wg, values.cuda(), indices.cuda(), bg, temperature=tau, reduction=reduction)
+    got = torch.autograd.grad(loss, (hg, wg, bg), grad_outputs=up.cuda() if reduction == 'none' else torch.ones_like(loss))
+    h, w = h.double(), w.double()
+    z = h @ w.t() + b.double()
+    _, _, dz, q, coef = _formula(z, p, at, live, tau, reduction, up)
+    A = (h.abs() @ w.abs().t() + b.double().abs()).amax(1, keepdim=True)
+    cq = coef * q * (2 * (d + 8) * U * A / tau + 2.0 ** -18 + U16[dt] ** 2)  # logits, exponentials, the two parts
+    lost = coef.max() * 2.0 ** -37 if dt == torch.float16 else 0.0  # f16: subnormals of the scaled parts
+    for x, ref, size, length, floor in ((got[0], dz @ w, (cq @ w.abs()), v, w.abs().sum(0)), (got[1], dz.t() @ h, cq.t() @ h.abs(), n, h.abs().sum(0)),
+                                        (got[2], dz.sum(0), cq.sum(0), n, torch.tensor(float(n)))):
+        terms = (coef * q) @ w.abs() if length == v else (coef * q).t() @ h.abs() if ref.dim() == 2 else (coef * q).sum(0)
+        bound = U16[dt] * ref.abs() * (1 + 2.0 ** -8) + size + (length + 64) * U * terms + lost * floor + (2.0 ** -25 if dt == torch.float16 else 1e-37)
+        off = (x.cpu().double() - ref).abs()
+        assert torch.all(off <= bound), float((off / bound).max())
