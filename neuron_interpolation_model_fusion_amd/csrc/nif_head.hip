@@ -1032,14 +1032,20 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
 // dz are multiplied with.  Where one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
 // near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
 // the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  Where no row counts the arriving gradient is not read
-// (there may be none, and zeros stay zeros whatever it holds).  The other blocks: gradient 0 for rows without a target.
+// (there may be none, and zeros stay zeros whatever it holds).  inv_scale[1]: the power of two that takes that largest one
+// to [2^37, 2^38), for `rest`.  The other blocks: gradient 0 for rows without a target, and `rest` cleared.
 template <typename W>
 __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict__ grad, int per_row, int mean, Targets tg,
                                                          const int* __restrict__ rows, const int* __restrict__ inv,
                                                          const int* __restrict__ count, const float* __restrict__ sums, int64_t rows_all,
                                                          int f16, float* __restrict__ coef,
                                                          float* __restrict__ cp, float* __restrict__ inv_scale, W* __restrict__ out,
-                                                         int64_t ld, int d) {
+                                                         int64_t ld, int d, int64_t clearing, long long* __restrict__ rest, int classes) {
+  if (row_block() > clearing) {
+    const int64_t c = (row_block() - 1 - clearing) * 1024 + threadIdx.x;
+    if (rest && c < classes) rest[c] = 0;
+    return;
+  }
   if (row_block() > 0) {
     const int64_t r = (row_block() - 1) * 4 + (threadIdx.x >> 8);
     if (r < rows_all && inv[r] < 0)
@@ -1050,7 +1056,7 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
   const int n = *count;
   const float w = tg.tau * (mean ? 1.f / max(1, n) : 1.f), all = per_row || n == 0 ? 1.f : grad[0] * w;
   float scale = 1.f;
-  if (f16) {
+  if (f16 || rest) {
     float top = 0.f;
     for (int i = threadIdx.x; i < n; i += 1024) {
       const float c = (per_row ? fabsf(grad[rows[i]] * w) : 1.f) * fmaxf(1.f, tg.P[rows[i]]);
@@ -1060,11 +1066,12 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
     __syncthreads();
     for (int v = 0; v < 16; ++v) top = fmaxf(top, sh[v]);
+    int e = 0;
     if (top > 0.f && top < INFINITY) {
-      int e;
       frexpf(top, &e);  // top in [2^(e-1), 2^e)
-      scale = ldexpf(1.f, max(-100, min(100, 14 - e)));
+      if (f16) scale = ldexpf(1.f, max(-100, min(100, 14 - e)));
     }
+    if (threadIdx.x == 0) inv_scale[1] = ldexpf(1.f, max(-100, min(100, 38 - (f16 ? 14 : e))));
   }
   if (threadIdx.x == 0) *inv_scale = all / scale;
   for (int i = threadIdx.x; i < n; i += 1024) {
@@ -1075,10 +1082,11 @@ __global__ __launch_bounds__(1024) void head_coef_kernel(const float* __restrict
 }
 
 // The targets' entries of a piece of dz: coef (P s - sum of the row's p with that class).  The first of equal classes
-// writes, with the sum over all of them in order; dz2: the second part, or null.  One wave per packed row.
+// writes, with the sum over all of them in order; dz2: the second part, or null.  rest: what the rounding takes off, for
+// dbias, added up over the rows in whole numbers of 1 / fix (whose order does not matter), or null.  One wave per packed row.
 template <class W, class U>
 __device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U&& z_of, float top, float coef, float cp, int v0,
-                                               int v1, W* dz, W* dz2, int lane) {
+                                               int v1, W* dz, W* dz2, long long* rest, float fix, int lane) {
   const int* at = tg.at + src * tg.k;
   const float* p = tg.p + src * tg.k;
   for (int k0 = 0; k0 < tg.k; k0 += 64) {
@@ -1101,6 +1109,10 @@ __device__ __forceinline__ void target_entries(const Targets& tg, int64_t src, U
       const float x = cp * expf((z_of(k, v) - top) * tg.inv_tau) - coef * sum;
       dz[v - v0] = (W)x;
       if (dz2) dz2[v - v0] = (W)(x - (float)(W)x);
+      if (rest) {
+        const float r = (x - (float)(W)x) * fix;
+        if (fabsf(r) < 0x1p40f) atomicAdd((unsigned long long*)(rest + v - v0), (unsigned long long)llrintf(r));  // not NaN or inf
+      }
     }
   }
 }
@@ -1108,19 +1120,28 @@ template <class T>
 __global__ __launch_bounds__(256) void head_targets_kernel(Targets tg, const int* __restrict__ rows, const int* __restrict__ count,
                                                            const float* __restrict__ zk, const float* __restrict__ tops,
                                                            const float* __restrict__ coef, const float* __restrict__ cp, int v0, int v1,
-                                                           typename T::t* __restrict__ dz, int64_t ldz, int two) {
+                                                           typename T::t* __restrict__ dz, int64_t ldz, int two, long long* rest,
+                                                           const float* __restrict__ inv_scale) {
   const int64_t i = row_block() * 4 + (threadIdx.x >> 6);
   if (i >= *count) return;
   target_entries(tg, rows[i], [&](int k, int) { return zk[i * tg.k + k]; }, tops[i], coef[i], cp[i], v0, v1, dz + i * ldz,
-                 two ? dz + (i + two) * ldz : nullptr, threadIdx.x & 63);
+                 two ? dz + (i + two) * ldz : nullptr, rest, inv_scale[1], threadIdx.x & 63);
 }
 
-// dbias of a piece: column sums of dz (of both parts) over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
+// dbias of a piece: column sums of dz (of both parts, or with what the targets' entries lost, `rest`, which is left cleared for
+// the next piece) over stretches of packed rows (256 columns a block, 8 a thread), joined in order by
 // head_bias_join_kernel where there are several.  Bound by the read of dz (2048 x 32000 f16, 125 MB: 20 us).
+__device__ __forceinline__ float take_rest(long long* rest, int c, const float* inv_scale) {
+  if (!rest) return 0.f;
+  const long long r = rest[c];
+  rest[c] = 0;
+  return (float)((double)r / (double)inv_scale[1]);
+}
 template <class T>
 __global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __restrict__ dz, int64_t ldz, int cols,
                                                         const int* __restrict__ count, int two, int stretch, float* __restrict__ part,
-                                                        const float* __restrict__ inv_scale, typename T::t* __restrict__ out) {
+                                                        const float* __restrict__ inv_scale, typename T::t* __restrict__ out,
+                                                        long long* __restrict__ rest) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   __shared__ float sh[8][256 + 8];
   const int c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8, group = threadIdx.x >> 5;
@@ -1151,17 +1172,19 @@ __global__ __launch_bounds__(256) void head_bias_kernel(const typename T::t* __r
   if (gridDim.y > 1)
     part[(int64_t)blockIdx.y * cols + c] = sum;
   else
-    out[c] = (typename T::t)(sum * *inv_scale);
+    out[c] = (typename T::t)((sum + take_rest(rest, c, inv_scale)) * *inv_scale);
 }
 template <class T>
 __global__ __launch_bounds__(256) void head_bias_join_kernel(const float* __restrict__ part, int cols, const int* __restrict__ count, int stretch,
-                                                             const float* __restrict__ inv_scale, void* __restrict__ out) {
+                                                             const float* __restrict__ inv_scale, void* __restrict__ out,
+                                                             long long* __restrict__ rest) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   const int stretches = (*count + stretch - 1) / stretch;
   float s = 0.f;
 #pragma unroll 8
   for (int q = 0; q < stretches; ++q) s += part[(int64_t)q * cols + c];
+  s += take_rest(rest, c, inv_scale);
   s *= *inv_scale;
   ((typename T::t*)out)[c] = (typename T::t)s;
 }
@@ -1241,7 +1264,8 @@ template <class T>
 __global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restrict__ z, int64_t ldu, int v0, int cols, Targets tg,
                                                            const int* __restrict__ rows, const int* __restrict__ count,
                                                            const float* __restrict__ tops, const float* __restrict__ coef,
-                                                           const float* __restrict__ cp, typename T::t* dz, int64_t ldz, int two) {
+                                                           const float* __restrict__ cp, typename T::t* dz, int64_t ldz, int two,
+                                                           long long* rest, const float* __restrict__ inv_scale) {
   typedef __attribute__((ext_vector_type(8))) typename T::t Eight;
   const int n = *count, c0 = blockIdx.y * KEPT_DZ, c = c0 + threadIdx.x * 8;
   const int64_t i = blockIdx.x;
@@ -1275,7 +1299,8 @@ __global__ __launch_bounds__(256) void head_kept_dz_kernel(const float* __restri
   __syncthreads();  // the entries are stored again behind the others
   if (threadIdx.x < 64)
     target_entries(tg, rows[i], [&](int, int v) { return z[i * ldu + v]; }, top, coef[i], k, v0 + c0, v0 + min(cols, c0 + KEPT_DZ),
-                   dz + i * ldz + c0, two ? dz + (i + two) * ldz + c0 : nullptr, threadIdx.x);
+                   dz + i * ldz + c0, two ? dz + (i + two) * ldz + c0 : nullptr, rest ? rest + c0 : nullptr,
+                   inv_scale[1], threadIdx.x);
 }
 
 // ---- small heads ----------------------------------------------------------------------------------------------
@@ -1734,7 +1759,7 @@ static void pack_rows(const nif_head_desc* h, const Plan& p, char* state, hipStr
 }
 
 struct BwdSpace {
-  size_t coef, cp, scale, dz, w, acc, part, bytes;
+  size_t coef, cp, scale, dz, w, acc, part, rest, bytes;
   int64_t ldz, dh_ld, part_rows;  // part_rows: of a split's partial sums of dhidden
   int stretch;
   Shape dh, dw;
@@ -1751,7 +1776,7 @@ static BwdSpace backward_space(const Plan& p) {
   size_t at = 0;
   b.coef = take(at, (size_t)p.cap * 4);
   b.cp = take(at, (size_t)p.cap * 4);
-  b.scale = take(at, 4);
+  b.scale = take(at, 8);
   b.dz = take(at, (size_t)p.cap * b.ldz * p.e);
   b.w = take(at, p.pack_b ? (size_t)p.piece * p.ldd * p.e : 0);
   b.acc = take(at, p.piece < p.v ? (size_t)p.cap * b.dh_ld * 4 : 0);
@@ -1764,8 +1789,14 @@ static BwdSpace backward_space(const Plan& p) {
   const size_t part_b = (size_t)((p.n + b.stretch - 1) / b.stretch) * p.piece * 4;
   const size_t part = part_h > part_w ? part_h : part_w;
   b.part = take(at, part > part_b ? part : part_b);
+  b.rest = take(at, p.e == 2 && !p.two ? (size_t)p.piece * 8 : 0);
   b.bytes = at;
   return b;
+}
+
+// where dbias keeps what the rounding of dz takes off the targets' entries; null where there is no need
+static long long* rest_of(const Plan& p, const BwdSpace& b, char* ws, const void* dbias) {
+  return dbias && p.e == 2 && !p.two ? (long long*)(ws + b.rest) : nullptr;
 }
 
 template <class T>
@@ -1784,6 +1815,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
   W* dz = (W*)(ws + b.dz);
   float* acc = (float*)(ws + b.acc);
   float* part = (float*)(ws + b.part);
+  long long* rest = rest_of(p, b, ws, dbias);
   const int f32 = h->dtype == NIF_F32;
   for (int v0 = 0; v0 < p.v; v0 += p.piece) {
     const int vc = p.v - v0 < p.piece ? p.v - v0 : p.piece;
@@ -1793,7 +1825,7 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     if (p.keep) {
       hipLaunchKernelGGL(head_kept_dz_kernel<T>, dim3((unsigned)round_up(p.n, K_PAD), (unsigned)((b.ldz + KEPT_DZ - 1) / KEPT_DZ)), dim3(256),
                          0, st, (const float*)(state + p.s_z), p.ldu, v0, vc, tg, rows, count, tops, coef, cp, dz, b.ldz,
-                         p.two);
+                         p.two, rest, inv_scale);
     } else {
       GemmArgs g = {};
       g.A = w;
@@ -1814,15 +1846,15 @@ static void backward_products(const nif_head_desc* h, const Plan& p, const char*
     }
     if (p.n > 0 && !p.keep)
       hipLaunchKernelGGL(head_targets_kernel<T>, row_grid((p.n + 3) / 4), dim3(256), 0, st, tg, rows, count, zk, tops, coef, cp, v0,
-                       v0 + vc, dz, b.ldz, p.two);
+                       v0 + vc, dz, b.ldz, p.two, rest, inv_scale);
     if (dbias) {
       W* out = (W*)dbias + v0;
       const unsigned stretches = (unsigned)((p.n + b.stretch - 1) / b.stretch);
       if (p.n > 0)
         hipLaunchKernelGGL(head_bias_kernel<T>, dim3((vc + 255) / 256, stretches), dim3(256), 0, st, dz, b.ldz, vc, count, p.two, b.stretch, part,
-                           inv_scale, out);
+                           inv_scale, out, rest);
       if (stretches != 1)
-        hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale, out);
+        hipLaunchKernelGGL(head_bias_join_kernel<T>, dim3((vc + 255) / 256), dim3(256), 0, st, part, vc, count, b.stretch, inv_scale, out, rest);
     }
     if (dweight) {  // [classes of the piece][features] = dz^T hidden, contraction over the packed rows
       GemmArgs g = {};
@@ -2028,10 +2060,11 @@ extern "C" int nif_head_backward(const nif_head_desc* h, const float* grad_loss,
   const BwdSpace b = backward_space(p);
   const auto prepare = [&](auto* out) {
     const int64_t clearing = out && p.n > 0 ? (p.n + 3) / 4 : 0;
-    hipLaunchKernelGGL(head_coef_kernel, row_grid(1 + clearing), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
+    long long* rest = rest_of(p, b, (char*)ws, dbias);
+    hipLaunchKernelGGL(head_coef_kernel, row_grid(1 + clearing + (rest ? (p.piece + 1023) / 1024 : 0)), dim3(1024), 0, st, grad_loss, h->reduction == NIF_REDUCE_NONE,
                        h->reduction == NIF_REDUCE_MEAN, targets_of(h, p, (char*)s), (const int*)(s + p.s_rows), (const int*)(s + p.s_inv),
                        (const int*)(s + p.s_count), (const float*)(s + p.s_sum), p.n, h->dtype == NIF_F16, (float*)((char*)ws + b.coef), (float*)((char*)ws + b.cp),
-                       (float*)((char*)ws + b.scale), out, lddh, p.d);
+                       (float*)((char*)ws + b.scale), out, lddh, p.d, clearing, rest, p.piece);
   };
   if (h->dtype == NIF_F32)
     prepare((float*)dhidden);

@@ -358,3 +358,45 @@ def test_gradients_of_few_rows_are_rounded_once(ops, dt, k, n, d, v, reduction):
         bound = U16[dt] * ref.abs() * (1 + 2.0 ** -8) + size + (length + 64) * U * terms + lost * floor + (2.0 ** -25 if dt == torch.float16 else 1e-37)
         off = (x.cpu().double() - ref).abs()
         assert torch.all(off <= bound), float((off / bound).max())
+
+
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('reduction', ['mean', 'none'])
+@pytest.mark.parametrize('n, d, v, k', [(65, 64, 9001, 13), (200, 72, 300, 8), (130, 40, 60001, 100), (700, 67, 3001, 2), (2100, 64, 520, None),
+                                        (600, 64, 700, 9), (1500, 16, 500001, 5)])
+def test_the_bias_gradient_keeps_what_its_targets_entries_round_off(ops, dt, reduction, n, d, v, k):
+    """A class has few targets, so their entries' rounding does not average out in its column sum: it is added back.  What is
+    left is that of the P s of every row, and the entries' own without it where a target falls."""
+    g = torch.Generator(device='cuda').manual_seed(n + v)
+    h = torch.randn(n, d, generator=g, device='cuda').to(dt)
+    w = (torch.randn(v, d, generator=g, device='cuda') / math.sqrt(d)).to(dt)
+    b = torch.zeros(v, dtype=dt, device='cuda').requires_grad_()
+    tau = 1.0 if k is None else 2.0
+    up = torch.rand(n, generator=g, device='cuda') + 0.5 if reduction == 'none' else None
+    if k is None:
+        y = torch.randint(0, v, (n,), generator=g, device='cuda')
+        at, p = y[:, None], torch.ones(n, 1, device='cuda').double()
+        loss = ops.linear_cross_entropy(h, w, y, b, reduction=reduction)
+    else:
+        values = 2 * torch.randn(n, k, generator=g, device='cuda')
+        at = (torch.randint(0, v, (n, 1), generator=g, device='cuda') + torch.arange(k, device='cuda') * max(1, v // k)) % v
+        p = torch.softmax(values.double() / tau, 1)
+        loss = ops.linear_topk_distillation(h, w, values, at, b, temperature=tau, reduction=reduction)
+    for _ in range(2):  # the second pass finds the buffers of the first
+        got, = torch.autograd.grad(loss, b, grad_outputs=up if reduction == 'none' else torch.ones_like(loss), retain_graph=True)
+    c = tau * (up.double() if reduction == 'none' else torch.full((n,), 1.0 / n, device='cuda').double())
+    ref, left, q, terms = (torch.zeros(v, dtype=torch.float64, device='cuda') for _ in range(4))
+    for lo in range(0, n, 100):
+        part = slice(lo, min(n, lo + 100))
+        z = (h[part].double() @ w.double().t()) / tau
+        s = torch.softmax(z, 1) * c[part, None]
+        A = (h[part].double().abs() @ w.double().abs().t()).amax(1, keepdim=True)
+        cp = c[part, None] * p[part]
+        q += (s * (2 * (d + 8) * U * A / tau + 2.0 ** -18)).sum(0) + 2.0 ** -18 * torch.zeros_like(ref).index_add_(0, at[part].reshape(-1), cp.reshape(-1))
+        ref += s.sum(0).index_add_(0, at[part].reshape(-1), -cp.reshape(-1))
+        left += s.scatter(1, at[part], 0.0).sum(0)
+        terms += s.sum(0).index_add_(0, at[part].reshape(-1), cp.reshape(-1))
+    bound = U16[dt] * (1 + 2.0 ** -8) * (ref.abs() + left) + q + (n + 64) * U * terms \
+        + (2.0 ** -25 + n * c.max() * 2.0 ** -37 if dt == torch.float16 else 1e-37)
+    off = (got.double() - ref).abs()
+    assert torch.all(off <= bound), float((off / bound).max())
