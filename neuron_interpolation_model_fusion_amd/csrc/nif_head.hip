@@ -964,7 +964,8 @@ template <int ROWS>
 __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __restrict__ stats, int64_t stat_ld, int tiles, Targets tg,
                                                                 const int* __restrict__ rows, const int* __restrict__ count,
                                                                 float* __restrict__ tops, float* __restrict__ sums,
-                                                                const float* __restrict__ zk, const float* __restrict__ z, int64_t ldz, float* loss,
+                                                                const float* __restrict__ zk, const float* __restrict__ z, int64_t ldz,
+                                                                float* loss,
                                                                 int64_t all_rows, int reduction, int* done, float* __restrict__ reduced) {
   constexpr int PARTS = FINISH_NT / ROWS;
   __shared__ float sh_top[ROWS][PARTS + 1], sh_sum[ROWS][PARTS + 1];
@@ -996,7 +997,8 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
       double s = 0.0;
       for (int k = lane; k < tg.k; k += 64)
         s += target_term(tg, src, k,
-                         ((double)(z ? z[i * ldz + max(0, tg.at[src * tg.k + k])] : zk[i * tg.k + k]) - (double)all) * (double)tg.inv_tau,
+                         ((double)(z ? z[i * ldz + max(0, tg.at[src * tg.k + k])] : zk[i * tg.k + k]) - (double)all) *
+                             (double)tg.inv_tau,
                          log_sum);
       s = wave_sum_f64(s);
       if (lane == 0) {
@@ -1029,8 +1031,8 @@ __global__ __launch_bounds__(FINISH_NT) void head_finish_kernel(const float2* __
 }
 
 // First block: dz = coef[i] (P s - p) with cp[i] = coef[i] * P[i] / (the row's sum of exponentials), and what the products of
-// dz are multiplied with.  Where one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits: the row's largest entry, mostly
-// near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
+// dz are multiplied with.  Where one gradient arrives for all rows, dz goes without it and it joins at the end, in 32 bits:
+// the row's largest entry, mostly near -1, then keeps its bits.  f16 holds nothing below 2^-24, so there dz is scaled by the power of two that takes
 // the largest |coef| max(1, P) to [2^13, 2^14) (|dz| is no larger).  Where no row counts the arriving gradient is not read
 // (there may be none, and zeros stay zeros whatever it holds).  inv_scale[1]: the power of two that takes that largest one
 // to [2^37, 2^38), for `rest`.  The other blocks: gradient 0 for rows without a target, and `rest` cleared.

@@ -1088,7 +1088,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     accuracy and 16-bit ones accumulate in 32 bits.  Under 16-bit inputs and more than 64 rows the gradient of the logits is
     rounded to their type before its products with hidden and weight: beside the rounding of the gradients themselves that is
     hardly seen for labels, and makes the error 1.4 times as large for distillation (f16 2.1e-4 -> 2.9e-4 relative, bf16
-    1.7e-3 -> 2.3e-3); float32 inputs do without, and of up to 64 rows it is held in two 16-bit parts.  Infinite features or weights make losses NaN in float32 beyond small heads; mask classes by
+    1.7e-3 -> 2.3e-3); float32 inputs do without, and of up to 64 rows it is held in two 16-bit parts; bias's gradient does not show it.  Infinite features or weights make losses NaN in float32 beyond small heads; mask classes by
     the bias, with -inf or the type's lowest value.
 
     Memory beyond the gradients: the packed hidden rows; forward 8 bytes a row for every 32 (few rows) to 128 classes;

@@ -400,3 +400,40 @@ def test_the_bias_gradient_keeps_what_its_targets_entries_round_off(ops, dt, red
         + (2.0 ** -25 + n * c.max() * 2.0 ** -37 if dt == torch.float16 else 1e-37)
     off = (got.double() - ref).abs()
     assert torch.all(off <= bound), float((off / bound).max())
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('n, v', [(5, 5003), (40, 20011), (96, 9001), (700, 600)])
+def test_captured_steps_with_a_bias(ops, dt, n, v):
+    """Replayed with new inputs, rows that are left out among them, eager steps of the same between: the buffers of one step
+    are those of the next."""
+    g = torch.Generator(device='cuda').manual_seed(n)
+    d, k = 72, 7
+    h, w, b = (torch.zeros(*s, dtype=dt, device='cuda', requires_grad=True) for s in ((n, d), (v, d), (v,)))
+    values, indices = torch.zeros(n, k, device='cuda'), torch.zeros(n, k, dtype=torch.int32, device='cuda')
+
+    def step():
+        loss = ops.linear_topk_distillation(h, w, values, indices, b, temperature=2.0)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w, b)))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        with torch.no_grad():
+            for t in (h, w, b):
+                t.copy_(torch.randn(t.shape, generator=g, device='cuda') / 3)
+            values.copy_(torch.randn(n, k, generator=g, device='cuda'))
+            indices.copy_(torch.randint(0, v, (n, k), generator=g, device='cuda'))
+            indices[turn::3] = -1
+            if turn == 2:
+                indices.fill_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, c in zip(got, step()):
+            assert torch.equal(a, c)
+        torch.cuda.synchronize()
